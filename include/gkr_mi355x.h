@@ -91,6 +91,11 @@ int gkr_ctx_create(int device, gkr_ctx** out);  /* replaces GpuSumcheckExecutor:
  * digit sums on the matrix cores); other matrices, and every matrix of a
  * context created with GKR_INT8_WEIGHTS=0 in the environment, are read as
  * u32.  Proofs are identical. */
+/* The same on a stream of the caller's (hipStream_t; NULL is the device's
+ * default stream), which must outlive the context: calls are ordered with the
+ * caller's other work on it, and every launch is issued before its call
+ * returns (a context of its own stream issues them from a thread of its own). */
+int gkr_ctx_create_on_stream(int device, void* stream, gkr_ctx** out);
 void gkr_ctx_destroy(gkr_ctx* ctx);
 int gkr_ctx_synchronize(gkr_ctx* ctx);
 /* Per-kernel timing (HIP events on the context stream), for benchmarks.
@@ -175,6 +180,8 @@ int gkr_matrix_invalidate(gkr_ctx* ctx, gkr_matrix* m);
 /* Fill a new resident matrix on the device from the documented synthetic
  * generator (counter-mode SplitMix64; kind 0 uniform M31, kind 1 int8-range). */
 int gkr_matrix_synthetic(gkr_ctx* ctx, uint64_t rows, uint64_t cols, int kind, uint64_t seed, gkr_matrix** out);
+/* A new resident matrix of zeros (asynchronous), e.g. for the outputs below. */
+int gkr_matrix_zeros(gkr_ctx* ctx, uint64_t rows, uint64_t cols, gkr_matrix** out);
 int gkr_matrix_download(gkr_ctx* ctx, const gkr_matrix* m, uint32_t* host);
 void gkr_matrix_free(gkr_matrix* m);
 /* Host-side copy of the synthetic generator, for callers that need the same
@@ -368,6 +375,76 @@ int gkr_matmul_forward(gkr_ctx* ctx, const gkr_matrix* a, const gkr_matrix* b, g
  * product with a given B also builds and keeps B's digit planes (one pass
  * over B plus a host round trip).                                          */
 int gkr_matmul_forward_into(gkr_ctx* ctx, const gkr_matrix* a, const gkr_matrix* b, gkr_matrix* out);
+
+/* ------------------------------------------------------------------ witness operators
+ * What the forward pass of a transformer layer computes around its plain
+ * products, over canonical M31 words, into existing matrices.  All are exact
+ * and asynchronous on the context stream: nothing is allocated once the
+ * context's buffers have grown and the weights' digit planes are there (built
+ * on the first product with a weight, as for gkr_matmul_forward_into).  An
+ * output matrix has the shape of the product and shares no memory with the
+ * inputs or another output, except where said.  NULL is no such operand.
+ *
+ * Activations: 0 none; 1 ReLU, z where z <= 2^30 - 1 (the words of
+ * numbers >= 0) and 0 elsewhere; 2 .. 5 the lookup table that
+ * gkr_prove_activation_layer proves, f(z mod 2^table_log_size) as
+ * gkr_activation_table gives it (table_log_size 1 .. 24, 0 = the default).    */
+
+/* Z = A B + bias, Y = act(Z) + residual (mod P): Y into out, Z into pre.
+ * A is m x k, B k x n; bias 1 x n, residual, pre and out m x n.  The residual
+ * may be the output itself (added in place).  Replaces the reference's GEMM,
+ * add, ReLU and table kernels of the forward pass (engine/src/gpu_sumcheck.rs:418-512). */
+int gkr_matmul_forward_fused(gkr_ctx* ctx, const gkr_matrix* a, const gkr_matrix* b, const gkr_matrix* bias,
+                             uint32_t activation_type, uint32_t table_log_size, const gkr_matrix* residual,
+                             gkr_matrix* pre, gkr_matrix* out);
+/* The gated feed-forward block: G = A Wg, U = A Wu, H = act(G) * U (mod P),
+ * element by element: H into out, and G, act(G) and U, which the walk's
+ * layers read, into gate, act and up.                                        */
+int gkr_gated_forward(gkr_ctx* ctx, const gkr_matrix* a, const gkr_matrix* wg, const gkr_matrix* wu,
+                      uint32_t activation_type, uint32_t table_log_size, gkr_matrix* gate, gkr_matrix* act,
+                      gkr_matrix* up, gkr_matrix* out);
+
+/* A paged cache of keys and values: n_pages pages of page_tokens tokens (a
+ * multiple of 64) for n_kv_heads heads of head_dim values (1 .. 256), shared
+ * by up to max_seqs sequences of up to max_tokens tokens (at most 2^21).  The
+ * pages hold digit planes in the matrix cores' operand order: four bytes a
+ * value, or one in an int8 cache (int8 != 0), whose values are -128 .. 127 as
+ * words.  The cache belongs to its context; sequences are small numbers.     */
+typedef struct gkr_kv_cache gkr_kv_cache;
+int gkr_kv_cache_new(gkr_ctx* ctx, uint32_t n_kv_heads, uint32_t head_dim, uint32_t n_pages, uint32_t page_tokens,
+                     uint32_t max_seqs, uint32_t max_tokens, int int8, gkr_kv_cache** out);
+void gkr_kv_cache_free(gkr_kv_cache* cache);
+/* A new, empty sequence; its end, which gives its pages back. */
+int gkr_kv_cache_new_sequence(gkr_kv_cache* cache, uint32_t* seq);
+int gkr_kv_cache_free_sequence(gkr_kv_cache* cache, uint32_t seq);
+/* Drops the tokens behind the first n_tokens (a rejected draft), with their pages. */
+int gkr_kv_cache_truncate(gkr_kv_cache* cache, uint32_t seq, uint32_t n_tokens);
+int gkr_kv_cache_length(const gkr_kv_cache* cache, uint32_t seq, uint32_t* n_tokens);
+int gkr_kv_cache_free_pages(const gkr_kv_cache* cache, uint32_t* n_pages);
+/* Appends counts[i] tokens to sequence seqs[i], the rows of k and v (each
+ * n_kv_heads * head_dim wide, head by head) in that order; their number is the
+ * sum of the counts.  All of them or, on an error, none: too few pages or too
+ * long a sequence (GKR_ERR_NOMEM), or a word outside an int8 cache's range
+ * (GKR_ERR_INVALID; for this check, and only on int8 caches, the call waits
+ * for the stream).                                                           */
+int gkr_kv_cache_append(gkr_ctx* ctx, gkr_kv_cache* cache, const uint32_t* seqs, const uint32_t* counts, size_t n,
+                        const gkr_matrix* k, const gkr_matrix* v);
+/* Attention of n_rows new tokens: row i of q (n_heads * head_dim words, query
+ * head h on kv head h / (n_heads / n_kv_heads)) over the first lens[i] tokens
+ * of sequence seqs[i] (lens == NULL: all of its tokens; one sequence may have
+ * several rows, as the tokens of a prompt).  For each head and token j seen
+ *   x_j = q . k_j + score_offset (mod P),
+ *   e_j = 2^16 2^min(floor((x_j mod 2^table_log_size) / 2^16), 10), the softmax
+ *         table's entry at x_j (gkr_activation_table, type 4; 0 = default size),
+ * and out = sum_j e_j c(v_j) / sum_j e_j with centered values c(v), rounded to
+ * whole numbers, halves away from zero (0 where nothing is seen).  Also, where
+ * given: weighted = sum_j e_j c(v_j) mod P (as out), sums = sum_j e_j mod P
+ * (n_rows x n_heads), scores = x_j (row i * n_heads + h, at least as many
+ * columns as the longest row; 0 behind a row's last token).                  */
+int gkr_attention_forward(gkr_ctx* ctx, const gkr_kv_cache* cache, const gkr_matrix* q, const uint32_t* seqs,
+                          const uint32_t* lens, size_t n_rows, uint32_t n_heads, uint32_t score_offset,
+                          uint32_t table_log_size, gkr_matrix* weighted, gkr_matrix* sums, gkr_matrix* scores,
+                          gkr_matrix* out);
 
 /* MLE commitments: Poseidon Merkle roots (engine/src/crypto/poseidon_merkle.rs:255-280,
  * root_only_parallel) over securefield_to_felt leaves (poseidon_channel.rs:59-69),

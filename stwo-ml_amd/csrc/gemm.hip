@@ -41,7 +41,7 @@ static int pack_planes(gkr_ctx* c, const uint32_t* X, uint64_t outer, uint64_t K
   return GKR_OK;
 }
 
-static int weight_planes(gkr_ctx* c, gkr_matrix* b) {
+int weight_planes(gkr_ctx* c, gkr_matrix* b) {
   if (b->bplanes) return GKR_OK;
   int np;
   TRY(digit_planes_needed(c, b->dev, b->rows * b->cols, &np));
@@ -59,7 +59,7 @@ static int weight_planes(gkr_ctx* c, gkr_matrix* b) {
   return GKR_OK;
 }
 
-static int matmul_forward(gkr_ctx* c, const gkr_matrix* a, gkr_matrix* b, uint32_t* C) {
+int matmul_forward(gkr_ctx* c, const gkr_matrix* a, gkr_matrix* b, uint32_t* C) {
   const uint64_t m = a->rows, k = a->cols, n = b->cols;
   TRY(weight_planes(c, b));
   const uint64_t nsteps = (k + kGemmK - 1) / kGemmK;

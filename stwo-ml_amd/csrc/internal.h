@@ -24,6 +24,7 @@
 #include "../../include/gkr_mi355x.h"
 #include "field.h"
 #include <functional>
+#include <initializer_list>
 
 #include "kernels.h"
 #include "launcher.h"
@@ -105,7 +106,7 @@ enum Slot {
   S_MULT, S_MIN, S_MOUT, S_D0, S_D1, S_W0, S_W1, S_E0, S_M0, S_M1, S_COLPART,
   S_MK0, S_MK1, S_MKSTEP, S_MKROOT, S_OPL, S_OPI, S_GEMMA, S_GEMMB, S_GEMMP, S_FA2, S_FB2, S_EQPARTS, S_TRIPCNT, S_TRIPMB, S_LKINV, S_LKHIST, S_LDIG, S_R8FLAG, S_PTWAIT, S_EXTA, S_EXTB, S_GRAM, S_NORMSUM, S_NORMROW,
   S_LKARENA, S_LKFOLD, S_LKDESC, S_LKPART, S_LKRES, S_LKTAB,
-  S_BIND, S_BINDEQ, S_BINDDESC, S_BINDPART, S_BINDRES, S_BINDVIRT, S_NSLOTS
+  S_BIND, S_BINDEQ, S_BINDDESC, S_BINDPART, S_BINDRES, S_BINDVIRT, S_WITG, S_WITU, S_ATTP, S_NSLOTS
 };
 // Timer ids: device kernels (HIP events) and host-side phases (Fiat-Shamir
 // hashing inside the reducers, waiting for trip results, waiting for the
@@ -179,6 +180,22 @@ struct gkr_matrix {
 // rebuilt on the next use.
 int drop_derived(gkr_ctx* c, gkr_matrix* m);
 
+// gemm.hip: a matrix's digit planes as the B operand of the forward product
+// (kept with it), and that product into C.
+int weight_planes(gkr_ctx* c, gkr_matrix* b);
+int matmul_forward(gkr_ctx* c, const gkr_matrix* a, gkr_matrix* b, uint32_t* C);
+// logup.hip: an activation table's output column, resident on the device.
+int device_table(gkr_ctx* c, uint32_t tag, uint32_t log_size, uint32_t** out);
+
+// witness.hip: operand checks of the witness operators.  Every given matrix
+// (null: none) is alive on c, and no output shares memory with an input or
+// another output; m has the shape rows x cols.
+int check_operands(gkr_ctx* c, const char* what, std::initializer_list<const gkr_matrix*> ins,
+                   std::initializer_list<const gkr_matrix*> outs);
+int check_shape(const char* what, const char* name, const gkr_matrix* m, uint64_t rows, uint64_t cols);
+// attend.hip: frees a cache's device memory (its handle stays).
+void release_cache(gkr_kv_cache* cache);
+
 struct gkr_qvec {
   gkr_ctx* ctx;
   qm31* dev;
@@ -215,6 +232,7 @@ struct gkr_ctx {
   void* hbuf[H_NSLOTS] = {};
   size_t hcap[H_NSLOTS] = {};
   hipStream_t stream = nullptr;
+  bool own_stream = true;  // false: the caller's (gkr_ctx_create_on_stream), not destroyed here
   void* buf[S_NSLOTS] = {};
   size_t cap[S_NSLOTS] = {};
   qm31* h_res = nullptr;  // pinned result staging (64 QM31)
@@ -240,6 +258,7 @@ struct gkr_ctx {
   std::map<uint64_t, std::vector<uint32_t>> tables;  // (tag << 32 | log) -> table outputs
   std::set<gkr_matrix*> matrices;  // live matrices; detached when the context is destroyed
   std::set<gkr_qvec*> qvecs;       // live QM31 vectors; detached likewise
+  std::set<gkr_kv_cache*> caches;  // live key-value caches; detached likewise
   uint64_t mult_zero_entries = 0;  // leading entries of S_MULT known to be zero once the queued work is done
   std::map<uint64_t, uint32_t*> dev_tables;  // (tag << 32 | log) -> resident device copy of the table outputs
   std::map<uint64_t, felt> table_commitments;  // (tag << 32 | log) -> poseidon_hash_many([tag, log])

@@ -18,7 +18,7 @@ const std::vector<uint32_t>& cached_table(gkr_ctx* c, uint32_t tag, uint32_t log
 }
 // The table's outputs resident on the device, uploaded on first use and kept
 // for the context's lifetime (a model alternates between a few tables).
-static int device_table(gkr_ctx* c, uint32_t tag, uint32_t log_size, uint32_t** out) {
+int device_table(gkr_ctx* c, uint32_t tag, uint32_t log_size, uint32_t** out) {
   const uint64_t key = ((uint64_t)tag << 32) | log_size;
   auto it = c->dev_tables.find(key);
   if (it != c->dev_tables.end()) {

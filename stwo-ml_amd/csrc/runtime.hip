@@ -392,7 +392,7 @@ int dot_m31(gkr_ctx* c, const uint32_t* v, const qm31* eq, uint64_t n, qm31* out
 }
 // ------------------------------------------------------------------ context ABI
 extern "C" void gkr_ctx_destroy(gkr_ctx* c);
-extern "C" int gkr_ctx_create(int device, gkr_ctx** out) {
+static int create_context(int device, bool own_stream, hipStream_t stream, gkr_ctx** out) {
   if (!out) return fail(GKR_ERR_INVALID, "null out");
   int n = 0;
   HIP_CHECK(hipGetDeviceCount(&n));
@@ -402,7 +402,9 @@ extern "C" int gkr_ctx_create(int device, gkr_ctx** out) {
   c->device = device;
   const char* i8 = getenv("GKR_INT8_WEIGHTS");
   c->int8_weights = !(i8 && i8[0] == '0' && i8[1] == 0);  // default on; GKR_INT8_WEIGHTS=0: u32 restriction
-  if (hipStreamCreateWithFlags(&c->stream, hipStreamNonBlocking) != hipSuccess) {
+  c->own_stream = own_stream;
+  c->stream = stream;
+  if (own_stream && hipStreamCreateWithFlags(&c->stream, hipStreamNonBlocking) != hipSuccess) {
     delete c;
     return fail(GKR_ERR_DEVICE, "hipStreamCreate failed");
   }
@@ -436,11 +438,17 @@ extern "C" int gkr_ctx_create(int device, gkr_ctx** out) {
   c->vmailbox->seq = 0;
   c->vmailbox->expired = 0;
   // Launches are issued by a thread of their own unless GKR_ASYNC_LAUNCH=0
-  // (the launch cost then falls on the caller's thread).
+  // (the launch cost then falls on the caller's thread).  On a caller's stream
+  // they are issued before the call returns, so that what the caller puts on
+  // the stream next comes behind them.
   const char* al = getenv("GKR_ASYNC_LAUNCH");
-  if (!(al && al[0] == '0' && al[1] == 0)) c->launcher.reset(new Launcher(device));
+  if (own_stream && !(al && al[0] == '0' && al[1] == 0)) c->launcher.reset(new Launcher(device));
   *out = c;
   return GKR_OK;
+}
+extern "C" int gkr_ctx_create(int device, gkr_ctx** out) { return create_context(device, true, nullptr, out); }
+extern "C" int gkr_ctx_create_on_stream(int device, void* stream, gkr_ctx** out) {
+  return create_context(device, false, (hipStream_t)stream, out);
 }
 extern "C" void gkr_ctx_destroy(gkr_ctx* c) {
   if (!c) return;
@@ -449,7 +457,7 @@ extern "C" void gkr_ctx_destroy(gkr_ctx* c) {
     c->launcher->drain();
     c->launcher.reset();
   }
-  if (c->stream) (void)hipStreamSynchronize(c->stream);
+  if (c->stream || !c->own_stream) (void)hipStreamSynchronize(c->stream);
   for (auto& p : c->pending) {
     (void)hipEventDestroy(p.e0);
     (void)hipEventDestroy(p.e1);
@@ -469,6 +477,7 @@ extern "C" void gkr_ctx_destroy(gkr_ctx* c) {
     v->dev = nullptr;
     v->ctx = nullptr;
   }
+  for (gkr_kv_cache* k : c->caches) release_cache(k);
   for (int s = 0; s < S_NSLOTS; s++)
     if (c->buf[s]) (void)hipFree(c->buf[s]);
   for (auto& t : c->dev_tables) (void)hipFree(t.second);
@@ -481,7 +490,7 @@ extern "C" void gkr_ctx_destroy(gkr_ctx* c) {
     if (c->hbuf[s]) (void)hipHostFree(c->hbuf[s]);
   if (c->h_vec) (void)hipHostFree(c->h_vec);
   if (c->h_out) (void)hipHostFree(c->h_out);
-  if (c->stream) (void)hipStreamDestroy(c->stream);
+  if (c->stream && c->own_stream) (void)hipStreamDestroy(c->stream);
   delete c;
 }
 extern "C" int gkr_ctx_debug(gkr_ctx* c, int op, uint64_t arg) {
@@ -589,6 +598,21 @@ extern "C" int gkr_matrix_synthetic(gkr_ctx* c, uint64_t rows, uint64_t cols, in
     drain(c);
     (void)hipFree(d);
     return rc;
+  }
+  *out = new_matrix(c, d, rows, cols, true);
+  return GKR_OK;
+}
+extern "C" int gkr_matrix_zeros(gkr_ctx* c, uint64_t rows, uint64_t cols, gkr_matrix** out) {
+  if (!c || !out) return fail(GKR_ERR_INVALID, "null argument");
+  if (rows == 0 || cols == 0 || rows > (1ull << 40) / cols)
+    return fail(GKR_ERR_INVALID, "matrix of zeros: %llux%llu", (unsigned long long)rows, (unsigned long long)cols);
+  HIP_TRY(hipSetDevice(c->device));
+  uint32_t* d = nullptr;
+  HIP_TRY(hipMalloc(&d, rows * cols * sizeof(uint32_t)));
+  const hipError_t e = hipMemsetAsync(d, 0, rows * cols * sizeof(uint32_t), c->stream);
+  if (e != hipSuccess) {
+    (void)hipFree(d);
+    return fail(GKR_ERR_DEVICE, "matrix of zeros: %s", hipGetErrorString(e));
   }
   *out = new_matrix(c, d, rows, cols, true);
   return GKR_OK;

@@ -144,6 +144,7 @@ SIGNATURES = [
     ("gkr_channel_export", C.c_int, [_P, _U32P]),
     ("gkr_channel_import", C.c_int, [_P, _U32P]),
     ("gkr_ctx_create", C.c_int, [C.c_int, C.POINTER(_P)]),
+    ("gkr_ctx_create_on_stream", C.c_int, [C.c_int, _P, C.POINTER(_P)]),
     ("gkr_ctx_destroy", None, [_P]),
     ("gkr_ctx_synchronize", C.c_int, [_P]),
     ("gkr_ctx_set_timing", C.c_int, [_P, C.c_int]),
@@ -156,6 +157,7 @@ SIGNATURES = [
     ("gkr_matrix_upload", C.c_int, [_P, _U32P, C.c_uint64, C.c_uint64, C.POINTER(_P)]),
     ("gkr_matrix_wrap_device", C.c_int, [_P, _P, C.c_uint64, C.c_uint64, C.POINTER(_P)]),
     ("gkr_matrix_synthetic", C.c_int, [_P, C.c_uint64, C.c_uint64, C.c_int, C.c_uint64, C.POINTER(_P)]),
+    ("gkr_matrix_zeros", C.c_int, [_P, C.c_uint64, C.c_uint64, C.POINTER(_P)]),
     ("gkr_matrix_download", C.c_int, [_P, _P, _U32P]),
     ("gkr_matrix_free", None, [_P]),
     ("gkr_synthetic_value", C.c_uint32, [C.c_int, C.c_uint64, C.c_uint64]),
@@ -225,6 +227,19 @@ SIGNATURES = [
                                  C.POINTER(C.c_uint32), _PQ]),
     ("gkr_matmul_forward", C.c_int, [_P, _P, _P, C.POINTER(_P)]),
     ("gkr_matmul_forward_into", C.c_int, [_P, _P, _P, _P]),
+    ("gkr_matmul_forward_fused", C.c_int, [_P, _P, _P, _P, C.c_uint32, C.c_uint32, _P, _P, _P]),
+    ("gkr_gated_forward", C.c_int, [_P, _P, _P, _P, C.c_uint32, C.c_uint32, _P, _P, _P, _P]),
+    ("gkr_kv_cache_new", C.c_int, [_P, C.c_uint32, C.c_uint32, C.c_uint32, C.c_uint32, C.c_uint32, C.c_uint32, C.c_int,
+                                   C.POINTER(_P)]),
+    ("gkr_kv_cache_free", None, [_P]),
+    ("gkr_kv_cache_new_sequence", C.c_int, [_P, _U32P]),
+    ("gkr_kv_cache_free_sequence", C.c_int, [_P, C.c_uint32]),
+    ("gkr_kv_cache_truncate", C.c_int, [_P, C.c_uint32, C.c_uint32]),
+    ("gkr_kv_cache_length", C.c_int, [_P, C.c_uint32, _U32P]),
+    ("gkr_kv_cache_free_pages", C.c_int, [_P, _U32P]),
+    ("gkr_kv_cache_append", C.c_int, [_P, _P, _U32P, _U32P, C.c_size_t, _P, _P]),
+    ("gkr_attention_forward", C.c_int, [_P, _P, _P, _U32P, _U32P, C.c_size_t, C.c_uint32, C.c_uint32, C.c_uint32, _P,
+                                        _P, _P, _P]),
     ("gkr_weight_commitment", C.c_int, [_P, _P, _PF]),
     ("gkr_weight_commitments", C.c_int, [_P, C.POINTER(_P), C.c_size_t, _PF]),
     ("gkr_mle_commitment", C.c_int, [_P, _P, _PF]),
@@ -404,11 +419,16 @@ class PoseidonChannel:
 
 # ------------------------------------------------------------------ device
 class Context:
-    """A device context: one HIP stream plus its device buffers."""
+    """A device context: one HIP stream plus its device buffers.  `stream`: a stream of the caller's (its
+    address, e.g. torch.cuda.current_stream().cuda_stream) that the context works on and that outlives it; such a program
+    imports torch first, so that both use its HIP runtime."""
 
-    def __init__(self, device: int = 0):
+    def __init__(self, device: int = 0, stream: Optional[int] = None):
         h = C.c_void_p()
-        _check(lib().gkr_ctx_create(device, C.byref(h)))
+        if stream is None:
+            _check(lib().gkr_ctx_create(device, C.byref(h)))
+        else:
+            _check(lib().gkr_ctx_create_on_stream(device, C.c_void_p(stream), C.byref(h)))
         self._h = h.value
 
     def close(self):
@@ -475,6 +495,12 @@ class Context:
     def synthetic(self, rows: int, cols: int, kind: int, seed: int) -> "Matrix":
         h = C.c_void_p()
         _check(lib().gkr_matrix_synthetic(self._h, rows, cols, kind, seed, C.byref(h)))
+        return Matrix(self, h.value, rows, cols)
+
+    def zeros(self, rows: int, cols: int) -> "Matrix":
+        """gkr_matrix_zeros: a new resident matrix of zeros."""
+        h = C.c_void_p()
+        _check(lib().gkr_matrix_zeros(self._h, rows, cols, C.byref(h)))
         return Matrix(self, h.value, rows, cols)
 
     # ZkmlOps
@@ -613,6 +639,42 @@ class Context:
     def matmul_forward_into(self, a: "Matrix", b: "Matrix", out: "Matrix") -> None:
         """gkr_matmul_forward_into: C = A * B mod P written into an existing matrix."""
         _check(lib().gkr_matmul_forward_into(self._h, a.handle, b.handle, out.handle))
+
+    # witness operators
+    def matmul_forward_fused(self, a: "Matrix", b: "Matrix", out: "Matrix", bias: Optional["Matrix"] = None,
+                             activation: int = 0, table_log_size: int = 0, residual: Optional["Matrix"] = None,
+                             pre: Optional["Matrix"] = None) -> None:
+        """gkr_matmul_forward_fused: out = act(A B + bias) + residual mod P, pre = A B + bias."""
+        _check(lib().gkr_matmul_forward_fused(self._h, a.handle, b.handle, _handle(bias), activation, table_log_size,
+                                              _handle(residual), _handle(pre), out.handle))
+
+    def gated_forward(self, a: "Matrix", wg: "Matrix", wu: "Matrix", out: "Matrix", activation: int = 5,
+                      table_log_size: int = 0, gate: Optional["Matrix"] = None, act: Optional["Matrix"] = None,
+                      up: Optional["Matrix"] = None) -> None:
+        """gkr_gated_forward: out = act(A Wg) * (A Wu) mod P; the parts into gate, act and up."""
+        _check(lib().gkr_gated_forward(self._h, a.handle, wg.handle, wu.handle, activation, table_log_size,
+                                       _handle(gate), _handle(act), _handle(up), out.handle))
+
+    def kv_cache(self, n_kv_heads: int, head_dim: int, n_pages: int, page_tokens: int = 64, max_seqs: int = 64,
+                 max_tokens: int = 65536, int8: bool = False) -> "KvCache":
+        """gkr_kv_cache_new: a paged key-value cache on this context."""
+        h = C.c_void_p()
+        _check(lib().gkr_kv_cache_new(self._h, n_kv_heads, head_dim, n_pages, page_tokens, max_seqs, max_tokens,
+                                      int(int8), C.byref(h)))
+        return KvCache(self, h.value)
+
+    def attention_forward(self, cache: "KvCache", q: "Matrix", seqs: Sequence[int], n_heads: int, out: "Matrix",
+                          lens: Optional[Sequence[int]] = None, score_offset: int = 0, table_log_size: int = 0,
+                          weighted: Optional["Matrix"] = None, sums: Optional["Matrix"] = None,
+                          scores: Optional["Matrix"] = None) -> None:
+        """gkr_attention_forward: row i of q over the first lens[i] tokens (all, without lens) of sequence seqs[i]."""
+        n = len(seqs)
+        if lens is not None and len(lens) != n:
+            raise ValueError(f"{n} sequences and {len(lens)} lengths")
+        c_lens = None if lens is None else (C.c_uint32 * max(1, n))(*lens)
+        _check(lib().gkr_attention_forward(self._h, cache.handle, q.handle, (C.c_uint32 * max(1, n))(*seqs), c_lens, n,
+                                           n_heads, score_offset, table_log_size, _handle(weighted), _handle(sums),
+                                           _handle(scores), out.handle))
 
     def weight_commitment(self, b: "Matrix") -> int:
         """gkr_weight_commitment: commit_mle_root_only(matrix_to_mle_col_major_padded(B))."""
@@ -960,6 +1022,60 @@ class Matrix:
     def free(self):
         if self._h:
             lib().gkr_matrix_free(self._h)
+            self._h = None
+
+    def __del__(self):
+        if _lib is not None and getattr(self, "_h", None):
+            self.free()
+
+
+def _handle(m: Optional["Matrix"]) -> Optional[int]:
+    return None if m is None else m.handle
+
+
+class KvCache:
+    """A paged key-value cache (gkr_kv_cache); made by Context.kv_cache."""
+
+    def __init__(self, ctx: "Context", handle: int):
+        self.ctx, self._h = ctx, handle
+
+    @property
+    def handle(self) -> int:
+        return self._h
+
+    def new_sequence(self) -> int:
+        s = C.c_uint32()
+        _check(lib().gkr_kv_cache_new_sequence(self._h, C.byref(s)))
+        return s.value
+
+    def free_sequence(self, seq: int) -> None:
+        _check(lib().gkr_kv_cache_free_sequence(self._h, seq))
+
+    def truncate(self, seq: int, n_tokens: int) -> None:
+        """Drop the tokens behind the first n_tokens."""
+        _check(lib().gkr_kv_cache_truncate(self._h, seq, n_tokens))
+
+    def length(self, seq: int) -> int:
+        n = C.c_uint32()
+        _check(lib().gkr_kv_cache_length(self._h, seq, C.byref(n)))
+        return n.value
+
+    def free_pages(self) -> int:
+        n = C.c_uint32()
+        _check(lib().gkr_kv_cache_free_pages(self._h, C.byref(n)))
+        return n.value
+
+    def append(self, seqs: Sequence[int], counts: Sequence[int], k: "Matrix", v: "Matrix") -> None:
+        """gkr_kv_cache_append: counts[i] tokens for sequence seqs[i], the rows of k and v in that order."""
+        n = len(seqs)
+        if len(counts) != n:
+            raise ValueError(f"{n} sequences and {len(counts)} counts")
+        _check(lib().gkr_kv_cache_append(self.ctx.handle, self._h, (C.c_uint32 * max(1, n))(*seqs),
+                                         (C.c_uint32 * max(1, n))(*counts), n, k.handle, v.handle))
+
+    def free(self) -> None:
+        if self._h:
+            lib().gkr_kv_cache_free(self._h)
             self._h = None
 
     def __del__(self):

@@ -1,0 +1,253 @@
+"""The fused product and the gated block (gkr_matmul_forward_fused, gkr_gated_forward) against whole-number
+arithmetic: every activation, with and without bias, residual and parts, rows on both sides of each rule on
+sizes, int8-range and general operands, and what is refused."""
+import ctypes
+
+import numpy as np
+import pytest
+
+import gkr_mi355x as G
+
+pytestmark = pytest.mark.gpu
+P = G.P
+RELU, GELU, SIGMOID, SOFTMAX, SILU = 1, 2, 3, 4, 5
+
+
+def product(a, b):
+    """A B mod P: bytes of A by 16-bit halves of B, every partial sum below 2^53."""
+    a, b = a.astype(np.int64), b.astype(np.int64)
+    out = np.zeros((a.shape[0], b.shape[1]), np.int64)
+    for i in range(4):
+        for j in range(2):
+            s = ((a >> (8 * i)) & 255).astype(np.float64) @ ((b >> (16 * j)) & 0xFFFF).astype(np.float64)
+            out = (out + s.astype(np.int64) % P * pow(2, 8 * i + 16 * j, P)) % P
+    return out
+
+
+def activate(z, act, log):
+    if act == 0:
+        return z
+    if act == RELU:
+        return np.where(z <= (1 << 30) - 1, z, 0)
+    log = log or (20 if act == SOFTMAX else 16)
+    return G.activation_table(act, log).astype(np.int64)[z % (1 << log)]
+
+
+def words(rng, shape, kind):
+    if kind == 0:
+        return rng.integers(0, P, size=shape, dtype=np.uint32)
+    v = rng.integers(-127, 128, size=shape)
+    return np.where(v < 0, v + P, v).astype(np.uint32)
+
+
+def check_fused(ctx, m, k, n, xk, wk, act=0, log=0, bias=True, residual=True, pre=True, seed=1, x=None):
+    rng = np.random.default_rng(seed + m * 31 + k * 7 + n)
+    A, B = words(rng, (m, k), xk) if x is None else x, words(rng, (k, n), wk)
+    bv, rv = words(rng, (1, n), 0), words(rng, (m, n), 0)
+    out, z = ctx.zeros(m, n), ctx.zeros(m, n)
+    a, b, bm, rm = ctx.upload(A), ctx.upload(B), ctx.upload(bv), ctx.upload(rv)
+    ref = product(A, B)
+    if bias:
+        ref = (ref + bv) % P
+    y = activate(ref, act, log)
+    if residual:
+        y = (y + rv) % P
+    for _ in range(2):  # the second finds the weight's planes built
+        ctx.matmul_forward_fused(a, b, out, bias=bm if bias else None, activation=act, table_log_size=log,
+                                 residual=rm if residual else None, pre=z if pre else None)
+        assert np.array_equal(out.download(), y)
+        if pre:
+            assert np.array_equal(z.download(), ref)
+
+
+def check_gated(ctx, m, k, n, xk, wk, act=SILU, log=0, trace=True, seed=2):
+    rng = np.random.default_rng(seed + m * 31 + k * 7 + n)
+    A, Wg, Wu = words(rng, (m, k), xk), words(rng, (k, n), wk), words(rng, (k, n), wk)
+    a, wg, wu = ctx.upload(A), ctx.upload(Wg), ctx.upload(Wu)
+    out, g, t, u = (ctx.zeros(m, n) for _ in range(4))
+    gate, up = product(A, Wg), product(A, Wu)
+    ac = activate(gate, act, log)
+    for _ in range(2):
+        ctx.gated_forward(a, wg, wu, out, activation=act, table_log_size=log, **(dict(gate=g, act=t, up=u) if trace else {}))
+        assert np.array_equal(out.download(), ac * up % P)
+        if trace:
+            assert np.array_equal(g.download(), gate)
+            assert np.array_equal(t.download(), ac)
+            assert np.array_equal(u.download(), up)
+
+
+@pytest.mark.parametrize("act,log", [(0, 0), (RELU, 0), (GELU, 0), (SIGMOID, 0), (SOFTMAX, 0), (SILU, 0), (SILU, 1),
+                                     (GELU, 20)])
+def test_activations(gpu_ctx, act, log):
+    for bias, residual, pre in ((True, True, True), (False, False, False), (False, True, False)):
+        check_fused(gpu_ctx, 5, 100, 70, 0, 1, act, log, bias, residual, pre)
+
+
+@pytest.mark.parametrize("m", [1, 2, 3, 4, 5, 8, 9, 16, 17, 32, 33, 64, 65, 100, 129, 300])
+@pytest.mark.parametrize("k,n", [(1, 1), (33, 31), (576, 192), (1000, 333)])
+def test_row_counts(gpu_ctx, m, k, n):
+    for xk in (1, 0):
+        for wk in (1, 0):
+            check_fused(gpu_ctx, m, k, n, xk, wk, GELU)
+            check_gated(gpu_ctx, m, k, n, xk, wk)
+
+
+# long sums (several splits or passes of K), one row to many
+@pytest.mark.parametrize("m,k,n", [(1, 40001, 40), (3, 20000, 65), (8, 13825, 31), (40, 17000, 96), (70, 33001, 33),
+                                   (200, 9001, 260), (2, 140001, 3), (33, 131073, 5)])
+def test_long_sums(gpu_ctx, m, k, n):
+    for xk, wk in ((1, 1), (0, 1), (0, 0)):
+        check_fused(gpu_ctx, m, k, n, xk, wk, 0)
+    check_gated(gpu_ctx, m, k, n, 0, 1)
+
+
+@pytest.mark.parametrize("m,k,n", [(1, 300, 13824), (512, 700, 1100), (300, 4000, 2100), (64, 2048, 5120)])
+def test_wide(gpu_ctx, m, k, n):
+    for xk in (1, 0):
+        check_fused(gpu_ctx, m, k, n, xk, 1, 0)
+        check_gated(gpu_ctx, m, k, n, xk, 1)
+
+
+@pytest.mark.parametrize("m,k", [(1, 40000), (8, 9000), (64, 9000), (260, 5000)])
+@pytest.mark.parametrize("fill", [P - 1, P // 2, P // 2 + 1, P - 128, 127])
+def test_extreme_words(gpu_ctx, m, k, fill):
+    """Operands of one repeated word: every digit sum at its largest."""
+    n = 40
+    A, B = np.full((m, k), fill, np.uint32), np.full((k, n), P - 128, np.uint32)
+    want = np.full((m, n), (fill - P if fill > P // 2 else fill) * -128 * k % P)
+    out = gpu_ctx.zeros(m, n)
+    gpu_ctx.matmul_forward_fused(gpu_ctx.upload(A), gpu_ctx.upload(B), out)
+    assert np.array_equal(out.download(), want)
+    B[:] = P // 2 + 1
+    c = P // 2 + 1 - P
+    gpu_ctx.matmul_forward_fused(gpu_ctx.upload(A), gpu_ctx.upload(B), out)
+    assert np.array_equal(out.download(), np.full((m, n), (fill - P if fill > P // 2 else fill) * c * k % P))
+
+
+@pytest.mark.parametrize("m,k,n", [(2, 65, 40), (30, 600, 100), (300, 300, 300), (260, 2000, 500)])
+def test_one_high_word(gpu_ctx, m, k, n):
+    """A single word outside the int8 range, in the last place, after a call without one and before another."""
+    rng = np.random.default_rng(4)
+    x = words(rng, (m, k), 1)
+    check_fused(gpu_ctx, m, k, n, 1, 1, x=x)
+    x[-1, -1] = 1 << 20
+    check_fused(gpu_ctx, m, k, n, 1, 1, x=x)
+    check_fused(gpu_ctx, m, k, n, 1, 1, seed=9)
+
+
+@pytest.mark.parametrize("m,k,n", [(1, 4000, 500), (40, 4000, 500), (300, 900, 700)])
+def test_weights_of_two_and_three_planes(gpu_ctx, m, k, n):
+    rng = np.random.default_rng(6)
+    for bits in (12, 20):
+        B = rng.integers(0, 1 << bits, size=(k, n), dtype=np.uint32)
+        A = words(rng, (m, k), 0)
+        out = gpu_ctx.zeros(m, n)
+        gpu_ctx.matmul_forward_fused(gpu_ctx.upload(A), gpu_ctx.upload(B), out)
+        assert np.array_equal(out.download(), product(A, B))
+        H = gpu_ctx.zeros(m, n)  # a gate and an up weight of different plane counts
+        W2 = words(rng, (k, n), 1)
+        gpu_ctx.gated_forward(gpu_ctx.upload(A), gpu_ctx.upload(B), gpu_ctx.upload(W2), H, activation=RELU)
+        assert np.array_equal(H.download(), activate(product(A, B), RELU, 0) * product(A, W2) % P)
+
+
+@pytest.mark.parametrize("m", [1, 20, 300])
+def test_residual_in_place(gpu_ctx, m):
+    rng = np.random.default_rng(5)
+    A, B, R = words(rng, (m, 500), 0), words(rng, (500, 130), 1), words(rng, (m, 130), 0)
+    a, b, h = gpu_ctx.upload(A), gpu_ctx.upload(B), gpu_ctx.upload(R)
+    ref = R.astype(np.int64)
+    for _ in range(3):
+        gpu_ctx.matmul_forward_fused(a, b, h, residual=h)
+        ref = (ref + product(A, B)) % P
+        assert np.array_equal(h.download(), ref)
+
+
+def test_changed_weights_and_outputs(gpu_ctx):
+    """An output that was a weight is no longer taken from its old planes."""
+    rng = np.random.default_rng(8)
+    A, B, W = words(rng, (4, 64), 1), words(rng, (64, 64), 1), words(rng, (64, 64), 1)
+    a, b, w, out = gpu_ctx.upload(A), gpu_ctx.upload(B), gpu_ctx.upload(W), gpu_ctx.zeros(4, 64)
+    gpu_ctx.matmul_forward_fused(a, w, out)
+    gpu_ctx.matmul_forward_fused(b, b, w)
+    gpu_ctx.matmul_forward_fused(a, w, out)
+    assert np.array_equal(out.download(), product(A, product(B, B)))
+
+
+def test_refusals(gpu_ctx):
+    a, b, out = gpu_ctx.zeros(3, 40), gpu_ctx.zeros(40, 50), gpu_ctx.zeros(3, 50)
+    other = G.Context(0)
+    stray = other.zeros(3, 50)
+    part = gpu_ctx.wrap_device(out.device_ptr + 4, 1, 50)
+    half = gpu_ctx.wrap_device(out.device_ptr, 2, 50)
+    bad = [dict(bias=gpu_ctx.zeros(1, 49)), dict(bias=gpu_ctx.zeros(3, 50)), dict(residual=gpu_ctx.zeros(3, 51)),
+           dict(pre=gpu_ctx.zeros(2, 50)), dict(pre=out), dict(residual=stray), dict(pre=stray), dict(bias=part),
+           dict(pre=half), dict(activation=6), dict(activation=SILU, table_log_size=25)]
+    for kw in bad:
+        with pytest.raises(G.GkrError) as e:
+            gpu_ctx.matmul_forward_fused(a, b, out, **kw)
+        assert e.value.code == 1, kw
+    shifted = gpu_ctx.wrap_device(gpu_ctx.zeros(4, 50).device_ptr, 3, 50)
+    for args in ((a, a, out), (a, b, a), (a, b, gpu_ctx.zeros(3, 40)), (stray, b, out)):
+        with pytest.raises(G.GkrError):
+            gpu_ctx.matmul_forward_fused(*args)
+    with pytest.raises(G.GkrError):
+        gpu_ctx.matmul_forward_fused(a, b, out, residual=gpu_ctx.wrap_device(out.device_ptr + 200, 3, 50))
+    for kw in (dict(gate=out), dict(act=gpu_ctx.zeros(3, 49)), dict(up=stray), dict(activation=9)):
+        with pytest.raises(G.GkrError):
+            gpu_ctx.gated_forward(a, b, b, out, **kw)
+    with pytest.raises(G.GkrError):
+        gpu_ctx.gated_forward(a, b, gpu_ctx.zeros(40, 51), out)
+    with pytest.raises(G.GkrError):
+        gpu_ctx.zeros(0, 3)
+    del shifted
+    gpu_ctx.matmul_forward_fused(a, b, out)  # and the context goes on
+    assert not out.download().any()
+    other.close()
+
+
+def test_refused_launch_leaves_the_context_usable(gpu_ctx):
+    for m in (1, 40, 300):
+        a, b, out = gpu_ctx.synthetic(m, 64, 0, 1), gpu_ctx.synthetic(64, 96, 1, 2), gpu_ctx.zeros(m, 96)
+        gpu_ctx.matmul_forward_fused(a, b, out)
+        want = out.download()
+        for nth in (1, 2):
+            gpu_ctx.debug(G.DEBUG_REFUSE_LAUNCH, nth)
+            try:
+                gpu_ctx.matmul_forward_fused(a, b, out)
+                gpu_ctx.matmul_forward_fused(a, b, out)
+                gpu_ctx.synchronize()
+            except G.GkrError:
+                pass
+            gpu_ctx.debug(G.DEBUG_REFUSE_LAUNCH, 0)
+            try:
+                gpu_ctx.matmul_forward_fused(a, b, out)
+            except G.GkrError:  # the launcher thread's refusal, told by the next call
+                gpu_ctx.matmul_forward_fused(a, b, out)
+            assert np.array_equal(out.download(), want)
+
+
+def test_on_the_callers_stream():
+    """A context on a stream of the caller's (one of its own, then the default one): ordered with the copies
+    and fills that the caller puts on it before and behind each call."""
+    G.lib()
+    hip = ctypes.CDLL("libamdhip64.so.7")  # the runtime the library has loaded
+    vp, size = ctypes.c_void_p, ctypes.c_size_t
+    copy, fill, stream = hip.hipMemcpyAsync, hip.hipMemsetAsync, vp()
+    copy.argtypes, fill.argtypes = [vp, vp, size, ctypes.c_int, vp], [vp, ctypes.c_int, size, vp]
+    assert hip.hipStreamCreate(ctypes.byref(stream)) == 0
+    to_device, within_device = 1, 3
+    rng = np.random.default_rng(3)
+    B = words(rng, (700, 300), 1)
+    for s in (stream, vp()):
+        ctx = G.Context(0, stream=s.value or 0)
+        a, b, o, kept = ctx.zeros(4, 700), ctx.upload(B), ctx.zeros(4, 300), ctx.zeros(4, 300)
+        for i in range(20):
+            A = words(rng, (4, 700), i % 2)
+            assert copy(a.device_ptr, A.ctypes.data, A.nbytes, to_device, s) == 0
+            ctx.matmul_forward_fused(a, b, o)
+            assert copy(kept.device_ptr, o.device_ptr, 4800, within_device, s) == 0
+            assert fill(o.device_ptr, 0, 4800, s) == 0
+            assert hip.hipStreamSynchronize(s) == 0
+            assert np.array_equal(kept.download(), product(A, B)) and not o.download().any()
+        ctx.close()
+    assert hip.hipStreamDestroy(stream) == 0
