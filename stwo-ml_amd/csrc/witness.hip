@@ -2,6 +2,7 @@
 // feed-forward block (kernels in witness.h).
 #include "internal.h"
 #include "activations.h"
+#include "gemm.h"
 #include "witness.h"
 
 static bool overlap(const gkr_matrix* x, const gkr_matrix* y) {
@@ -47,6 +48,35 @@ static int activation_arg(gkr_ctx* c, const char* what, uint32_t tag, uint32_t l
   arg->mask = (1u << log_size) - 1;
   return GKR_OK;
 }
+// Longest inner size of the kernels here: a digit sum stays below 2^31.
+// Beyond it (no model's layer) the forward product's passes of K are used,
+// with the element-wise work in a launch behind.
+constexpr uint64_t kMaxInner = 131071;
+
+static WitWeight wit_weight(const gkr_matrix* w) { return WitWeight{w->bplanes, (uint32_t)w->bnplanes}; }
+
+// One to four rows (k_rows).
+template <bool GATED, class End>
+static int rows_product(gkr_ctx* c, const gkr_matrix* a, const gkr_matrix* w0, const gkr_matrix* w1, const End& end) {
+  const uint32_t m = (uint32_t)a->rows, k = (uint32_t)a->cols;
+  const uint64_t n = w0->cols, ctiles = (n + kGemmTile - 1) / kGemmTile;
+  const bool one = w0->bnplanes == 1 && w1->bnplanes == 1;
+  auto launch = [&](auto kernel, uint32_t mr) {
+    const uint32_t lds = std::min<uint32_t>(kRowLds, 4 * mr * ((k + 63) / 64 * 64));
+    GKR_LAUNCH(c, kernel, dim3((uint32_t)ctiles), dim3(64 * kRowWaves), lds, a->dev, wit_weight(w0), wit_weight(w1), m, k,
+               (uint32_t)n, end);
+  };
+  if (m == 1) one ? launch(k_rows<1, 1, GATED, End>, 1) : launch(k_rows<1, 4, GATED, End>, 1);
+  else if (m == 2) one ? launch(k_rows<2, 1, GATED, End>, 2) : launch(k_rows<2, 4, GATED, End>, 2);
+  else one ? launch(k_rows<4, 1, GATED, End>, 4) : launch(k_rows<4, 4, GATED, End>, 4);
+  return check_launch(c);
+}
+// A grid of kernels with 1024 threads takes this many column tiles.
+constexpr uint64_t kRowMaxTiles = 1ull << 21;
+static bool few_rows(uint64_t m, uint64_t k, uint64_t n) {
+  return m <= 4 && k <= kMaxInner && n <= kRowMaxTiles * kGemmTile;
+}
+
 static dim3 end_grid(uint64_t count) { return dim3((uint32_t)std::min<uint64_t>((count + 255) / 256, 1u << 20)); }
 
 extern "C" int gkr_matmul_forward_fused(gkr_ctx* c, const gkr_matrix* a, const gkr_matrix* b, const gkr_matrix* bias,
@@ -76,6 +106,8 @@ extern "C" int gkr_matmul_forward_fused(gkr_ctx* c, const gkr_matrix* a, const g
   e.out = out->dev;
   TRY(drop_derived(c, out));
   if (pre) TRY(drop_derived(c, pre));
+  TRY(weight_planes(c, const_cast<gkr_matrix*>(b)));
+  if (few_rows(m, a->cols, n)) return rows_product<false>(c, a, b, b, e);
   uint32_t* z;
   TRY(ensureT(c, S_WITG, m * n, &z));
   TRY(matmul_forward(c, a, const_cast<gkr_matrix*>(b), z));
@@ -107,6 +139,9 @@ extern "C" int gkr_gated_forward(gkr_ctx* c, const gkr_matrix* a, const gkr_matr
   e.out = out->dev;
   for (gkr_matrix* w : {gate, act, up, out})
     if (w) TRY(drop_derived(c, w));
+  TRY(weight_planes(c, const_cast<gkr_matrix*>(wg)));
+  TRY(weight_planes(c, const_cast<gkr_matrix*>(wu)));
+  if (few_rows(m, a->cols, n)) return rows_product<true>(c, a, wg, wu, e);
   uint32_t *g, *u;
   TRY(ensureT(c, S_WITG, m * n, &g));
   TRY(ensureT(c, S_WITU, m * n, &u));
