@@ -118,11 +118,19 @@ __device__ __forceinline__ void att_finish(const AttOut& o, uint64_t at, int64_t
   if (o.weighted) o.weighted[at] = shift16(signed_mod_p(total));
 }
 
+// A store of four scores, on a 4-byte boundary at least.
+struct __attribute__((packed, aligned(4))) Scores4 {
+  uint32_t v[4];
+};
+
 // One workgroup: up to 16 query heads of one kv head, `bpw` blocks of one row.
 // Four blocks a step: wave w forms the scores and weights of block w, all
-// waves read the four blocks' weights from LDS, and wave w takes the dims 16
-// (w + 4 i) .. + 15 of the values.  NP planes of the cache; DT = dims / 64
-// rounded up.
+// waves read the four blocks' weights from LDS (two buffers, one barrier a
+// step), and wave w takes the dims 16 (w + 4 i) .. + 15 of the values.  The
+// loads run ahead: a wave holds NS of its four token tiles of keys and NS of
+// the step's four blocks of values, and refills each as it has used it, across
+// steps (values are loaded before their weights are known).
+// NP planes of the cache; DT = dims / 64 rounded up.
 template <int NP, int DT>
 static __global__ void __launch_bounds__(256) k_attend(KvPool p, AttRowArgs rows, uint32_t bpw,
                                                        const uint32_t* __restrict__ q, uint32_t heads,
@@ -130,32 +138,78 @@ static __global__ void __launch_bounds__(256) k_attend(KvPool p, AttRowArgs rows
                                                        int64_t* __restrict__ part, uint32_t* __restrict__ part_z,
                                                        AttOut o) {
   constexpr int NG = NP + 3, NV = NP + 1;  // digit groups of the scores and of the weighted sums
-  __shared__ v4i weights[4][2][64];
+  constexpr int NS = NP * DT <= 4 ? 4 : NP * DT <= 8 ? 2 : 1;
+  __shared__ v4i weights[2][4][2][64];
   __shared__ uint32_t zsum[4][16];
-  const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 15, quarter = lane >> 4;
+  const uint32_t lane = threadIdx.x & 63, col = lane & 15, quarter = lane >> 4;
+  const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   uint32_t r = 0;
   while (r + 1 < rows.n && rows.e[r + 1].part0 <= blockIdx.x) r++;
   const uint32_t group = heads / p.kv_heads, tiles = (group + kAttHeads - 1) / kAttHeads;
   const uint32_t kvh = blockIdx.y / tiles, h0 = blockIdx.y % tiles * kAttHeads;
   const uint32_t mine = group - h0 < kAttHeads ? group - h0 : kAttHeads;  // heads of this workgroup
-  const uint32_t len = rows.e[r].len, nblocks = (len + kAttBlock - 1) / kAttBlock;
+  const uint32_t seq = rows.e[r].seq, len = rows.e[r].len, nblocks = (len + kAttBlock - 1) / kAttBlock;
   const uint64_t row = row0 + r;
   const uint32_t b0 = (blockIdx.x - rows.e[r].part0) * bpw;
   const uint32_t head0 = kvh * group + h0;
-  const uint64_t plane = (uint64_t)p.chunks * 1024;
+  const uint32_t plane = p.chunks * 1024;
+  const uint32_t b_end = b0 + bpw, seen_end = b_end < nblocks ? b_end : nblocks;
+
+  v4i kd[NS][DT][NP], vd[NS][DT][NP];
+  const int8_t *kbase = nullptr, *vbase[4] = {};
+  auto key_block = [&](uint32_t b) {  // this wave's block of the step from b: past the end, the last one again
+    const uint32_t block = b + wave < seen_end ? b + wave : seen_end - 1;
+    kbase = p.k + kv_block(p, seq, block, kvh);
+  };
+  auto load_keys = [&](int slot, int t) {
+#pragma unroll
+    for (int s = 0; s < DT; s++) {
+      const uint32_t chunk = 4 * s + quarter;  // past the dims the query's digits are zero
+      const uint32_t at = (chunk < p.chunks ? chunk : p.chunks - 1) * 1024 + 256 * t + 16 * col;
+#pragma unroll
+      for (int pk = 0; pk < NP; pk++) kd[slot][s][pk] = __builtin_nontemporal_load((const v4i*)(kbase + (at + pk * plane)));
+    }
+  };
+  auto value_blocks = [&](uint32_t b) {
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+      const uint32_t block = b + j < seen_end ? b + j : seen_end - 1;
+      vbase[j] = p.v + kv_block(p, seq, block, kvh);
+    }
+  };
+  auto load_values = [&](int slot, int j) {
+#pragma unroll
+    for (int i = 0; i < DT; i++) {
+      const uint32_t tile = wave + 4 * i < p.chunks ? wave + 4 * i : p.chunks - 1;  // past the dims: not stored
+#pragma unroll
+      for (int pv = 0; pv < NP; pv++)
+        vd[slot][i][pv] = __builtin_nontemporal_load((const v4i*)(vbase[j] + (tile * 1024 + pv * plane + 16 * lane)));
+    }
+  };
+  if (b0 < seen_end) {
+    key_block(b0);
+    value_blocks(b0);
+#pragma unroll
+    for (int t = 0; t < NS; t++) load_keys(t, t);
+#pragma unroll
+    for (int j = 0; j < NS; j++) load_values(j, j);
+  }
 
   v4i qd[DT][4];  // the query's digits: head col, dims 16 (4 s + quarter) .. + 15
 #pragma unroll
   for (int s = 0; s < DT; s++) {
-    uint32_t w[4][4] = {};
+    uint32_t w[4][4];
 #pragma unroll
-    for (int i = 0; i < 16; i++) {
-      const uint32_t d = 16 * (4 * s + quarter) + i;
-      const uint32_t x = col < mine && d < p.dim ? q[(row * heads + head0 + col) * p.dim + d] : 0u;
-      int32_t dg[4];
-      balanced_digits(center_m31(x), dg);
+    for (int i = 0; i < 4; i++) {
+      uint32_t d[4], out[4];
 #pragma unroll
-      for (int g = 0; g < 4; g++) w[g][i >> 2] |= ((uint32_t)dg[g] & 0xffu) << (8 * (i & 3));
+      for (int j = 0; j < 4; j++) {
+        const uint32_t dim = 16 * (4 * s + quarter) + 4 * i + j;
+        d[j] = digit_bytes(col < mine && dim < p.dim ? q[(row * heads + head0 + col) * p.dim + dim] : 0u);
+      }
+      transpose_bytes(d, out);
+#pragma unroll
+      for (int g = 0; g < 4; g++) w[g][i] = out[g];
     }
 #pragma unroll
     for (int g = 0; g < 4; g++) qd[s][g] = v4i{(int)w[g][0], (int)w[g][1], (int)w[g][2], (int)w[g][3]};
@@ -166,79 +220,77 @@ static __global__ void __launch_bounds__(256) k_attend(KvPool p, AttRowArgs rows
 #pragma unroll
     for (int g = 0; g < NV; g++) acc[i][g] = v4i{0, 0, 0, 0};
   uint32_t z = 0;
-  const uint32_t b_end = b0 + bpw, seen_end = b_end < nblocks ? b_end : nblocks;
-  const uint32_t walk_end = o.scores ? b_end : seen_end;  // scores behind the last token are cleared
-  for (uint32_t b = b0; b < walk_end; b += 4) {
-    const uint32_t block = b + wave;
-    v4i w0 = v4i{0, 0, 0, 0}, w1 = v4i{0, 0, 0, 0};
-    uint32_t x[4][4] = {};
-    if (block < seen_end) {
-      const int8_t* kb = p.k + kv_block(p, rows.e[r].seq, block, kvh) + 16 * col;
+  uint32_t* const my_scores =
+      o.scores && col < mine ? o.scores + (row * heads + head0 + col) * o.score_cols : nullptr;
+  auto store_scores = [&](uint32_t block, int t, const uint32_t (&x)[4]) {
+    const uint64_t tok = (uint64_t)block * kAttBlock + 16 * t + 4 * quarter;
+    if (!my_scores || block >= b_end || tok >= o.score_cols) return;
+    if (tok + 4 <= o.score_cols)
+      *(Scores4*)(my_scores + tok) = Scores4{{x[0], x[1], x[2], x[3]}};
+    else
+      for (int v = 0; v < 4; v++)
+        if (tok + v < o.score_cols) my_scores[tok + v] = x[v];
+  };
+  uint32_t b = b0;
+  for (uint32_t turn = 0; b < seen_end; b += 4, turn ^= 1) {
+    const uint32_t block = b + wave, first = block * kAttBlock + 4 * quarter;
+    v4i w0, w1;
 #pragma unroll
-      for (int t = 0; t < 4; t++) {
-        v4i sc[NG];
+    for (int t = 0; t < 4; t++) {
+      v4i sc[NG];
 #pragma unroll
-        for (int g = 0; g < NG; g++) sc[g] = v4i{0, 0, 0, 0};
+      for (int g = 0; g < NG; g++) sc[g] = v4i{0, 0, 0, 0};
 #pragma unroll
-        for (int s = 0; s < DT; s++) {
-          const uint32_t chunk = 4 * s + quarter;  // past the dims the query's digits are zero
-          const int8_t* at = kb + (chunk < p.chunks ? chunk : p.chunks - 1) * 1024 + 256 * t;
+      for (int s = 0; s < DT; s++)
 #pragma unroll
-          for (int pk = 0; pk < NP; pk++) {
-            const v4i kd = *(const v4i*)(at + pk * plane);
+        for (int pk = 0; pk < NP; pk++)
 #pragma unroll
-            for (int g = 0; g < 4; g++) sc[pk + g] = __builtin_amdgcn_mfma_i32_16x16x64_i8(kd, qd[s][g], sc[pk + g], 0, 0, 0);
-          }
-        }
+          for (int g = 0; g < 4; g++)
+            sc[pk + g] = __builtin_amdgcn_mfma_i32_16x16x64_i8(kd[t % NS][s][pk], qd[s][g], sc[pk + g], 0, 0, 0);
+      if (t + NS == 4 && b + 4 < seen_end) key_block(b + 4);
+      if (t + NS < 4 || b + 4 < seen_end) load_keys(t % NS, (t + NS) % 4);
+      uint32_t x[4], lo = 0, hi = 0;
 #pragma unroll
-        for (int v = 0; v < 4; v++) {
-          // sum_g 256^g sc[g], below 2^52, with 2^32 = 2 (mod P)
-          int64_t sum = (int64_t)sc[0][v] + ((int64_t)sc[1][v] << 8) + ((int64_t)sc[2][v] << 16) + ((int64_t)sc[3][v] << 24);
-          if constexpr (NP > 1)
-            sum += ((int64_t)sc[4][v] << 1) + ((int64_t)sc[5][v] << 9) + ((int64_t)sc[6][v] << 17);
-          const uint32_t xv = m31_add(m31_reduce64((uint64_t)(sum + ((int64_t)P << 24))), offset);
-          const bool seen = block * kAttBlock + 16 * t + 4 * quarter + v < len;
-          uint32_t g = (xv & mask) >> 16;
-          g = g < 10 ? g : 10;
-          const uint32_t e = seen ? 1u << g : 0u;  // digits base 256, balanced: 128 is 256 - 128
-          x[t][v] = seen ? xv : 0u;
-          z += e;
-          w0[t] |= (int)((e & 0xffu) << (8 * v));
-          w1[t] |= (int)(((e + 0x80u) >> 8) << (8 * v));
-        }
+      for (int v = 0; v < 4; v++) {
+        // sum_g 256^g sc[g], below 2^52, with 2^32 = 2 (mod P)
+        int64_t sum = (int64_t)sc[0][v] + ((int64_t)sc[1][v] << 8) + ((int64_t)sc[2][v] << 16) + ((int64_t)sc[3][v] << 24);
+        if constexpr (NP > 1)
+          sum += ((int64_t)sc[4][v] << 1) + ((int64_t)sc[5][v] << 9) + ((int64_t)sc[6][v] << 17);
+        const uint32_t xv = m31_add(m31_reduce64((uint64_t)(sum + ((int64_t)P << 24))), offset);
+        const bool seen = block < seen_end && first + 16 * t + v < len;
+        uint32_t g = (xv & mask) >> 16;
+        g = g < 10 ? g : 10;
+        const uint32_t e = seen ? 1u << g : 0u;  // digits base 256, balanced: 128 is 256 - 128
+        x[v] = seen ? xv : 0u;
+        z += e;
+        lo |= (e & 0xffu) << (8 * v);
+        hi |= ((e + 0x80u) >> 8) << (8 * v);
       }
+      w0[t] = (int)lo;
+      w1[t] = (int)hi;
+      store_scores(block, t, x);
     }
-    if (o.scores && col < mine) {
-      uint32_t* out = o.scores + (row * heads + head0 + col) * o.score_cols;
-#pragma unroll
-      for (int t = 0; t < 4; t++)
-#pragma unroll
-        for (int v = 0; v < 4; v++) {
-          const uint64_t tok = (uint64_t)block * kAttBlock + 16 * t + 4 * quarter + v;
-          if (tok < o.score_cols && block < b_end) out[tok] = x[t][v];
-        }
-    }
-    if (b >= seen_end) continue;  // uniform: only scores to clear
-    weights[wave][0][lane] = w0;
-    weights[wave][1][lane] = w1;
+    weights[turn][wave][0][lane] = w0;
+    weights[turn][wave][1][lane] = w1;
     __syncthreads();
-    const uint32_t nb = seen_end - b < 4 ? seen_end - b : 4;
-    for (uint32_t j = 0; j < nb; j++) {
-      const int8_t* vb = p.v + kv_block(p, rows.e[r].seq, b + j, kvh) + 16 * lane;
-      const v4i e0 = weights[j][0][lane], e1 = weights[j][1][lane];
 #pragma unroll
-      for (int i = 0; i < DT; i++) {
-        const uint32_t tile = wave + 4 * i;
-        if (tile >= p.chunks) continue;  // uniform in the wave
+    for (int j = 0; j < 4; j++) {  // blocks past the end have no weight
+      const v4i e0 = weights[turn][j][0][lane], e1 = weights[turn][j][1][lane];
+#pragma unroll
+      for (int i = 0; i < DT; i++)
 #pragma unroll
         for (int pv = 0; pv < NP; pv++) {
-          const v4i vd = *(const v4i*)(vb + tile * 1024 + pv * plane);
-          acc[i][pv] = __builtin_amdgcn_mfma_i32_16x16x64_i8(e0, vd, acc[i][pv], 0, 0, 0);
-          acc[i][pv + 1] = __builtin_amdgcn_mfma_i32_16x16x64_i8(e1, vd, acc[i][pv + 1], 0, 0, 0);
+          acc[i][pv] = __builtin_amdgcn_mfma_i32_16x16x64_i8(e0, vd[j % NS][i][pv], acc[i][pv], 0, 0, 0);
+          acc[i][pv + 1] = __builtin_amdgcn_mfma_i32_16x16x64_i8(e1, vd[j % NS][i][pv], acc[i][pv + 1], 0, 0, 0);
         }
-      }
+      if (j + NS == 4 && b + 4 < seen_end) value_blocks(b + 4);
+      if (j + NS < 4 || b + 4 < seen_end) load_values(j % NS, (j + NS) % 4);
     }
-    __syncthreads();
+  }
+  if (o.scores) {  // scores behind the last token are cleared
+    const uint32_t none[4] = {0, 0, 0, 0};
+    for (; b < b_end; b += 4)
+      for (int t = 0; t < 4; t++) store_scores(b + wave, t, none);
   }
   z += __shfl_xor(z, 16);
   z += __shfl_xor(z, 32);
@@ -269,20 +321,32 @@ static __global__ void __launch_bounds__(256) k_attend(KvPool p, AttRowArgs rows
   }
 }
 
-// Joins the parts of rows that have several: workgroup (row, head), a thread per dim.
-static __global__ void k_attend_join(AttRowArgs rows, uint32_t n_parts, uint32_t heads, uint32_t dim, uint32_t row0,
-                                     const int64_t* __restrict__ part, const uint32_t* __restrict__ part_z, AttOut o) {
-  const uint32_t r = blockIdx.x, h = blockIdx.y;
+// Joins the parts of rows that have several: workgroup (row, head), whose
+// eight waves take the parts in turn and a lane up to four dims.
+static __global__ void __launch_bounds__(512) k_attend_join(AttRowArgs rows, uint32_t n_parts, uint32_t heads,
+                                                            uint32_t dim, uint32_t row0,
+                                                            const int64_t* __restrict__ part,
+                                                            const uint32_t* __restrict__ part_z, AttOut o) {
+  __shared__ unsigned long long total[256];
+  __shared__ uint32_t z;
+  const uint32_t r = blockIdx.x, h = blockIdx.y, tid = threadIdx.x;
   const uint32_t first = rows.e[r].part0, last = r + 1 < rows.n ? rows.e[r + 1].part0 : n_parts;
   if (last - first == 1) return;
-  uint32_t z = 0;
-  for (uint32_t i = first; i < last; i++) z += part_z[(uint64_t)i * heads + h];
-  for (uint32_t d = threadIdx.x; d < dim; d += blockDim.x) {
-    int64_t total = 0;
-    for (uint32_t i = first; i < last; i++) total += part[((uint64_t)i * heads + h) * dim + d];
-    att_finish(o, ((uint64_t)(row0 + r) * heads + h) * dim + d, total, z);
+  if (tid < 256) total[tid] = 0;
+  if (tid == 0) z = 0;
+  __syncthreads();
+  for (uint32_t d = tid & 63; d < dim; d += 64) {
+    int64_t t = 0;
+#pragma unroll 8
+    for (uint32_t i = first + (tid >> 6); i < last; i += 8) t += part[((uint64_t)i * heads + h) * dim + d];
+    atomicAdd(&total[d], (unsigned long long)t);
   }
-  if (threadIdx.x == 0 && o.sums) o.sums[(uint64_t)(row0 + r) * heads + h] = shift16(m31_from_u32(z));
+  uint32_t mine = 0;
+  for (uint32_t i = first + tid; i < last; i += 512) mine += part_z[(uint64_t)i * heads + h];
+  if (mine) atomicAdd(&z, mine);
+  __syncthreads();
+  if (tid < dim) att_finish(o, ((uint64_t)(row0 + r) * heads + h) * dim + tid, (int64_t)total[tid], z);
+  if (tid == 0 && o.sums) o.sums[(uint64_t)(row0 + r) * heads + h] = shift16(m31_from_u32(z));
 }
 
 }  // namespace gkr

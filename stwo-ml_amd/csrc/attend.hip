@@ -273,7 +273,7 @@ extern "C" int gkr_attention_forward(gkr_ctx* c, const gkr_kv_cache* k, const gk
     }
     TRY(check_launch(c));
     if (parts > n) {
-      GKR_LAUNCH(c, k_attend_join, dim3(n, heads), dim3(128), 0, rows, parts, heads, pool.dim, (uint32_t)row0, part, part_z, o);
+      GKR_LAUNCH(c, k_attend_join, dim3(n, heads), dim3(512), 0, rows, parts, heads, pool.dim, (uint32_t)row0, part, part_z, o);
       TRY(check_launch(c));
     }
   }

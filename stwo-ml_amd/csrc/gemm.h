@@ -50,6 +50,21 @@ __device__ __forceinline__ void balanced_digits(int32_t v, int32_t (&d)[4]) {
   }
 }
 
+// The four balanced digits of a word, one to a byte: adding 128 at each lower
+// digit makes them plain base-256 digits, each 128 too large.
+__device__ __forceinline__ uint32_t digit_bytes(uint32_t x) {
+  return ((uint32_t)center_m31(x) + 0x00808080u) ^ 0x00808080u;
+}
+// out[p] = the p-th bytes of w[0..3].
+__device__ __forceinline__ void transpose_bytes(const uint32_t (&w)[4], uint32_t (&out)[4]) {
+  const uint32_t a = __builtin_amdgcn_perm(w[1], w[0], 0x05010400), b = __builtin_amdgcn_perm(w[3], w[2], 0x05010400);
+  const uint32_t c = __builtin_amdgcn_perm(w[1], w[0], 0x07030602), d = __builtin_amdgcn_perm(w[3], w[2], 0x07030602);
+  out[0] = __builtin_amdgcn_perm(b, a, 0x05040100);
+  out[1] = __builtin_amdgcn_perm(b, a, 0x07060302);
+  out[2] = __builtin_amdgcn_perm(d, c, 0x05040100);
+  out[3] = __builtin_amdgcn_perm(d, c, 0x07060302);
+}
+
 // Which planes of X (count canonical M31 values, 16-byte aligned when VEC) are
 // non-zero: bit p of *mask (zero before the launch).  Grid-stride, an OR
 // across the workgroup in LDS, then at most one vector atomic per workgroup.

@@ -53,20 +53,6 @@ struct WitWeight {
   uint32_t count;  // planes that are not zero everywhere
 };
 
-// The four balanced digits of a word, one to a byte: adding 128 at each lower
-// digit makes them plain base-256 digits, each 128 too large.
-__device__ __forceinline__ uint32_t digit_bytes(uint32_t x) {
-  return ((uint32_t)center_m31(x) + 0x00808080u) ^ 0x00808080u;
-}
-// out[p] = the p-th bytes of w[0..3].
-__device__ __forceinline__ void transpose_bytes(const uint32_t (&w)[4], uint32_t (&out)[4]) {
-  const uint32_t a = __builtin_amdgcn_perm(w[1], w[0], 0x05010400), b = __builtin_amdgcn_perm(w[3], w[2], 0x05010400);
-  const uint32_t c = __builtin_amdgcn_perm(w[1], w[0], 0x07030602), d = __builtin_amdgcn_perm(w[3], w[2], 0x07030602);
-  out[0] = __builtin_amdgcn_perm(b, a, 0x05040100);
-  out[1] = __builtin_amdgcn_perm(b, a, 0x07060302);
-  out[2] = __builtin_amdgcn_perm(d, c, 0x05040100);
-  out[3] = __builtin_amdgcn_perm(d, c, 0x07060302);
-}
 // sum_p 256^p s[p] mod P for digit sums of fewer than 2^31 in magnitude.
 __device__ __forceinline__ uint32_t digit_sum_mod_p(const int32_t (&s)[4]) {
   const int64_t t = (int64_t)s[0] + ((int64_t)s[1] << 8) + ((int64_t)s[2] << 16) + ((int64_t)s[3] << 24);  // < 2^56
