@@ -233,32 +233,36 @@ extern "C" int gkr_attention_forward(gkr_ctx* c, const gkr_kv_cache* k, const gk
     const uint32_t n = (uint32_t)std::min<size_t>(kAttRows, n_rows - row0);
     AttRowArgs rows{};
     rows.n = n;
-    uint64_t blocks = 0;
-    auto row_blocks = [&](uint32_t i) {  // of the tokens seen, or of the scores to write
-      const uint64_t t = scores ? scores->cols : rows.e[i].len;
-      return (uint32_t)((t + kAttBlock - 1) / kAttBlock);
-    };
+    rows.wide = wide;
+    uint64_t all_steps = 0, longest_steps = 0;
     for (uint32_t i = 0; i < n; i++) {
-      const uint32_t seq = seqs[row0 + i];
+      const uint32_t seq = seqs[row0 + i], len = lens ? lens[row0 + i] : k->book->seq(seq).len;
+      const uint64_t tokens = scores ? scores->cols : len;  // the scores behind the last token are cleared
+      rows.e[i].step0 = all_steps;
       rows.e[i].seq = seq;
-      rows.e[i].len = lens ? lens[row0 + i] : k->book->seq(seq).len;
-      blocks += row_blocks(i);
+      rows.e[i].len = len;
+      const uint64_t row_steps = std::max<uint64_t>(1, (tokens + 4 * kAttBlock - 1) / (4 * kAttBlock));
+      rows.e[i].steps = (uint32_t)row_steps;
+      all_steps += wide * row_steps;
+      longest_steps = std::max(longest_steps, row_steps);
     }
-    uint32_t bpw = (uint32_t)std::min<uint64_t>(kAttMaxBlocks, (blocks * wide + 1023) / 1024);
-    bpw = std::max(4u, (bpw + 3) / 4 * 4);
-    uint32_t parts = 0;
-    for (uint32_t i = 0; i < n; i++) {
-      rows.e[i].part0 = parts;
-      parts += std::max(1u, (row_blocks(i) + bpw - 1) / bpw);
-    }
+    // as many workgroups as fit at once, with equal shares; more where a share would be too long
+    const uint32_t fit = kAttWaveGroups[pool.planes == 1 ? 0 : 1];
+    const uint64_t groups = std::max<uint64_t>(std::min<uint64_t>(fit, all_steps),
+                                               (all_steps + kAttMaxSteps - 2) / (kAttMaxSteps - 1));
+    if (groups > 1u << 23) return fail(GKR_ERR_INVALID, "%s: too many tokens and heads for one launch", what);
+    rows.share = all_steps / groups;
+    rows.extra = all_steps % groups;
+    const uint64_t segments = (uint64_t)n * wide, part_heads = std::min(kAttHeads, heads / pool.kv_heads);
     int64_t* part = nullptr;
     uint32_t* part_z = nullptr;
-    if (parts > n) {
-      TRY(ensureT(c, S_ATTP, (uint64_t)parts * (width + heads), &part));
-      part_z = reinterpret_cast<uint32_t*>(part + (uint64_t)parts * width);
+    const bool join = groups > 1 && all_steps > segments;  // with one step a segment none is shared
+    if (join) {
+      TRY(ensureT(c, S_ATTP, (segments + groups) * part_heads * (pool.dim + 1), &part));
+      part_z = reinterpret_cast<uint32_t*>(part + (segments + groups) * part_heads * pool.dim);
     }
     auto launch = [&](auto kernel) {
-      GKR_LAUNCH(c, kernel, dim3(parts, wide), dim3(256), 0, pool, rows, bpw, q->dev, heads, (uint32_t)row0, offset, mask,
+      GKR_LAUNCH(c, kernel, dim3((uint32_t)groups), dim3(256), 0, pool, pool.pages, rows, q->dev, heads, (uint32_t)row0, offset, mask,
                  part, part_z, o);
     };
     const uint32_t steps = (pool.dim + 63) / 64;
@@ -272,8 +276,13 @@ extern "C" int gkr_attention_forward(gkr_ctx* c, const gkr_kv_cache* k, const gk
       else launch(k_attend<4, 4>);
     }
     TRY(check_launch(c));
-    if (parts > n) {
-      GKR_LAUNCH(c, k_attend_join, dim3(n, heads), dim3(512), 0, rows, parts, heads, pool.dim, (uint32_t)row0, part, part_z, o);
+    if (join) {
+      auto launch_join = [&](auto kernel, uint32_t threads) {
+        GKR_LAUNCH(c, kernel, dim3((uint32_t)segments, (uint32_t)part_heads), dim3(threads), 0, rows, heads,
+                   pool.kv_heads, pool.dim, (uint32_t)row0, part, part_z, o);
+      };
+      if (longest_steps * groups <= 6 * all_steps) launch_join(k_attend_join<1>, steps * 64);
+      else launch_join(k_attend_join<8>, 512);
       TRY(check_launch(c));
     }
   }

@@ -19,11 +19,13 @@ namespace gkr {
 constexpr uint32_t kAttBlock = 64;         // tokens per block
 constexpr uint32_t kMaxTokens = 1u << 21;  // per sequence: sums of weights below 2^31, weighted sums below 2^61
 
-// Byte of (token in the block, dim) in a plane of the block's keys and of its
-// values (attend.h: the matrix cores' operand orders).
-KV_HD uint32_t kv_key_byte(uint32_t token, uint32_t dim) { return dim / 16 * 1024 + 16 * token + dim % 16; }
-KV_HD uint32_t kv_value_byte(uint32_t token, uint32_t dim) {
-  return dim / 16 * 1024 + 256 * (token / 4 % 4) + 16 * (dim % 16) + 4 * (token / 16) + token % 4;
+// Byte of a plane's digit of (token in the block, dim), among the block's keys
+// and among its values (attend.h: the matrix cores' operand orders).
+KV_HD uint32_t kv_key_byte(uint32_t token, uint32_t dim, uint32_t plane, uint32_t planes) {
+  return (dim / 16 * planes + plane) * 1024 + 16 * token + dim % 16;
+}
+KV_HD uint32_t kv_value_byte(uint32_t token, uint32_t dim, uint32_t plane, uint32_t planes) {
+  return (dim / 16 * planes + plane) * 1024 + 256 * (token / 4 % 4) + 16 * (dim % 16) + 4 * (token / 16) + token % 4;
 }
 
 class KvBook {

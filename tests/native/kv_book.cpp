@@ -27,6 +27,10 @@ int kvb_extend(KvBook* b, const uint32_t* seqs, const uint32_t* counts, size_t n
   if (undo) b->back(before);
   return 1;
 }
-uint32_t kvb_key_byte(uint32_t token, uint32_t dim) { return kv_key_byte(token, dim); }
-uint32_t kvb_value_byte(uint32_t token, uint32_t dim) { return kv_value_byte(token, dim); }
+uint32_t kvb_key_byte(uint32_t token, uint32_t dim, uint32_t plane, uint32_t planes) {
+  return kv_key_byte(token, dim, plane, planes);
+}
+uint32_t kvb_value_byte(uint32_t token, uint32_t dim, uint32_t plane, uint32_t planes) {
+  return kv_value_byte(token, dim, plane, planes);
+}
 }

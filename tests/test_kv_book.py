@@ -97,12 +97,13 @@ def test_lengths_near_the_type_range(lib):
     lib.kvb_free(b)
 
 
+@pytest.mark.parametrize("planes", [1, 4])
 @pytest.mark.parametrize("dim", [1, 16, 80, 256])
-def test_every_value_has_its_byte(lib, dim):
+def test_every_value_has_its_byte(lib, dim, planes):
     chunks = (dim + 15) // 16
     for at in (lib.kvb_key_byte, lib.kvb_value_byte):
-        seen = {at(t, d) for t in range(64) for d in range(dim)}
-        assert len(seen) == 64 * dim and max(seen) < 1024 * chunks
+        seen = {at(t, d, p, planes) for t in range(64) for d in range(dim) for p in range(planes)}
+        assert len(seen) == 64 * dim * planes and max(seen) < 1024 * chunks * planes
     # four tokens 4 i .. 4 i + 3 of a dim are neighbours among the values
-    assert all(lib.kvb_value_byte(4 * i + v, 3 % dim) == lib.kvb_value_byte(4 * i, 3 % dim) + v
+    assert all(lib.kvb_value_byte(4 * i + v, 3 % dim, 0, planes) == lib.kvb_value_byte(4 * i, 3 % dim, 0, planes) + v
                for i in range(16) for v in range(4))
