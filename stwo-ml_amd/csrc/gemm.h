@@ -273,8 +273,9 @@ __device__ __forceinline__ bool gemm_group(uint32_t rgroups, uint32_t cgroups, u
   return cg < cgroups;
 }
 constexpr uint64_t kGemmMaxGroups = 1ull << 23;  // of 256 threads: half of the 2^32 that a dimension takes
-inline dim3 gemm_group_grid(uint64_t rgroups, uint64_t cgroups, uint64_t splits, uint32_t* rgroups_arg) {
-  const uint64_t z = rgroups * cgroups / kGemmMaxGroups + 1, rows = (rgroups + z - 1) / z;
+inline dim3 gemm_group_grid(uint64_t rgroups, uint64_t cgroups, uint64_t splits, uint32_t* rgroups_arg,
+                            uint64_t max_groups = kGemmMaxGroups) {
+  const uint64_t z = rgroups * cgroups / max_groups + 1, rows = (rgroups + z - 1) / z;
   *rgroups_arg = (uint32_t)rows;
   return dim3((uint32_t)((rows * cgroups + 7) / 8 * 8), (uint32_t)splits, (uint32_t)z);
 }

@@ -184,6 +184,7 @@ int drop_derived(gkr_ctx* c, gkr_matrix* m);
 // (kept with it), and that product into C.
 int weight_planes(gkr_ctx* c, gkr_matrix* b);
 int matmul_forward(gkr_ctx* c, const gkr_matrix* a, gkr_matrix* b, uint32_t* C);
+int gemm_masks(gkr_ctx* c, uint32_t** mask, uint32_t** next_mask);
 // logup.hip: an activation table's output column, resident on the device.
 int device_table(gkr_ctx* c, uint32_t tag, uint32_t log_size, uint32_t** out);
 

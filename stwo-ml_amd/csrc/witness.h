@@ -15,37 +15,81 @@ struct ActArg {
   const uint32_t* table;
   uint32_t mask, relu;
 };
-__device__ __forceinline__ uint32_t activate(const ActArg& a, uint32_t z) {
-  if (a.table) return a.table[z & a.mask];
-  return a.relu && z > (P >> 1) ? 0u : z;
+// E elements of a thread at once: their loads go out together.
+template <int E>
+__device__ __forceinline__ void activate(const ActArg& a, uint32_t (&z)[E]) {
+  if (a.table) {
+#pragma unroll
+    for (int e = 0; e < E; e++) z[e] = a.table[z[e] & a.mask];
+  } else if (a.relu) {
+#pragma unroll
+    for (int e = 0; e < E; e++) z[e] = z[e] > (P >> 1) ? 0u : z[e];
+  }
 }
 
-// What happens to a sum of the product (fused) or a pair of sums (gated).
+// What happens to a sum of the product (fused) or a pair of sums (gated), for E
+// elements (row-major place `at`, column `col`) of a thread: fetch() before the
+// sums are there, store() with them.  Places that are not `ok` are not touched.
 struct FusedEnd {
   ActArg act;
   const uint32_t* bias;      // n
   const uint32_t* residual;  // m x n; may be out (read by the thread that writes the element)
   uint32_t* pre;
   uint32_t* out;
+  template <int E>
+  struct Fetched {
+    uint32_t bias[E], residual[E];
+  };
+  template <int E>
+  __device__ __forceinline__ void fetch(const uint64_t (&at)[E], const uint64_t (&col)[E], const bool (&ok)[E],
+                                        Fetched<E>& f) const {
+#pragma unroll
+    for (int e = 0; e < E; e++) {
+      f.bias[e] = bias && ok[e] ? bias[col[e]] : 0u;
+      f.residual[e] = residual && ok[e] ? residual[at[e]] : 0u;
+    }
+  }
+  template <int E>
+  __device__ __forceinline__ void store(const uint64_t (&at)[E], const bool (&ok)[E], const Fetched<E>& f,
+                                        uint32_t (&z)[1][E]) const {
+#pragma unroll
+    for (int e = 0; e < E; e++) z[0][e] = m31_add(z[0][e], f.bias[e]);
+    uint32_t y[E];
+#pragma unroll
+    for (int e = 0; e < E; e++) y[e] = z[0][e];
+    activate(act, y);
+#pragma unroll
+    for (int e = 0; e < E; e++)
+      if (ok[e]) {
+        if (pre) pre[at[e]] = z[0][e];
+        out[at[e]] = m31_add(y[e], f.residual[e]);
+      }
+  }
 };
-__device__ __forceinline__ void fused_end(const FusedEnd& e, uint64_t at, uint64_t col, uint32_t z) {
-  if (e.bias) z = m31_add(z, e.bias[col]);
-  if (e.pre) e.pre[at] = z;
-  uint32_t y = activate(e.act, z);
-  if (e.residual) y = m31_add(y, e.residual[at]);
-  e.out[at] = y;
-}
 struct GatedEnd {
   ActArg act;
   uint32_t *gate, *act_out, *up, *out;
+  template <int E>
+  struct Fetched {};
+  template <int E>
+  __device__ __forceinline__ void fetch(const uint64_t (&)[E], const uint64_t (&)[E], const bool (&)[E], Fetched<E>&) const {}
+  template <int E>
+  __device__ __forceinline__ void store(const uint64_t (&at)[E], const bool (&ok)[E], const Fetched<E>&,
+                                        uint32_t (&z)[2][E]) const {
+    uint32_t y[E];
+#pragma unroll
+    for (int e = 0; e < E; e++) y[e] = z[0][e];
+    activate(act, y);
+#pragma unroll
+    for (int e = 0; e < E; e++)
+      if (ok[e]) {
+        if (gate) gate[at[e]] = z[0][e];
+        if (act_out) act_out[at[e]] = y[e];
+        if (up) up[at[e]] = z[1][e];
+        out[at[e]] = m31_mul(y[e], z[1][e]);
+      }
+  }
 };
-__device__ __forceinline__ void gated_end(const GatedEnd& e, uint64_t at, uint32_t g, uint32_t u) {
-  const uint32_t a = activate(e.act, g);
-  if (e.gate) e.gate[at] = g;
-  if (e.act_out) e.act_out[at] = a;
-  if (e.up) e.up[at] = u;
-  e.out[at] = m31_mul(a, u);
-}
 
 // A digit plane stack of a weight: planes of kGemmBlockBytes blocks (gemm.h).
 struct WitWeight {
@@ -159,10 +203,14 @@ static __global__ void __launch_bounds__(64 * kRowWaves) k_rows(const uint32_t* 
 #pragma unroll
           for (int v = 0; v < 4; v++) atomicAdd(&sums[i][q][quarter][v][16 * h + col], acc[i][q][h][v]);
   }
-  __syncthreads();
   const uint32_t r = threadIdx.x / 32, c = threadIdx.x % 32, column = ct * kGemmTile + c;
-  if (r >= m || column >= n) return;
-  uint32_t z[NW];
+  const bool ok[1] = {r < m && column < n};
+  const uint64_t at[1] = {(uint64_t)r * n + column}, cols[1] = {column};
+  typename End::template Fetched<1> fetched;
+  end.fetch(at, cols, ok, fetched);
+  __syncthreads();
+  if (!ok[0]) return;
+  uint32_t z[NW][1];
 #pragma unroll
   for (int i = 0; i < NW; i++) {
     uint64_t t = 0;
@@ -171,23 +219,257 @@ static __global__ void __launch_bounds__(64 * kRowWaves) k_rows(const uint32_t* 
       const int32_t s[4] = {sums[i][q][r][0][c], sums[i][q][r][1][c], sums[i][q][r][2][c], sums[i][q][r][3][c]};
       t += (uint64_t)digit_sum_mod_p(s) << (8 * q);
     }
-    z[i] = m31_reduce64(t);
+    z[i][0] = m31_reduce64(t);
   }
-  if constexpr (GATED)
-    gated_end(end, (uint64_t)r * n + column, z[0], z[1]);
-  else
-    fused_end(end, (uint64_t)r * n + column, column, z[0]);
+  end.store(at, ok, fetched, z);
 }
 
-// One thread per element, behind the products.
-static __global__ void k_fused_end(const uint32_t* __restrict__ z, uint64_t count, uint64_t n, FusedEnd e) {
-  for (uint64_t i = (uint64_t)blockIdx.x * blockDim.x + threadIdx.x; i < count; i += (uint64_t)gridDim.x * blockDim.x)
-    fused_end(e, i, i % n, z[i]);
+// More rows: the rows' digits are packed first, as operand blocks (gemm.h) in
+// two forms, one of which the product reads: plane 0 alone, row r as row r, and
+// all four planes interleaved, plane p of row r as row 4 r + p, so that a lane
+// of an accumulator holds the four digit sums of its elements.  *mask gets a
+// bit where a digit above plane 0 is not zero, and *clear, the mask of the next
+// product on the stream, is zeroed.  A thread takes 16 words of a row; rows
+// past m are left as they are (their sums are not stored).
+template <bool VEC>
+static __global__ void __launch_bounds__(256) k_wit_pack(const uint32_t* __restrict__ X, uint64_t m, uint64_t k,
+                                                         uint64_t nsteps, int8_t* __restrict__ one,
+                                                         int8_t* __restrict__ four, uint32_t* __restrict__ mask,
+                                                         uint32_t* __restrict__ clear) {
+  const uint64_t at = (uint64_t)blockIdx.x * blockDim.x + threadIdx.x;  // (row / 8, step, row % 8, half)
+  if (at == 0) *clear = 0;
+  const uint32_t half = (uint32_t)at & 1, row8 = (uint32_t)(at >> 1) & 7;
+  const uint64_t blk = at >> 4, rt8 = blk / nsteps, step = blk - rt8 * nsteps, row = 8 * rt8 + row8;
+  uint32_t high = 0;
+  if (row < m) {
+    const uint64_t k0 = step * kGemmK + 16 * half;
+    uint32_t w[4][4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      uint32_t d[4], out[4];
+      if constexpr (VEC) {
+        const uint4 x = k0 + 4 * i < k ? *(const uint4*)(X + row * k + k0 + 4 * i) : make_uint4(0, 0, 0, 0);
+        d[0] = digit_bytes(x.x);
+        d[1] = digit_bytes(x.y);
+        d[2] = digit_bytes(x.z);
+        d[3] = digit_bytes(x.w);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 4; j++) d[j] = digit_bytes(k0 + 4 * i + j < k ? X[row * k + k0 + 4 * i + j] : 0u);
+      }
+      transpose_bytes(d, out);
+#pragma unroll
+      for (int p = 0; p < 4; p++) w[p][i] = out[p];
+      high |= out[1] | out[2] | out[3];
+    }
+    int8_t* const f = four + blk * kGemmBlockBytes + 512 * half + 64 * row8;
+#pragma unroll
+    for (int p = 0; p < 4; p++) *(uint4*)(f + 16 * p) = make_uint4(w[p][0], w[p][1], w[p][2], w[p][3]);
+    *(uint4*)(one + ((row >> 5) * nsteps + step) * kGemmBlockBytes + 512 * half + 16 * (row & 31)) =
+        make_uint4(w[0][0], w[0][1], w[0][2], w[0][3]);
+  }
+  // atomics on one address take about 20 ns each, one after another: only while the bit is missing
+  if (__any(high != 0) && (threadIdx.x & 63) == 0 && !*(volatile const uint32_t*)mask) atomicOr(mask, 1u);
 }
-static __global__ void k_gated_end(const uint32_t* __restrict__ g, const uint32_t* __restrict__ u, uint64_t count,
-                                   GatedEnd e) {
-  for (uint64_t i = (uint64_t)blockIdx.x * blockDim.x + threadIdx.x; i < count; i += (uint64_t)gridDim.x * blockDim.x)
-    gated_end(e, i, g[i], u[i]);
+
+// How a product of several rows is cut, for rows of one plane and of four: row
+// groups, K splits and K steps per split.
+struct WitPlan {
+  uint32_t rtiles, rgroups, splits, steps;
+};
+struct WitProduct {
+  const int8_t *one, *four;  // the packed rows
+  const uint32_t* mask;
+  WitWeight w[2];
+  uint64_t m, n;
+  uint32_t nsteps, ctiles, cgroups;
+  WitPlan plan[2];
+  uint32_t* part;  // [split][matrix][m][n] where there are splits
+};
+
+// Up to 64 rows: a stream of the weights.  A workgroup has one column tile of
+// each matrix and WR * RT row tiles of 32 (packed) rows; its W waves are WR
+// down the rows, RT tiles each, by W / WR that take the K steps in turn,
+// operands straight from memory into registers with U steps in flight; the
+// waves' sums meet in LDS.  WR goes with the rows' planes (WR1, WR4), so that
+// both take the same registers.
+template <int RT, int PB, bool GATED, int W, int WR, bool FOUR, class End>
+__device__ __forceinline__ void wit_tiles(const WitProduct& g, int32_t* sums, uint32_t rg, uint32_t cg, uint32_t split,
+                                          const End& end) {
+  constexpr int NW = GATED ? 2 : 1, NB = NW * PB, WK = W / WR, TILES = WR * RT;
+  constexpr int U = W == 16 ? (RT + NB <= 2 ? 6 : RT + NB <= 3 ? 4 : 2) : (RT + NB <= 3 ? 6 : RT + NB <= 4 ? 3 : 2);
+  const WitPlan& plan = g.plan[FOUR ? 1 : 0];
+  const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const uint32_t wr = wave % WR, wk = wave / WR;
+  const uint32_t s0 = split * plan.steps, s1 = s0 + plan.steps < g.nsteps ? s0 + plan.steps : g.nsteps;
+  const uint64_t plane = (uint64_t)g.ctiles * g.nsteps * kGemmBlockBytes;
+  const int8_t* ab[RT];
+  const int8_t* bb[NW][PB];
+#pragma unroll
+  for (int i = 0; i < RT; i++) {  // tiles past the edge are the last one again, and not stored
+    const uint32_t rt = rg * TILES + wr * RT + i < plan.rtiles ? rg * TILES + wr * RT + i : plan.rtiles - 1;
+    ab[i] = (FOUR ? g.four : g.one) + (uint64_t)rt * g.nsteps * kGemmBlockBytes;
+  }
+#pragma unroll
+  for (int x = 0; x < NW; x++)
+#pragma unroll
+    for (int q = 0; q < PB; q++)
+      bb[x][q] = g.w[x].planes + (q < (int)g.w[x].count ? q : 0) * plane + (uint64_t)cg * g.nsteps * kGemmBlockBytes;
+  v4i a[U][RT], b[U][NW][PB];
+  auto load = [&](int u, uint32_t s) {
+    const uint32_t at = (s < s1 ? s : s1 - 1) * kGemmBlockBytes + 16 * lane;  // past the end: again, unused
+#pragma unroll
+    for (int x = 0; x < NW; x++)
+#pragma unroll
+      for (int q = 0; q < PB; q++)
+        if (q == 0 || q < (int)g.w[x].count)
+          b[u][x][q] = WR == 1 ? __builtin_nontemporal_load((const v4i*)(bb[x][q] + at)) : *(const v4i*)(bb[x][q] + at);
+#pragma unroll
+    for (int i = 0; i < RT; i++) a[u][i] = *(const v4i*)(ab[i] + at);
+  };
+#pragma unroll
+  for (int u = 0; u < U; u++) load(u, s0 + wk + u * WK);
+  for (uint32_t i = threadIdx.x; i < TILES * NB * 1024; i += 64 * W) sums[i] = 0;
+  v16i acc[RT][NW][PB];
+#pragma unroll
+  for (int i = 0; i < RT; i++)
+#pragma unroll
+    for (int x = 0; x < NW; x++)
+#pragma unroll
+      for (int q = 0; q < PB; q++)
+#pragma unroll
+        for (int v = 0; v < 16; v++) acc[i][x][q][v] = 0;
+#pragma unroll 1
+  for (uint32_t s = s0 + wk; s < s1; s += U * WK) {
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+      if (s + u * WK < s1) {  // uniform
+#pragma unroll
+        for (int x = 0; x < NW; x++)
+#pragma unroll
+          for (int q = 0; q < PB; q++)
+            if (q == 0 || q < (int)g.w[x].count) {
+#pragma unroll
+              for (int i = 0; i < RT; i++)
+                acc[i][x][q] = __builtin_amdgcn_mfma_i32_32x32x32_i8(a[u][i], b[u][x][q], acc[i][x][q], 0, 0, 0);
+            }
+        load(u, s + (u + U) * WK);
+      }
+    }
+  }
+  // this thread's elements
+  constexpr uint32_t ROWS = FOUR ? 8 : 32;  // of a tile
+  constexpr int ALL = TILES * ROWS * 32, E = ALL <= 64 * W ? 1 : ALL / (64 * W);
+  static_assert(E * 64 * W == ALL || E == 1, "whole elements");
+  uint64_t at[E], cols[E];
+  uint32_t rows[E];
+  bool ok[E];
+  const uint32_t c = threadIdx.x % 32;
+#pragma unroll
+  for (int e = 0; e < E; e++) {
+    rows[e] = threadIdx.x / 32 + e * 2 * W;
+    const uint64_t row = (uint64_t)rg * (TILES * ROWS) + rows[e];
+    cols[e] = (uint64_t)cg * 32 + c;
+    at[e] = row * g.n + cols[e];
+    ok[e] = rows[e] < TILES * ROWS && row < g.m && cols[e] < g.n;
+  }
+  typename End::template Fetched<E> fetched;
+  if (plan.splits == 1) end.fetch(at, cols, ok, fetched);
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < RT; i++)
+#pragma unroll
+    for (int x = 0; x < NW; x++)
+#pragma unroll
+      for (int q = 0; q < PB; q++)
+#pragma unroll
+        for (int v = 0; v < 16; v++)
+          atomicAdd(&sums[(((wr * RT + i) * NB + x * PB + q) * 32 + 8 * (v / 4) + 4 * (lane >> 5) + v % 4) * 32 + (lane & 31)],
+                    acc[i][x][q][v]);
+  __syncthreads();
+  uint32_t z[NW][E];
+#pragma unroll
+  for (int e = 0; e < E; e++) {
+    const uint32_t r = rows[e] < TILES * ROWS ? rows[e] : 0;
+#pragma unroll
+    for (int x = 0; x < NW; x++) {
+      uint64_t t = 0;
+#pragma unroll
+      for (int q = 0; q < PB; q++) {
+        const int32_t* const from = sums + (r / ROWS * NB + x * PB + q) * 1024 + c;
+        uint32_t one;
+        if constexpr (FOUR) {
+          const uint32_t r4 = 4 * (r % 8);
+          const int32_t d[4] = {from[r4 * 32], from[r4 * 32 + 32], from[r4 * 32 + 64], from[r4 * 32 + 96]};
+          one = digit_sum_mod_p(d);
+        } else {
+          one = gemm_mod_p(from[r % 32 * 32]);
+        }
+        t += (uint64_t)one << (8 * q);
+      }
+      z[x][e] = m31_reduce64(t);
+    }
+  }
+  if (plan.splits == 1) {
+    end.store(at, ok, fetched, z);
+  } else {
+#pragma unroll
+    for (int e = 0; e < E; e++)
+#pragma unroll
+      for (int x = 0; x < NW; x++)
+        if (ok[e]) g.part[(uint64_t)(split * NW + x) * g.m * g.n + at[e]] = z[x][e];
+  }
+}
+template <int RT, int PB, bool GATED, int W, int WR1, int WR4, class End>
+static __global__ void __launch_bounds__(64 * W) k_wit_tiles(WitProduct g, uint32_t rgroups, End end) {
+  __shared__ int32_t sums[(WR1 > WR4 ? WR1 : WR4) * RT * PB * (GATED ? 2 : 1) * 1024];
+  const bool four = *g.mask != 0;
+  const WitPlan& plan = g.plan[four ? 1 : 0];
+  uint32_t rg, cg;
+  if (!gemm_group(rgroups, g.cgroups, rg, cg) || rg >= plan.rgroups || blockIdx.y >= plan.splits) return;  // uniform
+  if (four)
+    wit_tiles<RT, PB, GATED, W, WR4, true>(g, sums, rg, cg, blockIdx.y, end);
+  else
+    wit_tiles<RT, PB, GATED, W, WR1, false>(g, sums, rg, cg, blockIdx.y, end);
+}
+
+// The end of a product whose K was split: a thread per element.
+template <bool GATED, class End>
+static __global__ void __launch_bounds__(256) k_wit_join(WitProduct g, End end) {
+  const uint32_t splits = g.plan[*g.mask != 0 ? 1 : 0].splits;
+  if (splits == 1) return;  // done where it was computed
+  constexpr int NW = GATED ? 2 : 1;
+  const uint64_t count = g.m * g.n;
+  for (uint64_t i = (uint64_t)blockIdx.x * blockDim.x + threadIdx.x; i < count; i += (uint64_t)gridDim.x * blockDim.x) {
+    const uint64_t at[1] = {i}, cols[1] = {i % g.n};
+    const bool ok[1] = {true};
+    typename End::template Fetched<1> fetched;
+    end.fetch(at, cols, ok, fetched);
+    uint32_t z[NW][1];
+#pragma unroll
+    for (int x = 0; x < NW; x++) {
+      uint64_t t = 0;
+      for (uint32_t s = 0; s < splits; s++) t += g.part[(uint64_t)(s * NW + x) * count + i];
+      z[x][0] = m31_reduce64(t);
+    }
+    end.store(at, ok, fetched, z);
+  }
+}
+
+// One thread per element, behind products of their own.
+template <bool GATED, class End>
+static __global__ void __launch_bounds__(256) k_wit_end(const uint32_t* __restrict__ z0, const uint32_t* __restrict__ z1,
+                                                        uint64_t count, uint64_t n, End end) {
+  for (uint64_t i = (uint64_t)blockIdx.x * blockDim.x + threadIdx.x; i < count; i += (uint64_t)gridDim.x * blockDim.x) {
+    const uint64_t at[1] = {i}, cols[1] = {i % n};
+    const bool ok[1] = {true};
+    typename End::template Fetched<1> fetched;
+    end.fetch(at, cols, ok, fetched);
+    uint32_t z[GATED ? 2 : 1][1];
+    z[0][0] = z0[i];
+    if constexpr (GATED) z[1][0] = z1[i];
+    end.store(at, ok, fetched, z);
+  }
 }
 
 }  // namespace gkr

@@ -77,6 +77,76 @@ static bool few_rows(uint64_t m, uint64_t k, uint64_t n) {
   return m <= 4 && k <= kMaxInner && n <= kRowMaxTiles * kGemmTile;
 }
 
+static dim3 end_grid(uint64_t count);
+
+// More rows: packed, multiplied (k_wit_tiles) and, where K is split, joined.
+template <bool GATED, class End>
+static int packed_product(gkr_ctx* c, const gkr_matrix* a, const gkr_matrix* w0, const gkr_matrix* w1, const End& end) {
+  const uint64_t m = a->rows, k = a->cols, n = w0->cols;
+  WitProduct g{};
+  g.m = m;
+  g.n = n;
+  g.nsteps = (uint32_t)((k + kGemmK - 1) / kGemmK);
+  const uint64_t ctiles = (n + kGemmTile - 1) / kGemmTile;
+  g.ctiles = (uint32_t)ctiles;
+  g.w[0] = wit_weight(w0);
+  g.w[1] = wit_weight(w1);
+  const uint64_t one_tiles = (m + 31) / 32, four_tiles = (m + 7) / 8;
+  int8_t* packed;
+  TRY(ensureT(c, S_GEMMA, (one_tiles + four_tiles) * g.nsteps * kGemmBlockBytes, &packed));
+  g.one = packed;
+  g.four = packed + one_tiles * g.nsteps * kGemmBlockBytes;
+  uint32_t *mask, *next_mask;
+  TRY(gemm_masks(c, &mask, &next_mask));
+  g.mask = mask;
+  const uint64_t slots = four_tiles * g.nsteps * 16;
+  const dim3 pack_grid((uint32_t)((slots + 255) / 256));
+  if (k % 4 == 0 && ((uintptr_t)a->dev & 15) == 0)
+    GKR_LAUNCH(c, k_wit_pack<true>, pack_grid, dim3(256), 0, a->dev, m, k, (uint64_t)g.nsteps, packed, const_cast<int8_t*>(g.four), mask, next_mask);
+  else
+    GKR_LAUNCH(c, k_wit_pack<false>, pack_grid, dim3(256), 0, a->dev, m, k, (uint64_t)g.nsteps, packed, const_cast<int8_t*>(g.four), mask, next_mask);
+  TRY(check_launch(c));
+
+  uint32_t max_splits = 1;
+  g.cgroups = g.ctiles;
+  auto launch = [&](auto kernel, uint32_t rt, uint32_t waves, uint32_t wr1, uint32_t wr4) -> int {
+    const uint64_t tiles[2] = {one_tiles, four_tiles}, group[2] = {rt * wr1, rt * wr4};
+    for (int i = 0; i < 2; i++) {
+      WitPlan& p = g.plan[i];
+      p.rtiles = (uint32_t)tiles[i];
+      p.rgroups = (uint32_t)((tiles[i] + group[i] - 1) / group[i]);
+      p.splits = 1;
+      p.steps = g.nsteps;
+      max_splits = std::max(max_splits, p.splits);
+    }
+    uint32_t rg;
+    const dim3 grid = gemm_group_grid(std::max(g.plan[0].rgroups, g.plan[1].rgroups), g.cgroups, max_splits, &rg,
+                                      kGemmMaxGroups / 4);
+    GKR_LAUNCH(c, kernel, grid, dim3(64 * waves), 0, g, rg, end);
+    return check_launch(c);
+  };
+#define GKR_WIT_TILES(RT, PB, W, WR1, WR4) launch(k_wit_tiles<RT, PB, GATED, W, WR1, WR4, End>, RT, W, WR1, WR4)
+  // sixteen waves a workgroup for one matrix, eight for two: the registers of
+  // sixteen hold no more accumulators
+  constexpr int W = GATED ? 8 : 16;
+  if (w0->bnplanes > 1 || w1->bnplanes > 1) TRY(GKR_WIT_TILES(1, 4, W, 1, 2));
+  else if (m <= 8) TRY(GKR_WIT_TILES(1, 1, W, 1, 1));
+  else if (m <= 16) TRY(GKR_WIT_TILES(1, 1, W, 1, 2));
+  else if (m <= 32) TRY(GKR_WIT_TILES(1, 1, W, 1, 4));
+  else TRY(GKR_WIT_TILES(2, 1, W, 1, 4));
+#undef GKR_WIT_TILES
+  if (max_splits > 1) {
+    auto join = k_wit_join<GATED, End>;
+    GKR_LAUNCH(c, join, end_grid(m * n), dim3(256), 0, g, end);
+    TRY(check_launch(c));
+  }
+  return GKR_OK;
+}
+// Sizes that the packed product's grids and 32-bit step offsets take.
+static bool packable(uint64_t m, uint64_t k, uint64_t n) {
+  return k <= kMaxInner && m <= 64 && n <= 1ull << 24 && m * k <= 1ull << 34;
+}
+
 static dim3 end_grid(uint64_t count) { return dim3((uint32_t)std::min<uint64_t>((count + 255) / 256, 1u << 20)); }
 
 extern "C" int gkr_matmul_forward_fused(gkr_ctx* c, const gkr_matrix* a, const gkr_matrix* b, const gkr_matrix* bias,
@@ -108,10 +178,12 @@ extern "C" int gkr_matmul_forward_fused(gkr_ctx* c, const gkr_matrix* a, const g
   if (pre) TRY(drop_derived(c, pre));
   TRY(weight_planes(c, const_cast<gkr_matrix*>(b)));
   if (few_rows(m, a->cols, n)) return rows_product<false>(c, a, b, b, e);
+  if (packable(m, a->cols, n)) return packed_product<false>(c, a, b, b, e);
   uint32_t* z;
   TRY(ensureT(c, S_WITG, m * n, &z));
   TRY(matmul_forward(c, a, const_cast<gkr_matrix*>(b), z));
-  GKR_LAUNCH(c, k_fused_end, end_grid(m * n), dim3(256), 0, z, m * n, n, e);
+  auto end = k_wit_end<false, FusedEnd>;
+  GKR_LAUNCH(c, end, end_grid(m * n), dim3(256), 0, z, z, m * n, n, e);
   return check_launch(c);
 }
 
@@ -142,11 +214,13 @@ extern "C" int gkr_gated_forward(gkr_ctx* c, const gkr_matrix* a, const gkr_matr
   TRY(weight_planes(c, const_cast<gkr_matrix*>(wg)));
   TRY(weight_planes(c, const_cast<gkr_matrix*>(wu)));
   if (few_rows(m, a->cols, n)) return rows_product<true>(c, a, wg, wu, e);
+  if (packable(m, a->cols, n)) return packed_product<true>(c, a, wg, wu, e);
   uint32_t *g, *u;
   TRY(ensureT(c, S_WITG, m * n, &g));
   TRY(ensureT(c, S_WITU, m * n, &u));
   TRY(matmul_forward(c, a, const_cast<gkr_matrix*>(wg), g));
   TRY(matmul_forward(c, a, const_cast<gkr_matrix*>(wu), u));
-  GKR_LAUNCH(c, k_gated_end, end_grid(m * n), dim3(256), 0, g, u, m * n, e);
+  auto end = k_wit_end<true, GatedEnd>;
+  GKR_LAUNCH(c, end, end_grid(m * n), dim3(256), 0, g, u, m * n, n, e);
   return check_launch(c);
 }
