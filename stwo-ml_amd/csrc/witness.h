@@ -433,6 +433,152 @@ static __global__ void __launch_bounds__(64 * W) k_wit_tiles(WitProduct g, uint3
     wit_tiles<RT, PB, GATED, W, WR1, false>(g, sums, rg, cg, blockIdx.y, end);
 }
 
+// More rows: 8 row tiles of (packed) rows by 8 column tiles of the weights (4 of
+// each of two matrices) a workgroup, through LDS.  Both operands lie in memory
+// as the matrix cores take them, so a tile's K step is 1 KB that one wave
+// copies and any wave reads back without bank conflicts.  A stage is four K
+// steps, 64 KB; while a stage is multiplied the next goes from registers to the
+// other half of LDS and the one after it is on its way from memory.  Eight
+// waves, two down the rows (four tiles each) by four across (two tiles, or one
+// of each matrix): 6 KB from LDS feed 8 matrix instructions of 32 cycles.
+constexpr int kBlockStage = 4;  // K steps
+template <bool GATED, bool FOUR, class End>
+__device__ __forceinline__ void wit_block(const WitProduct& g, v4i* lds, uint32_t rg, uint32_t cg, uint32_t split,
+                                          const End& end) {
+  constexpr int NW = GATED ? 2 : 1, CT = 8 / NW;  // column tiles of a workgroup
+  const WitPlan& plan = g.plan[FOUR ? 1 : 0];
+  const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const uint32_t s0 = split * plan.steps, s1 = s0 + plan.steps < g.nsteps ? s0 + plan.steps : g.nsteps;
+  // this wave copies the 8 row tiles (even waves) or column tiles (odd) of step wave / 2 of each stage
+  const int8_t* from[8];
+#pragma unroll
+  for (int i = 0; i < 8; i++) {  // tiles past the edges are the last one again, and not stored
+    if (wave & 1) {
+      const uint32_t ct = cg * CT + i / NW, t = ct < g.ctiles ? ct : g.ctiles - 1;
+      from[i] = g.w[i % NW].planes + (uint64_t)t * g.nsteps * kGemmBlockBytes;
+    } else {
+      const uint32_t rt = rg * 8 + i, t = rt < plan.rtiles ? rt : plan.rtiles - 1;
+      from[i] = (FOUR ? g.four : g.one) + (uint64_t)t * g.nsteps * kGemmBlockBytes;
+    }
+  }
+  v4i in[8];
+  auto load = [&](uint32_t s) {  // of the stage from step s
+    const uint32_t step = s + wave / 2, at = (step < s1 ? step : s1 - 1) * kGemmBlockBytes + 16 * lane;
+#pragma unroll
+    for (int i = 0; i < 8; i++) in[i] = *(const v4i*)(from[i] + at);
+  };
+  auto put = [&](uint32_t half) {
+#pragma unroll
+    for (int i = 0; i < 8; i++) lds[(half * 8 * kBlockStage * 2 + wave * 8 + i) * 64 + lane] = in[i];
+  };
+  const uint32_t wr = wave & 1, wc = wave >> 1;
+  v16i acc[4][2];
+#pragma unroll
+  for (int i = 0; i < 4; i++)
+#pragma unroll
+    for (int j = 0; j < 2; j++)
+#pragma unroll
+      for (int v = 0; v < 16; v++) acc[i][j][v] = 0;
+  auto multiply = [&](uint32_t half, int k) {
+    const v4i* const at = lds + (half * 8 * kBlockStage * 2 + k * 16) * 64 + lane;
+    v4i a[4], b[2];
+#pragma unroll
+    for (int j = 0; j < 2; j++) b[j] = at[(8 + wc * 2 + j) * 64];
+#pragma unroll
+    for (int i = 0; i < 4; i++) a[i] = at[(wr * 4 + i) * 64];
+#pragma unroll
+    for (int i = 0; i < 4; i++)
+#pragma unroll
+      for (int j = 0; j < 2; j++) acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(a[i], b[j], acc[i][j], 0, 0, 0);
+  };
+  load(s0);
+  put(0);
+  load(s0 + kBlockStage);
+  __syncthreads();
+  uint32_t half = 0, s = s0;
+#pragma unroll 1
+  for (; s + kBlockStage <= s1; s += kBlockStage, half ^= 1) {
+    put(half ^ 1);
+    load(s + 2 * kBlockStage);
+    __builtin_amdgcn_sched_barrier(0);  // left to itself the compiler issues the loads last
+#pragma unroll
+    for (int k = 0; k < kBlockStage; k++) multiply(half, k);
+    __syncthreads();
+  }
+  for (int k = 0; s + k < s1; k++) multiply(half, k);  // a last, shorter stage
+  // The end, half of a wave's tiles at a time: through its 16 KB of LDS into
+  // rows, eight elements a lane and turn.
+  __syncthreads();
+  constexpr uint32_t ROWS = FOUR ? 8 : 32, TI = 4 / NW;  // of a tile; tiles down the rows at a time
+  constexpr int E = 8;
+  int32_t* const mine = (int32_t*)lds + wave * 4096;
+#pragma unroll
+  for (uint32_t part = 0; part < 2; part++) {
+#pragma unroll
+    for (uint32_t t = 0; t < 4; t++) {
+      const v16i& from = GATED ? acc[part * TI + t / 2][t % 2] : acc[t][part];
+#pragma unroll
+      for (int v = 0; v < 16; v++) mine[t * 1024 + (8 * (v / 4) + 4 * (lane >> 5) + v % 4) * 32 + (lane & 31)] = from[v];
+    }
+    const uint32_t tile0 = rg * 8 + wr * 4 + (GATED ? part * TI : 0), c = lane & 31;
+    const uint64_t col = ((uint64_t)cg * CT + (GATED ? wc : wc * 2 + part)) * 32 + c;
+#pragma unroll 1
+    for (uint32_t r0 = 0; r0 < TI * ROWS; r0 += 2 * E) {
+      uint64_t at[E], cols[E];
+      bool ok[E];
+#pragma unroll
+      for (int e = 0; e < E; e++) {
+        const uint64_t row = (uint64_t)tile0 * ROWS + r0 + 2 * e + (lane >> 5);
+        at[e] = row * g.n + col;
+        cols[e] = col;
+        ok[e] = row < g.m && col < g.n;
+      }
+      typename End::template Fetched<E> fetched;
+      if (plan.splits == 1) end.fetch(at, cols, ok, fetched);
+      uint32_t z[NW][E];
+#pragma unroll
+      for (int e = 0; e < E; e++) {
+        const uint32_t r = r0 + 2 * e + (lane >> 5);
+#pragma unroll
+        for (int x = 0; x < NW; x++) {
+          const int32_t* const t = mine + (r / ROWS * NW + x) * 1024 + c;
+          if constexpr (FOUR) {
+            const uint32_t r4 = 4 * (r % 8);
+            const int32_t d[4] = {t[r4 * 32], t[r4 * 32 + 32], t[r4 * 32 + 64], t[r4 * 32 + 96]};
+            z[x][e] = digit_sum_mod_p(d);
+          } else {
+            z[x][e] = gemm_mod_p(t[r % 32 * 32]);
+          }
+        }
+      }
+      if (plan.splits == 1) {
+        end.store(at, ok, fetched, z);
+      } else {
+#pragma unroll
+        for (int e = 0; e < E; e++)
+#pragma unroll
+          for (int x = 0; x < NW; x++)
+            if (ok[e]) g.part[(uint64_t)(split * NW + x) * g.m * g.n + at[e]] = z[x][e];
+      }
+    }
+  }
+}
+template <bool GATED, class End>
+static __global__ void __launch_bounds__(512) k_wit_blocks(WitProduct g, End end) {
+  __shared__ v4i lds[2 * 16 * kBlockStage * 64];
+  const bool four = *g.mask != 0;
+  const WitPlan& plan = g.plan[four ? 1 : 0];
+  // as gemm_group, over the groups that this product has
+  const uint64_t groups = (uint64_t)plan.rgroups * g.cgroups, per_xcd = (groups + 7) / 8;
+  const uint64_t i = blockIdx.x >> 3, at = (blockIdx.x & 7) * per_xcd + i;
+  if (i >= per_xcd || at >= groups || blockIdx.y >= plan.splits) return;  // uniform
+  const uint32_t rg = (uint32_t)(at % plan.rgroups), cg = (uint32_t)(at / plan.rgroups);
+  if (four)
+    wit_block<GATED, true>(g, lds, rg, cg, blockIdx.y, end);
+  else
+    wit_block<GATED, false>(g, lds, rg, cg, blockIdx.y, end);
+}
+
 // The end of a product whose K was split: a thread per element.
 template <bool GATED, class End>
 static __global__ void __launch_bounds__(256) k_wit_join(WitProduct g, End end) {

@@ -79,6 +79,24 @@ static bool few_rows(uint64_t m, uint64_t k, uint64_t n) {
 
 static dim3 end_grid(uint64_t count);
 
+// K splits of k_wit_blocks: a workgroup fills a CU, and a K step takes it about
+// 0.25 us, so the steps of the last, partly filled round of the 256 CUs are
+// weighed against the parts' way through memory (8 bytes an element and split
+// at 4 TB/s, and 5 us for the joining launch).
+static uint32_t block_splits(uint64_t groups, uint32_t nsteps, uint64_t elements) {
+  uint32_t best = 1;
+  double best_us = 0;
+  for (uint32_t s = 1; s <= 16 && (s == 1 || nsteps / s >= 16); s++) {
+    const uint64_t rounds = (groups * s + 255) / 256, steps = (nsteps + s - 1) / s;
+    const double us = 0.25 * (double)(rounds * (steps + 8)) + (s > 1 ? 5.0 + (double)s * (double)elements * 2e-6 : 0.0);
+    if (s == 1 || us < best_us) {
+      best = s;
+      best_us = us;
+    }
+  }
+  return best;
+}
+
 // More rows: packed, multiplied (k_wit_tiles) and, where K is split, joined.
 template <bool GATED, class End>
 static int packed_product(gkr_ctx* c, const gkr_matrix* a, const gkr_matrix* w0, const gkr_matrix* w1, const End& end) {
@@ -107,22 +125,38 @@ static int packed_product(gkr_ctx* c, const gkr_matrix* a, const gkr_matrix* w0,
     GKR_LAUNCH(c, k_wit_pack<false>, pack_grid, dim3(256), 0, a->dev, m, k, (uint64_t)g.nsteps, packed, const_cast<int8_t*>(g.four), mask, next_mask);
   TRY(check_launch(c));
 
-  uint32_t max_splits = 1;
-  g.cgroups = g.ctiles;
-  auto launch = [&](auto kernel, uint32_t rt, uint32_t waves, uint32_t wr1, uint32_t wr4) -> int {
-    const uint64_t tiles[2] = {one_tiles, four_tiles}, group[2] = {rt * wr1, rt * wr4};
+  uint32_t max_splits = 1, max_rgroups = 1;
+  // group: row tiles of a workgroup, for rows of one plane and of four
+  auto plans = [&](uint32_t group1, uint32_t group4, auto splits_of) -> int {
+    const uint64_t tiles[2] = {one_tiles, four_tiles};
+    const uint32_t group[2] = {group1, group4};
     for (int i = 0; i < 2; i++) {
       WitPlan& p = g.plan[i];
       p.rtiles = (uint32_t)tiles[i];
       p.rgroups = (uint32_t)((tiles[i] + group[i] - 1) / group[i]);
-      p.splits = 1;
-      p.steps = g.nsteps;
+      p.splits = splits_of((uint64_t)p.rgroups * g.cgroups);
+      p.steps = (g.nsteps + p.splits - 1) / p.splits;
+      p.splits = (g.nsteps + p.steps - 1) / p.steps;
       max_splits = std::max(max_splits, p.splits);
+      max_rgroups = std::max(max_rgroups, p.rgroups);
     }
+    if (max_splits > 1) TRY(ensureT(c, S_GEMMP, (uint64_t)max_splits * (GATED ? 2 : 1) * m * n, &g.part));
+    return GKR_OK;
+  };
+  auto launch = [&](auto kernel, uint32_t rt, uint32_t waves, uint32_t wr1, uint32_t wr4) -> int {
+    g.cgroups = g.ctiles;
+    TRY(plans(rt * wr1, rt * wr4, [](uint64_t) { return 1u; }));
     uint32_t rg;
-    const dim3 grid = gemm_group_grid(std::max(g.plan[0].rgroups, g.plan[1].rgroups), g.cgroups, max_splits, &rg,
-                                      kGemmMaxGroups / 4);
+    const dim3 grid = gemm_group_grid(max_rgroups, g.cgroups, max_splits, &rg, kGemmMaxGroups / 4);
     GKR_LAUNCH(c, kernel, grid, dim3(64 * waves), 0, g, rg, end);
+    return check_launch(c);
+  };
+  auto launch_blocks = [&]() -> int {
+    g.cgroups = (uint32_t)((ctiles * (GATED ? 2 : 1) + 7) / 8);
+    TRY(plans(8, 8, [&](uint64_t groups) { return block_splits(groups, g.nsteps, m * n * (GATED ? 2 : 1)); }));
+    auto kernel = k_wit_blocks<GATED, End>;
+    const uint64_t groups = (uint64_t)max_rgroups * g.cgroups;
+    GKR_LAUNCH(c, kernel, dim3((uint32_t)((groups + 7) / 8 * 8), max_splits), dim3(512), 0, g, end);
     return check_launch(c);
   };
 #define GKR_WIT_TILES(RT, PB, W, WR1, WR4) launch(k_wit_tiles<RT, PB, GATED, W, WR1, WR4, End>, RT, W, WR1, WR4)
@@ -133,7 +167,8 @@ static int packed_product(gkr_ctx* c, const gkr_matrix* a, const gkr_matrix* w0,
   else if (m <= 8) TRY(GKR_WIT_TILES(1, 1, W, 1, 1));
   else if (m <= 16) TRY(GKR_WIT_TILES(1, 1, W, 1, 2));
   else if (m <= 32) TRY(GKR_WIT_TILES(1, 1, W, 1, 4));
-  else TRY(GKR_WIT_TILES(2, 1, W, 1, 4));
+  else if (m <= 64) TRY(GKR_WIT_TILES(2, 1, W, 1, 4));
+  else TRY(launch_blocks());
 #undef GKR_WIT_TILES
   if (max_splits > 1) {
     auto join = k_wit_join<GATED, End>;
@@ -144,7 +179,7 @@ static int packed_product(gkr_ctx* c, const gkr_matrix* a, const gkr_matrix* w0,
 }
 // Sizes that the packed product's grids and 32-bit step offsets take.
 static bool packable(uint64_t m, uint64_t k, uint64_t n) {
-  return k <= kMaxInner && m <= 64 && n <= 1ull << 24 && m * k <= 1ull << 34;
+  return k <= kMaxInner && m <= 1ull << 22 && n <= 1ull << 24 && m * k <= 1ull << 34;
 }
 
 static dim3 end_grid(uint64_t count) { return dim3((uint32_t)std::min<uint64_t>((count + 255) / 256, 1u << 20)); }
