@@ -462,15 +462,11 @@ __device__ __forceinline__ void wit_block(const WitProduct& g, v4i* lds, uint32_
     }
   }
   v4i in[8];
-  auto load = [&](uint32_t s) {  // of the stage from step s
+  auto load = [&](int i, uint32_t s) {  // tile i of the stage from step s
     const uint32_t step = s + wave / 2, at = (step < s1 ? step : s1 - 1) * kGemmBlockBytes + 16 * lane;
-#pragma unroll
-    for (int i = 0; i < 8; i++) in[i] = *(const v4i*)(from[i] + at);
+    in[i] = *(const v4i*)(from[i] + at);
   };
-  auto put = [&](uint32_t half) {
-#pragma unroll
-    for (int i = 0; i < 8; i++) lds[(half * 8 * kBlockStage * 2 + wave * 8 + i) * 64 + lane] = in[i];
-  };
+  auto put = [&](int i, uint32_t half) { lds[(half * 8 * kBlockStage * 2 + wave * 8 + i) * 64 + lane] = in[i]; };
   const uint32_t wr = wave & 1, wc = wave >> 1;
   v16i acc[4][2];
 #pragma unroll
@@ -479,33 +475,52 @@ __device__ __forceinline__ void wit_block(const WitProduct& g, v4i* lds, uint32_
     for (int j = 0; j < 2; j++)
 #pragma unroll
       for (int v = 0; v < 16; v++) acc[i][j][v] = 0;
-  auto multiply = [&](uint32_t half, int k) {
+  v4i a[2][4], b[2][2];  // a K step's operands, and the next one's
+  auto read = [&](int to, uint32_t half, int k) {
     const v4i* const at = lds + (half * 8 * kBlockStage * 2 + k * 16) * 64 + lane;
-    v4i a[4], b[2];
 #pragma unroll
-    for (int j = 0; j < 2; j++) b[j] = at[(8 + wc * 2 + j) * 64];
+    for (int j = 0; j < 2; j++) b[to][j] = at[(8 + wc * 2 + j) * 64];
 #pragma unroll
-    for (int i = 0; i < 4; i++) a[i] = at[(wr * 4 + i) * 64];
+    for (int i = 0; i < 4; i++) a[to][i] = at[(wr * 4 + i) * 64];
+  };
+  auto multiply = [&](int of) {
 #pragma unroll
     for (int i = 0; i < 4; i++)
 #pragma unroll
-      for (int j = 0; j < 2; j++) acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(a[i], b[j], acc[i][j], 0, 0, 0);
+      for (int j = 0; j < 2; j++) acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(a[of][i], b[of][j], acc[i][j], 0, 0, 0);
   };
-  load(s0);
-  put(0);
-  load(s0 + kBlockStage);
+#pragma unroll
+  for (int i = 0; i < 8; i++) load(i, s0);
+#pragma unroll
+  for (int i = 0; i < 8; i++) put(i, 0);
+#pragma unroll
+  for (int i = 0; i < 8; i++) load(i, s0 + kBlockStage);
   __syncthreads();
   uint32_t half = 0, s = s0;
 #pragma unroll 1
   for (; s + kBlockStage <= s1; s += kBlockStage, half ^= 1) {
-    put(half ^ 1);
-    load(s + 2 * kBlockStage);
-    __builtin_amdgcn_sched_barrier(0);  // left to itself the compiler issues the loads last
+    read(0, half, 0);
 #pragma unroll
-    for (int k = 0; k < kBlockStage; k++) multiply(half, k);
+    for (int k = 0; k < kBlockStage; k++) {
+      // the next step's operands, a quarter of the next stage and of the one
+      // after it go out before this step's products
+      if (k + 1 < kBlockStage) read((k + 1) & 1, half, k + 1);
+#pragma unroll
+      for (int i = 2 * k; i < 2 * k + 2; i++) {
+        put(i, half ^ 1);
+        load(i, s + 2 * kBlockStage);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+      multiply(k & 1);
+      __builtin_amdgcn_sched_barrier(0);
+    }
     __syncthreads();
   }
-  for (int k = 0; s + k < s1; k++) multiply(half, k);  // a last, shorter stage
+#pragma unroll 1
+  for (int k = 0; s + k < s1; k++) {  // a last, shorter stage
+    read(0, half, k);
+    multiply(0);
+  }
   // The end, half of a wave's tiles at a time: through its 16 KB of LDS into
   // rows, eight elements a lane and turn.
   __syncthreads();
