@@ -476,18 +476,13 @@ __device__ __forceinline__ void wit_block(const WitProduct& g, v4i* lds, uint32_
 #pragma unroll
       for (int v = 0; v < 16; v++) acc[i][j][v] = 0;
   v4i a[2][4], b[2][2];  // a K step's operands, and the next one's
-  auto read = [&](int to, uint32_t half, int k) {
+  auto read = [&](int to, uint32_t half, int k, int o) {  // operand o of six
     const v4i* const at = lds + (half * 8 * kBlockStage * 2 + k * 16) * 64 + lane;
-#pragma unroll
-    for (int j = 0; j < 2; j++) b[to][j] = at[(8 + wc * 2 + j) * 64];
-#pragma unroll
-    for (int i = 0; i < 4; i++) a[to][i] = at[(wr * 4 + i) * 64];
+    if (o < 2) b[to][o] = at[(8 + wc * 2 + o) * 64];
+    else a[to][o - 2] = at[(wr * 4 + o - 2) * 64];
   };
-  auto multiply = [&](int of) {
-#pragma unroll
-    for (int i = 0; i < 4; i++)
-#pragma unroll
-      for (int j = 0; j < 2; j++) acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(a[of][i], b[of][j], acc[i][j], 0, 0, 0);
+  auto multiply = [&](int of, int t) {  // product t of eight
+    acc[t / 2][t % 2] = __builtin_amdgcn_mfma_i32_32x32x32_i8(a[of][t / 2], b[of][t % 2], acc[t / 2][t % 2], 0, 0, 0);
   };
 #pragma unroll
   for (int i = 0; i < 8; i++) load(i, s0);
@@ -497,29 +492,38 @@ __device__ __forceinline__ void wit_block(const WitProduct& g, v4i* lds, uint32_
   for (int i = 0; i < 8; i++) load(i, s0 + kBlockStage);
   __syncthreads();
   uint32_t half = 0, s = s0;
+#pragma unroll
+  for (int o = 0; o < 6; o++) read(0, 0, 0, o);
+  // Between a K step's products go the next step's operands, one after each,
+  // and a third of the next stage's way to LDS: issued together they hold the
+  // matrix cores up, as all eight waves do it at the same time.  The barrier
+  // comes before a stage's last step, whose operands are there, so that the
+  // next stage's first are read under that step's products.
 #pragma unroll 1
   for (; s + kBlockStage <= s1; s += kBlockStage, half ^= 1) {
-    read(0, half, 0);
 #pragma unroll
     for (int k = 0; k < kBlockStage; k++) {
-      // the next step's operands, a quarter of the next stage and of the one
-      // after it go out before this step's products
-      if (k + 1 < kBlockStage) read((k + 1) & 1, half, k + 1);
+      const bool turn = k + 1 == kBlockStage;
+      if (turn) __syncthreads();
 #pragma unroll
-      for (int i = 2 * k; i < 2 * k + 2; i++) {
-        put(i, half ^ 1);
-        load(i, s + 2 * kBlockStage);
+      for (int t = 0; t < 8; t++) {
+        multiply(k & 1, t);
+        if (t < 6) read((k + 1) & 1, turn ? half ^ 1 : half, turn ? 0 : k + 1, t);
+        const int i = 3 * k + t / 2 - 1;
+        if (!turn && t >= 2 && t % 2 == 1 && i < 8) {
+          put(i, half ^ 1);
+          load(i, s + 2 * kBlockStage);
+        }
+        __builtin_amdgcn_sched_barrier(0);
       }
-      __builtin_amdgcn_sched_barrier(0);
-      multiply(k & 1);
-      __builtin_amdgcn_sched_barrier(0);
     }
-    __syncthreads();
   }
 #pragma unroll 1
   for (int k = 0; s + k < s1; k++) {  // a last, shorter stage
-    read(0, half, k);
-    multiply(0);
+#pragma unroll
+    for (int o = 0; o < 6; o++) read(0, half, k, o);
+#pragma unroll
+    for (int t = 0; t < 8; t++) multiply(0, t);
   }
   // The end, half of a wave's tiles at a time: through its 16 KB of LDS into
   // rows, eight elements a lane and turn.
@@ -578,20 +582,40 @@ __device__ __forceinline__ void wit_block(const WitProduct& g, v4i* lds, uint32_
     }
   }
 }
+// As gemm_group, in one grid dimension over the groups that a product has.
+__device__ __forceinline__ bool wit_group(uint32_t rgroups, uint32_t cgroups, uint32_t& rg, uint32_t& cg) {
+  const uint64_t groups = (uint64_t)rgroups * cgroups, per_xcd = (groups + 7) / 8;
+  const uint64_t i = blockIdx.x >> 3, at = (blockIdx.x & 7) * per_xcd + i;
+  rg = (uint32_t)(at % rgroups);
+  cg = (uint32_t)(at / rgroups);
+  return i < per_xcd && at < groups;
+}
 template <bool GATED, class End>
 static __global__ void __launch_bounds__(512) k_wit_blocks(WitProduct g, End end) {
   __shared__ v4i lds[2 * 16 * kBlockStage * 64];
   const bool four = *g.mask != 0;
   const WitPlan& plan = g.plan[four ? 1 : 0];
-  // as gemm_group, over the groups that this product has
-  const uint64_t groups = (uint64_t)plan.rgroups * g.cgroups, per_xcd = (groups + 7) / 8;
-  const uint64_t i = blockIdx.x >> 3, at = (blockIdx.x & 7) * per_xcd + i;
-  if (i >= per_xcd || at >= groups || blockIdx.y >= plan.splits) return;  // uniform
-  const uint32_t rg = (uint32_t)(at % plan.rgroups), cg = (uint32_t)(at / plan.rgroups);
+  uint32_t rg, cg;
+  if (!wit_group(plan.rgroups, g.cgroups, rg, cg) || blockIdx.y >= plan.splits) return;  // uniform
   if (four)
     wit_block<GATED, true>(g, lds, rg, cg, blockIdx.y, end);
   else
     wit_block<GATED, false>(g, lds, rg, cg, blockIdx.y, end);
+}
+// 65 to 256 rows: rows of one plane are still a stream of the weights
+// (wit_tiles, all of the rows in a workgroup), rows of four are blocks.
+template <int RT, int WR, bool GATED, class End>
+static __global__ void __launch_bounds__(512) k_wit_mixed(WitProduct g, End end) {
+  __shared__ v4i lds[2 * 16 * kBlockStage * 64];
+  static_assert(WR * RT * (GATED ? 2 : 1) * 4096 <= sizeof(lds), "the waves' sums");
+  const bool four = *g.mask != 0;
+  const WitPlan& plan = g.plan[four ? 1 : 0];
+  uint32_t rg, cg;
+  if (!wit_group(plan.rgroups, four ? g.cgroups : g.ctiles, rg, cg) || blockIdx.y >= plan.splits) return;  // uniform
+  if (four)
+    wit_block<GATED, true>(g, lds, rg, cg, blockIdx.y, end);
+  else
+    wit_tiles<RT, 1, GATED, 8, WR, false>(g, (int32_t*)lds, rg, cg, 0, end);
 }
 
 // The end of a product whose K was split: a thread per element.

@@ -127,39 +127,42 @@ static int packed_product(gkr_ctx* c, const gkr_matrix* a, const gkr_matrix* w0,
 
   uint32_t max_splits = 1, max_rgroups = 1;
   // group: row tiles of a workgroup, for rows of one plane and of four
-  auto plans = [&](uint32_t group1, uint32_t group4, auto splits_of) -> int {
-    const uint64_t tiles[2] = {one_tiles, four_tiles};
-    const uint32_t group[2] = {group1, group4};
-    for (int i = 0; i < 2; i++) {
-      WitPlan& p = g.plan[i];
-      p.rtiles = (uint32_t)tiles[i];
-      p.rgroups = (uint32_t)((tiles[i] + group[i] - 1) / group[i]);
-      p.splits = splits_of((uint64_t)p.rgroups * g.cgroups);
-      p.steps = (g.nsteps + p.splits - 1) / p.splits;
-      p.splits = (g.nsteps + p.steps - 1) / p.steps;
-      max_splits = std::max(max_splits, p.splits);
-      max_rgroups = std::max(max_rgroups, p.rgroups);
-    }
-    if (max_splits > 1) TRY(ensureT(c, S_GEMMP, (uint64_t)max_splits * (GATED ? 2 : 1) * m * n, &g.part));
+  auto plan = [&](int four, uint32_t group, auto splits_of) -> int {
+    const uint64_t tiles = four ? four_tiles : one_tiles;
+    WitPlan& p = g.plan[four];
+    p.rtiles = (uint32_t)tiles;
+    p.rgroups = (uint32_t)((tiles + group - 1) / group);
+    p.splits = splits_of((uint64_t)p.rgroups * g.cgroups);
+    p.steps = (g.nsteps + p.splits - 1) / p.splits;
+    p.splits = (g.nsteps + p.steps - 1) / p.steps;
+    max_splits = std::max(max_splits, p.splits);
+    max_rgroups = std::max(max_rgroups, p.rgroups);
+    if (p.splits > 1) TRY(ensureT(c, S_GEMMP, (uint64_t)max_splits * (GATED ? 2 : 1) * m * n, &g.part));
     return GKR_OK;
   };
-  auto launch = [&](auto kernel, uint32_t rt, uint32_t waves, uint32_t wr1, uint32_t wr4) -> int {
+  const auto whole = [](uint64_t) { return 1u; };
+  const auto split = [&](uint64_t groups) { return block_splits(groups, g.nsteps, m * n * (GATED ? 2 : 1)); };
+  auto launch_tiles = [&](auto kernel, uint32_t rt, uint32_t waves, uint32_t wr1, uint32_t wr4) -> int {
     g.cgroups = g.ctiles;
-    TRY(plans(rt * wr1, rt * wr4, [](uint64_t) { return 1u; }));
+    TRY(plan(0, rt * wr1, whole));
+    TRY(plan(1, rt * wr4, whole));
     uint32_t rg;
     const dim3 grid = gemm_group_grid(max_rgroups, g.cgroups, max_splits, &rg, kGemmMaxGroups / 4);
     GKR_LAUNCH(c, kernel, grid, dim3(64 * waves), 0, g, rg, end);
     return check_launch(c);
   };
-  auto launch_blocks = [&]() -> int {
+  // rows1: row tiles a workgroup has of rows of one plane that it streams the weights for; 0: blocks as for four
+  auto launch_blocks = [&](auto kernel, uint32_t rows1) -> int {
     g.cgroups = (uint32_t)((ctiles * (GATED ? 2 : 1) + 7) / 8);
-    TRY(plans(8, 8, [&](uint64_t groups) { return block_splits(groups, g.nsteps, m * n * (GATED ? 2 : 1)); }));
-    auto kernel = k_wit_blocks<GATED, End>;
-    const uint64_t groups = (uint64_t)max_rgroups * g.cgroups;
+    if (rows1) TRY(plan(0, rows1, whole));
+    else TRY(plan(0, 8, split));
+    TRY(plan(1, 8, split));
+    const uint64_t groups = std::max((uint64_t)g.plan[0].rgroups * (rows1 ? g.ctiles : g.cgroups),
+                                     (uint64_t)g.plan[1].rgroups * g.cgroups);
     GKR_LAUNCH(c, kernel, dim3((uint32_t)((groups + 7) / 8 * 8), max_splits), dim3(512), 0, g, end);
     return check_launch(c);
   };
-#define GKR_WIT_TILES(RT, PB, W, WR1, WR4) launch(k_wit_tiles<RT, PB, GATED, W, WR1, WR4, End>, RT, W, WR1, WR4)
+#define GKR_WIT_TILES(RT, PB, W, WR1, WR4) launch_tiles(k_wit_tiles<RT, PB, GATED, W, WR1, WR4, End>, RT, W, WR1, WR4)
   // sixteen waves a workgroup for one matrix, eight for two: the registers of
   // sixteen hold no more accumulators
   constexpr int W = GATED ? 8 : 16;
@@ -168,7 +171,9 @@ static int packed_product(gkr_ctx* c, const gkr_matrix* a, const gkr_matrix* w0,
   else if (m <= 16) TRY(GKR_WIT_TILES(1, 1, W, 1, 2));
   else if (m <= 32) TRY(GKR_WIT_TILES(1, 1, W, 1, 4));
   else if (m <= 64) TRY(GKR_WIT_TILES(2, 1, W, 1, 4));
-  else TRY(launch_blocks());
+  else if (m <= 128) TRY(launch_blocks(k_wit_mixed<GATED ? 2 : 4, GATED ? 2 : 1, GATED, End>, 4));
+  else if (m <= 256) TRY(launch_blocks(k_wit_mixed<GATED ? 2 : 4, GATED ? 4 : 2, GATED, End>, 8));
+  else TRY(launch_blocks(k_wit_blocks<GATED, End>, 0));
 #undef GKR_WIT_TILES
   if (max_splits > 1) {
     auto join = k_wit_join<GATED, End>;
@@ -179,7 +184,8 @@ static int packed_product(gkr_ctx* c, const gkr_matrix* a, const gkr_matrix* w0,
 }
 // Sizes that the packed product's grids and 32-bit step offsets take.
 static bool packable(uint64_t m, uint64_t k, uint64_t n) {
-  return k <= kMaxInner && m <= 1ull << 22 && n <= 1ull << 24 && m * k <= 1ull << 34;
+  return k <= kMaxInner && m <= 1ull << 22 && n <= 1ull << 24 && m * k <= 1ull << 34 &&
+         (m / 64 + 1) * (n / 128 + 1) <= 1ull << 22;
 }
 
 static dim3 end_grid(uint64_t count) { return dim3((uint32_t)std::min<uint64_t>((count + 255) / 256, 1u << 20)); }
