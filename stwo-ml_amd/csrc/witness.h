@@ -27,69 +27,124 @@ __device__ __forceinline__ void activate(const ActArg& a, uint32_t (&z)[E]) {
   }
 }
 
+// Words of a row-major m x n matrix from word `first` on, as a buffer: a lane
+// adds a 32-bit byte offset, and a place behind the matrix's last word (a tile's
+// rows past m; kOutside for columns past n) reads zero and is not written, with
+// no comparison for it.  A matrix that is not given has no bytes.
+typedef __amdgpu_buffer_rsrc_t WitBuffer;
+constexpr uint32_t kOutside = 0xfffffff0u;
+__device__ __forceinline__ WitBuffer wit_buffer(const uint32_t* p, uint64_t first, uint64_t count) {
+  const uint64_t bytes = p && first < count ? 4 * (count - first) : 0;
+  return __builtin_amdgcn_make_buffer_rsrc((void*)(p + (bytes ? first : 0)), 0,
+                                           (int)(uint32_t)(bytes < kOutside ? bytes : kOutside), 0x00027000);
+}
+__device__ __forceinline__ uint32_t wit_read(WitBuffer b, uint32_t at) {
+  return (uint32_t)__builtin_amdgcn_raw_buffer_load_b32(b, (int)at, 0, 0);
+}
+__device__ __forceinline__ void wit_write(WitBuffer b, uint32_t at, uint32_t x) {
+  __builtin_amdgcn_raw_buffer_store_b32((int)x, b, (int)at, 0, 0);
+}
+
 // What happens to a sum of the product (fused) or a pair of sums (gated), for E
-// elements (row-major place `at`, column `col`) of a thread: fetch() before the
-// sums are there, store() with them.  Places that are not `ok` are not touched.
+// elements (byte offsets `at` into the Tile) of a thread.  begin() takes the
+// sums and sends the loads out that they need, finish() stores, so that the next
+// elements' loads can go out before these ones' stores.  `bias`: the column's.
 struct FusedEnd {
   ActArg act;
   const uint32_t* bias;      // n
   const uint32_t* residual;  // m x n; may be out (read by the thread that writes the element)
   uint32_t* pre;
   uint32_t* out;
-  template <int E>
-  struct Fetched {
-    uint32_t bias[E], residual[E];
+  struct Tile {
+    WitBuffer residual, pre, out;
   };
   template <int E>
-  __device__ __forceinline__ void fetch(const uint64_t (&at)[E], const uint64_t (&col)[E], const bool (&ok)[E],
-                                        Fetched<E>& f) const {
+  struct Slot {
+    uint32_t z[E], y[E], residual[E];
+  };
+  __device__ __forceinline__ Tile tile(uint64_t first, uint64_t count) const {
+    return Tile{wit_buffer(residual, first, count), wit_buffer(pre, first, count), wit_buffer(out, first, count)};
+  }
+  __device__ __forceinline__ uint32_t column(uint64_t col, bool ok) const { return bias && ok ? bias[col] : 0u; }
+  template <int E>
+  __device__ __forceinline__ void begin(Slot<E>& s, const Tile& t, const uint32_t (&at)[E], uint32_t b,
+                                        const uint32_t (&z)[1][E]) const {
+    if (residual) {
 #pragma unroll
-    for (int e = 0; e < E; e++) {
-      f.bias[e] = bias && ok[e] ? bias[col[e]] : 0u;
-      f.residual[e] = residual && ok[e] ? residual[at[e]] : 0u;
+      for (int e = 0; e < E; e++) s.residual[e] = wit_read(t.residual, at[e]);
     }
+#pragma unroll
+    for (int e = 0; e < E; e++) s.y[e] = s.z[e] = m31_add(z[0][e], b);
+    activate(act, s.y);
   }
   template <int E>
-  __device__ __forceinline__ void store(const uint64_t (&at)[E], const bool (&ok)[E], const Fetched<E>& f,
-                                        uint32_t (&z)[1][E]) const {
+  __device__ __forceinline__ void finish(Slot<E>& s, const Tile& t, const uint32_t (&at)[E]) const {
+    if (pre) {
 #pragma unroll
-    for (int e = 0; e < E; e++) z[0][e] = m31_add(z[0][e], f.bias[e]);
-    uint32_t y[E];
+      for (int e = 0; e < E; e++) wit_write(t.pre, at[e], s.z[e]);
+    }
+    if (residual) {
 #pragma unroll
-    for (int e = 0; e < E; e++) y[e] = z[0][e];
-    activate(act, y);
+      for (int e = 0; e < E; e++) s.y[e] = m31_add(s.y[e], s.residual[e]);
+    }
 #pragma unroll
-    for (int e = 0; e < E; e++)
-      if (ok[e]) {
-        if (pre) pre[at[e]] = z[0][e];
-        out[at[e]] = m31_add(y[e], f.residual[e]);
-      }
+    for (int e = 0; e < E; e++) wit_write(t.out, at[e], s.y[e]);
   }
 };
 struct GatedEnd {
   ActArg act;
   uint32_t *gate, *act_out, *up, *out;
+  struct Tile {
+    WitBuffer gate, act, up, out;
+  };
   template <int E>
-  struct Fetched {};
+  struct Slot {
+    uint32_t z[E], y[E], u[E];
+  };
+  __device__ __forceinline__ Tile tile(uint64_t first, uint64_t count) const {
+    return Tile{wit_buffer(gate, first, count), wit_buffer(act_out, first, count), wit_buffer(up, first, count),
+                wit_buffer(out, first, count)};
+  }
+  __device__ __forceinline__ uint32_t column(uint64_t, bool) const { return 0; }
   template <int E>
-  __device__ __forceinline__ void fetch(const uint64_t (&)[E], const uint64_t (&)[E], const bool (&)[E], Fetched<E>&) const {}
-  template <int E>
-  __device__ __forceinline__ void store(const uint64_t (&at)[E], const bool (&ok)[E], const Fetched<E>&,
-                                        uint32_t (&z)[2][E]) const {
-    uint32_t y[E];
+  __device__ __forceinline__ void begin(Slot<E>& s, const Tile&, const uint32_t (&)[E], uint32_t,
+                                        const uint32_t (&z)[2][E]) const {
 #pragma unroll
-    for (int e = 0; e < E; e++) y[e] = z[0][e];
-    activate(act, y);
+    for (int e = 0; e < E; e++) {
+      s.y[e] = s.z[e] = z[0][e];
+      s.u[e] = z[1][e];
+    }
+    activate(act, s.y);
+  }
+  template <int E>
+  __device__ __forceinline__ void finish(Slot<E>& s, const Tile& t, const uint32_t (&at)[E]) const {
+    if (gate) {
 #pragma unroll
-    for (int e = 0; e < E; e++)
-      if (ok[e]) {
-        if (gate) gate[at[e]] = z[0][e];
-        if (act_out) act_out[at[e]] = y[e];
-        if (up) up[at[e]] = z[1][e];
-        out[at[e]] = m31_mul(y[e], z[1][e]);
-      }
+      for (int e = 0; e < E; e++) wit_write(t.gate, at[e], s.z[e]);
+    }
+    if (act_out) {
+#pragma unroll
+      for (int e = 0; e < E; e++) wit_write(t.act, at[e], s.y[e]);
+    }
+    if (up) {
+#pragma unroll
+      for (int e = 0; e < E; e++) wit_write(t.up, at[e], s.u[e]);
+    }
+#pragma unroll
+    for (int e = 0; e < E; e++) wit_write(t.out, at[e], m31_mul(s.y[e], s.u[e]));
   }
 };
+// A split's sums, into its part of each matrix.
+template <int NW, int E>
+__device__ __forceinline__ void wit_parts(uint32_t* part, uint32_t split, uint64_t first, uint64_t count,
+                                          const uint32_t (&at)[E], const uint32_t (&z)[NW][E]) {
+#pragma unroll
+  for (int x = 0; x < NW; x++) {
+    const WitBuffer b = wit_buffer(part + (uint64_t)(split * NW + x) * count, first, count);
+#pragma unroll
+    for (int e = 0; e < E; e++) wit_write(b, at[e], z[x][e]);
+  }
+}
 
 // A digit plane stack of a weight: planes of kGemmBlockBytes blocks (gemm.h).
 struct WitWeight {
@@ -204,12 +259,11 @@ static __global__ void __launch_bounds__(64 * kRowWaves) k_rows(const uint32_t* 
           for (int v = 0; v < 4; v++) atomicAdd(&sums[i][q][quarter][v][16 * h + col], acc[i][q][h][v]);
   }
   const uint32_t r = threadIdx.x / 32, c = threadIdx.x % 32, column = ct * kGemmTile + c;
-  const bool ok[1] = {r < m && column < n};
-  const uint64_t at[1] = {(uint64_t)r * n + column}, cols[1] = {column};
-  typename End::template Fetched<1> fetched;
-  end.fetch(at, cols, ok, fetched);
+  const bool ok = r < m && column < n;
+  const uint32_t at[1] = {4 * (r * n + column)};  // below 2^32: four rows of at most 2^26 words
+  const uint32_t bias = end.column(column, ok);
   __syncthreads();
-  if (!ok[0]) return;
+  if (!ok) return;
   uint32_t z[NW][1];
 #pragma unroll
   for (int i = 0; i < NW; i++) {
@@ -221,7 +275,10 @@ static __global__ void __launch_bounds__(64 * kRowWaves) k_rows(const uint32_t* 
     }
     z[i][0] = m31_reduce64(t);
   }
-  end.store(at, ok, fetched, z);
+  typename End::template Slot<1> slot;
+  const typename End::Tile tile = end.tile(0, (uint64_t)m * n);
+  end.begin(slot, tile, at, bias, z);
+  end.finish(slot, tile, at);
 }
 
 // More rows: the rows' digits are packed first, as operand blocks (gemm.h) in
@@ -361,20 +418,15 @@ __device__ __forceinline__ void wit_tiles(const WitProduct& g, int32_t* sums, ui
   constexpr uint32_t ROWS = FOUR ? 8 : 32;  // of a tile
   constexpr int ALL = TILES * ROWS * 32, E = ALL <= 64 * W ? 1 : ALL / (64 * W);
   static_assert(E * 64 * W == ALL || E == 1, "whole elements");
-  uint64_t at[E], cols[E];
-  uint32_t rows[E];
-  bool ok[E];
   const uint32_t c = threadIdx.x % 32;
+  const uint64_t col = (uint64_t)cg * 32 + c, first = (uint64_t)rg * (TILES * ROWS) * g.n + (uint64_t)cg * 32;
+  uint32_t at[E], rows[E];
 #pragma unroll
   for (int e = 0; e < E; e++) {
     rows[e] = threadIdx.x / 32 + e * 2 * W;
-    const uint64_t row = (uint64_t)rg * (TILES * ROWS) + rows[e];
-    cols[e] = (uint64_t)cg * 32 + c;
-    at[e] = row * g.n + cols[e];
-    ok[e] = rows[e] < TILES * ROWS && row < g.m && cols[e] < g.n;
+    at[e] = rows[e] < TILES * ROWS && col < g.n ? 4 * (rows[e] * (uint32_t)g.n + c) : kOutside;
   }
-  typename End::template Fetched<E> fetched;
-  if (plan.splits == 1) end.fetch(at, cols, ok, fetched);
+  const uint32_t bias = end.column(col, col < g.n);
   __syncthreads();
 #pragma unroll
   for (int i = 0; i < RT; i++)
@@ -411,13 +463,12 @@ __device__ __forceinline__ void wit_tiles(const WitProduct& g, int32_t* sums, ui
     }
   }
   if (plan.splits == 1) {
-    end.store(at, ok, fetched, z);
+    typename End::template Slot<E> slot;
+    const typename End::Tile tile = end.tile(first, g.m * g.n);
+    end.begin(slot, tile, at, bias, z);
+    end.finish(slot, tile, at);
   } else {
-#pragma unroll
-    for (int e = 0; e < E; e++)
-#pragma unroll
-      for (int x = 0; x < NW; x++)
-        if (ok[e]) g.part[(uint64_t)(split * NW + x) * g.m * g.n + at[e]] = z[x][e];
+    wit_parts(g.part, split, first, g.m * g.n, at, z);
   }
 }
 template <int RT, int PB, bool GATED, int W, int WR1, int WR4, class End>
@@ -539,45 +590,62 @@ __device__ __forceinline__ void wit_block(const WitProduct& g, v4i* lds, uint32_
 #pragma unroll
       for (int v = 0; v < 16; v++) mine[t * 1024 + (8 * (v / 4) + 4 * (lane >> 5) + v % 4) * 32 + (lane & 31)] = from[v];
     }
-    const uint32_t tile0 = rg * 8 + wr * 4 + (GATED ? part * TI : 0), c = lane & 31;
-    const uint64_t col = ((uint64_t)cg * CT + (GATED ? wc : wc * 2 + part)) * 32 + c;
-#pragma unroll 1
-    for (uint32_t r0 = 0; r0 < TI * ROWS; r0 += 2 * E) {
-      uint64_t at[E], cols[E];
-      bool ok[E];
+    const uint32_t tile0 = rg * 8 + wr * 4 + (GATED ? part * TI : 0), c = lane & 31, hi = lane >> 5;
+    const uint64_t col0 = ((uint64_t)cg * CT + (GATED ? wc : wc * 2 + part)) * 32;
+    const uint64_t first = (uint64_t)tile0 * ROWS * g.n + col0;
+    const uint32_t bias = end.column(col0 + c, col0 + c < g.n), pitch = 8 * (uint32_t)g.n;  // bytes of two rows
+    const uint32_t at0 = col0 + c < g.n ? 4 * (hi * (uint32_t)g.n + c) : kOutside;
+    const int32_t* const from = mine + hi * (FOUR ? 128 : 32) + c;
+    // rows r0 + 2 e + hi, r0 a multiple of 16
+    auto places = [&](uint32_t r0, uint32_t (&at)[E]) {
 #pragma unroll
-      for (int e = 0; e < E; e++) {
-        const uint64_t row = (uint64_t)tile0 * ROWS + r0 + 2 * e + (lane >> 5);
-        at[e] = row * g.n + col;
-        cols[e] = col;
-        ok[e] = row < g.m && col < g.n;
-      }
-      typename End::template Fetched<E> fetched;
-      if (plan.splits == 1) end.fetch(at, cols, ok, fetched);
-      uint32_t z[NW][E];
+      for (int e = 0; e < E; e++) at[e] = at0 == kOutside ? kOutside : at0 + (r0 / 2 + e) * pitch;
+    };
+    auto values = [&](uint32_t r0, uint32_t (&z)[NW][E]) {
 #pragma unroll
-      for (int e = 0; e < E; e++) {
-        const uint32_t r = r0 + 2 * e + (lane >> 5);
+      for (int e = 0; e < E; e++)
 #pragma unroll
         for (int x = 0; x < NW; x++) {
-          const int32_t* const t = mine + (r / ROWS * NW + x) * 1024 + c;
-          if constexpr (FOUR) {
-            const uint32_t r4 = 4 * (r % 8);
-            const int32_t d[4] = {t[r4 * 32], t[r4 * 32 + 32], t[r4 * 32 + 64], t[r4 * 32 + 96]};
+          if constexpr (FOUR) {  // a tile has eight rows, of four planes each
+            const int32_t* const t = from + (r0 / 8 * NW + e / 4 * NW + x) * 1024 + e % 4 * 256;
+            const int32_t d[4] = {t[0], t[32], t[64], t[96]};
             z[x][e] = digit_sum_mod_p(d);
           } else {
-            z[x][e] = gemm_mod_p(t[r % 32 * 32]);
+            z[x][e] = gemm_mod_p(from[(r0 / 32 * NW + x) * 1024 + r0 % 32 * 32 + e * 64]);
           }
         }
+    };
+    constexpr uint32_t ALL = TI * ROWS;
+    if (plan.splits == 1) {  // two turns at a time, the second's loads before the first's stores
+      const typename End::Tile tile = end.tile(first, g.m * g.n);
+      typename End::template Slot<E> slot[2];
+      auto begin = [&](int i, uint32_t r0) {
+        uint32_t at[E], z[NW][E];
+        places(r0, at);
+        values(r0, z);
+        end.begin(slot[i], tile, at, bias, z);
+      };
+      auto finish = [&](int i, uint32_t r0) {
+        uint32_t at[E];
+        places(r0, at);
+        end.finish(slot[i], tile, at);
+      };
+      static_assert(ALL % (4 * E) == 0 || ALL == 2 * E, "two turns");
+      begin(0, 0);
+#pragma unroll 1
+      for (uint32_t r0 = 0; r0 < ALL; r0 += 4 * E) {
+        if (ALL > 2 * E) begin(1, r0 + 2 * E);
+        finish(0, r0);
+        if (r0 + 4 * E < ALL) begin(0, r0 + 4 * E);
+        if (ALL > 2 * E) finish(1, r0 + 2 * E);
       }
-      if (plan.splits == 1) {
-        end.store(at, ok, fetched, z);
-      } else {
-#pragma unroll
-        for (int e = 0; e < E; e++)
-#pragma unroll
-          for (int x = 0; x < NW; x++)
-            if (ok[e]) g.part[(uint64_t)(split * NW + x) * g.m * g.n + at[e]] = z[x][e];
+    } else {
+#pragma unroll 1
+      for (uint32_t r0 = 0; r0 < ALL; r0 += 2 * E) {
+        uint32_t at[E], z[NW][E];
+        places(r0, at);
+        values(r0, z);
+        wit_parts(g.part, split, first, g.m * g.n, at, z);
       }
     }
   }
@@ -625,11 +693,9 @@ static __global__ void __launch_bounds__(256) k_wit_join(WitProduct g, End end) 
   if (splits == 1) return;  // done where it was computed
   constexpr int NW = GATED ? 2 : 1;
   const uint64_t count = g.m * g.n;
-  for (uint64_t i = (uint64_t)blockIdx.x * blockDim.x + threadIdx.x; i < count; i += (uint64_t)gridDim.x * blockDim.x) {
-    const uint64_t at[1] = {i}, cols[1] = {i % g.n};
-    const bool ok[1] = {true};
-    typename End::template Fetched<1> fetched;
-    end.fetch(at, cols, ok, fetched);
+  for (uint64_t first = (uint64_t)blockIdx.x * 256; first < count; first += (uint64_t)gridDim.x * 256) {
+    const uint64_t i = first + threadIdx.x < count ? first + threadIdx.x : count - 1;
+    const uint32_t at[1] = {4 * threadIdx.x}, bias = end.column(i % g.n, true);
     uint32_t z[NW][1];
 #pragma unroll
     for (int x = 0; x < NW; x++) {
@@ -637,7 +703,10 @@ static __global__ void __launch_bounds__(256) k_wit_join(WitProduct g, End end) 
       for (uint32_t s = 0; s < splits; s++) t += g.part[(uint64_t)(s * NW + x) * count + i];
       z[x][0] = m31_reduce64(t);
     }
-    end.store(at, ok, fetched, z);
+    typename End::template Slot<1> slot;
+    const typename End::Tile tile = end.tile(first, count);
+    end.begin(slot, tile, at, bias, z);
+    end.finish(slot, tile, at);
   }
 }
 
@@ -645,15 +714,16 @@ static __global__ void __launch_bounds__(256) k_wit_join(WitProduct g, End end) 
 template <bool GATED, class End>
 static __global__ void __launch_bounds__(256) k_wit_end(const uint32_t* __restrict__ z0, const uint32_t* __restrict__ z1,
                                                         uint64_t count, uint64_t n, End end) {
-  for (uint64_t i = (uint64_t)blockIdx.x * blockDim.x + threadIdx.x; i < count; i += (uint64_t)gridDim.x * blockDim.x) {
-    const uint64_t at[1] = {i}, cols[1] = {i % n};
-    const bool ok[1] = {true};
-    typename End::template Fetched<1> fetched;
-    end.fetch(at, cols, ok, fetched);
+  for (uint64_t first = (uint64_t)blockIdx.x * 256; first < count; first += (uint64_t)gridDim.x * 256) {
+    const uint64_t i = first + threadIdx.x < count ? first + threadIdx.x : count - 1;
+    const uint32_t at[1] = {4 * threadIdx.x}, bias = end.column(i % n, true);
     uint32_t z[GATED ? 2 : 1][1];
     z[0][0] = z0[i];
     if constexpr (GATED) z[1][0] = z1[i];
-    end.store(at, ok, fetched, z);
+    typename End::template Slot<1> slot;
+    const typename End::Tile tile = end.tile(first, count);
+    end.begin(slot, tile, at, bias, z);
+    end.finish(slot, tile, at);
   }
 }
 
