@@ -59,24 +59,6 @@ int weight_planes(gkr_ctx* c, gkr_matrix* b) {
   return GKR_OK;
 }
 
-// Two mask words, used in turn: the packing of one product clears the other's.
-int gemm_masks(gkr_ctx* c, uint32_t** mask, uint32_t** next_mask) {
-  if (!c->gemm_mask) {
-    drain(c);
-    uint32_t* w = nullptr;
-    HIP_TRY(hipMalloc(&w, 2 * sizeof(uint32_t)));
-    if (hipMemsetAsync(w, 0, 2 * sizeof(uint32_t), c->stream) != hipSuccess) {
-      (void)hipFree(w);
-      return fail(GKR_ERR_DEVICE, "clear of the digit masks failed");
-    }
-    c->gemm_mask = w;
-  }
-  *mask = c->gemm_mask + (c->gemm_turn & 1);
-  *next_mask = c->gemm_mask + (~c->gemm_turn & 1);
-  c->gemm_turn++;
-  return GKR_OK;
-}
-
 int matmul_forward(gkr_ctx* c, const gkr_matrix* a, gkr_matrix* b, uint32_t* C) {
   const uint64_t m = a->rows, k = a->cols, n = b->cols;
   TRY(weight_planes(c, b));
@@ -88,8 +70,20 @@ int matmul_forward(gkr_ctx* c, const gkr_matrix* a, gkr_matrix* b, uint32_t* C) 
   const int PB = b->bnplanes == 1 ? 1 : 4;
   int8_t* ap;
   TRY(ensureT(c, S_GEMMA, (size_t)4 * a_plane, &ap));
-  uint32_t *amask, *next_mask;
-  TRY(gemm_masks(c, &amask, &next_mask));
+  // two mask words, used in turn: the packing of one product clears the other's
+  if (!c->gemm_mask) {
+    drain(c);
+    uint32_t* w = nullptr;
+    HIP_TRY(hipMalloc(&w, 2 * sizeof(uint32_t)));
+    if (hipMemsetAsync(w, 0, 2 * sizeof(uint32_t), c->stream) != hipSuccess) {
+      (void)hipFree(w);
+      return fail(GKR_ERR_DEVICE, "clear of the digit masks failed");
+    }
+    c->gemm_mask = w;
+  }
+  uint32_t* amask = c->gemm_mask + (c->gemm_turn & 1);
+  uint32_t* next_mask = c->gemm_mask + (~c->gemm_turn & 1);
+  c->gemm_turn++;
   TRY(pack_planes(c, a->dev, m, k, false, 4, ap, amask, next_mask));
   const int8_t* bp = b->bplanes;
   if (PB > b->bnplanes) {  // a 2- or 3-plane weight: extend with zero planes in scratch

@@ -184,7 +184,6 @@ int drop_derived(gkr_ctx* c, gkr_matrix* m);
 // (kept with it), and that product into C.
 int weight_planes(gkr_ctx* c, gkr_matrix* b);
 int matmul_forward(gkr_ctx* c, const gkr_matrix* a, gkr_matrix* b, uint32_t* C);
-int gemm_masks(gkr_ctx* c, uint32_t** mask, uint32_t** next_mask);
 // logup.hip: an activation table's output column, resident on the device.
 int device_table(gkr_ctx* c, uint32_t tag, uint32_t log_size, uint32_t** out);
 
@@ -266,6 +265,8 @@ struct gkr_ctx {
   MerkleConsts* merkle_consts = nullptr;  // device copy, built on first use
   uint32_t* gemm_mask = nullptr;          // forward product: A's non-zero planes, two words in turn
   uint32_t gemm_turn = 0;
+  uint32_t* wit_mask = nullptr;           // the same for the witness operators (witness.hip)
+  uint32_t wit_turn = 0;
   f9::fe* merkle_pairs = nullptr;         // parents of int8-range leaf pairs (merkle.h), built on first use
   bool fb_pending = false;  // f_b of the last restriction still as column-chunk partials (S_COLPART)
   uint64_t fb_rows = 0, fb_pk = 0;

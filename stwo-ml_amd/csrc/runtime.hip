@@ -484,6 +484,7 @@ extern "C" void gkr_ctx_destroy(gkr_ctx* c) {
   if (c->merkle_consts) (void)hipFree(c->merkle_consts);
   if (c->merkle_pairs) (void)hipFree(c->merkle_pairs);
   if (c->gemm_mask) (void)hipFree(c->gemm_mask);
+  if (c->wit_mask) (void)hipFree(c->wit_mask);
   if (c->h_res) (void)hipHostFree(c->h_res);
   c->mring.reset();  // freed with the last proof record still holding a slot
   for (int s = 0; s < H_NSLOTS; s++)

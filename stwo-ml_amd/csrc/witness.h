@@ -284,17 +284,21 @@ static __global__ void __launch_bounds__(64 * kRowWaves) k_rows(const uint32_t* 
 // More rows: the rows' digits are packed first, as operand blocks (gemm.h) in
 // two forms, one of which the product reads: plane 0 alone, row r as row r, and
 // all four planes interleaved, plane p of row r as row 4 r + p, so that a lane
-// of an accumulator holds the four digit sums of its elements.  *mask gets a
-// bit where a digit above plane 0 is not zero, and *clear, the mask of the next
-// product on the stream, is zeroed.  A thread takes 16 words of a row; rows
+// of an accumulator holds the four digit sums of its elements.  Words of
+// the mask are set where a digit above plane 0 is not zero, and `clear`, the mask
+// of the next product on the stream, is zeroed.  A thread takes 16 words of a row; rows
 // past m are left as they are (their sums are not stored).
+constexpr uint32_t kMaskWords = 64, kMaskStride = 32;
+__device__ __forceinline__ bool wit_four(const uint32_t* mask) {  // the same in every wave
+  return __any(mask[kMaskStride * (threadIdx.x & 63)] != 0);
+}
 template <bool VEC>
 static __global__ void __launch_bounds__(256) k_wit_pack(const uint32_t* __restrict__ X, uint64_t m, uint64_t k,
                                                          uint64_t nsteps, int8_t* __restrict__ one,
                                                          int8_t* __restrict__ four, uint32_t* __restrict__ mask,
                                                          uint32_t* __restrict__ clear) {
   const uint64_t at = (uint64_t)blockIdx.x * blockDim.x + threadIdx.x;  // (row / 8, step, row % 8, half)
-  if (at == 0) *clear = 0;
+  if (at < kMaskWords) clear[kMaskStride * at] = 0;
   const uint32_t half = (uint32_t)at & 1, row8 = (uint32_t)(at >> 1) & 7;
   const uint64_t blk = at >> 4, rt8 = blk / nsteps, step = blk - rt8 * nsteps, row = 8 * rt8 + row8;
   uint32_t high = 0;
@@ -325,8 +329,12 @@ static __global__ void __launch_bounds__(256) k_wit_pack(const uint32_t* __restr
     *(uint4*)(one + ((row >> 5) * nsteps + step) * kGemmBlockBytes + 512 * half + 16 * (row & 31)) =
         make_uint4(w[0][0], w[0][1], w[0][2], w[0][3]);
   }
-  // atomics on one address take about 20 ns each, one after another: only while the bit is missing
-  if (__any(high != 0) && (threadIdx.x & 63) == 0 && !*(volatile const uint32_t*)mask) atomicOr(mask, 1u);
+  // stores to one address take about 20 ns each, one after another: 64 words on
+  // lines of their own, and only while a word is not set
+  if (__any(high != 0) && (threadIdx.x & 63) == 0) {
+    volatile uint32_t* const word = mask + kMaskStride * (blockIdx.x % kMaskWords);
+    if (!*word) *word = 1;
+  }
 }
 
 // How a product of several rows is cut, for rows of one plane and of four: row
@@ -474,7 +482,7 @@ __device__ __forceinline__ void wit_tiles(const WitProduct& g, int32_t* sums, ui
 template <int RT, int PB, bool GATED, int W, int WR1, int WR4, class End>
 static __global__ void __launch_bounds__(64 * W) k_wit_tiles(WitProduct g, uint32_t rgroups, End end) {
   __shared__ int32_t sums[(WR1 > WR4 ? WR1 : WR4) * RT * PB * (GATED ? 2 : 1) * 1024];
-  const bool four = *g.mask != 0;
+  const bool four = wit_four(g.mask);
   const WitPlan& plan = g.plan[four ? 1 : 0];
   uint32_t rg, cg;
   if (!gemm_group(rgroups, g.cgroups, rg, cg) || rg >= plan.rgroups || blockIdx.y >= plan.splits) return;  // uniform
@@ -493,10 +501,13 @@ static __global__ void __launch_bounds__(64 * W) k_wit_tiles(WitProduct g, uint3
 // waves, two down the rows (four tiles each) by four across (two tiles, or one
 // of each matrix): 6 KB from LDS feed 8 matrix instructions of 32 cycles.
 constexpr int kBlockStage = 4;  // K steps
-template <bool GATED, bool FOUR, class End>
+// Weights of several planes: a column tile's four planes are four of the eight,
+// two to a wave, whose sums two waves bring together.
+template <int PB, bool GATED, bool FOUR, class End>
 __device__ __forceinline__ void wit_block(const WitProduct& g, v4i* lds, uint32_t rg, uint32_t cg, uint32_t split,
                                           const End& end) {
-  constexpr int NW = GATED ? 2 : 1, CT = 8 / NW;  // column tiles of a workgroup
+  constexpr int NW = GATED ? 2 : 1, CT = 8 / (NW * PB);  // column tiles of a workgroup
+  static_assert(!GATED || PB == 1, "two matrices of one plane");
   const WitPlan& plan = g.plan[FOUR ? 1 : 0];
   const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const uint32_t s0 = split * plan.steps, s1 = s0 + plan.steps < g.nsteps ? s0 + plan.steps : g.nsteps;
@@ -505,8 +516,10 @@ __device__ __forceinline__ void wit_block(const WitProduct& g, v4i* lds, uint32_
 #pragma unroll
   for (int i = 0; i < 8; i++) {  // tiles past the edges are the last one again, and not stored
     if (wave & 1) {
-      const uint32_t ct = cg * CT + i / NW, t = ct < g.ctiles ? ct : g.ctiles - 1;
-      from[i] = g.w[i % NW].planes + (uint64_t)t * g.nsteps * kGemmBlockBytes;
+      const uint32_t ct = cg * CT + i / (NW * PB), t = ct < g.ctiles ? ct : g.ctiles - 1;
+      const uint32_t q = i % PB;  // a plane that the weight does not have is zero: no pointer
+      from[i] = q && q >= g.w[0].count ? nullptr
+                                       : g.w[i % NW].planes + ((uint64_t)q * g.ctiles + t) * g.nsteps * kGemmBlockBytes;
     } else {
       const uint32_t rt = rg * 8 + i, t = rt < plan.rtiles ? rt : plan.rtiles - 1;
       from[i] = (FOUR ? g.four : g.one) + (uint64_t)t * g.nsteps * kGemmBlockBytes;
@@ -515,7 +528,8 @@ __device__ __forceinline__ void wit_block(const WitProduct& g, v4i* lds, uint32_
   v4i in[8];
   auto load = [&](int i, uint32_t s) {  // tile i of the stage from step s
     const uint32_t step = s + wave / 2, at = (step < s1 ? step : s1 - 1) * kGemmBlockBytes + 16 * lane;
-    in[i] = *(const v4i*)(from[i] + at);
+    if (PB > 1 && !from[i]) in[i] = v4i{0, 0, 0, 0};  // uniform
+    else in[i] = *(const v4i*)(from[i] + at);
   };
   auto put = [&](int i, uint32_t half) { lds[(half * 8 * kBlockStage * 2 + wave * 8 + i) * 64 + lane] = in[i]; };
   const uint32_t wr = wave & 1, wc = wave >> 1;
@@ -580,8 +594,60 @@ __device__ __forceinline__ void wit_block(const WitProduct& g, v4i* lds, uint32_
   // rows, eight elements a lane and turn.
   __syncthreads();
   constexpr uint32_t ROWS = FOUR ? 8 : 32, TI = 4 / NW;  // of a tile; tiles down the rows at a time
-  constexpr int E = 8;
   int32_t* const mine = (int32_t*)lds + wave * 4096;
+  if constexpr (PB > 1) {
+    // two row tiles at a time; of a pair of waves with the same rows and column
+    // tile, one has planes 0 and 1 of both, one 2 and 3, and each ends one
+    constexpr int E = 4;
+    const uint32_t c = lane & 31, hi = lane >> 5, odd = wc & 1;
+    const int32_t* const low = (const int32_t*)lds + (wave & ~2u) * 4096;
+    const uint64_t col0 = ((uint64_t)cg * CT + wc / 2) * 32;
+    const uint32_t bias = end.column(col0 + c, col0 + c < g.n);
+#pragma unroll
+    for (uint32_t part = 0; part < 2; part++) {
+      if (part) __syncthreads();
+#pragma unroll
+      for (uint32_t t = 0; t < 4; t++)
+#pragma unroll
+        for (int v = 0; v < 16; v++)
+          mine[t * 1024 + (8 * (v / 4) + 4 * hi + v % 4) * 32 + c] = acc[part * 2 + t / 2][t % 2][v];
+      __syncthreads();
+      const uint64_t first = (uint64_t)(rg * 8 + wr * 4 + part * 2 + odd) * ROWS * g.n + col0;
+      const typename End::Tile tile = end.tile(plan.splits == 1 ? first : 0, plan.splits == 1 ? g.m * g.n : 0);
+#pragma unroll 1
+      for (uint32_t r0 = 0; r0 < ROWS; r0 += 2 * E) {
+        uint32_t at[E], z[1][E];
+#pragma unroll
+        for (int e = 0; e < E; e++) {
+          const uint32_t r = r0 + 2 * e + hi;
+          at[e] = col0 + c < g.n ? 4 * (r * (uint32_t)g.n + c) : kOutside;
+          uint64_t sum = 0;
+#pragma unroll
+          for (int q = 0; q < PB; q++) {
+            const int32_t* const t = low + (q / 2) * (2 * 4096) + (odd * 2 + q % 2) * 1024 + c;
+            uint32_t one;
+            if constexpr (FOUR) {
+              const int32_t d[4] = {t[r * 128], t[r * 128 + 32], t[r * 128 + 64], t[r * 128 + 96]};
+              one = digit_sum_mod_p(d);
+            } else {
+              one = gemm_mod_p(t[r * 32]);
+            }
+            sum += (uint64_t)one << (8 * q);
+          }
+          z[0][e] = m31_reduce64(sum);
+        }
+        if (plan.splits == 1) {
+          typename End::template Slot<E> slot;
+          end.begin(slot, tile, at, bias, z);
+          end.finish(slot, tile, at);
+        } else {
+          wit_parts(g.part, split, first, g.m * g.n, at, z);
+        }
+      }
+    }
+    return;
+  }
+  constexpr int E = 8;
 #pragma unroll
   for (uint32_t part = 0; part < 2; part++) {
 #pragma unroll
@@ -658,17 +724,17 @@ __device__ __forceinline__ bool wit_group(uint32_t rgroups, uint32_t cgroups, ui
   cg = (uint32_t)(at / rgroups);
   return i < per_xcd && at < groups;
 }
-template <bool GATED, class End>
+template <int PB, bool GATED, class End>
 static __global__ void __launch_bounds__(512) k_wit_blocks(WitProduct g, End end) {
   __shared__ v4i lds[2 * 16 * kBlockStage * 64];
-  const bool four = *g.mask != 0;
+  const bool four = wit_four(g.mask);
   const WitPlan& plan = g.plan[four ? 1 : 0];
   uint32_t rg, cg;
   if (!wit_group(plan.rgroups, g.cgroups, rg, cg) || blockIdx.y >= plan.splits) return;  // uniform
   if (four)
-    wit_block<GATED, true>(g, lds, rg, cg, blockIdx.y, end);
+    wit_block<PB, GATED, true>(g, lds, rg, cg, blockIdx.y, end);
   else
-    wit_block<GATED, false>(g, lds, rg, cg, blockIdx.y, end);
+    wit_block<PB, GATED, false>(g, lds, rg, cg, blockIdx.y, end);
 }
 // 65 to 256 rows: rows of one plane are still a stream of the weights
 // (wit_tiles, all of the rows in a workgroup), rows of four are blocks.
@@ -676,12 +742,12 @@ template <int RT, int WR, bool GATED, class End>
 static __global__ void __launch_bounds__(512) k_wit_mixed(WitProduct g, End end) {
   __shared__ v4i lds[2 * 16 * kBlockStage * 64];
   static_assert(WR * RT * (GATED ? 2 : 1) * 4096 <= sizeof(lds), "the waves' sums");
-  const bool four = *g.mask != 0;
+  const bool four = wit_four(g.mask);
   const WitPlan& plan = g.plan[four ? 1 : 0];
   uint32_t rg, cg;
   if (!wit_group(plan.rgroups, four ? g.cgroups : g.ctiles, rg, cg) || blockIdx.y >= plan.splits) return;  // uniform
   if (four)
-    wit_block<GATED, true>(g, lds, rg, cg, blockIdx.y, end);
+    wit_block<1, GATED, true>(g, lds, rg, cg, blockIdx.y, end);
   else
     wit_tiles<RT, 1, GATED, 8, WR, false>(g, (int32_t*)lds, rg, cg, 0, end);
 }
@@ -689,7 +755,7 @@ static __global__ void __launch_bounds__(512) k_wit_mixed(WitProduct g, End end)
 // The end of a product whose K was split: a thread per element.
 template <bool GATED, class End>
 static __global__ void __launch_bounds__(256) k_wit_join(WitProduct g, End end) {
-  const uint32_t splits = g.plan[*g.mask != 0 ? 1 : 0].splits;
+  const uint32_t splits = g.plan[wit_four(g.mask) ? 1 : 0].splits;
   if (splits == 1) return;  // done where it was computed
   constexpr int NW = GATED ? 2 : 1;
   const uint64_t count = g.m * g.n;
@@ -700,6 +766,7 @@ static __global__ void __launch_bounds__(256) k_wit_join(WitProduct g, End end) 
 #pragma unroll
     for (int x = 0; x < NW; x++) {
       uint64_t t = 0;
+#pragma unroll 8
       for (uint32_t s = 0; s < splits; s++) t += g.part[(uint64_t)(s * NW + x) * count + i];
       z[x][0] = m31_reduce64(t);
     }

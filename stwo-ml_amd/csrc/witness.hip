@@ -79,6 +79,25 @@ static bool few_rows(uint64_t m, uint64_t k, uint64_t n) {
 
 static dim3 end_grid(uint64_t count);
 
+// Two masks of the packing, used in turn: the packing of one product clears the other's.
+static int wit_masks(gkr_ctx* c, uint32_t** mask, uint32_t** next_mask) {
+  constexpr uint32_t words = kMaskWords * kMaskStride;
+  if (!c->wit_mask) {
+    drain(c);
+    uint32_t* w = nullptr;
+    HIP_TRY(hipMalloc(&w, 2 * words * sizeof(uint32_t)));
+    if (hipMemsetAsync(w, 0, 2 * words * sizeof(uint32_t), c->stream) != hipSuccess) {
+      (void)hipFree(w);
+      return fail(GKR_ERR_DEVICE, "clear of the digit masks failed");
+    }
+    c->wit_mask = w;
+  }
+  *mask = c->wit_mask + (c->wit_turn & 1) * words;
+  *next_mask = c->wit_mask + (~c->wit_turn & 1) * words;
+  c->wit_turn++;
+  return GKR_OK;
+}
+
 // K splits of k_wit_blocks: a workgroup fills a CU, and a K step takes it about
 // 0.25 us, so the steps of the last, partly filled round of the 256 CUs are
 // weighed against the parts' way through memory (8 bytes an element and split
@@ -115,7 +134,7 @@ static int packed_product(gkr_ctx* c, const gkr_matrix* a, const gkr_matrix* w0,
   g.one = packed;
   g.four = packed + one_tiles * g.nsteps * kGemmBlockBytes;
   uint32_t *mask, *next_mask;
-  TRY(gemm_masks(c, &mask, &next_mask));
+  TRY(wit_masks(c, &mask, &next_mask));
   g.mask = mask;
   const uint64_t slots = four_tiles * g.nsteps * 16;
   const dim3 pack_grid((uint32_t)((slots + 255) / 256));
@@ -152,8 +171,8 @@ static int packed_product(gkr_ctx* c, const gkr_matrix* a, const gkr_matrix* w0,
     return check_launch(c);
   };
   // rows1: row tiles a workgroup has of rows of one plane that it streams the weights for; 0: blocks as for four
-  auto launch_blocks = [&](auto kernel, uint32_t rows1) -> int {
-    g.cgroups = (uint32_t)((ctiles * (GATED ? 2 : 1) + 7) / 8);
+  auto launch_blocks = [&](auto kernel, uint32_t rows1, uint32_t pb) -> int {
+    g.cgroups = (uint32_t)((ctiles * (GATED ? 2 : 1) * pb + 7) / 8);
     if (rows1) TRY(plan(0, rows1, whole));
     else TRY(plan(0, 8, split));
     TRY(plan(1, 8, split));
@@ -166,14 +185,20 @@ static int packed_product(gkr_ctx* c, const gkr_matrix* a, const gkr_matrix* w0,
   // sixteen waves a workgroup for one matrix, eight for two: the registers of
   // sixteen hold no more accumulators
   constexpr int W = GATED ? 8 : 16;
-  if (w0->bnplanes > 1 || w1->bnplanes > 1) TRY(GKR_WIT_TILES(1, 4, W, 1, 2));
+  if (w0->bnplanes > 1 || w1->bnplanes > 1) {
+    if (GATED || m <= 64) {
+      TRY(GKR_WIT_TILES(1, 4, W, 1, 2));
+    } else if constexpr (!GATED) {
+      TRY(launch_blocks(k_wit_blocks<4, false, End>, 0, 4));
+    }
+  }
   else if (m <= 8) TRY(GKR_WIT_TILES(1, 1, W, 1, 1));
   else if (m <= 16) TRY(GKR_WIT_TILES(1, 1, W, 1, 2));
   else if (m <= 32) TRY(GKR_WIT_TILES(1, 1, W, 1, 4));
   else if (m <= 64) TRY(GKR_WIT_TILES(2, 1, W, 1, 4));
-  else if (m <= 128) TRY(launch_blocks(k_wit_mixed<GATED ? 2 : 4, GATED ? 2 : 1, GATED, End>, 4));
-  else if (m <= 256) TRY(launch_blocks(k_wit_mixed<GATED ? 2 : 4, GATED ? 4 : 2, GATED, End>, 8));
-  else TRY(launch_blocks(k_wit_blocks<GATED, End>, 0));
+  else if (m <= 128) TRY(launch_blocks(k_wit_mixed<GATED ? 2 : 4, GATED ? 2 : 1, GATED, End>, 4, 1));
+  else if (m <= 256) TRY(launch_blocks(k_wit_mixed<GATED ? 2 : 4, GATED ? 4 : 2, GATED, End>, 8, 1));
+  else TRY(launch_blocks(k_wit_blocks<1, GATED, End>, 0, 1));
 #undef GKR_WIT_TILES
   if (max_splits > 1) {
     auto join = k_wit_join<GATED, End>;
