@@ -716,25 +716,28 @@ __device__ __forceinline__ void wit_block(const WitProduct& g, v4i* lds, uint32_
     }
   }
 }
-// As gemm_group, in one grid dimension over the groups that a product has.
-__device__ __forceinline__ bool wit_group(uint32_t rgroups, uint32_t cgroups, uint32_t& rg, uint32_t& cg) {
-  const uint64_t groups = (uint64_t)rgroups * cgroups, per_xcd = (groups + 7) / 8;
-  const uint64_t i = blockIdx.x >> 3, at = (blockIdx.x & 7) * per_xcd + i;
-  rg = (uint32_t)(at % rgroups);
-  cg = (uint32_t)(at / rgroups);
-  return i < per_xcd && at < groups;
+// As gemm_group, over the groups and K splits that a product has, in one grid
+// dimension: those that it does not have come last, where they wait for no one.
+__device__ __forceinline__ bool wit_group(const WitPlan& plan, uint32_t cgroups, uint32_t& rg, uint32_t& cg,
+                                          uint32_t& split) {
+  const uint32_t groups = plan.rgroups * cgroups, per_xcd = (groups + 7) / 8;
+  split = blockIdx.x / (8 * per_xcd);
+  const uint32_t x = blockIdx.x % (8 * per_xcd), at = (x & 7) * per_xcd + (x >> 3);
+  rg = at % plan.rgroups;
+  cg = at / plan.rgroups;
+  return split < plan.splits && at < groups;
 }
 template <int PB, bool GATED, class End>
 static __global__ void __launch_bounds__(512) k_wit_blocks(WitProduct g, End end) {
   __shared__ v4i lds[2 * 16 * kBlockStage * 64];
   const bool four = wit_four(g.mask);
   const WitPlan& plan = g.plan[four ? 1 : 0];
-  uint32_t rg, cg;
-  if (!wit_group(plan.rgroups, g.cgroups, rg, cg) || blockIdx.y >= plan.splits) return;  // uniform
+  uint32_t rg, cg, split;
+  if (!wit_group(plan, g.cgroups, rg, cg, split)) return;  // uniform
   if (four)
-    wit_block<PB, GATED, true>(g, lds, rg, cg, blockIdx.y, end);
+    wit_block<PB, GATED, true>(g, lds, rg, cg, split, end);
   else
-    wit_block<PB, GATED, false>(g, lds, rg, cg, blockIdx.y, end);
+    wit_block<PB, GATED, false>(g, lds, rg, cg, split, end);
 }
 // 65 to 256 rows: rows of one plane are still a stream of the weights
 // (wit_tiles, all of the rows in a workgroup), rows of four are blocks.
@@ -744,35 +747,45 @@ static __global__ void __launch_bounds__(512) k_wit_mixed(WitProduct g, End end)
   static_assert(WR * RT * (GATED ? 2 : 1) * 4096 <= sizeof(lds), "the waves' sums");
   const bool four = wit_four(g.mask);
   const WitPlan& plan = g.plan[four ? 1 : 0];
-  uint32_t rg, cg;
-  if (!wit_group(plan.rgroups, four ? g.cgroups : g.ctiles, rg, cg) || blockIdx.y >= plan.splits) return;  // uniform
+  uint32_t rg, cg, split;
+  if (!wit_group(plan, four ? g.cgroups : g.ctiles, rg, cg, split)) return;  // uniform
   if (four)
-    wit_block<1, GATED, true>(g, lds, rg, cg, blockIdx.y, end);
+    wit_block<1, GATED, true>(g, lds, rg, cg, split, end);
   else
     wit_tiles<RT, 1, GATED, 8, WR, false>(g, (int32_t*)lds, rg, cg, 0, end);
 }
 
-// The end of a product whose K was split: a thread per element.
+// The end of a product whose K was split: four elements a thread.
 template <bool GATED, class End>
 static __global__ void __launch_bounds__(256) k_wit_join(WitProduct g, End end) {
   const uint32_t splits = g.plan[wit_four(g.mask) ? 1 : 0].splits;
   if (splits == 1) return;  // done where it was computed
   constexpr int NW = GATED ? 2 : 1;
   const uint64_t count = g.m * g.n;
-  for (uint64_t first = (uint64_t)blockIdx.x * 256; first < count; first += (uint64_t)gridDim.x * 256) {
-    const uint64_t i = first + threadIdx.x < count ? first + threadIdx.x : count - 1;
-    const uint32_t at[1] = {4 * threadIdx.x}, bias = end.column(i % g.n, true);
-    uint32_t z[NW][1];
+  constexpr int E = 4;
+  for (uint64_t first = (uint64_t)blockIdx.x * (256 * E); first < count; first += (uint64_t)gridDim.x * (256 * E)) {
+    uint64_t t[NW][E] = {};
+    uint32_t at[E], z[NW][E];
 #pragma unroll
-    for (int x = 0; x < NW; x++) {
-      uint64_t t = 0;
-#pragma unroll 8
-      for (uint32_t s = 0; s < splits; s++) t += g.part[(uint64_t)(s * NW + x) * count + i];
-      z[x][0] = m31_reduce64(t);
-    }
-    typename End::template Slot<1> slot;
+    for (int e = 0; e < E; e++) at[e] = 4 * (threadIdx.x + 256 * e);
+#pragma unroll 2
+    for (uint32_t s = 0; s < splits; s++)
+#pragma unroll
+      for (int x = 0; x < NW; x++) {
+        const WitBuffer part = wit_buffer(g.part + (uint64_t)(s * NW + x) * count, first, count);
+#pragma unroll
+        for (int e = 0; e < E; e++) t[x][e] += wit_read(part, at[e]);
+      }
+#pragma unroll
+    for (int x = 0; x < NW; x++)
+#pragma unroll
+      for (int e = 0; e < E; e++) {
+        z[x][e] = m31_reduce64(t[x][e]);
+        if (x == 0) z[0][e] = m31_add(z[0][e], end.column((first + threadIdx.x + 256 * e) % g.n, true));
+      }
+    typename End::template Slot<E> slot;
     const typename End::Tile tile = end.tile(first, count);
-    end.begin(slot, tile, at, bias, z);
+    end.begin(slot, tile, at, 0, z);
     end.finish(slot, tile, at);
   }
 }

@@ -98,19 +98,28 @@ static int wit_masks(gkr_ctx* c, uint32_t** mask, uint32_t** next_mask) {
   return GKR_OK;
 }
 
-// K splits of k_wit_blocks: a workgroup fills a CU, and a K step takes it about
-// 0.25 us, so the steps of the last, partly filled round of the 256 CUs are
-// weighed against the parts' way through memory (8 bytes an element and split
-// at 4 TB/s, and 5 us for the joining launch).
-static uint32_t block_splits(uint64_t groups, uint32_t nsteps, uint64_t elements) {
-  uint32_t best = 1;
-  double best_us = 0;
+// What the two kinds of kernel take, in us, to choose between them; fitted to 27
+// products of 40 to 512 rows, k 100 to 13824, n 900 to 13824, rows and weights
+// of one plane and of four, which each kind took 10 to 330 us for: within a
+// quarter, and the better one taken in all but two (by 1.1 and 1.2 times).
+// k_wit_tiles: 8 us for each round of the workgroups that fit at once (`slots`),
+// and the operands' way from the second-level cache, 17 GB/ms; kb is a
+// workgroup's K step.
+static double tiles_us(uint64_t groups, uint32_t slots, uint32_t nsteps, uint32_t kb) {
+  return 8.0 * (double)((groups + slots - 1) / slots) + (double)groups * nsteps * kb / 17000.0;
+}
+// k_wit_blocks: a workgroup fills a CU; a K step takes it 0.27 us where few run
+// and 0.5 on all 256 (the matrix cores slow down).  K splits fill the last
+// round, against the parts' way through memory and a launch to join them.
+static double blocks_us(uint64_t groups, uint32_t nsteps, uint64_t elements, uint32_t* splits) {
+  double best = 0;
   for (uint32_t s = 1; s <= 16 && (s == 1 || nsteps / s >= 16); s++) {
     const uint64_t rounds = (groups * s + 255) / 256, steps = (nsteps + s - 1) / s;
-    const double us = 0.25 * (double)(rounds * (steps + 8)) + (s > 1 ? 5.0 + (double)s * (double)elements * 2e-6 : 0.0);
-    if (s == 1 || us < best_us) {
-      best = s;
-      best_us = us;
+    const double step = 0.27 + 0.23 * std::min(1.0, (double)(groups * s) / 256);
+    const double us = 12.0 + step * (double)(rounds * steps) + (s > 1 ? 5.0 + (double)s * (double)elements * 2e-6 : 0.0);
+    if (s == 1 || us < best) {
+      best = us;
+      *splits = s;
     }
   }
   return best;
@@ -146,12 +155,12 @@ static int packed_product(gkr_ctx* c, const gkr_matrix* a, const gkr_matrix* w0,
 
   uint32_t max_splits = 1, max_rgroups = 1;
   // group: row tiles of a workgroup, for rows of one plane and of four
-  auto plan = [&](int four, uint32_t group, auto splits_of) -> int {
+  auto plan = [&](int four, uint32_t group, uint32_t splits) -> int {
     const uint64_t tiles = four ? four_tiles : one_tiles;
     WitPlan& p = g.plan[four];
     p.rtiles = (uint32_t)tiles;
     p.rgroups = (uint32_t)((tiles + group - 1) / group);
-    p.splits = splits_of((uint64_t)p.rgroups * g.cgroups);
+    p.splits = splits;
     p.steps = (g.nsteps + p.splits - 1) / p.splits;
     p.splits = (g.nsteps + p.steps - 1) / p.steps;
     max_splits = std::max(max_splits, p.splits);
@@ -159,46 +168,62 @@ static int packed_product(gkr_ctx* c, const gkr_matrix* a, const gkr_matrix* w0,
     if (p.splits > 1) TRY(ensureT(c, S_GEMMP, (uint64_t)max_splits * (GATED ? 2 : 1) * m * n, &g.part));
     return GKR_OK;
   };
-  const auto whole = [](uint64_t) { return 1u; };
-  const auto split = [&](uint64_t groups) { return block_splits(groups, g.nsteps, m * n * (GATED ? 2 : 1)); };
   auto launch_tiles = [&](auto kernel, uint32_t rt, uint32_t waves, uint32_t wr1, uint32_t wr4) -> int {
     g.cgroups = g.ctiles;
-    TRY(plan(0, rt * wr1, whole));
-    TRY(plan(1, rt * wr4, whole));
+    TRY(plan(0, rt * wr1, 1));
+    TRY(plan(1, rt * wr4, 1));
     uint32_t rg;
-    const dim3 grid = gemm_group_grid(max_rgroups, g.cgroups, max_splits, &rg, kGemmMaxGroups / 4);
+    const dim3 grid = gemm_group_grid(max_rgroups, g.cgroups, 1, &rg, kGemmMaxGroups / 4);
     GKR_LAUNCH(c, kernel, grid, dim3(64 * waves), 0, g, rg, end);
     return check_launch(c);
   };
+  // the block kernels' column groups, and what they take (splits[]) for rows of one plane and of four
+  constexpr uint32_t NW = GATED ? 2 : 1;
+  const bool general = w0->bnplanes > 1 || w1->bnplanes > 1;
+  const uint64_t bgroups = (ctiles * NW * (general ? 4 : 1) + 7) / 8, elements = m * n * NW;
+  uint32_t splits[2] = {1, 1};
+  const double blocks[2] = {blocks_us((one_tiles + 7) / 8 * bgroups, g.nsteps, elements, &splits[0]),
+                            blocks_us((four_tiles + 7) / 8 * bgroups, g.nsteps, elements, &splits[1])};
   // rows1: row tiles a workgroup has of rows of one plane that it streams the weights for; 0: blocks as for four
-  auto launch_blocks = [&](auto kernel, uint32_t rows1, uint32_t pb) -> int {
-    g.cgroups = (uint32_t)((ctiles * (GATED ? 2 : 1) * pb + 7) / 8);
-    if (rows1) TRY(plan(0, rows1, whole));
-    else TRY(plan(0, 8, split));
-    TRY(plan(1, 8, split));
-    const uint64_t groups = std::max((uint64_t)g.plan[0].rgroups * (rows1 ? g.ctiles : g.cgroups),
-                                     (uint64_t)g.plan[1].rgroups * g.cgroups);
-    GKR_LAUNCH(c, kernel, dim3((uint32_t)((groups + 7) / 8 * 8), max_splits), dim3(512), 0, g, end);
+  auto launch_blocks = [&](auto kernel, uint32_t rows1) -> int {
+    g.cgroups = (uint32_t)bgroups;
+    TRY(plan(0, rows1 ? rows1 : 8, rows1 ? 1 : splits[0]));
+    TRY(plan(1, 8, splits[1]));
+    uint64_t grid = 0;
+    for (int i = 0; i < 2; i++) {
+      const uint64_t groups = (uint64_t)g.plan[i].rgroups * (i == 0 && rows1 ? g.ctiles : g.cgroups);
+      grid = std::max(grid, (groups + 7) / 8 * 8 * g.plan[i].splits);
+    }
+    GKR_LAUNCH(c, kernel, dim3((uint32_t)grid), dim3(512), 0, g, end);
     return check_launch(c);
   };
 #define GKR_WIT_TILES(RT, PB, W, WR1, WR4) launch_tiles(k_wit_tiles<RT, PB, GATED, W, WR1, WR4, End>, RT, W, WR1, WR4)
   // sixteen waves a workgroup for one matrix, eight for two: the registers of
   // sixteen hold no more accumulators
   constexpr int W = GATED ? 8 : 16;
-  if (w0->bnplanes > 1 || w1->bnplanes > 1) {
-    if (GATED || m <= 64) {
+  if (general) {
+    const double tiles = tiles_us(one_tiles * ctiles, 256, g.nsteps, 1 + 4 * NW) +
+                         tiles_us((four_tiles + 1) / 2 * ctiles, 256, g.nsteps, 2 * (1 + 4 * NW));
+    if (GATED || tiles <= blocks[0] + blocks[1]) {
       TRY(GKR_WIT_TILES(1, 4, W, 1, 2));
     } else if constexpr (!GATED) {
-      TRY(launch_blocks(k_wit_blocks<4, false, End>, 0, 4));
+      TRY(launch_blocks(k_wit_blocks<4, false, End>, 0));
     }
-  }
-  else if (m <= 8) TRY(GKR_WIT_TILES(1, 1, W, 1, 1));
+  } else if (m <= 8) TRY(GKR_WIT_TILES(1, 1, W, 1, 1));
   else if (m <= 16) TRY(GKR_WIT_TILES(1, 1, W, 1, 2));
   else if (m <= 32) TRY(GKR_WIT_TILES(1, 1, W, 1, 4));
   else if (m <= 64) TRY(GKR_WIT_TILES(2, 1, W, 1, 4));
-  else if (m <= 128) TRY(launch_blocks(k_wit_mixed<GATED ? 2 : 4, GATED ? 2 : 1, GATED, End>, 4, 1));
-  else if (m <= 256) TRY(launch_blocks(k_wit_mixed<GATED ? 2 : 4, GATED ? 4 : 2, GATED, End>, 8, 1));
-  else TRY(launch_blocks(k_wit_blocks<1, GATED, End>, 0, 1));
+  else {
+    const uint64_t rows64 = (m + 63) / 64;
+    const double tiles = tiles_us(rows64 * ctiles, 512, g.nsteps, 2 + NW) + tiles_us(rows64 * ctiles, 512, g.nsteps, 4 * (2 + NW));
+    constexpr uint32_t RT = GATED ? 2 : 4, WR = GATED ? 2 : 1;
+    const uint32_t down = m <= 128 ? WR : 2 * WR;  // waves down the rows of k_wit_mixed
+    const double mixed = m <= 256 ? tiles_us(ctiles, 256, g.nsteps, down * (RT + NW)) + blocks[1] : 1e30;
+    if (tiles <= std::min(mixed, blocks[0] + blocks[1])) TRY(GKR_WIT_TILES(2, 1, W, 1, 4));
+    else if (mixed > blocks[0] + blocks[1]) TRY(launch_blocks(k_wit_blocks<1, GATED, End>, 0));
+    else if (m <= 128) TRY(launch_blocks(k_wit_mixed<RT, WR, GATED, End>, RT * WR));
+    else TRY(launch_blocks(k_wit_mixed<RT, 2 * WR, GATED, End>, 2 * RT * WR));
+  }
 #undef GKR_WIT_TILES
   if (max_splits > 1) {
     auto join = k_wit_join<GATED, End>;
