@@ -17,6 +17,12 @@ def product(a, b):
     """A B mod P: bytes of A by 16-bit halves of B, every partial sum below 2^53."""
     a, b = a.astype(np.int64), b.astype(np.int64)
     out = np.zeros((a.shape[0], b.shape[1]), np.int64)
+    if np.all((b < 128) | (b >= P - 128)):  # int8-range B as signed numbers, 16-bit halves of A
+        c = np.where(b > P // 2, b - P, b).astype(np.float64)
+        for i in range(2):
+            s = ((a >> (16 * i)) & 0xFFFF).astype(np.float64) @ c
+            out = (out + s.astype(np.int64) % P * pow(2, 16 * i, P)) % P
+        return out
     for i in range(4):
         for j in range(2):
             s = ((a >> (8 * i)) & 255).astype(np.float64) @ ((b >> (16 * j)) & 0xFFFF).astype(np.float64)
@@ -106,6 +112,28 @@ def test_wide(gpu_ctx, m, k, n):
     for xk in (1, 0):
         check_fused(gpu_ctx, m, k, n, xk, 1, 0)
         check_gated(gpu_ctx, m, k, n, xk, 1)
+
+
+# more than 64 rows and enough work for blocks of 8 x 8 tiles, for all rows streamed through one workgroup
+# where they have one plane, and for K splits; ragged edges, and K steps that end inside a stage of four
+@pytest.mark.parametrize("m,k,n", [(100, 5121, 5101), (200, 2605, 5101), (130, 1130, 5131), (260, 500, 4099),
+                                   (513, 2001, 2003), (300, 100, 9001)])
+def test_blocks(gpu_ctx, m, k, n):
+    for xk in (1, 0):
+        check_fused(gpu_ctx, m, k, n, xk, 1, GELU)
+        check_gated(gpu_ctx, m, k, n, xk, 1)
+
+
+@pytest.mark.parametrize("m,k,n", [(100, 2605, 3001), (130, 500, 5131), (300, 100, 4099), (513, 801, 2003)])
+def test_blocks_of_general_weights(gpu_ctx, m, k, n):
+    for xk in (1, 0):
+        check_fused(gpu_ctx, m, k, n, xk, 0, SILU)
+    rng = np.random.default_rng(m)
+    for bits in (12, 20):  # two and three planes
+        A, B = words(rng, (m, k), 0), rng.integers(0, 1 << bits, size=(k, n), dtype=np.uint32)
+        out = gpu_ctx.zeros(m, n)
+        gpu_ctx.matmul_forward_fused(gpu_ctx.upload(A), gpu_ctx.upload(B), out)
+        assert np.array_equal(out.download(), product(A, B))
 
 
 @pytest.mark.parametrize("m,k", [(1, 40000), (8, 9000), (64, 9000), (260, 5000)])
