@@ -46,9 +46,10 @@ __device__ __forceinline__ void wit_write(WitBuffer b, uint32_t at, uint32_t x) 
 }
 
 // What happens to a sum of the product (fused) or a pair of sums (gated), for E
-// elements (byte offsets `at` into the Tile) of a thread.  begin() takes the
-// sums and sends the loads out that they need, finish() stores, so that the next
-// elements' loads can go out before these ones' stores.  `bias`: the column's.
+// elements (byte offsets `at` into the Tile) of a thread.  fetch() sends out the
+// loads that need no sums, begin() takes the sums and sends out those that do,
+// finish() stores, so that the next elements' loads can go out before these
+// ones' stores.  `bias`: the column's.
 struct FusedEnd {
   ActArg act;
   const uint32_t* bias;      // n
@@ -67,12 +68,14 @@ struct FusedEnd {
   }
   __device__ __forceinline__ uint32_t column(uint64_t col, bool ok) const { return bias && ok ? bias[col] : 0u; }
   template <int E>
-  __device__ __forceinline__ void begin(Slot<E>& s, const Tile& t, const uint32_t (&at)[E], uint32_t b,
-                                        const uint32_t (&z)[1][E]) const {
+  __device__ __forceinline__ void fetch(Slot<E>& s, const Tile& t, const uint32_t (&at)[E]) const {
     if (residual) {
 #pragma unroll
       for (int e = 0; e < E; e++) s.residual[e] = wit_read(t.residual, at[e]);
     }
+  }
+  template <int E>
+  __device__ __forceinline__ void begin(Slot<E>& s, uint32_t b, const uint32_t (&z)[1][E]) const {
 #pragma unroll
     for (int e = 0; e < E; e++) s.y[e] = s.z[e] = m31_add(z[0][e], b);
     activate(act, s.y);
@@ -107,8 +110,9 @@ struct GatedEnd {
   }
   __device__ __forceinline__ uint32_t column(uint64_t, bool) const { return 0; }
   template <int E>
-  __device__ __forceinline__ void begin(Slot<E>& s, const Tile&, const uint32_t (&)[E], uint32_t,
-                                        const uint32_t (&z)[2][E]) const {
+  __device__ __forceinline__ void fetch(Slot<E>&, const Tile&, const uint32_t (&)[E]) const {}
+  template <int E>
+  __device__ __forceinline__ void begin(Slot<E>& s, uint32_t, const uint32_t (&z)[2][E]) const {
 #pragma unroll
     for (int e = 0; e < E; e++) {
       s.y[e] = s.z[e] = z[0][e];
@@ -158,27 +162,28 @@ __device__ __forceinline__ uint32_t digit_sum_mod_p(const int32_t (&s)[4]) {
   return m31_reduce64((uint64_t)(t + ((int64_t)P << 26)));
 }
 
-// One to four rows.  The rows' digit planes are rows of one product: row' 4 i
-// + p of the 16 that v_mfma_i32_16x16x64_i8 takes is plane p of row i, so
-// general words cost no more than int8-range ones, and lane 16 i + c of the
-// accumulator holds the four digit sums of row i, column c.
+// Few rows.  The rows' digit planes are rows of one product: row' 4 i + p is
+// plane p of row i, 16 of them to a v_mfma_i32_16x16x64_i8, so general words cost
+// no more than int8-range ones, and lane 16 j + c of the accumulator of tile t
+// holds the four digit sums of row 4 t + j, column c.
 //
 // A workgroup has 32 columns of the weights and all of K: it lays the rows'
-// digits out in LDS (kRowLds bytes at a time) and its waves take K pairs of 32
-// in turn, a pair's 2 KB per plane in two loads, U pairs in flight; then the
-// waves' sums meet in LDS (integers: any order gives the same).  No packing
-// launch, no partial sums in memory: bound by the weights' bytes (packing, the
-// product, its splits' sum and the epilogue as launches of their own, then
-// this: 1 x 576 x 192 11.4 -> 4.7 us, 1 x 13824 x 5120 39.1 -> 16.2, 4.4 TB/s;
-// gated 1 x 5120 x 13824 47.0 -> 28.7, 4.9 TB/s, where a copy reaches 4.8).
+// digits out in LDS (one to four rows kRowLds bytes at a time, more rows at
+// once) and its waves take K pairs of 32 in turn, a pair's 2 KB per plane in two
+// loads, U pairs in flight; then the waves' sums meet in LDS (integers: any
+// order gives the same).  No packing launch, no partial sums in memory: bound by
+// the weights' bytes (packing, the product, its splits' sum and the epilogue as
+// launches of their own, then this: 1 x 576 x 192 11.4 -> 4.7 us, 1 x 13824 x
+// 5120 39.1 -> 16.2, 4.4 TB/s; gated 1 x 5120 x 13824 47.0 -> 28.7, 4.9 TB/s,
+// where a copy reaches 4.8).
 constexpr uint32_t kRowWaves = 16;
 constexpr uint32_t kRowLds = 65536;
 template <int MR, int PB, bool GATED, class End>
 static __global__ void __launch_bounds__(64 * kRowWaves) k_rows(const uint32_t* __restrict__ X, WitWeight w0, WitWeight w1,
                                                                 uint32_t m, uint32_t k, uint32_t n, End end) {
-  constexpr int NW = GATED ? 2 : 1, U = PB == 1 ? 4 : 1;
+  constexpr int NW = GATED ? 2 : 1, RT = MR <= 4 ? 1 : MR / 4, U = PB > 1 ? 1 : MR > 4 ? 2 : 4;
   constexpr uint32_t kChunk = kRowLds / (4 * MR);  // K per LDS fill
-  static_assert(kChunk / 64 % (kRowWaves * U) == 0, "a fill ends where the loads in flight start over");
+  static_assert(MR > 4 || kChunk / 64 % (kRowWaves * U) == 0, "a fill ends where the loads in flight start over");
   extern __shared__ __align__(16) int8_t digits[];  // [K / 16][4 MR][16]
   __shared__ int32_t sums[NW][PB][MR][4][32];
   const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6, ct = blockIdx.x;
@@ -204,13 +209,15 @@ static __global__ void __launch_bounds__(64 * kRowWaves) k_rows(const uint32_t* 
 #pragma unroll
   for (int u = 0; u < U; u++) load(u, wave + u * kRowWaves);
   for (uint32_t i = threadIdx.x; i < NW * PB * MR * 128; i += blockDim.x) (&sums[0][0][0][0][0])[i] = 0;
-  v4i acc[NW][PB][2];
+  v4i acc[NW][PB][2][RT];
 #pragma unroll
   for (int i = 0; i < NW; i++)
 #pragma unroll
     for (int q = 0; q < PB; q++)
 #pragma unroll
-      for (int h = 0; h < 2; h++) acc[i][q][h] = v4i{0, 0, 0, 0};
+      for (int h = 0; h < 2; h++)
+#pragma unroll
+        for (int t = 0; t < RT; t++) acc[i][q][h][t] = v4i{0, 0, 0, 0};
   uint32_t pair = wave;
   for (uint32_t k0 = 0; k0 < k; k0 += kChunk) {
     const uint32_t left = k - k0 < kChunk ? k - k0 : kChunk, fill = (left + 63) / 64 * 64;
@@ -232,7 +239,10 @@ static __global__ void __launch_bounds__(64 * kRowWaves) k_rows(const uint32_t* 
 #pragma unroll
       for (int u = 0; u < U; u++) {
         if (pair < pair1) {  // uniform in the wave
-          const v4i a = *(const v4i*)(digits + ((4 * (pair - pair0) + quarter) * (4 * MR) + col % (4 * MR)) * 16);
+          v4i a[RT];
+#pragma unroll
+          for (int t = 0; t < RT; t++)
+            a[t] = *(const v4i*)(digits + ((4 * (pair - pair0) + quarter) * (4 * MR) + (16 * t + col) % (4 * MR)) * 16);
 #pragma unroll
           for (int i = 0; i < NW; i++)
 #pragma unroll
@@ -240,7 +250,9 @@ static __global__ void __launch_bounds__(64 * kRowWaves) k_rows(const uint32_t* 
               if (q == 0 || q < (int)w[i].count) {
 #pragma unroll
                 for (int h = 0; h < 2; h++)
-                  acc[i][q][h] = __builtin_amdgcn_mfma_i32_16x16x64_i8(a, b[u][i][q][h], acc[i][q][h], 0, 0, 0);
+#pragma unroll
+                  for (int t = 0; t < RT; t++)
+                    acc[i][q][h][t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(a[t], b[u][i][q][h], acc[i][q][h][t], 0, 0, 0);
               }
           load(u, pair + U * kRowWaves);
           pair += kRowWaves;
@@ -248,20 +260,27 @@ static __global__ void __launch_bounds__(64 * kRowWaves) k_rows(const uint32_t* 
       }
     }
   }
-  if (quarter < MR) {
 #pragma unroll
-    for (int i = 0; i < NW; i++)
+  for (int t = 0; t < RT; t++) {
+    const uint32_t row = 4 * t + quarter;
+    if (row < MR) {
 #pragma unroll
-      for (int q = 0; q < PB; q++)
+      for (int i = 0; i < NW; i++)
 #pragma unroll
-        for (int h = 0; h < 2; h++)
+        for (int q = 0; q < PB; q++)
 #pragma unroll
-          for (int v = 0; v < 4; v++) atomicAdd(&sums[i][q][quarter][v][16 * h + col], acc[i][q][h][v]);
+          for (int h = 0; h < 2; h++)
+#pragma unroll
+            for (int v = 0; v < 4; v++) atomicAdd(&sums[i][q][row][v][16 * h + col], acc[i][q][h][t][v]);
+    }
   }
   const uint32_t r = threadIdx.x / 32, c = threadIdx.x % 32, column = ct * kGemmTile + c;
   const bool ok = r < m && column < n;
-  const uint32_t at[1] = {4 * (r * n + column)};  // below 2^32: four rows of at most 2^26 words
+  const uint32_t at[1] = {4 * (r * n + column)};  // below 2^32: sixteen rows of at most 2^26 words
   const uint32_t bias = end.column(column, ok);
+  typename End::template Slot<1> slot;
+  const typename End::Tile tile = end.tile(0, (uint64_t)m * n);
+  if (ok) end.fetch(slot, tile, at);
   __syncthreads();
   if (!ok) return;
   uint32_t z[NW][1];
@@ -275,9 +294,7 @@ static __global__ void __launch_bounds__(64 * kRowWaves) k_rows(const uint32_t* 
     }
     z[i][0] = m31_reduce64(t);
   }
-  typename End::template Slot<1> slot;
-  const typename End::Tile tile = end.tile(0, (uint64_t)m * n);
-  end.begin(slot, tile, at, bias, z);
+  end.begin(slot, bias, z);
   end.finish(slot, tile, at);
 }
 
@@ -362,7 +379,7 @@ template <int RT, int PB, bool GATED, int W, int WR, bool FOUR, class End>
 __device__ __forceinline__ void wit_tiles(const WitProduct& g, int32_t* sums, uint32_t rg, uint32_t cg, uint32_t split,
                                           const End& end) {
   constexpr int NW = GATED ? 2 : 1, NB = NW * PB, WK = W / WR, TILES = WR * RT;
-  constexpr int U = W == 16 ? (RT + NB <= 2 ? 6 : RT + NB <= 3 ? 4 : 2) : (RT + NB <= 3 ? 6 : RT + NB <= 4 ? 3 : 2);
+  constexpr int U = W == 16 ? (RT + NB <= 2 ? 8 : RT + NB <= 3 ? 6 : 2) : (RT + NB <= 3 ? 6 : RT + NB <= 4 ? 3 : 2);
   const WitPlan& plan = g.plan[FOUR ? 1 : 0];
   const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const uint32_t wr = wave % WR, wk = wave / WR;
@@ -435,6 +452,9 @@ __device__ __forceinline__ void wit_tiles(const WitProduct& g, int32_t* sums, ui
     at[e] = rows[e] < TILES * ROWS && col < g.n ? 4 * (rows[e] * (uint32_t)g.n + c) : kOutside;
   }
   const uint32_t bias = end.column(col, col < g.n);
+  typename End::template Slot<E> slot;
+  const typename End::Tile tile = end.tile(first, plan.splits == 1 ? g.m * g.n : 0);
+  end.fetch(slot, tile, at);
   __syncthreads();
 #pragma unroll
   for (int i = 0; i < RT; i++)
@@ -471,9 +491,7 @@ __device__ __forceinline__ void wit_tiles(const WitProduct& g, int32_t* sums, ui
     }
   }
   if (plan.splits == 1) {
-    typename End::template Slot<E> slot;
-    const typename End::Tile tile = end.tile(first, g.m * g.n);
-    end.begin(slot, tile, at, bias, z);
+    end.begin(slot, bias, z);
     end.finish(slot, tile, at);
   } else {
     wit_parts(g.part, split, first, g.m * g.n, at, z);
@@ -638,7 +656,8 @@ __device__ __forceinline__ void wit_block(const WitProduct& g, v4i* lds, uint32_
         }
         if (plan.splits == 1) {
           typename End::template Slot<E> slot;
-          end.begin(slot, tile, at, bias, z);
+          end.fetch(slot, tile, at);
+          end.begin(slot, bias, z);
           end.finish(slot, tile, at);
         } else {
           wit_parts(g.part, split, first, g.m * g.n, at, z);
@@ -688,8 +707,9 @@ __device__ __forceinline__ void wit_block(const WitProduct& g, v4i* lds, uint32_
       auto begin = [&](int i, uint32_t r0) {
         uint32_t at[E], z[NW][E];
         places(r0, at);
+        end.fetch(slot[i], tile, at);
         values(r0, z);
-        end.begin(slot[i], tile, at, bias, z);
+        end.begin(slot[i], bias, z);
       };
       auto finish = [&](int i, uint32_t r0) {
         uint32_t at[E];
@@ -785,7 +805,8 @@ static __global__ void __launch_bounds__(256) k_wit_join(WitProduct g, End end) 
       }
     typename End::template Slot<E> slot;
     const typename End::Tile tile = end.tile(first, count);
-    end.begin(slot, tile, at, 0, z);
+    end.fetch(slot, tile, at);
+    end.begin(slot, 0, z);
     end.finish(slot, tile, at);
   }
 }
@@ -802,7 +823,8 @@ static __global__ void __launch_bounds__(256) k_wit_end(const uint32_t* __restri
     if constexpr (GATED) z[1][0] = z1[i];
     typename End::template Slot<1> slot;
     const typename End::Tile tile = end.tile(first, count);
-    end.begin(slot, tile, at, bias, z);
+    end.fetch(slot, tile, at);
+    end.begin(slot, bias, z);
     end.finish(slot, tile, at);
   }
 }

@@ -55,7 +55,8 @@ constexpr uint64_t kMaxInner = 131071;
 
 static WitWeight wit_weight(const gkr_matrix* w) { return WitWeight{w->bplanes, (uint32_t)w->bnplanes}; }
 
-// One to four rows (k_rows).
+static dim3 end_grid(uint64_t count) { return dim3((uint32_t)std::min<uint64_t>((count + 255) / 256, 1u << 20)); }
+// Few rows (k_rows).
 template <bool GATED, class End>
 static int rows_product(gkr_ctx* c, const gkr_matrix* a, const gkr_matrix* w0, const gkr_matrix* w1, const End& end) {
   const uint32_t m = (uint32_t)a->rows, k = (uint32_t)a->cols;
@@ -68,16 +69,20 @@ static int rows_product(gkr_ctx* c, const gkr_matrix* a, const gkr_matrix* w0, c
   };
   if (m == 1) one ? launch(k_rows<1, 1, GATED, End>, 1) : launch(k_rows<1, 4, GATED, End>, 1);
   else if (m == 2) one ? launch(k_rows<2, 1, GATED, End>, 2) : launch(k_rows<2, 4, GATED, End>, 2);
-  else one ? launch(k_rows<4, 1, GATED, End>, 4) : launch(k_rows<4, 4, GATED, End>, 4);
+  else if (m <= 4) one ? launch(k_rows<4, 1, GATED, End>, 4) : launch(k_rows<4, 4, GATED, End>, 4);
+  else if (m <= 8) launch(k_rows<8, 1, GATED, End>, 8);
+  else launch(k_rows<16, 1, GATED, End>, 16);
   return check_launch(c);
 }
-// A grid of kernels with 1024 threads takes this many column tiles.
-constexpr uint64_t kRowMaxTiles = 1ull << 21;
-static bool few_rows(uint64_t m, uint64_t k, uint64_t n) {
-  return m <= 4 && k <= kMaxInner && n <= kRowMaxTiles * kGemmTile;
+// Whether k_rows takes it: up to four rows; five to sixteen by weights of one
+// plane while their digits fit in LDS at once (every workgroup makes them
+// again, which takes it longer beyond than a launch that packs them).
+static bool few_rows(const gkr_matrix* a, const gkr_matrix* w0, const gkr_matrix* w1) {
+  const uint64_t m = a->rows, k = a->cols;
+  if (k > kMaxInner || w0->cols > 1ull << 26) return false;
+  if (m <= 4) return true;
+  return m <= 16 && w0->bnplanes == 1 && w1->bnplanes == 1 && (m <= 8 ? 8 : 16) * 4 * ((k + 63) / 64 * 64) <= kRowLds;
 }
-
-static dim3 end_grid(uint64_t count);
 
 // Two masks of the packing, used in turn: the packing of one product clears the other's.
 static int wit_masks(gkr_ctx* c, uint32_t** mask, uint32_t** next_mask) {
@@ -239,7 +244,6 @@ static bool packable(uint64_t m, uint64_t k, uint64_t n) {
          (m / 64 + 1) * (n / 128 + 1) <= 1ull << 22;
 }
 
-static dim3 end_grid(uint64_t count) { return dim3((uint32_t)std::min<uint64_t>((count + 255) / 256, 1u << 20)); }
 
 extern "C" int gkr_matmul_forward_fused(gkr_ctx* c, const gkr_matrix* a, const gkr_matrix* b, const gkr_matrix* bias,
                                         uint32_t tag, uint32_t table_log, const gkr_matrix* residual, gkr_matrix* pre,
@@ -269,7 +273,7 @@ extern "C" int gkr_matmul_forward_fused(gkr_ctx* c, const gkr_matrix* a, const g
   TRY(drop_derived(c, out));
   if (pre) TRY(drop_derived(c, pre));
   TRY(weight_planes(c, const_cast<gkr_matrix*>(b)));
-  if (few_rows(m, a->cols, n)) return rows_product<false>(c, a, b, b, e);
+  if (few_rows(a, b, b)) return rows_product<false>(c, a, b, b, e);
   if (packable(m, a->cols, n)) return packed_product<false>(c, a, b, b, e);
   uint32_t* z;
   TRY(ensureT(c, S_WITG, m * n, &z));
@@ -305,7 +309,7 @@ extern "C" int gkr_gated_forward(gkr_ctx* c, const gkr_matrix* a, const gkr_matr
     if (w) TRY(drop_derived(c, w));
   TRY(weight_planes(c, const_cast<gkr_matrix*>(wg)));
   TRY(weight_planes(c, const_cast<gkr_matrix*>(wu)));
-  if (few_rows(m, a->cols, n)) return rows_product<true>(c, a, wg, wu, e);
+  if (few_rows(a, wg, wu)) return rows_product<true>(c, a, wg, wu, e);
   if (packable(m, a->cols, n)) return packed_product<true>(c, a, wg, wu, e);
   uint32_t *g, *u;
   TRY(ensureT(c, S_WITG, m * n, &g));
