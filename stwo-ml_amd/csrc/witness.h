@@ -235,30 +235,38 @@ static __global__ void __launch_bounds__(64 * kRowWaves) k_rows(const uint32_t* 
     }
     __syncthreads();
     const uint32_t pair0 = k0 / 64, pair1 = pair0 + fill / 64;
-    while (pair < pair1) {
+    auto multiply = [&](int u) {
+      v4i a[RT];
+#pragma unroll
+      for (int t = 0; t < RT; t++)
+        a[t] = *(const v4i*)(digits + ((4 * (pair - pair0) + quarter) * (4 * MR) + (16 * t + col) % (4 * MR)) * 16);
+#pragma unroll
+      for (int i = 0; i < NW; i++)
+#pragma unroll
+        for (int q = 0; q < PB; q++)
+          if (q == 0 || q < (int)w[i].count) {
+#pragma unroll
+            for (int h = 0; h < 2; h++)
+#pragma unroll
+              for (int t = 0; t < RT; t++)
+                acc[i][q][h][t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(a[t], b[u][i][q][h], acc[i][q][h][t], 0, 0, 0);
+          }
+    };
+    // U pairs at a time without a branch between: with one, a wait for any load would be for all
+    while (pair + (U - 1) * kRowWaves < pair1) {
 #pragma unroll
       for (int u = 0; u < U; u++) {
-        if (pair < pair1) {  // uniform in the wave
-          v4i a[RT];
-#pragma unroll
-          for (int t = 0; t < RT; t++)
-            a[t] = *(const v4i*)(digits + ((4 * (pair - pair0) + quarter) * (4 * MR) + (16 * t + col) % (4 * MR)) * 16);
-#pragma unroll
-          for (int i = 0; i < NW; i++)
-#pragma unroll
-            for (int q = 0; q < PB; q++)
-              if (q == 0 || q < (int)w[i].count) {
-#pragma unroll
-                for (int h = 0; h < 2; h++)
-#pragma unroll
-                  for (int t = 0; t < RT; t++)
-                    acc[i][q][h][t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(a[t], b[u][i][q][h], acc[i][q][h][t], 0, 0, 0);
-              }
-          load(u, pair + U * kRowWaves);
-          pair += kRowWaves;
-        }
+        multiply(u);
+        load(u, pair + U * kRowWaves);
+        pair += kRowWaves;
       }
     }
+#pragma unroll
+    for (int u = 0; u < U - 1; u++)
+      if (pair < pair1) {  // the last pairs of all: their loads are out
+        multiply(u);
+        pair += kRowWaves;
+      }
   }
 #pragma unroll
   for (int t = 0; t < RT; t++) {
@@ -421,24 +429,30 @@ __device__ __forceinline__ void wit_tiles(const WitProduct& g, int32_t* sums, ui
       for (int q = 0; q < PB; q++)
 #pragma unroll
         for (int v = 0; v < 16; v++) acc[i][x][q][v] = 0;
+  auto multiply = [&](int u) {
+#pragma unroll
+    for (int x = 0; x < NW; x++)
+#pragma unroll
+      for (int q = 0; q < PB; q++)
+        if (q == 0 || q < (int)g.w[x].count) {
+#pragma unroll
+          for (int i = 0; i < RT; i++)
+            acc[i][x][q] = __builtin_amdgcn_mfma_i32_32x32x32_i8(a[u][i], b[u][x][q], acc[i][x][q], 0, 0, 0);
+        }
+  };
+  uint32_t s = s0 + wk;
+  // U steps at a time without a branch between: with one, a wait for any load would be for all
 #pragma unroll 1
-  for (uint32_t s = s0 + wk; s < s1; s += U * WK) {
+  for (; s + (U - 1) * WK < s1; s += U * WK) {
 #pragma unroll
     for (int u = 0; u < U; u++) {
-      if (s + u * WK < s1) {  // uniform
-#pragma unroll
-        for (int x = 0; x < NW; x++)
-#pragma unroll
-          for (int q = 0; q < PB; q++)
-            if (q == 0 || q < (int)g.w[x].count) {
-#pragma unroll
-              for (int i = 0; i < RT; i++)
-                acc[i][x][q] = __builtin_amdgcn_mfma_i32_32x32x32_i8(a[u][i], b[u][x][q], acc[i][x][q], 0, 0, 0);
-            }
-        load(u, s + (u + U) * WK);
-      }
+      multiply(u);
+      load(u, s + (u + U) * WK);
     }
   }
+#pragma unroll
+  for (int u = 0; u < U - 1; u++)
+    if (s + u * WK < s1) multiply(u);
   // this thread's elements
   constexpr uint32_t ROWS = FOUR ? 8 : 32;  // of a tile
   constexpr int ALL = TILES * ROWS * 32, E = ALL <= 64 * W ? 1 : ALL / (64 * W);
