@@ -60,33 +60,87 @@ struct KvAppend {
     uint64_t row;                     // its first row of k and v
   } e[kAttRows];
 };
-// A workgroup takes four token positions 4 i .. 4 i + 3 of a sequence; a
-// thread, one value of them at a time (neighbours read neighbouring words).
-// Bytes are stored one by one, so tokens that were there stay.  A word outside
-// an int8 cache's range sets *bad (host memory).
+// A workgroup takes four token positions 4 i .. 4 i + 3 of a sequence; tokens
+// that were there stay.  A word outside an int8 cache's range sets *bad (host
+// memory).  DIMS = 4 (dims a multiple of 4): a thread takes four dims of the
+// four tokens, whose digits are four bytes next to each other a token among the
+// keys and, where all four tokens are new, a dim among the values (65537 tokens
+// of 8 x 128 general values: 982 us a value and byte at a time, 567 so);
+// DIMS = 1: a value at a time.
+template <int DIMS>
 static __global__ void __launch_bounds__(256) k_kv_append(KvPool p, KvAppend a, const uint32_t* __restrict__ k,
                                                           const uint32_t* __restrict__ v, uint32_t* bad) {
   uint32_t i = 0;
-  while (i + 1 < a.n && a.e[i + 1].quad0 <= blockIdx.x) i++;
+  for (uint32_t up = a.n; up - i > 1;) {  // the last entry that begins at or before this group
+    const uint32_t mid = (i + up) / 2;
+    if (a.e[mid].quad0 <= blockIdx.x) i = mid;
+    else up = mid;
+  }
   const uint32_t pos = a.e[i].pos, end = pos + a.e[i].count;
   const uint32_t t0 = (pos / 4 + (blockIdx.x - a.e[i].quad0)) * 4;  // never crosses a block
-  const uint32_t width = p.kv_heads * p.dim, block = t0 / kAttBlock;
-  for (uint32_t w = threadIdx.x; w < width; w += blockDim.x) {
+  const uint32_t width = p.kv_heads * p.dim, block = t0 / kAttBlock, in = t0 % kAttBlock;
+  uint32_t high = 0;
+  for (uint32_t w = threadIdx.x * DIMS; w < width; w += blockDim.x * DIMS) {
     const uint32_t head = w / p.dim, d = w % p.dim;
     const uint64_t base = kv_block(p, a.e[i].seq, block, head);
-    for (uint32_t t = t0 < pos ? pos : t0; t < t0 + 4 && t < end; t++) {
-      const uint64_t at = (a.e[i].row + (t - pos)) * width + w;
-      const uint32_t in = t % kAttBlock;
-      int32_t dk[4], dv[4];
-      balanced_digits(center_m31(k[at]), dk);
-      balanced_digits(center_m31(v[at]), dv);
-      if (p.planes == 1 && (dk[1] | dk[2] | dk[3] | dv[1] | dv[2] | dv[3])) *(volatile uint32_t*)bad = 1;
-      for (uint32_t q = 0; q < p.planes; q++) {
-        p.k[base + kv_key_byte(in, d, q, p.planes)] = (int8_t)dk[q];
-        p.v[base + kv_value_byte(in, d, q, p.planes)] = (int8_t)dv[q];
+    uint32_t kx[4][DIMS], vx[4][DIMS];  // places that are not new read a new one's, unused
+#pragma unroll
+    for (uint32_t t = 0; t < 4; t++) {
+      const uint32_t token = t0 + t < pos ? pos : t0 + t < end ? t0 + t : end - 1;
+      const uint64_t at = (a.e[i].row + (token - pos)) * width + w;
+      if constexpr (DIMS == 4) {
+        const v4i_word kq = *(const v4i_word*)(k + at), vq = *(const v4i_word*)(v + at);
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+          kx[t][j] = (uint32_t)kq[j];
+          vx[t][j] = (uint32_t)vq[j];
+        }
+      } else {
+        kx[t][0] = k[at];
+        vx[t][0] = v[at];
+      }
+    }
+    uint32_t vd[DIMS][4];  // [dim][token]: digits
+#pragma unroll
+    for (uint32_t t = 0; t < 4; t++) {
+      uint32_t kd[4] = {}, out[4];
+#pragma unroll
+      for (int j = 0; j < DIMS; j++) {
+        kd[j] = digit_bytes(kx[t][j]);
+        vd[j][t] = digit_bytes(vx[t][j]);
+      }
+      transpose_bytes(kd, out);
+      high |= out[1] | out[2] | out[3];
+      if (t0 + t < pos || t0 + t >= end) continue;
+#pragma unroll
+      for (uint32_t q = 0; q < 4; q++) {
+        if (q >= p.planes) break;
+        int8_t* const to = p.k + base + kv_key_byte(in + t, d, q, p.planes);
+        if constexpr (DIMS == 4) *(uint32_t*)to = out[q];
+        else *to = (int8_t)out[q];
+      }
+    }
+    const bool whole = t0 >= pos && t0 + 4 <= end;
+#pragma unroll
+    for (uint32_t j = 0; j < DIMS; j++) {
+      uint32_t out[4];
+      transpose_bytes(vd[j], out);
+      high |= out[1] | out[2] | out[3];
+#pragma unroll
+      for (uint32_t q = 0; q < 4; q++) {
+        if (q >= p.planes) break;
+        int8_t* const to = p.v + base + kv_value_byte(in, d + j, q, p.planes);
+        if (whole) {
+          *(uint32_t*)to = out[q];
+        } else {
+#pragma unroll
+          for (uint32_t t = 0; t < 4; t++)
+            if (t0 + t >= pos && t0 + t < end) to[t] = (int8_t)(out[q] >> (8 * t));
+        }
       }
     }
   }
+  if (p.planes == 1 && high) *(volatile uint32_t*)bad = 1;
 }
 
 // The rows of a launch.  Their work lies on a line: row by row, kv head (and
@@ -124,16 +178,17 @@ __device__ __forceinline__ uint32_t shift16(uint32_t r) { return m31_reduce62((u
 __device__ __forceinline__ void att_finish(const AttOut& o, uint64_t at, int64_t total, uint32_t z) {
   uint32_t mean = 0;
   if (z) {
-    const uint64_t u = (uint64_t)(total < 0 ? -total : total);
-    const uint32_t r = (uint32_t)((2 * u + z) / (2 * (uint64_t)z));  // |c(v)| <= 2^30: r too
+    // floor((2 |total| + z) / 2 z): |c(v)| <= 2^30, so at most 2^30; the quotient in
+    // 53 bits is off by one at most
+    const uint64_t num = 2 * (uint64_t)(total < 0 ? -total : total) + z, den = 2 * (uint64_t)z;
+    uint32_t r = (uint32_t)((double)num / (double)den);
+    const int64_t rest = (int64_t)(num - (uint64_t)r * den);
+    r += rest < 0 ? -1 : rest >= (int64_t)den ? 1 : 0;
     mean = total < 0 ? m31_neg(r) : r;
   }
   o.out[at] = mean;
   if (o.weighted) o.weighted[at] = shift16(signed_mod_p(total));
 }
-
-// Four words on a word's boundary.
-typedef int v4i_word __attribute__((ext_vector_type(4), aligned(4)));
 
 // A block of the pool as a buffer: loads add a 32-bit lane offset to its scalar
 // descriptor, and those of a block of no bytes return without touching memory.

@@ -142,7 +142,10 @@ static int append_launches(gkr_ctx* c, gkr_kv_cache* k, const uint32_t* counts,
   KvAppend a{};
   uint32_t quads = 0;
   auto store = [&]() -> int {
-    if (quads) GKR_LAUNCH(c, k_kv_append, dim3(quads), dim3(256), 0, k->pool, a, kw, vw, k->bad);
+    if (quads && k->pool.dim % 4 == 0)
+      GKR_LAUNCH(c, k_kv_append<4>, dim3(quads), dim3(256), 0, k->pool, a, kw, vw, k->bad);
+    else if (quads)
+      GKR_LAUNCH(c, k_kv_append<1>, dim3(quads), dim3(256), 0, k->pool, a, kw, vw, k->bad);
     a.n = quads = 0;
     return check_launch(c);
   };

@@ -32,6 +32,7 @@ namespace gkr {
 
 typedef int v4i __attribute__((ext_vector_type(4)));
 typedef int v16i __attribute__((ext_vector_type(16)));
+typedef int v4i_word __attribute__((ext_vector_type(4), aligned(4)));  // four words on a word's boundary
 
 constexpr int kGemmK = 32;     // K per MFMA step
 constexpr int kGemmTile = 32;  // rows / columns per wave tile

@@ -173,17 +173,20 @@ __device__ __forceinline__ uint32_t digit_sum_mod_p(const int32_t (&s)[4]) {
 // loads, U pairs in flight; then the waves' sums meet in LDS (integers: any
 // order gives the same).  No packing launch, no partial sums in memory: bound by
 // the weights' bytes (packing, the product, its splits' sum and the epilogue as
-// launches of their own, then this: 1 x 576 x 192 11.4 -> 4.7 us, 1 x 13824 x
-// 5120 39.1 -> 16.2, 4.4 TB/s; gated 1 x 5120 x 13824 47.0 -> 28.7, 4.9 TB/s,
-// where a copy reaches 4.8).
-constexpr uint32_t kRowWaves = 16;
+// launches of their own, then this: 1 x 576 x 192 11.4 -> 4.7 us; 1 x 13824 x
+// 5120 39.1 -> 14.7, 4.8 TB/s; gated 1 x 5120 x 13824 47.0 -> 24.1, 5.9 TB/s,
+// where a read of 4 GiB reaches 6.4).  The rows' words are asked for before the
+// weights: behind them they came last, and the layout with them (17.2 and 29.3
+// us, also with sixteen waves for the gated pair's 432 column tiles).
+// W waves: sixteen, or eight, of which two workgroups fit a CU, where there are
+// more column tiles than CUs.
 constexpr uint32_t kRowLds = 65536;
-template <int MR, int PB, bool GATED, class End>
-static __global__ void __launch_bounds__(64 * kRowWaves) k_rows(const uint32_t* __restrict__ X, WitWeight w0, WitWeight w1,
-                                                                uint32_t m, uint32_t k, uint32_t n, End end) {
+template <int MR, int PB, bool GATED, int W, class End>
+static __global__ void __launch_bounds__(64 * W, PB == 1 || !GATED ? 4 : 2)
+    k_rows(const uint32_t* __restrict__ X, WitWeight w0, WitWeight w1, uint32_t m, uint32_t k, uint32_t n, End end) {
   constexpr int NW = GATED ? 2 : 1, RT = MR <= 4 ? 1 : MR / 4, U = PB > 1 ? 1 : MR > 4 ? 2 : 4;
   constexpr uint32_t kChunk = kRowLds / (4 * MR);  // K per LDS fill
-  static_assert(MR > 4 || kChunk / 64 % (kRowWaves * U) == 0, "a fill ends where the loads in flight start over");
+  static_assert(MR > 4 || kChunk / 64 % (W * U) == 0, "a fill ends where the loads in flight start over");
   extern __shared__ __align__(16) int8_t digits[];  // [K / 16][4 MR][16]
   __shared__ int32_t sums[NW][PB][MR][4][32];
   const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6, ct = blockIdx.x;
@@ -206,8 +209,41 @@ static __global__ void __launch_bounds__(64 * kRowWaves) k_rows(const uint32_t* 
             b[u][i][q][h] = __builtin_nontemporal_load((const v4i*)(w[i].planes + q * plane + at + 256 * h));
         }
   };
+  // four words of a row a thread: quad t of a fill from k0
+  auto words = [&](uint32_t t, uint32_t k0, uint32_t left, uint32_t quads, uint32_t (&x)[4]) {
+    const uint32_t i = t / quads, kk = t % quads * 4;
+    const uint32_t* const from = X + (uint64_t)i * k + k0 + kk;
+    if (i < m && kk + 4 <= left) {
+      const v4i_word q = *(const v4i_word*)from;
 #pragma unroll
-  for (int u = 0; u < U; u++) load(u, wave + u * kRowWaves);
+      for (int j = 0; j < 4; j++) x[j] = (uint32_t)q[j];
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; j++) x[j] = i < m && kk + j < left ? from[j] : 0u;
+    }
+  };
+  auto lay_out = [&](uint32_t t, uint32_t quads, const uint32_t (&x)[4]) {
+    const uint32_t i = t / quads, kk = t % quads * 4;
+    uint32_t d[4], out[4];
+#pragma unroll
+    for (int j = 0; j < 4; j++) d[j] = digit_bytes(x[j]);
+    transpose_bytes(d, out);
+#pragma unroll
+    for (int p = 0; p < 4; p++)
+      *(uint32_t*)(digits + (kk / 16 * (4 * MR) + 4 * i + p) * 16 + kk % 16) = out[p];
+  };
+  // the first rows' words go out before the weights' loads, which are then in
+  // flight while the words are laid out
+  constexpr int XQ = 4;
+  uint32_t x[XQ][4];
+  {
+    const uint32_t left = k < kChunk ? k : kChunk, quads = (left + 63) / 64 * 16;
+#pragma unroll
+    for (int q = 0; q < XQ; q++)
+      if (threadIdx.x + q * 64 * W < MR * quads) words(threadIdx.x + q * 64 * W, 0, left, quads, x[q]);
+  }
+#pragma unroll
+  for (int u = 0; u < U; u++) load(u, wave + u * W);
   for (uint32_t i = threadIdx.x; i < NW * PB * MR * 128; i += blockDim.x) (&sums[0][0][0][0][0])[i] = 0;
   v4i acc[NW][PB][2][RT];
 #pragma unroll
@@ -222,16 +258,16 @@ static __global__ void __launch_bounds__(64 * kRowWaves) k_rows(const uint32_t* 
   for (uint32_t k0 = 0; k0 < k; k0 += kChunk) {
     const uint32_t left = k - k0 < kChunk ? k - k0 : kChunk, fill = (left + 63) / 64 * 64;
     if (k0) __syncthreads();
-    for (uint32_t t = threadIdx.x; t < MR * (fill / 4); t += blockDim.x) {
-      const uint32_t i = t / (fill / 4), kk = t % (fill / 4) * 4;
-      uint32_t d[4], out[4];
+    uint32_t t = threadIdx.x;
+    if (k0 == 0) {
 #pragma unroll
-      for (int j = 0; j < 4; j++)
-        d[j] = i < m && kk + j < left ? digit_bytes(X[(uint64_t)i * k + k0 + kk + j]) : 0u;
-      transpose_bytes(d, out);
-#pragma unroll
-      for (int p = 0; p < 4; p++)
-        *(uint32_t*)(digits + (kk / 16 * (4 * MR) + 4 * i + p) * 16 + kk % 16) = out[p];
+      for (int q = 0; q < XQ; q++, t += 64 * W)
+        if (t < MR * (fill / 4)) lay_out(t, fill / 4, x[q]);
+    }
+    for (; t < MR * (fill / 4); t += 64 * W) {
+      uint32_t later[4];
+      words(t, k0, left, fill / 4, later);
+      lay_out(t, fill / 4, later);
     }
     __syncthreads();
     const uint32_t pair0 = k0 / 64, pair1 = pair0 + fill / 64;
@@ -253,19 +289,19 @@ static __global__ void __launch_bounds__(64 * kRowWaves) k_rows(const uint32_t* 
           }
     };
     // U pairs at a time without a branch between: with one, a wait for any load would be for all
-    while (pair + (U - 1) * kRowWaves < pair1) {
+    while (pair + (U - 1) * W < pair1) {
 #pragma unroll
       for (int u = 0; u < U; u++) {
         multiply(u);
-        load(u, pair + U * kRowWaves);
-        pair += kRowWaves;
+        load(u, pair + U * W);
+        pair += W;
       }
     }
 #pragma unroll
     for (int u = 0; u < U - 1; u++)
       if (pair < pair1) {  // the last pairs of all: their loads are out
         multiply(u);
-        pair += kRowWaves;
+        pair += W;
       }
   }
 #pragma unroll

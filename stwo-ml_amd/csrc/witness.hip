@@ -62,16 +62,26 @@ static int rows_product(gkr_ctx* c, const gkr_matrix* a, const gkr_matrix* w0, c
   const uint32_t m = (uint32_t)a->rows, k = (uint32_t)a->cols;
   const uint64_t n = w0->cols, ctiles = (n + kGemmTile - 1) / kGemmTile;
   const bool one = w0->bnplanes == 1 && w1->bnplanes == 1;
-  auto launch = [&](auto kernel, uint32_t mr) {
+  auto launch = [&](auto kernel, uint32_t mr, uint32_t waves) {
     const uint32_t lds = std::min<uint32_t>(kRowLds, 4 * mr * ((k + 63) / 64 * 64));
-    GKR_LAUNCH(c, kernel, dim3((uint32_t)ctiles), dim3(64 * kRowWaves), lds, a->dev, wit_weight(w0), wit_weight(w1), m, k,
+    GKR_LAUNCH(c, kernel, dim3((uint32_t)ctiles), dim3(64 * waves), lds, a->dev, wit_weight(w0), wit_weight(w1), m, k,
                (uint32_t)n, end);
   };
-  if (m == 1) one ? launch(k_rows<1, 1, GATED, End>, 1) : launch(k_rows<1, 4, GATED, End>, 1);
-  else if (m == 2) one ? launch(k_rows<2, 1, GATED, End>, 2) : launch(k_rows<2, 4, GATED, End>, 2);
-  else if (m <= 4) one ? launch(k_rows<4, 1, GATED, End>, 4) : launch(k_rows<4, 4, GATED, End>, 4);
-  else if (m <= 8) launch(k_rows<8, 1, GATED, End>, 8);
-  else launch(k_rows<16, 1, GATED, End>, 16);
+  const bool many = ctiles > 256;
+  // two matrices of general weights: eight waves of twice the registers
+#define GKR_ROWS(MR)                                                                \
+  do {                                                                              \
+    if (!one && (many || GATED)) launch(k_rows<MR, 4, GATED, 8, End>, MR, 8);       \
+    else if (!one) launch(k_rows<MR, 4, GATED, GATED ? 8 : 16, End>, MR, 16);       \
+    else if (many) launch(k_rows<MR, 1, GATED, 8, End>, MR, 8);                     \
+    else launch(k_rows<MR, 1, GATED, 16, End>, MR, 16);                             \
+  } while (0)
+  if (m == 1) GKR_ROWS(1);
+  else if (m == 2) GKR_ROWS(2);
+  else if (m <= 4) GKR_ROWS(4);
+  else if (m <= 8) many ? launch(k_rows<8, 1, GATED, 8, End>, 8, 8) : launch(k_rows<8, 1, GATED, 16, End>, 8, 16);
+  else many ? launch(k_rows<16, 1, GATED, 8, End>, 16, 8) : launch(k_rows<16, 1, GATED, 16, End>, 16, 16);
+#undef GKR_ROWS
   return check_launch(c);
 }
 // Whether k_rows takes it: up to four rows; five to sixteen by weights of one

@@ -114,6 +114,15 @@ def test_wide(gpu_ctx, m, k, n):
         check_gated(gpu_ctx, m, k, n, xk, 1)
 
 
+# few rows by more column tiles than the chip has CUs
+@pytest.mark.parametrize("m,k,n", [(1, 1025, 8225), (2, 700, 9001), (4, 16400, 8193), (7, 500, 8500), (16, 300, 8300)])
+def test_few_rows_many_columns(gpu_ctx, m, k, n):
+    for xk, wk in ((1, 1), (0, 1), (0, 0)):
+        check_fused(gpu_ctx, m, k, n, xk, wk, RELU)
+        if k < 2000:
+            check_gated(gpu_ctx, m, k, n, xk, wk)
+
+
 # more than 64 rows and enough work for blocks of 8 x 8 tiles, for all rows streamed through one workgroup
 # where they have one plane, and for K splits; ragged edges, and K steps that end inside a stage of four
 @pytest.mark.parametrize("m,k,n", [(100, 5121, 5101), (200, 2605, 5101), (130, 1130, 5131), (260, 500, 4099),
