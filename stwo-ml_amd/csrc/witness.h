@@ -353,7 +353,6 @@ constexpr uint32_t kMaskWords = 64, kMaskStride = 32;
 __device__ __forceinline__ bool wit_four(const uint32_t* mask) {  // the same in every wave
   return __any(mask[kMaskStride * (threadIdx.x & 63)] != 0);
 }
-template <bool VEC>
 static __global__ void __launch_bounds__(256) k_wit_pack(const uint32_t* __restrict__ X, uint64_t m, uint64_t k,
                                                          uint64_t nsteps, int8_t* __restrict__ one,
                                                          int8_t* __restrict__ four, uint32_t* __restrict__ mask,
@@ -362,23 +361,27 @@ static __global__ void __launch_bounds__(256) k_wit_pack(const uint32_t* __restr
   if (at < kMaskWords) clear[kMaskStride * at] = 0;
   const uint32_t half = (uint32_t)at & 1, row8 = (uint32_t)(at >> 1) & 7;
   const uint64_t blk = at >> 4, rt8 = blk / nsteps, step = blk - rt8 * nsteps, row = 8 * rt8 + row8;
-  uint32_t high = 0;
+  uint32_t high = 0, w[4][4];
   if (row < m) {
     const uint64_t k0 = step * kGemmK + 16 * half;
-    uint32_t w[4][4];
+    const uint32_t* const from = X + row * k + k0;
+    uint32_t x[4][4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      if (k0 + 4 * i + 4 <= k) {
+        const v4i_word q = *(const v4i_word*)(from + 4 * i);
+#pragma unroll
+        for (int j = 0; j < 4; j++) x[i][j] = (uint32_t)q[j];
+      } else {
+#pragma unroll
+        for (int j = 0; j < 4; j++) x[i][j] = k0 + 4 * i + j < k ? from[4 * i + j] : 0u;
+      }
+    }
 #pragma unroll
     for (int i = 0; i < 4; i++) {
       uint32_t d[4], out[4];
-      if constexpr (VEC) {
-        const uint4 x = k0 + 4 * i < k ? *(const uint4*)(X + row * k + k0 + 4 * i) : make_uint4(0, 0, 0, 0);
-        d[0] = digit_bytes(x.x);
-        d[1] = digit_bytes(x.y);
-        d[2] = digit_bytes(x.z);
-        d[3] = digit_bytes(x.w);
-      } else {
 #pragma unroll
-        for (int j = 0; j < 4; j++) d[j] = digit_bytes(k0 + 4 * i + j < k ? X[row * k + k0 + 4 * i + j] : 0u);
-      }
+      for (int j = 0; j < 4; j++) d[j] = digit_bytes(x[i][j]);
       transpose_bytes(d, out);
 #pragma unroll
       for (int p = 0; p < 4; p++) w[p][i] = out[p];
@@ -387,12 +390,14 @@ static __global__ void __launch_bounds__(256) k_wit_pack(const uint32_t* __restr
     int8_t* const f = four + blk * kGemmBlockBytes + 512 * half + 64 * row8;
 #pragma unroll
     for (int p = 0; p < 4; p++) *(uint4*)(f + 16 * p) = make_uint4(w[p][0], w[p][1], w[p][2], w[p][3]);
-    *(uint4*)(one + ((row >> 5) * nsteps + step) * kGemmBlockBytes + 512 * half + 16 * (row & 31)) =
-        make_uint4(w[0][0], w[0][1], w[0][2], w[0][3]);
   }
-  // stores to one address take about 20 ns each, one after another: 64 words on
-  // lines of their own, and only while a word is not set
-  if (__any(high != 0) && (threadIdx.x & 63) == 0) {
+  if (!__any(high != 0)) {  // with a higher digit anywhere plane 0 alone is not read
+    if (row < m)
+      *(uint4*)(one + ((row >> 5) * nsteps + step) * kGemmBlockBytes + 512 * half + 16 * (row & 31)) =
+          make_uint4(w[0][0], w[0][1], w[0][2], w[0][3]);
+  } else if ((threadIdx.x & 63) == 0) {
+    // stores to one address take about 20 ns each, one after another: 64 words
+    // on lines of their own, and only while a word is not set
     volatile uint32_t* const word = mask + kMaskStride * (blockIdx.x % kMaskWords);
     if (!*word) *word = 1;
   }

@@ -94,7 +94,9 @@ static bool few_rows(const gkr_matrix* a, const gkr_matrix* w0, const gkr_matrix
   return m <= 16 && w0->bnplanes == 1 && w1->bnplanes == 1 && (m <= 8 ? 8 : 16) * 4 * ((k + 63) / 64 * 64) <= kRowLds;
 }
 
-// Two masks of the packing, used in turn: the packing of one product clears the other's.
+// Two masks of the packing, used in turn: the packing of one product clears the
+// other's.  A mask that is set says that rows may have four planes, which is right
+// for all rows: a captured product may find its own from the last replay.
 static int wit_masks(gkr_ctx* c, uint32_t** mask, uint32_t** next_mask) {
   constexpr uint32_t words = kMaskWords * kMaskStride;
   if (!c->wit_mask) {
@@ -162,10 +164,8 @@ static int packed_product(gkr_ctx* c, const gkr_matrix* a, const gkr_matrix* w0,
   g.mask = mask;
   const uint64_t slots = four_tiles * g.nsteps * 16;
   const dim3 pack_grid((uint32_t)((slots + 255) / 256));
-  if (k % 4 == 0 && ((uintptr_t)a->dev & 15) == 0)
-    GKR_LAUNCH(c, k_wit_pack<true>, pack_grid, dim3(256), 0, a->dev, m, k, (uint64_t)g.nsteps, packed, const_cast<int8_t*>(g.four), mask, next_mask);
-  else
-    GKR_LAUNCH(c, k_wit_pack<false>, pack_grid, dim3(256), 0, a->dev, m, k, (uint64_t)g.nsteps, packed, const_cast<int8_t*>(g.four), mask, next_mask);
+  GKR_LAUNCH(c, k_wit_pack, pack_grid, dim3(256), 0, a->dev, m, k, (uint64_t)g.nsteps, packed,
+             const_cast<int8_t*>(g.four), mask, next_mask);
   TRY(check_launch(c));
 
   uint32_t max_splits = 1, max_rgroups = 1;

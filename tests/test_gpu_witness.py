@@ -288,3 +288,67 @@ def test_on_the_callers_stream():
             assert np.array_equal(kept.download(), product(A, B)) and not o.download().any()
         ctx.close()
     assert hip.hipStreamDestroy(stream) == 0
+
+
+def test_captured_into_a_graph():
+    """Products of one row, 40 and 200 rows, the gated block, and attention with its join, captured once and
+    replayed over changed inputs, int8-range and general in turn, with calls of the context's own between."""
+    from test_gpu_attention import attend
+
+    G.lib()
+    hip = ctypes.CDLL("libamdhip64.so.7")
+    vp, size = ctypes.c_void_p, ctypes.c_size_t
+    copy, stream, graph, run = hip.hipMemcpyAsync, vp(), vp(), vp()
+    copy.argtypes = [vp, vp, size, ctypes.c_int, vp]
+    hip.hipStreamBeginCapture.argtypes, hip.hipStreamEndCapture.argtypes = [vp, ctypes.c_int], [vp, ctypes.POINTER(vp)]
+    hip.hipGraphInstantiate.argtypes = [ctypes.POINTER(vp), vp, vp, vp, size]
+    hip.hipGraphLaunch.argtypes, hip.hipGraphExecDestroy.argtypes, hip.hipGraphDestroy.argtypes = [vp, vp], [vp], [vp]
+    assert hip.hipStreamCreate(ctypes.byref(stream)) == 0
+    ctx = G.Context(0, stream=stream.value)
+    rng = np.random.default_rng(11)
+    k, n, kv_len = 500, 300, 2000
+    W, V = words(rng, (k, n), 1), words(rng, (k, n), 1)
+    w, v = ctx.upload(W), ctx.upload(V)
+    rows = (1, 40, 200)
+    xs = {m: ctx.zeros(m, k) for m in rows}
+    fused, gated = {m: ctx.zeros(m, n) for m in rows}, {m: ctx.zeros(m, n) for m in rows}
+    keys, values = words(rng, (kv_len, 64), 0), words(rng, (kv_len, 64), 0)
+    cache = ctx.kv_cache(1, 64, n_pages=40, max_seqs=1, max_tokens=kv_len)
+    seq = cache.new_sequence()
+    cache.append([seq], [kv_len], ctx.upload(keys), ctx.upload(values))
+    q, att = ctx.zeros(1, 128), ctx.zeros(1, 128)
+
+    def calls():
+        for m in rows:
+            ctx.matmul_forward_fused(xs[m], w, fused[m], activation=GELU)
+            ctx.gated_forward(xs[m], w, v, gated[m])
+        ctx.attention_forward(cache, q, [seq], 2, att, score_offset=1 << 19)
+
+    calls()  # planes, tables and buffers are there from here on
+    ctx.synchronize()
+    thread_local = 1
+    assert hip.hipStreamBeginCapture(stream, thread_local) == 0
+    calls()
+    assert hip.hipStreamEndCapture(stream, ctypes.byref(graph)) == 0
+    assert hip.hipGraphInstantiate(ctypes.byref(run), graph, None, None, 0) == 0
+    for turn in range(4):
+        host = {m: words(rng, (m, k), turn % 2) for m in rows}
+        Q = words(rng, (1, 128), 0)
+        for dev, h in [(xs[m], host[m]) for m in rows] + [(q, Q)]:
+            assert copy(dev.device_ptr, h.ctypes.data, h.nbytes, 1, stream) == 0
+        assert hip.hipGraphLaunch(run, stream) == 0
+        got = [{m: o[m].download() for m in rows} for o in (fused, gated)] + [att.download()]
+        for m in rows:
+            z = product(host[m], W)
+            assert np.array_equal(got[0][m], activate(z, GELU, 0))
+            assert np.array_equal(got[1][m], activate(z, SILU, 0) * product(host[m], V) % P)
+        assert np.array_equal(got[2][0], attend(Q[0], keys, values, 2, 1, 1 << 19, 20)[0])
+        if turn != 2:  # an eager call between two replays
+            other = words(rng, (40, k), 1 - turn % 2)
+            out = ctx.zeros(40, n)
+            ctx.matmul_forward_fused(ctx.upload(other), w, out)
+            assert np.array_equal(out.download(), product(other, W))
+    assert hip.hipGraphExecDestroy(run) == 0 and hip.hipGraphDestroy(graph) == 0
+    cache.free()
+    ctx.close()
+    assert hip.hipStreamDestroy(stream) == 0
