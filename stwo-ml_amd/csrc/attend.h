@@ -168,6 +168,14 @@ struct AttOut {
   uint64_t score_cols;
 };
 
+// Byte B of each of four words.
+template <int B>
+__device__ __forceinline__ uint32_t pick_bytes(const uint32_t (&w)[4]) {
+  constexpr uint32_t sel = 0x0c0c0400u + 0x101u * B;  // byte B of the first, of the second, zeros
+  return __builtin_amdgcn_perm(w[1], w[0], sel) | __builtin_amdgcn_perm(w[3], w[2], sel) << 16;
+}
+// A signed 32-bit number above -P mod P.
+__device__ __forceinline__ uint32_t signed32_mod_p(int32_t x) { return umin32((uint32_t)x, (uint32_t)x + P); }
 // A signed whole number mod P.
 __device__ __forceinline__ uint32_t signed_mod_p(int64_t x) {
   const uint32_t r = m31_reduce64((uint64_t)(x < 0 ? -x : x));
@@ -358,11 +366,12 @@ static __global__ void __launch_bounds__(256, NP * DT <= 2 ? 2 : 1)
       const bool same = b + 4 < cur.seen_end;
       const uint32_t n_seq = same ? cur.seq : next.seq, n_kvh = same ? cur.kvh : next.kvh;
       const uint32_t n_b = same ? b + 4 : 4 * next.s0, n_end = same ? cur.seen_end : loaded ? next.seen_end : 0;
+      // tokens of the block that are seen, from this lane's first on
+      const int left = block < cur.seen_end ? (int)(len - first) : 0;
       v4i w0, w1, x[4];
 #pragma unroll
       for (int t = 0; t < 4; t++) {
         v4i sc[NG];
-        uint32_t lo = 0, hi = 0;
 #pragma unroll
         for (int g = 0; g < NG; g++) sc[g] = v4i{0, 0, 0, 0};
 #pragma unroll
@@ -374,22 +383,29 @@ static __global__ void __launch_bounds__(256, NP * DT <= 2 ? 2 : 1)
               sc[pk + g] = __builtin_amdgcn_mfma_i32_16x16x64_i8(kd[t % NS][s][pk], qd[s][g], sc[pk + g], 0, 0, 0);
         if (t + NS == 4) key_block(n_seq, n_kvh, n_b, n_end);
         load_keys(t % NS, (t + NS) % 4);
+        uint32_t e[4], e8[4];
 #pragma unroll
         for (int v = 0; v < 4; v++) {
-          // sum_g 256^g sc[g], below 2^52, with 2^32 = 2 (mod P)
-          int64_t sum = (int64_t)sc[0][v] + ((int64_t)sc[1][v] << 8) + ((int64_t)sc[2][v] << 16) + ((int64_t)sc[3][v] << 24);
-          if constexpr (NP > 1)
-            sum += ((int64_t)sc[4][v] << 1) + ((int64_t)sc[5][v] << 9) + ((int64_t)sc[6][v] << 17);
-          const uint32_t xv = m31_add(m31_reduce64((uint64_t)(sum + ((int64_t)P << 24))), offset);
-          const bool seen = block < cur.seen_end && first + 16 * t + v < len;
+          uint32_t xv;
+          if constexpr (NP == 1) {
+            // |sc[g]| <= 2^22: pairs in 32 bits, the upper one turned by 16 of 31 bits
+            const uint32_t low = signed32_mod_p(sc[0][v] + (sc[1][v] << 8)), high = signed32_mod_p(sc[2][v] + (sc[3][v] << 8));
+            xv = m31_add(m31_add(low, ((high << 16) & P) | (high >> 15)), offset);
+          } else {
+            // sum_g 256^g sc[g], below 2^52, with 2^32 = 2 (mod P)
+            int64_t sum = (int64_t)sc[0][v] + ((int64_t)sc[1][v] << 8) + ((int64_t)sc[2][v] << 16) + ((int64_t)sc[3][v] << 24);
+            if constexpr (NP > 1)
+              sum += ((int64_t)sc[4][v] << 1) + ((int64_t)sc[5][v] << 9) + ((int64_t)sc[6][v] << 17);
+            xv = m31_add(m31_reduce64((uint64_t)(sum + ((int64_t)P << 24))), offset);
+          }
+          x[t][v] = (int)xv;
           uint32_t g = (xv & mask) >> 16;
           g = g < 10 ? g : 10;
-          const uint32_t e = seen ? 1u << g : 0u;  // digits base 256, balanced: 128 is 256 - 128
-          x[t][v] = (int)(seen ? xv : 0u);
-          z += e;
-          lo |= (e & 0xffu) << (8 * v);
-          hi |= ((e + 0x80u) >> 8) << (8 * v);
+          e[v] = 16 * t + v < left ? 1u << g : 0u;
+          e8[v] = e[v] + 0x80u;  // digits base 256, balanced: 128 is 256 - 128
+          z += e[v];
         }
+        const uint32_t lo = pick_bytes<0>(e), hi = pick_bytes<1>(e8);
         w0[t] = (int)lo;
         w1[t] = (int)hi;
       }
@@ -400,13 +416,18 @@ static __global__ void __launch_bounds__(256, NP * DT <= 2 ? 2 : 1)
         uint32_t* const out = scores + col * o.score_cols + tok;
         if ((uint64_t)block * kAttBlock + kAttBlock <= o.score_cols) {
 #pragma unroll
-          for (int t = 0; t < 4; t++) *(v4i_word*)(out + 16 * t) = x[t];
+          for (int t = 0; t < 4; t++) {
+            v4i_word seen;
+#pragma unroll
+            for (int v = 0; v < 4; v++) seen[v] = 16 * t + v < left ? x[t][v] : 0;
+            *(v4i_word*)(out + 16 * t) = seen;
+          }
         } else {
 #pragma unroll
           for (int t = 0; t < 4; t++)
 #pragma unroll
             for (int v = 0; v < 4; v++)
-              if (tok + 16 * t + v < o.score_cols) out[16 * t + v] = (uint32_t)x[t][v];
+              if (tok + 16 * t + v < o.score_cols) out[16 * t + v] = 16 * t + v < left ? (uint32_t)x[t][v] : 0u;
         }
       }
       __syncthreads();

@@ -175,10 +175,15 @@ static int append(gkr_ctx* c, gkr_kv_cache* k, const uint32_t* seqs, const uint3
   std::string why;
   if (!k->book->extend(seqs, counts, n, &before, &why)) return fail(GKR_ERR_NOMEM, "cache append: %s", why.c_str());
   int rc = append_launches(c, k, counts, before, km->dev, vm->dev);
-  if (rc == GKR_OK && k->pool.planes == 1) {
-    rc = sync(c);
-    if (rc == GKR_OK && *(volatile uint32_t*)k->bad)
-      rc = fail(GKR_ERR_INVALID, "cache append: a word outside -128 .. 127 for an int8 cache");
+  if (k->pool.planes == 1) {
+    if (rc != GKR_OK) {  // a launch was refused: one before it may still set the word
+      drain(c);
+      (void)hipStreamSynchronize(c->stream);
+    } else {
+      rc = sync(c);
+      if (rc == GKR_OK && *(volatile uint32_t*)k->bad)
+        rc = fail(GKR_ERR_INVALID, "cache append: a word outside -128 .. 127 for an int8 cache");
+    }
     *(volatile uint32_t*)k->bad = 0;
   }
   if (rc != GKR_OK) k->book->back(before);

@@ -251,7 +251,7 @@ static int packed_product(gkr_ctx* c, const gkr_matrix* a, const gkr_matrix* w0,
 // and of a workgroup's rows (256 of 2^21 words).
 static bool packable(uint64_t m, uint64_t k, uint64_t n) {
   return k <= kMaxInner && m <= 1ull << 22 && n <= 1ull << 21 && m * k <= 1ull << 34 &&
-         (m / 64 + 1) * (n / 128 + 1) <= 1ull << 22;
+         (m / 64 + 1) * (n / 128 + 1) <= 1ull << 21;
 }
 
 
