@@ -20,15 +20,6 @@ void release_cache(gkr_kv_cache* k) {
   k->table = k->bad = nullptr;
   k->ctx = nullptr;
 }
-// A C entry point's body: running out of host memory is an error code.
-template <class F>
-static int guarded(F f) {
-  try {
-    return f();
-  } catch (const std::bad_alloc&) {
-    return fail(GKR_ERR_NOMEM, "out of host memory");
-  }
-}
 
 extern "C" int gkr_kv_cache_new(gkr_ctx* c, uint32_t kv_heads, uint32_t dim, uint32_t n_pages, uint32_t page_tokens,
                                 uint32_t max_seqs, uint32_t max_tokens, int int8, gkr_kv_cache** out) {
@@ -197,10 +188,9 @@ extern "C" int gkr_kv_cache_append(gkr_ctx* c, gkr_kv_cache* k, const uint32_t* 
   return guarded([&] { return append(c, k, seqs, counts, n, km, vm); });
 }
 
-extern "C" int gkr_attention_forward(gkr_ctx* c, const gkr_kv_cache* k, const gkr_matrix* q, const uint32_t* seqs,
-                                     const uint32_t* lens, size_t n_rows, uint32_t heads, uint32_t offset,
-                                     uint32_t table_log, gkr_matrix* weighted, gkr_matrix* sums, gkr_matrix* scores,
-                                     gkr_matrix* out) {
+static int attention_forward(gkr_ctx* c, const gkr_kv_cache* k, const gkr_matrix* q, const uint32_t* seqs,
+                             const uint32_t* lens, size_t n_rows, uint32_t heads, uint32_t offset, uint32_t table_log,
+                             gkr_matrix* weighted, gkr_matrix* sums, gkr_matrix* scores, gkr_matrix* out) {
   static const char what[] = "attention";
   if (!c || !k || !q || !out || !seqs) return fail(GKR_ERR_INVALID, "null argument");
   if (k->ctx != c) return fail(GKR_ERR_INVALID, "key-value cache belongs to another (or a destroyed) context");
@@ -295,4 +285,13 @@ extern "C" int gkr_attention_forward(gkr_ctx* c, const gkr_kv_cache* k, const gk
     }
   }
   return GKR_OK;
+}
+
+extern "C" int gkr_attention_forward(gkr_ctx* c, const gkr_kv_cache* k, const gkr_matrix* q, const uint32_t* seqs,
+                                     const uint32_t* lens, size_t n_rows, uint32_t heads, uint32_t offset,
+                                     uint32_t table_log, gkr_matrix* weighted, gkr_matrix* sums, gkr_matrix* scores,
+                                     gkr_matrix* out) {
+  return guarded([&] {
+    return attention_forward(c, k, q, seqs, lens, n_rows, heads, offset, table_log, weighted, sums, scores, out);
+  });
 }

@@ -17,6 +17,7 @@
 #include <map>
 #include <memory>
 #include <mutex>
+#include <new>
 #include <set>
 #include <string>
 #include <vector>
@@ -186,6 +187,16 @@ int weight_planes(gkr_ctx* c, gkr_matrix* b);
 int matmul_forward(gkr_ctx* c, const gkr_matrix* a, gkr_matrix* b, uint32_t* C);
 // logup.hip: an activation table's output column, resident on the device.
 int device_table(gkr_ctx* c, uint32_t tag, uint32_t log_size, uint32_t** out);
+
+// A C entry point's body: running out of host memory is an error code.
+template <class F>
+inline int guarded(F f) {
+  try {
+    return f();
+  } catch (const std::bad_alloc&) {
+    return fail(GKR_ERR_NOMEM, "out of host memory");
+  }
+}
 
 // witness.hip: operand checks of the witness operators.  Every given matrix
 // (null: none) is alive on c, and no output shares memory with an input or

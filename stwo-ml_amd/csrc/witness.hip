@@ -254,10 +254,8 @@ static bool packable(uint64_t m, uint64_t k, uint64_t n) {
          (m / 64 + 1) * (n / 128 + 1) <= 1ull << 21;
 }
 
-
-extern "C" int gkr_matmul_forward_fused(gkr_ctx* c, const gkr_matrix* a, const gkr_matrix* b, const gkr_matrix* bias,
-                                        uint32_t tag, uint32_t table_log, const gkr_matrix* residual, gkr_matrix* pre,
-                                        gkr_matrix* out) {
+static int fused_forward(gkr_ctx* c, const gkr_matrix* a, const gkr_matrix* b, const gkr_matrix* bias, uint32_t tag,
+                         uint32_t table_log, const gkr_matrix* residual, gkr_matrix* pre, gkr_matrix* out) {
   static const char what[] = "fused product";
   if (!c || !a || !b || !out) return fail(GKR_ERR_INVALID, "null argument");
   TRY(check_operands(c, what, {a, b, bias}, {pre, out}));
@@ -293,9 +291,8 @@ extern "C" int gkr_matmul_forward_fused(gkr_ctx* c, const gkr_matrix* a, const g
   return check_launch(c);
 }
 
-extern "C" int gkr_gated_forward(gkr_ctx* c, const gkr_matrix* a, const gkr_matrix* wg, const gkr_matrix* wu,
-                                 uint32_t tag, uint32_t table_log, gkr_matrix* gate, gkr_matrix* act, gkr_matrix* up,
-                                 gkr_matrix* out) {
+static int gated_forward(gkr_ctx* c, const gkr_matrix* a, const gkr_matrix* wg, const gkr_matrix* wu, uint32_t tag,
+                         uint32_t table_log, gkr_matrix* gate, gkr_matrix* act, gkr_matrix* up, gkr_matrix* out) {
   static const char what[] = "gated block";
   if (!c || !a || !wg || !wu || !out) return fail(GKR_ERR_INVALID, "null argument");
   TRY(check_operands(c, what, {a, wg, wu}, {gate, act, up, out}));
@@ -329,4 +326,15 @@ extern "C" int gkr_gated_forward(gkr_ctx* c, const gkr_matrix* a, const gkr_matr
   auto end = k_wit_end<true, GatedEnd>;
   GKR_LAUNCH(c, end, end_grid(m * n), dim3(256), 0, g, u, m * n, n, e);
   return check_launch(c);
+}
+
+extern "C" int gkr_matmul_forward_fused(gkr_ctx* c, const gkr_matrix* a, const gkr_matrix* b, const gkr_matrix* bias,
+                                        uint32_t tag, uint32_t table_log, const gkr_matrix* residual, gkr_matrix* pre,
+                                        gkr_matrix* out) {
+  return guarded([&] { return fused_forward(c, a, b, bias, tag, table_log, residual, pre, out); });
+}
+extern "C" int gkr_gated_forward(gkr_ctx* c, const gkr_matrix* a, const gkr_matrix* wg, const gkr_matrix* wu,
+                                 uint32_t tag, uint32_t table_log, gkr_matrix* gate, gkr_matrix* act, gkr_matrix* up,
+                                 gkr_matrix* out) {
+  return guarded([&] { return gated_forward(c, a, wg, wu, tag, table_log, gate, act, up, out); });
 }
