@@ -347,55 +347,59 @@ static __global__ void __launch_bounds__(64 * W, PB == 1 || !GATED ? 4 : 2)
 // all four planes interleaved, plane p of row r as row 4 r + p, so that a lane
 // of an accumulator holds the four digit sums of its elements.  Words of
 // the mask are set where a digit above plane 0 is not zero, and `clear`, the mask
-// of the next product on the stream, is zeroed.  A thread takes 16 words of a row; rows
-// past m are left as they are (their sums are not stored).
+// of the next product on the stream, is zeroed.  A wave takes a block of eight
+// rows, four words a lane, and a quad's lanes exchange them so that each stores
+// one plane's 16 bytes: loads and stores of whole lines (512 x 13824 words 15 us,
+// 3.7 TB/s; 16 words a lane, every load and store a quarter of its lines, 19 us).
+// Two or four blocks a wave gain 1 to 3 us there and cost 37 x 1537 0.5 to 1.7.
+// Rows past m are left as they are (their sums are not stored).
 constexpr uint32_t kMaskWords = 64, kMaskStride = 32;
 __device__ __forceinline__ bool wit_four(const uint32_t* mask) {  // the same in every wave
   return __any(mask[kMaskStride * (threadIdx.x & 63)] != 0);
 }
+// Word p of a quad's lane q and word q of its lane p change places.
+__device__ __forceinline__ void quad_transpose(uint32_t (&x)[4]) {
+#pragma unroll
+  for (int bit = 1; bit <= 2; bit *= 2)
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      if (i & bit) continue;
+      const bool upper = threadIdx.x & bit;
+      const int give = (int)(upper ? x[i] : x[i + bit]);
+      const uint32_t take = (uint32_t)(bit == 1 ? __builtin_amdgcn_mov_dpp(give, 0xb1, 0xf, 0xf, true)    // lanes 1 0 3 2
+                                                : __builtin_amdgcn_mov_dpp(give, 0x4e, 0xf, 0xf, true));  // 2 3 0 1
+      (upper ? x[i] : x[i + bit]) = take;
+    }
+}
 static __global__ void __launch_bounds__(256) k_wit_pack(const uint32_t* __restrict__ X, uint64_t m, uint64_t k,
-                                                         uint64_t nsteps, int8_t* __restrict__ one,
+                                                         uint32_t nsteps, int8_t* __restrict__ one,
                                                          int8_t* __restrict__ four, uint32_t* __restrict__ mask,
                                                          uint32_t* __restrict__ clear) {
-  const uint64_t at = (uint64_t)blockIdx.x * blockDim.x + threadIdx.x;  // (row / 8, step, row % 8, half)
-  if (at < kMaskWords) clear[kMaskStride * at] = 0;
-  const uint32_t half = (uint32_t)at & 1, row8 = (uint32_t)(at >> 1) & 7;
-  const uint64_t blk = at >> 4, rt8 = blk / nsteps, step = blk - rt8 * nsteps, row = 8 * rt8 + row8;
-  uint32_t high = 0, w[4][4];
-  if (row < m) {
-    const uint64_t k0 = step * kGemmK + 16 * half;
-    const uint32_t* const from = X + row * k + k0;
-    uint32_t x[4][4];
+  if (blockIdx.x == 0 && threadIdx.x < kMaskWords) clear[kMaskStride * threadIdx.x] = 0;
+  const uint32_t q = threadIdx.x & 3, row8 = threadIdx.x >> 2 & 7, half = threadIdx.x >> 5 & 1;
+  const uint32_t blk = (uint32_t)__builtin_amdgcn_readfirstlane((int)(blockIdx.x * 4 + (threadIdx.x >> 6)));
+  const uint32_t rt8 = blk / nsteps, step = blk - rt8 * nsteps;
+  const uint64_t row = 8 * (uint64_t)rt8 + row8, k0 = (uint64_t)step * kGemmK + 16 * half + 4 * q;
+  const uint32_t* const from = X + row * k + k0;
+  uint32_t d[4], w[4];
+  if (row < m && k0 + 4 <= k) {
+    const v4i_word x = *(const v4i_word*)from;
 #pragma unroll
-    for (int i = 0; i < 4; i++) {
-      if (k0 + 4 * i + 4 <= k) {
-        const v4i_word q = *(const v4i_word*)(from + 4 * i);
+    for (int j = 0; j < 4; j++) d[j] = digit_bytes((uint32_t)x[j]);
+  } else {
 #pragma unroll
-        for (int j = 0; j < 4; j++) x[i][j] = (uint32_t)q[j];
-      } else {
-#pragma unroll
-        for (int j = 0; j < 4; j++) x[i][j] = k0 + 4 * i + j < k ? from[4 * i + j] : 0u;
-      }
-    }
-#pragma unroll
-    for (int i = 0; i < 4; i++) {
-      uint32_t d[4], out[4];
-#pragma unroll
-      for (int j = 0; j < 4; j++) d[j] = digit_bytes(x[i][j]);
-      transpose_bytes(d, out);
-#pragma unroll
-      for (int p = 0; p < 4; p++) w[p][i] = out[p];
-      high |= out[1] | out[2] | out[3];
-    }
-    int8_t* const f = four + blk * kGemmBlockBytes + 512 * half + 64 * row8;
-#pragma unroll
-    for (int p = 0; p < 4; p++) *(uint4*)(f + 16 * p) = make_uint4(w[p][0], w[p][1], w[p][2], w[p][3]);
+    for (int j = 0; j < 4; j++) d[j] = digit_bytes(row < m && k0 + j < k ? from[j] : 0u);
   }
-  if (!__any(high != 0)) {  // with a higher digit anywhere plane 0 alone is not read
-    if (row < m)
-      *(uint4*)(one + ((row >> 5) * nsteps + step) * kGemmBlockBytes + 512 * half + 16 * (row & 31)) =
-          make_uint4(w[0][0], w[0][1], w[0][2], w[0][3]);
-  } else if ((threadIdx.x & 63) == 0) {
+  transpose_bytes(d, w);
+  const bool high = __any((w[1] | w[2] | w[3]) != 0);
+  quad_transpose(w);  // plane q of the row's 16 words
+  if (row < m) {
+    const uint4 words = make_uint4(w[0], w[1], w[2], w[3]);
+    *(uint4*)(four + (uint64_t)blk * kGemmBlockBytes + 512 * half + 64 * row8 + 16 * q) = words;
+    if (!high && q == 0)  // with a higher digit anywhere plane 0 alone is not read
+      *(uint4*)(one + ((row >> 5) * nsteps + step) * kGemmBlockBytes + 512 * half + 16 * (row & 31)) = words;
+  }
+  if (high && (threadIdx.x & 63) == 0) {
     // stores to one address take about 20 ns each, one after another: 64 words
     // on lines of their own, and only while a word is not set
     volatile uint32_t* const word = mask + kMaskStride * (blockIdx.x % kMaskWords);
@@ -830,7 +834,10 @@ static __global__ void __launch_bounds__(512) k_wit_mixed(WitProduct g, End end)
     wit_tiles<RT, 1, GATED, 8, WR, false>(g, (int32_t*)lds, rg, cg, 0, end);
 }
 
-// The end of a product whose K was split: four elements a thread.
+// The end of a product whose K was split: four elements a thread, four parts'
+// loads together.  Bound by the parts' way through memory: 512 x 5120 of three
+// parts 10.6 us, 3.9 TB/s (two at a time and the residual behind them 15.4).
+constexpr uint32_t kJoinParts = 4;
 template <bool GATED, class End>
 static __global__ void __launch_bounds__(256) k_wit_join(WitProduct g, End end) {
   const uint32_t splits = g.plan[wit_four(g.mask) ? 1 : 0].splits;
@@ -839,28 +846,39 @@ static __global__ void __launch_bounds__(256) k_wit_join(WitProduct g, End end) 
   const uint64_t count = g.m * g.n;
   constexpr int E = 4;
   for (uint64_t first = (uint64_t)blockIdx.x * (256 * E); first < count; first += (uint64_t)gridDim.x * (256 * E)) {
+    const uint32_t column = (uint32_t)(first % g.n);
     uint64_t t[NW][E] = {};
     uint32_t at[E], z[NW][E];
 #pragma unroll
     for (int e = 0; e < E; e++) at[e] = 4 * (threadIdx.x + 256 * e);
-#pragma unroll 2
-    for (uint32_t s = 0; s < splits; s++)
+    typename End::template Slot<E> slot;
+    const typename End::Tile tile = end.tile(first, count);
+    end.fetch(slot, tile, at);
+    for (uint32_t s0 = 0; s0 < splits; s0 += kJoinParts) {  // those past the last have no bytes and read zero
+      uint32_t part[kJoinParts][NW][E];
 #pragma unroll
-      for (int x = 0; x < NW; x++) {
-        const WitBuffer part = wit_buffer(g.part + (uint64_t)(s * NW + x) * count, first, count);
+      for (uint32_t s = 0; s < kJoinParts; s++)
 #pragma unroll
-        for (int e = 0; e < E; e++) t[x][e] += wit_read(part, at[e]);
-      }
+        for (int x = 0; x < NW; x++) {
+          const WitBuffer from =
+              wit_buffer(g.part + (uint64_t)((s0 + s) * NW + x) * count, first, s0 + s < splits ? count : 0);
+#pragma unroll
+          for (int e = 0; e < E; e++) part[s][x][e] = wit_read(from, at[e]);
+        }
+#pragma unroll
+      for (uint32_t s = 0; s < kJoinParts; s++)
+#pragma unroll
+        for (int x = 0; x < NW; x++)
+#pragma unroll
+          for (int e = 0; e < E; e++) t[x][e] += part[s][x][e];
+    }
 #pragma unroll
     for (int x = 0; x < NW; x++)
 #pragma unroll
       for (int e = 0; e < E; e++) {
         z[x][e] = m31_reduce64(t[x][e]);
-        if (x == 0) z[0][e] = m31_add(z[0][e], end.column((first + threadIdx.x + 256 * e) % g.n, true));
+        if (x == 0) z[0][e] = m31_add(z[0][e], end.column((column + threadIdx.x + 256 * e) % (uint32_t)g.n, true));
       }
-    typename End::template Slot<E> slot;
-    const typename End::Tile tile = end.tile(first, count);
-    end.fetch(slot, tile, at);
     end.begin(slot, 0, z);
     end.finish(slot, tile, at);
   }

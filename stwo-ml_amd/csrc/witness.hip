@@ -162,9 +162,8 @@ static int packed_product(gkr_ctx* c, const gkr_matrix* a, const gkr_matrix* w0,
   uint32_t *mask, *next_mask;
   TRY(wit_masks(c, &mask, &next_mask));
   g.mask = mask;
-  const uint64_t slots = four_tiles * g.nsteps * 16;
-  const dim3 pack_grid((uint32_t)((slots + 255) / 256));
-  GKR_LAUNCH(c, k_wit_pack, pack_grid, dim3(256), 0, a->dev, m, k, (uint64_t)g.nsteps, packed,
+  const dim3 pack_grid((uint32_t)((four_tiles * g.nsteps + 3) / 4));
+  GKR_LAUNCH(c, k_wit_pack, pack_grid, dim3(256), 0, a->dev, m, k, g.nsteps, packed,
              const_cast<int8_t*>(g.four), mask, next_mask);
   TRY(check_launch(c));
 
@@ -242,7 +241,7 @@ static int packed_product(gkr_ctx* c, const gkr_matrix* a, const gkr_matrix* w0,
 #undef GKR_WIT_TILES
   if (max_splits > 1) {
     auto join = k_wit_join<GATED, End>;
-    GKR_LAUNCH(c, join, end_grid(m * n), dim3(256), 0, g, end);
+    GKR_LAUNCH(c, join, end_grid((m * n + 3) / 4), dim3(256), 0, g, end);
     TRY(check_launch(c));
   }
   return GKR_OK;
