@@ -219,7 +219,7 @@ __device__ __forceinline__ v4i kv_load(__amdgpu_buffer_rsrc_t block, uint32_t at
 // LDS in small loops: unrolled over registers, the code of a short segment took
 // longer to fetch than to run.
 // Bound by the cache's bytes: 64 rows of up to 4096 int8 tokens, 8 kv heads of
-// 128, 59 us and 5 us of k_attend_join (4.2 TB/s; one workgroup per row, head
+// 128, 56 us and 5 us of k_attend_join (4.7 TB/s; one workgroup per row, head
 // and 20 blocks, whatever the lengths, 82 us); one row of 65537 general tokens
 // 94 us and 7 (5.7 TB/s), 10 more with its 2.6 M scores.  Here 1024 workgroups
 // for int8 caches (512: 72 us, 2048: 93), 256 of a wave per SIMD for general

@@ -173,8 +173,8 @@ __device__ __forceinline__ uint32_t digit_sum_mod_p(const int32_t (&s)[4]) {
 // loads, U pairs in flight; then the waves' sums meet in LDS (integers: any
 // order gives the same).  No packing launch, no partial sums in memory: bound by
 // the weights' bytes (packing, the product, its splits' sum and the epilogue as
-// launches of their own, then this: 1 x 576 x 192 11.4 -> 4.7 us; 1 x 13824 x
-// 5120 39.1 -> 14.7, 4.8 TB/s; gated 1 x 5120 x 13824 47.0 -> 24.1, 5.9 TB/s,
+// launches of their own, then this: 1 x 576 x 192 11.4 -> 4.5 us; 1 x 13824 x
+// 5120 39.1 -> 14.0, 5.1 TB/s; gated 1 x 5120 x 13824 47.0 -> 23.2, 6.1 TB/s,
 // where a read of 4 GiB reaches 6.4).  The rows' words are asked for before the
 // weights: behind them they came last, and the layout with them (17.2 and 29.3
 // us, also with sixteen waves for the gated pair's 432 column tiles).
@@ -427,7 +427,11 @@ struct WitProduct {
 // down the rows, RT tiles each, by W / WR that take the K steps in turn,
 // operands straight from memory into registers with U steps in flight; the
 // waves' sums meet in LDS.  WR goes with the rows' planes (WR1, WR4), so that
-// both take the same registers.
+// both take the same registers.  Bound by the weights' bytes where there are
+// many column tiles (gated 64 x 5120 x 13824 with 14 MB of outputs 36 us, 4.3
+// TB/s), by a workgroup's chain of first loads, steps, sums and stores where
+// there are few (64 x 5120 x 5120 13 us for 28 MB; 37 x 1537 x 1111 of general
+// words 11 us).
 template <int RT, int PB, bool GATED, int W, int WR, bool FOUR, class End>
 __device__ __forceinline__ void wit_tiles(const WitProduct& g, int32_t* sums, uint32_t rg, uint32_t cg, uint32_t split,
                                           const End& end) {
@@ -577,6 +581,10 @@ static __global__ void __launch_bounds__(64 * W) k_wit_tiles(WitProduct g, uint3
 // other half of LDS and the one after it is on its way from memory.  Eight
 // waves, two down the rows (four tiles each) by four across (two tiles, or one
 // of each matrix): 6 KB from LDS feed 8 matrix instructions of 32 cycles.
+// Bound by the matrix cores: 512 x 13824 x 5120 of general rows (2.9e11
+// operations) 133 to 144 us with its parts' stores, 2.0 to 2.2 POP/s, where a
+// library product of 8192^3 reaches 2.17; gated 512 x 5120 x 13824 of one plane
+// 93 to 96 us, about 15 of them the 7 M table look-ups at the end (a line each).
 constexpr int kBlockStage = 4;  // K steps
 // Weights of several planes: a column tile's four planes are four of the eight,
 // two to a wave, whose sums two waves bring together.
