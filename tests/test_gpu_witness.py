@@ -133,6 +133,14 @@ def test_blocks(gpu_ctx, m, k, n):
         check_gated(gpu_ctx, m, k, n, xk, 1)
 
 
+# five to sixteen K splits (more than are joined at a time) by few columns
+@pytest.mark.parametrize("m,k,n", [(200, 13825, 1030), (520, 9001, 1030), (100, 33001, 1111), (270, 20001, 900)])
+def test_many_splits(gpu_ctx, m, k, n):
+    for xk in (1, 0):
+        check_fused(gpu_ctx, m, k, n, xk, 1, SIGMOID)
+        check_gated(gpu_ctx, m, k, n, xk, 1)
+
+
 @pytest.mark.parametrize("m,k,n", [(100, 2605, 3001), (130, 500, 5131), (300, 100, 4099), (513, 801, 2003)])
 def test_blocks_of_general_weights(gpu_ctx, m, k, n):
     for xk in (1, 0):
