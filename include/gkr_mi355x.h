@@ -424,9 +424,10 @@ int gkr_kv_cache_free_pages(const gkr_kv_cache* cache, uint32_t* n_pages);
 /* Appends counts[i] tokens to sequence seqs[i], the rows of k and v (each
  * n_kv_heads * head_dim wide, head by head) in that order; their number is the
  * sum of the counts.  All of them or, on an error, none: too few pages or too
- * long a sequence (GKR_ERR_NOMEM), or a word outside an int8 cache's range
- * (GKR_ERR_INVALID; for this check, and only on int8 caches, the call waits
- * for the stream).                                                           */
+ * long a sequence (GKR_ERR_NOMEM), a launch that the runtime refuses
+ * (GKR_ERR_DEVICE; the call returns once all of its launches have been
+ * issued), or a word outside an int8 cache's range (GKR_ERR_INVALID; for this
+ * check, and only on int8 caches, the call waits for the stream).            */
 int gkr_kv_cache_append(gkr_ctx* ctx, gkr_kv_cache* cache, const uint32_t* seqs, const uint32_t* counts, size_t n,
                         const gkr_matrix* k, const gkr_matrix* v);
 /* Attention of n_rows new tokens: row i of q (n_heads * head_dim words, query

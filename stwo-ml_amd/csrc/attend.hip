@@ -64,6 +64,12 @@ extern "C" int gkr_kv_cache_new(gkr_ctx* c, uint32_t kv_heads, uint32_t dim, uin
   }
   k->pool.pages = k->table;
   *k->bad = 0;
+  // entries that no append has set name a page that there is
+  const hipError_t e = hipMemsetAsync(k->table, 0, (uint64_t)max_seqs * width * sizeof(uint32_t), c->stream);
+  if (e != hipSuccess) {
+    gkr_kv_cache_free(k);
+    return fail(GKR_ERR_DEVICE, "key-value cache: clear of the page table: %s", hipGetErrorString(e));
+  }
   *out = k;
   return GKR_OK;
 }
@@ -116,9 +122,13 @@ extern "C" int gkr_kv_cache_free_pages(const gkr_kv_cache* k, uint32_t* n) {
 static int append_launches(gkr_ctx* c, gkr_kv_cache* k, const uint32_t* counts,
                            const std::vector<KvBook::Before>& before, const uint32_t* kw, const uint32_t* vw) {
   KvSlots slots{};
+  // the tokens' stores go by the table: an entry that was not set names another sequence's page, so none is
+  // launched before the runtime has taken these launches
   auto set_pages = [&]() -> int {
-    if (slots.n) GKR_LAUNCH(c, k_kv_pages, dim3(1), dim3(256), 0, k->table, slots);
+    if (slots.n == 0) return GKR_OK;
+    GKR_LAUNCH(c, k_kv_pages, dim3(1), dim3(256), 0, k->table, slots);
     slots.n = 0;
+    drain(c);
     return check_launch(c);
   };
   for (size_t i = 0; i < before.size(); i++) {
@@ -165,7 +175,19 @@ static int append(gkr_ctx* c, gkr_kv_cache* k, const uint32_t* seqs, const uint3
   std::vector<KvBook::Before> before;  // lengths and pages first; taken back if anything fails
   std::string why;
   if (!k->book->extend(seqs, counts, n, &before, &why)) return fail(GKR_ERR_NOMEM, "cache append: %s", why.c_str());
+  struct Undo {
+    KvBook& book;
+    const std::vector<KvBook::Before>& before;
+    bool kept = false;
+    ~Undo() {
+      if (!kept) book.back(before);
+    }
+  } undo{*k->book, before};
   int rc = append_launches(c, k, counts, before, km->dev, vm->dev);
+  if (rc == GKR_OK) {  // a launcher thread's refusal is there once it has issued them all
+    drain(c);
+    rc = check_launch(c);
+  }
   if (k->pool.planes == 1) {
     if (rc != GKR_OK) {  // a launch was refused: one before it may still set the word
       drain(c);
@@ -177,7 +199,7 @@ static int append(gkr_ctx* c, gkr_kv_cache* k, const uint32_t* seqs, const uint3
     }
     *(volatile uint32_t*)k->bad = 0;
   }
-  if (rc != GKR_OK) k->book->back(before);
+  undo.kept = rc == GKR_OK;
   return rc;
 }
 extern "C" int gkr_kv_cache_append(gkr_ctx* c, gkr_kv_cache* k, const uint32_t* seqs, const uint32_t* counts, size_t n,

@@ -238,3 +238,57 @@ def test_refusals(gpu_ctx):
     mine.free()
     gpu_ctx.attention_forward(cache, q, [s], 4, out)
     gpu_ctx.synchronize()
+
+
+@pytest.mark.parametrize("callers_stream", [False, True])
+@pytest.mark.parametrize("int8", [True, False])
+@pytest.mark.parametrize("launch", [1, 2])
+def test_refused_append(launch, int8, callers_stream):
+    """A launch of an append that the runtime refuses (the page table's, the tokens') fails that call, whichever
+    thread issues it, and leaves lengths and pages as they were; the same append then goes through."""
+    ctx = G.Context(0, stream=0) if callers_stream else G.Context(0)
+    rng = np.random.default_rng(launch)
+    cache = ctx.kv_cache(2, 64, n_pages=12, max_seqs=3, max_tokens=512, int8=int8)
+    seqs, ks, vs = fill(ctx, cache, rng, [70, 0], 128, int8)
+    for turn in range(3):
+        counts = [100, 65] if turn < 2 else [3, 1]  # the last needs no page: its first launch is the tokens'
+        k, v = words(rng, (sum(counts), 128), int8), words(rng, (sum(counts), 128), int8)
+        up = ctx.upload(k), ctx.upload(v)
+        before = [cache.length(s) for s in seqs], cache.free_pages()
+        ctx.debug(G.DEBUG_REFUSE_LAUNCH, launch if turn < 2 else 1)
+        with pytest.raises(G.GkrError) as e:
+            cache.append(seqs, counts, *up)
+        assert e.value.code == 2
+        assert ([cache.length(s) for s in seqs], cache.free_pages()) == before
+        ctx.debug(G.DEBUG_REFUSE_LAUNCH, 0)
+        cache.append(seqs, counts, *up)
+        for i, part in enumerate((slice(0, counts[0]), slice(counts[0], None))):
+            ks[i], vs[i] = np.concatenate([ks[i], k[part]]), np.concatenate([vs[i], v[part]])
+        run_and_check(ctx, cache, seqs, ks, vs, 6, 2, 64, int8, seed=turn)
+    cache.free()
+    ctx.close()
+
+
+def test_append_behind_a_refused_launch():
+    """A launch refused on the launcher thread whose call has returned is told by an append behind it, which then
+    keeps nothing."""
+    ctx = G.Context(0)
+    rng = np.random.default_rng(5)
+    cache = ctx.kv_cache(1, 64, n_pages=8, max_seqs=2, max_tokens=256)
+    seqs, ks, vs = fill(ctx, cache, rng, [30], 64, False)
+    a, b, out = ctx.synthetic(1, 64, 0, 1), ctx.synthetic(64, 96, 1, 2), ctx.zeros(1, 96)
+    ctx.matmul_forward_fused(a, b, out)
+    k, v = words(rng, (64, 64), False), words(rng, (64, 64), False)
+    up = ctx.upload(k), ctx.upload(v)
+    before = cache.length(seqs[0]), cache.free_pages()
+    ctx.debug(G.DEBUG_REFUSE_LAUNCH, 1)
+    with pytest.raises(G.GkrError) as e:  # by the product itself where its launch was issued in time
+        ctx.matmul_forward_fused(a, b, out)
+        cache.append(seqs, [64], *up)
+    assert e.value.code == 2
+    assert (cache.length(seqs[0]), cache.free_pages()) == before
+    ctx.debug(G.DEBUG_REFUSE_LAUNCH, 0)
+    cache.append(seqs, [64], *up)
+    run_and_check(ctx, cache, seqs, [np.concatenate([ks[0], k])], [np.concatenate([vs[0], v])], 2, 1, 64, False)
+    cache.free()
+    ctx.close()
