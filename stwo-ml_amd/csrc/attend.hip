@@ -35,6 +35,10 @@ extern "C" int gkr_kv_cache_new(gkr_ctx* c, uint32_t kv_heads, uint32_t dim, uin
   const uint32_t width = (max_tokens + page_tokens - 1) / page_tokens, chunks = (dim + 15) / 16;
   if ((uint64_t)max_seqs * width > 1ull << 32)
     return fail(GKR_ERR_INVALID, "key-value cache: a page table of %u x %u", max_seqs, width);
+  uint64_t bytes;
+  if (!kv_pool_bytes(n_pages, page_tokens, kv_heads, dim, int8 ? 1 : 4, &bytes))
+    return fail(GKR_ERR_INVALID, "key-value cache: %u pages of %u tokens, %u heads of %u values: pools of more than 2^48 bytes",
+                n_pages, page_tokens, kv_heads, dim);
   HIP_TRY(hipSetDevice(c->device));
   gkr_kv_cache* k = nullptr;
   const int rc = guarded([&]() -> int {
@@ -53,7 +57,6 @@ extern "C" int gkr_kv_cache_new(gkr_ctx* c, uint32_t kv_heads, uint32_t dim, uin
     delete k;
     return rc;
   }
-  const uint64_t bytes = (uint64_t)n_pages * kv_heads * k->pool.page_blocks * k->pool.planes * chunks * 1024;
   drain(c);
   if (hipMalloc(&k->pool.k, bytes) != hipSuccess || hipMalloc(&k->pool.v, bytes) != hipSuccess ||
       hipMalloc(&k->table, (uint64_t)max_seqs * width * sizeof(uint32_t)) != hipSuccess ||

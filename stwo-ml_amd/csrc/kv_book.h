@@ -28,6 +28,17 @@ KV_HD uint32_t kv_value_byte(uint32_t token, uint32_t dim, uint32_t plane, uint3
   return (dim / 16 * planes + plane) * 1024 + 256 * (token / 4 % 4) + 16 * (dim % 16) + 4 * (token / 16) + token % 4;
 }
 
+// Bytes of one of a cache's two pools: 1 KB per page, kv head, block of 64
+// tokens, plane and 16 dims.  False if it is more than 2^48, beyond any device;
+// the product of the sizes that a cache takes can pass 2^64.
+inline bool kv_pool_bytes(uint32_t n_pages, uint32_t page_tokens, uint32_t kv_heads, uint32_t dim, uint32_t planes,
+                          uint64_t* bytes) {
+  const uint64_t page = (uint64_t)kv_heads * (page_tokens / kAttBlock) * planes * ((dim + 15) / 16) * 1024;  // <= 2^38
+  if (n_pages > (1ull << 48) / page) return false;
+  *bytes = n_pages * page;
+  return true;
+}
+
 class KvBook {
  public:
   struct Seq {

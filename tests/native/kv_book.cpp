@@ -30,6 +30,10 @@ int kvb_extend(KvBook* b, const uint32_t* seqs, const uint32_t* counts, size_t n
 uint32_t kvb_key_byte(uint32_t token, uint32_t dim, uint32_t plane, uint32_t planes) {
   return kv_key_byte(token, dim, plane, planes);
 }
+int kvb_pool_bytes(uint32_t n_pages, uint32_t page_tokens, uint32_t kv_heads, uint32_t dim, uint32_t planes,
+                   uint64_t* bytes) {
+  return kv_pool_bytes(n_pages, page_tokens, kv_heads, dim, planes, bytes);
+}
 uint32_t kvb_value_byte(uint32_t token, uint32_t dim, uint32_t plane, uint32_t planes) {
   return kv_value_byte(token, dim, plane, planes);
 }

@@ -292,3 +292,12 @@ def test_append_behind_a_refused_launch():
     run_and_check(ctx, cache, seqs, [np.concatenate([ks[0], k])], [np.concatenate([vs[0], v])], 2, 1, 64, False)
     cache.free()
     ctx.close()
+
+
+def test_refused_pools(gpu_ctx):
+    """Pools whose size passes 64 bits (the first one's is 2^64, nothing after the wrap) or any device's memory."""
+    for n_pages, page_tokens, heads, dim, int8 in ((1 << 26, 65536, 4096, 256, False), ((1 << 26) + 1, 65536, 4096, 256, False),
+                                                   (1 << 28, 65536, 4096, 256, True), ((1 << 10) + 1, 65536, 4096, 256, False)):
+        with pytest.raises(G.GkrError) as e:
+            gpu_ctx.kv_cache(heads, dim, n_pages=n_pages, page_tokens=page_tokens, max_seqs=1, max_tokens=64, int8=int8)
+        assert e.value.code == 1, (n_pages, int8)

@@ -107,3 +107,18 @@ def test_every_value_has_its_byte(lib, dim, planes):
     # four tokens 4 i .. 4 i + 3 of a dim are neighbours among the values
     assert all(lib.kvb_value_byte(4 * i + v, 3 % dim, 0, planes) == lib.kvb_value_byte(4 * i, 3 % dim, 0, planes) + v
                for i in range(16) for v in range(4))
+
+
+@pytest.mark.parametrize("n_pages,page_tokens,kv_heads,dim,planes", [
+    (1, 64, 1, 1, 1), (16, 64, 8, 128, 1), (1000, 192, 3, 80, 4), (1 << 10, 65536, 4096, 256, 4),
+    ((1 << 10) + 1, 65536, 4096, 256, 4), (1 << 26, 65536, 4096, 256, 4), ((1 << 26) + 1, 65536, 4096, 256, 4),
+    ((1 << 32) - 1, 65536, 4096, 256, 4), ((1 << 32) - 1, 64, 1, 1, 1), (1 << 31, 64, 128, 16, 1),
+    ((1 << 31) + 1, 64, 128, 16, 1), ((1 << 32) - 1, 64, 4096, 250, 4)])
+def test_pool_bytes(lib, n_pages, page_tokens, kv_heads, dim, planes):
+    """A pool's size against whole numbers of any length; sizes that would wrap around 64 bits (2^26 pages of 65536
+    tokens, 4096 heads of 256 general values: exactly 2^64) are refused."""
+    want = n_pages * (page_tokens // 64) * kv_heads * planes * -(-dim // 16) * 1024
+    got = C.c_uint64(12345)
+    fits = lib.kvb_pool_bytes(n_pages, page_tokens, kv_heads, dim, planes, C.byref(got))
+    assert fits == (want <= 1 << 48)
+    assert got.value == (want if fits else 12345)
