@@ -573,6 +573,15 @@ static __global__ void __launch_bounds__(64 * W) k_wit_tiles(WitProduct g, uint3
     wit_tiles<RT, PB, GATED, W, WR1, false>(g, sums, rg, cg, blockIdx.y, end);
 }
 
+// Between a wave's stores to LDS and its lanes' reads of each other's words, and
+// between those reads and the next stores: the wave's LDS instructions run in
+// order, but the compiler sees one lane's addresses, which it may prove apart
+// and put in another order.
+__device__ __forceinline__ void wave_exchange() {
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+}
+
 // More rows: 8 row tiles of (packed) rows by 8 column tiles of the weights (4 of
 // each of two matrices) a workgroup, through LDS.  Both operands lie in memory
 // as the matrix cores take them, so a tile's K step is 1 KB that one wave
@@ -736,12 +745,14 @@ __device__ __forceinline__ void wit_block(const WitProduct& g, v4i* lds, uint32_
   constexpr int E = 8;
 #pragma unroll
   for (uint32_t part = 0; part < 2; part++) {
+    if (part) wave_exchange();
 #pragma unroll
     for (uint32_t t = 0; t < 4; t++) {
       const v16i& from = GATED ? acc[part * TI + t / 2][t % 2] : acc[t][part];
 #pragma unroll
       for (int v = 0; v < 16; v++) mine[t * 1024 + (8 * (v / 4) + 4 * (lane >> 5) + v % 4) * 32 + (lane & 31)] = from[v];
     }
+    wave_exchange();
     const uint32_t tile0 = rg * 8 + wr * 4 + (GATED ? part * TI : 0), c = lane & 31, hi = lane >> 5;
     const uint64_t col0 = ((uint64_t)cg * CT + (GATED ? wc : wc * 2 + part)) * 32;
     const uint64_t first = (uint64_t)tile0 * ROWS * g.n + col0;

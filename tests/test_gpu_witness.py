@@ -360,3 +360,23 @@ def test_captured_into_a_graph():
     cache.free()
     ctx.close()
     assert hip.hipStreamDestroy(stream) == 0
+
+
+# short sums, so that blocks of 8 x 8 tiles are nearly all end: lanes exchange their sums through LDS, half of a
+# wave's tiles at a time; K splits leave them as parts (the last two)
+@pytest.mark.parametrize("m,k,n", [(512, 33, 8192), (300, 65, 6001), (257, 1, 4129), (520, 9001, 1030), (200, 13825, 1030)])
+def test_block_ends(gpu_ctx, m, k, n):
+    rng = np.random.default_rng(m)
+    for xk in (1, 0):
+        A, B, C2, R = words(rng, (m, k), xk), words(rng, (k, n), 1), words(rng, (k, n), 1), words(rng, (m, n), 0)
+        a, b, c2, h, z = (gpu_ctx.upload(x) for x in (A, B, C2, R, R))
+        p, q, ref = product(A, B), product(A, C2), R.astype(np.int64)
+        for _ in range(3):  # added in place: a word that another lane's reads or stores went past shows
+            gpu_ctx.matmul_forward_fused(a, b, h, residual=h, pre=z)
+            ref = (ref + p) % P
+            assert np.array_equal(h.download(), ref) and np.array_equal(z.download(), p)
+        out, parts = gpu_ctx.upload(R), [gpu_ctx.upload(R) for _ in range(3)]
+        gpu_ctx.gated_forward(a, b, c2, out, activation=RELU, gate=parts[0], act=parts[1], up=parts[2])
+        act = activate(p, RELU, 0)
+        for got, want in zip([out] + parts, (act * q % P, p, act, q)):
+            assert np.array_equal(got.download(), want)
