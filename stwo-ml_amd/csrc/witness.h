@@ -6,6 +6,7 @@
 
 #include "field.h"
 #include "gemm.h"
+#include "witness_sizes.h"
 
 namespace gkr {
 
@@ -32,7 +33,6 @@ __device__ __forceinline__ void activate(const ActArg& a, uint32_t (&z)[E]) {
 // rows past m; kOutside for columns past n) reads zero and is not written, with
 // no comparison for it.  A matrix that is not given has no bytes.
 typedef __amdgpu_buffer_rsrc_t WitBuffer;
-constexpr uint32_t kOutside = 0xfffffff0u;
 __device__ __forceinline__ WitBuffer wit_buffer(const uint32_t* p, uint64_t first, uint64_t count) {
   const uint64_t bytes = p && first < count ? 4 * (count - first) : 0;
   return __builtin_amdgcn_make_buffer_rsrc((void*)(p + (bytes ? first : 0)), 0,
@@ -180,7 +180,6 @@ __device__ __forceinline__ uint32_t digit_sum_mod_p(const int32_t (&s)[4]) {
 // us, also with sixteen waves for the gated pair's 432 column tiles).
 // W waves: sixteen, or eight, of which two workgroups fit a CU, where there are
 // more column tiles than CUs.
-constexpr uint32_t kRowLds = 65536;
 template <int MR, int PB, bool GATED, int W, class End>
 static __global__ void __launch_bounds__(64 * W, PB == 1 || !GATED ? 4 : 2)
     k_rows(const uint32_t* __restrict__ X, WitWeight w0, WitWeight w1, uint32_t m, uint32_t k, uint32_t n, End end) {
@@ -320,7 +319,7 @@ static __global__ void __launch_bounds__(64 * W, PB == 1 || !GATED ? 4 : 2)
   }
   const uint32_t r = threadIdx.x / 32, c = threadIdx.x % 32, column = ct * kGemmTile + c;
   const bool ok = r < m && column < n;
-  const uint32_t at[1] = {4 * (r * n + column)};  // below 2^32: sixteen rows of at most 2^26 words
+  const uint32_t at[1] = {4 * (r * n + column)};  // inside the buffer: few_rows_fit
   const uint32_t bias = end.column(column, ok);
   typename End::template Slot<1> slot;
   const typename End::Tile tile = end.tile(0, (uint64_t)m * n);

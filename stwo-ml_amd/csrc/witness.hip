@@ -48,11 +48,6 @@ static int activation_arg(gkr_ctx* c, const char* what, uint32_t tag, uint32_t l
   arg->mask = (1u << log_size) - 1;
   return GKR_OK;
 }
-// Longest inner size of the kernels here: a digit sum stays below 2^31.
-// Beyond it (no model's layer) the forward product's passes of K are used,
-// with the element-wise work in a launch behind.
-constexpr uint64_t kMaxInner = 131071;
-
 static WitWeight wit_weight(const gkr_matrix* w) { return WitWeight{w->bplanes, (uint32_t)w->bnplanes}; }
 
 static dim3 end_grid(uint64_t count) { return dim3((uint32_t)std::min<uint64_t>((count + 255) / 256, 1u << 20)); }
@@ -84,14 +79,8 @@ static int rows_product(gkr_ctx* c, const gkr_matrix* a, const gkr_matrix* w0, c
 #undef GKR_ROWS
   return check_launch(c);
 }
-// Whether k_rows takes it: up to four rows; five to sixteen by weights of one
-// plane while their digits fit in LDS at once (every workgroup makes them
-// again, which takes it longer beyond than a launch that packs them).
 static bool few_rows(const gkr_matrix* a, const gkr_matrix* w0, const gkr_matrix* w1) {
-  const uint64_t m = a->rows, k = a->cols;
-  if (k > kMaxInner || w0->cols > 1ull << 26) return false;
-  if (m <= 4) return true;
-  return m <= 16 && w0->bnplanes == 1 && w1->bnplanes == 1 && (m <= 8 ? 8 : 16) * 4 * ((k + 63) / 64 * 64) <= kRowLds;
+  return few_rows_fit(a->rows, a->cols, w0->cols, w0->bnplanes == 1 && w1->bnplanes == 1);
 }
 
 // Two masks of the packing, used in turn: the packing of one product clears the

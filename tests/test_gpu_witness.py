@@ -380,3 +380,25 @@ def test_block_ends(gpu_ctx, m, k, n):
         act = activate(p, RELU, 0)
         for got, want in zip([out] + parts, (act * q % P, p, act, q)):
             assert np.array_equal(got.download(), want)
+
+
+def test_sixteen_rows_of_the_most_columns(gpu_ctx):
+    """16 x 2^26 words, an output of 2^32 bytes, and one column fewer: the last words are there, with their
+    residual, and so are those of a gated block."""
+    rng = np.random.default_rng(7)
+    for n in (1 << 26, (1 << 26) - 1):
+        A, tail = words(rng, (16, 1), 1), 70
+        a, b = gpu_ctx.upload(A), gpu_ctx.synthetic(1, n, 1, 3)
+        res, out = gpu_ctx.synthetic(16, n, 0, 4), gpu_ctx.synthetic(16, n, 0, 5)
+
+        def last(m, row):  # the last words of a row
+            return gpu_ctx.wrap_device(m.device_ptr + 4 * (row * n + n - tail), 1, tail).download().astype(np.int64)[0]
+
+        B = last(b, 0)
+        gpu_ctx.matmul_forward_fused(a, b, out, residual=res)
+        for row in (0, 7, 15):
+            assert np.array_equal(last(out, row), (int(A[row, 0]) * B + last(res, row)) % P)
+        gpu_ctx.gated_forward(a, b, b, out, activation=0)
+        for row in (0, 15):
+            z = int(A[row, 0]) * B % P
+            assert np.array_equal(last(out, row), z * z % P)
