@@ -151,8 +151,9 @@ static int packed_product(gkr_ctx* c, const gkr_matrix* a, const gkr_matrix* w0,
   uint32_t *mask, *next_mask;
   TRY(wit_masks(c, &mask, &next_mask));
   g.mask = mask;
-  const dim3 pack_grid((uint32_t)((four_tiles * g.nsteps + 3) / 4));
-  GKR_LAUNCH(c, k_wit_pack, pack_grid, dim3(256), 0, a->dev, m, k, g.nsteps, packed,
+  static_assert(kProductStep == kGemmK, "packable");
+  const dim3 pack_grid((uint32_t)pack_groups(m, k));
+  GKR_LAUNCH(c, k_wit_pack, pack_grid, dim3(kPackThreads), 0, a->dev, m, k, g.nsteps, packed,
              const_cast<int8_t*>(g.four), mask, next_mask);
   TRY(check_launch(c));
 
@@ -234,12 +235,6 @@ static int packed_product(gkr_ctx* c, const gkr_matrix* a, const gkr_matrix* w0,
     TRY(check_launch(c));
   }
   return GKR_OK;
-}
-// Sizes that the packed product's grids take, and its 32-bit offsets of steps
-// and of a workgroup's rows (256 of 2^21 words).
-static bool packable(uint64_t m, uint64_t k, uint64_t n) {
-  return k <= kMaxInner && m <= 1ull << 22 && n <= 1ull << 21 && m * k <= 1ull << 34 &&
-         (m / 64 + 1) * (n / 128 + 1) <= 1ull << 21;
 }
 
 static int fused_forward(gkr_ctx* c, const gkr_matrix* a, const gkr_matrix* b, const gkr_matrix* bias, uint32_t tag,

@@ -24,4 +24,17 @@ inline bool few_rows_fit(uint64_t m, uint64_t k, uint64_t n, bool one_plane) {
   return one_plane && (m <= 8 ? 8 : 16) * 4 * ((k + 63) / 64 * 64) <= kRowLds;
 }
 
+constexpr uint64_t kProductStep = 32;     // K per operand block (gemm.h)
+constexpr uint64_t kPackThreads = 256;    // of k_wit_pack, a block of eight rows a wave
+inline uint64_t pack_groups(uint64_t m, uint64_t k) {
+  return ((m + 7) / 8 * ((k + kProductStep - 1) / kProductStep) + 3) / 4;
+}
+// Whether the packed product takes it: its grids (the packing's has fewer than
+// 2^32 threads, as any dimension), its 32-bit counts of blocks and its offsets
+// of steps and of a workgroup's rows (256 of 2^21 words).
+inline bool packable(uint64_t m, uint64_t k, uint64_t n) {
+  return k <= kMaxInner && m <= 1ull << 22 && n <= 1ull << 21 && pack_groups(m, k) * kPackThreads < 1ull << 32 &&
+         (m / 64 + 1) * (n / 128 + 1) <= 1ull << 21;
+}
+
 }  // namespace gkr

@@ -20,6 +20,8 @@ def lib():
     L = C.CDLL(OUT)
     L.ws_outside.restype = L.ws_row_lds.restype = C.c_uint32
     L.ws_max_inner.restype = C.c_uint64
+    L.ws_pack_groups.restype = C.c_uint64
+    L.ws_pack_groups.argtypes, L.ws_packable.argtypes = [C.c_uint64] * 2, [C.c_uint64] * 3
     L.ws_few_rows_fit.argtypes = [C.c_uint64, C.c_uint64, C.c_uint64, C.c_int]
     return L
 
@@ -48,3 +50,25 @@ def test_few_rows(lib):
     assert lib.ws_few_rows_fit(16, 1, (1 << 26) - 1, 1) and lib.ws_few_rows_fit(15, 1, 1 << 26, 1)
     assert lib.ws_few_rows_fit(4, 131071, 1 << 26, 0) and lib.ws_few_rows_fit(16, 1024, 5120, 1)
     assert lib.ws_few_rows_fit(8, 2048, 5120, 1) and not lib.ws_few_rows_fit(8, 2049, 5120, 1)
+
+
+def test_packed_product(lib):
+    """Every grid of a packed product that is admitted has fewer than 2^32 threads in a dimension: the packing's (131072
+    x 131071 words would have 2^32), and the products', a workgroup of up to 1024 threads for each group of row and
+    column tiles; a workgroup's rows and the packed blocks are counted in 32 bits."""
+    for m in around(5, 64, 512, 1 << 17, 1 << 20, 1 << 22):
+        for k in around(1, 1024, 4096, 16384, lib.ws_max_inner()):
+            groups = -(-(-(-m // 8) * -(-k // 32)) // 4)
+            assert lib.ws_pack_groups(m, k) == groups
+            for n in around(1, 128, 5120, 1 << 16, 1 << 21):
+                if not lib.ws_packable(m, k, n):
+                    continue
+                assert k <= lib.ws_max_inner() and 4 * 256 * n < 1 << 32
+                assert groups * 256 < 1 << 32 and 4 * groups < 1 << 32, (m, k)
+                assert -(-m // 64) * -(-n // 64) * 512 < 1 << 32  # blocks, four planes of both
+                runs = -(-m // 16) * -(-n // 32) // (1 << 21) + 1  # the streamed products' runs of row groups
+                assert runs < 65536 and (-(-m // 16) // runs + 1) * -(-n // 32) * 1024 < 1 << 32
+    for m, k in ((1 << 17, 131071), (1 << 22, 4096), (1 << 22, 4095), ((1 << 20) - 7, 16384)):
+        assert m * k <= 1 << 34 and not lib.ws_packable(m, k, 32)
+    for m, k, n in ((1 << 17, 131040, 32), (1 << 22, 4064, 32), (512, 13824, 5120), (5, 131071, 1 << 21)):
+        assert lib.ws_packable(m, k, n)
