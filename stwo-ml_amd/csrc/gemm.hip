@@ -17,7 +17,8 @@ static int digit_planes_needed(gkr_ctx* c, const uint32_t* X, uint64_t count, in
     GKR_LAUNCH(c, k_digit_mask<true>, grid, dim3(256), 0, X, count, dmask);
   else
     GKR_LAUNCH(c, k_digit_mask<false>, grid, dim3(256), 0, X, count, dmask);
-  HIP_TRY(hipGetLastError());
+  drain(c);
+  TRY(check_launch(c));  // refused on the launcher thread, it would leave no plane
   uint32_t mask = 0;
   HIP_TRY(hipMemcpyAsync(&mask, dmask, 4, hipMemcpyDeviceToHost, c->stream));
   HIP_TRY(hipStreamSynchronize(c->stream));
@@ -48,9 +49,10 @@ int weight_planes(gkr_ctx* c, gkr_matrix* b) {
   const uint64_t ntiles = (b->cols + kGemmTile - 1) / kGemmTile, nsteps = (b->rows + kGemmK - 1) / kGemmK;
   int8_t* d = nullptr;
   HIP_TRY(hipMalloc(&d, (size_t)np * ntiles * nsteps * kGemmBlockBytes));
-  const int rc = pack_planes(c, b->dev, b->cols, b->rows, true, np, d);
+  int rc = pack_planes(c, b->dev, b->cols, b->rows, true, np, d);
+  drain(c);
+  if (rc == GKR_OK) rc = check_launch(c);
   if (rc != GKR_OK) {
-    drain(c);
     (void)hipFree(d);
     return rc;
   }

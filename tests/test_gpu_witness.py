@@ -402,3 +402,27 @@ def test_sixteen_rows_of_the_most_columns(gpu_ctx):
         for row in (0, 15):
             z = int(A[row, 0]) * B % P
             assert np.array_equal(last(out, row), z * z % P)
+
+
+@pytest.mark.parametrize("callers_stream", [False, True])
+@pytest.mark.parametrize("launch", [1, 2])
+@pytest.mark.parametrize("m", [1, 40])
+def test_refused_launch_of_the_weights_planes(m, launch, callers_stream):
+    """A refused launch of those that make a weight's planes (which planes there are, their packing) fails the
+    call, and nothing of it is kept: the same call then gives the product, here of weights of four planes."""
+    rng = np.random.default_rng(m)
+    A, B = words(rng, (m, 300), 0), words(rng, (300, 70), 0)
+    for call in ("matmul_forward_fused", "matmul_forward_into", "gated_forward"):
+        ctx = G.Context(0, stream=0) if callers_stream else G.Context(0)
+        a, b, out = ctx.upload(A), ctx.upload(B), ctx.synthetic(m, 70, 0, 3)
+        args = (a, b, b, out) if call == "gated_forward" else (a, b, out)
+        kw = dict(activation=0) if call == "gated_forward" else {}
+        ctx.debug(G.DEBUG_REFUSE_LAUNCH, launch)
+        with pytest.raises(G.GkrError) as e:
+            getattr(ctx, call)(*args, **kw)
+        assert e.value.code == 2
+        ctx.debug(G.DEBUG_REFUSE_LAUNCH, 0)
+        getattr(ctx, call)(*args, **kw)
+        want = product(A, B)
+        assert np.array_equal(out.download(), want * want % P if call == "gated_forward" else want), call
+        ctx.close()
