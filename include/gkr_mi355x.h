@@ -97,6 +97,10 @@ int gkr_ctx_create(int device, gkr_ctx** out);  /* replaces GpuSumcheckExecutor:
  * returns (a context of its own stream issues them from a thread of its own). */
 int gkr_ctx_create_on_stream(int device, void* stream, gkr_ctx** out);
 void gkr_ctx_destroy(gkr_ctx* ctx);
+/* Waits for the context's work.  A launch that the runtime refused after the
+ * call that queued it had returned is told here, by gkr_matrix_download or by
+ * the context's next call, whichever comes first (GKR_ERR_DEVICE, once): what
+ * that call was to write is then not to be used. */
 int gkr_ctx_synchronize(gkr_ctx* ctx);
 /* Per-kernel timing (HIP events on the context stream), for benchmarks.
  * ids: 0 restrict_cols (weight and activation side of a matmul in one

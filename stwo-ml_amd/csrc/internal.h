@@ -451,15 +451,22 @@ struct HostTimer {
   }
 };
 void collect_timing(gkr_ctx* c);
+// Waits for the stream; a launch refused since the last check is an error here.
 int sync(gkr_ctx* c);
-// Launch errors of the calling thread and of c's launcher thread (the first
-// error its ring's launches returned), never another context's.
-inline int check_launch(gkr_ctx* c) {
-  hipError_t e = hipGetLastError();
-  if (e == hipSuccess && c && c->launcher) e = c->launcher->take_error();
+inline int launch_failed(gkr_ctx* c, hipError_t e) {
   if (e == hipSuccess) return GKR_OK;
   if (c) c->trip_count_valid = false;  // a launch that did not run has not counted its workgroups
   return fail(GKR_ERR_DEVICE, "kernel launch: %s", hipGetErrorString(e));
+}
+// Launch errors of c's launcher thread (the first error its ring's launches
+// returned), never another context's.
+inline int launcher_refusal(gkr_ctx* c) {
+  return launch_failed(c, c && c->launcher ? c->launcher->take_error() : hipSuccess);
+}
+// The same, and those of the calling thread.
+inline int check_launch(gkr_ctx* c) {
+  const hipError_t e = hipGetLastError();
+  return e == hipSuccess ? launcher_refusal(c) : launch_failed(c, e);
 }
 static inline unsigned grid_for(uint64_t n, uint64_t per_block = kBlock) {
   uint64_t g = (n + per_block - 1) / per_block;

@@ -106,7 +106,7 @@ void collect_timing(gkr_ctx* c) {
 int sync(gkr_ctx* c) {
   HIP_TRY(hipStreamSynchronize(c->stream));
   if (c->timing) collect_timing(c);
-  return GKR_OK;
+  return launcher_refusal(c);
 }
 
 PointArg make_point(const qm31* r, int n) {

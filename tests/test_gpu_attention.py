@@ -301,3 +301,31 @@ def test_refused_pools(gpu_ctx):
         with pytest.raises(G.GkrError) as e:
             gpu_ctx.kv_cache(heads, dim, n_pages=n_pages, page_tokens=page_tokens, max_seqs=1, max_tokens=64, int8=int8)
         assert e.value.code == 1, (n_pages, int8)
+
+
+@pytest.mark.parametrize("callers_stream", [False, True])
+@pytest.mark.parametrize("int8", [True, False])
+def test_every_refused_launch_is_told(int8, callers_stream):
+    """A refused launch of attention (its kernel's, its join's) fails the call or the wait behind it; the next
+    call writes the whole output again."""
+    ctx = G.Context(0, stream=0) if callers_stream else G.Context(0)
+    rng = np.random.default_rng(3)
+    cache = ctx.kv_cache(2, 64, n_pages=90, max_seqs=1, max_tokens=5001, int8=int8)
+    seqs, ks, vs = fill(ctx, cache, rng, [5001], 128, int8)
+    q = words(rng, (1, 384), int8)
+    qd = ctx.upload(q)
+    want = attend(q[0], ks[0], vs[0], 6, 2, 1 << 19, 20)[0]
+    for launch in (1, 2):
+        for wait in (ctx.synchronize, lambda: out.download()):
+            out = ctx.synthetic(1, 384, 0, launch)
+            ctx.debug(G.DEBUG_REFUSE_LAUNCH, launch)
+            with pytest.raises(G.GkrError) as e:
+                ctx.attention_forward(cache, qd, seqs, 6, out, score_offset=1 << 19)
+                wait()
+            assert e.value.code == 2, launch
+            ctx.debug(G.DEBUG_REFUSE_LAUNCH, 0)
+            out = ctx.synthetic(1, 384, 0, launch + 10)
+            ctx.attention_forward(cache, qd, seqs, 6, out, score_offset=1 << 19)
+            assert np.array_equal(out.download()[0], want), launch
+    cache.free()
+    ctx.close()

@@ -426,3 +426,32 @@ def test_refused_launch_of_the_weights_planes(m, launch, callers_stream):
         want = product(A, B)
         assert np.array_equal(out.download(), want * want % P if call == "gated_forward" else want), call
         ctx.close()
+
+
+@pytest.mark.parametrize("callers_stream", [False, True])
+@pytest.mark.parametrize("m,k,n,launches", [(1, 64, 96, 1), (40, 64, 96, 2), (300, 64, 96, 2), (200, 13825, 1030, 3)])
+def test_every_refused_launch_is_told(m, k, n, launches, callers_stream):
+    """Whichever launch of a product, of one kernel to three, is refused, the call or the wait behind it says so,
+    and the next call writes the whole output again."""
+    ctx = G.Context(0, stream=0) if callers_stream else G.Context(0)
+    rng = np.random.default_rng(m)
+    A, B = words(rng, (m, k), 0), words(rng, (k, n), 1)
+    a, b, want = ctx.upload(A), ctx.upload(B), product(A, B)
+    ctx.matmul_forward_fused(a, b, ctx.zeros(m, n))  # the planes are there
+    ctx.synchronize()
+    for call in ("matmul_forward_fused", "gated_forward"):
+        weights, kw, ref = ((b,), {}, want) if call == "matmul_forward_fused" else ((b, b), dict(activation=0), want * want % P)
+        for nth in range(1, launches + 1):
+            for wait in (ctx.synchronize, lambda: out.download()):
+                out = ctx.synthetic(m, n, 0, nth)
+                ctx.debug(G.DEBUG_REFUSE_LAUNCH, nth)
+                with pytest.raises(G.GkrError) as e:
+                    getattr(ctx, call)(a, *weights, out, **kw)
+                    wait()
+                assert e.value.code == 2, (call, nth)
+                ctx.debug(G.DEBUG_REFUSE_LAUNCH, 0)
+                ctx.synchronize()  # told once
+                out = ctx.synthetic(m, n, 0, nth + 10)
+                getattr(ctx, call)(a, *weights, out, **kw)
+                assert np.array_equal(out.download(), ref), (call, nth)
+    ctx.close()
