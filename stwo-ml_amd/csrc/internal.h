@@ -246,6 +246,11 @@ struct gkr_ctx {
   bool own_stream = true;  // false: the caller's (gkr_ctx_create_on_stream), not destroyed here
   void* buf[S_NSLOTS] = {};
   size_t cap[S_NSLOTS] = {};
+  // buffers whose address a captured graph of the caller's may hold, and those
+  // of them that were outgrown: freed with the context, as a replay may still
+  // come after it
+  bool in_graph[S_NSLOTS] = {};
+  std::vector<void*> outgrown;
   qm31* h_res = nullptr;  // pinned result staging (64 QM31)
   std::shared_ptr<MultRing> mring;  // LogUp multiplicities, host side (ensure_host_mult)
   uint32_t* h_mult = nullptr;  // the current activation layer's slot of mring (written by its table pass)

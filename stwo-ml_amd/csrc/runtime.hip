@@ -32,13 +32,18 @@ int ensure(gkr_ctx* c, Slot s, size_t bytes, void** out) {
     }
     return fail(GKR_ERR_NOMEM, "the allocation-free entry point needs device buffer %d (%zu bytes)", (int)s, bytes);
   }
+  hipStreamCaptureStatus capture = hipStreamCaptureStatusNone;
+  if (!c->own_stream && c->stream) HIP_TRY(hipStreamIsCapturing(c->stream, &capture));  // (the default stream never is)
+  if (capture != hipStreamCaptureStatusNone) c->in_graph[s] = true;
   if (c->cap[s] < bytes) {
     if (s == S_TRIPCNT) c->trip_count_valid = false;  // fresh memory must be zeroed
     if (s == S_MULT) c->mult_zero_entries = 0;
     if (s == S_TRIPMB) c->tripmb_valid = false;
-    if (c->buf[s]) HIP_TRY(hipFree(c->buf[s]));
+    if (c->buf[s] && c->in_graph[s]) c->outgrown.push_back(c->buf[s]);
+    else if (c->buf[s]) HIP_TRY(hipFree(c->buf[s]));
     c->buf[s] = nullptr;
     c->cap[s] = 0;
+    c->in_graph[s] = capture != hipStreamCaptureStatusNone;
     size_t want = bytes < 4096 ? 4096 : bytes;
     HIP_TRY(hipMalloc(&c->buf[s], want));
     c->cap[s] = want;
@@ -480,6 +485,7 @@ extern "C" void gkr_ctx_destroy(gkr_ctx* c) {
   for (gkr_kv_cache* k : c->caches) release_cache(k);
   for (int s = 0; s < S_NSLOTS; s++)
     if (c->buf[s]) (void)hipFree(c->buf[s]);
+  for (void* b : c->outgrown) (void)hipFree(b);
   for (auto& t : c->dev_tables) (void)hipFree(t.second);
   if (c->merkle_consts) (void)hipFree(c->merkle_consts);
   if (c->merkle_pairs) (void)hipFree(c->merkle_pairs);

@@ -455,3 +455,66 @@ def test_every_refused_launch_is_told(m, k, n, launches, callers_stream):
                 getattr(ctx, call)(a, *weights, out, **kw)
                 assert np.array_equal(out.download(), ref), (call, nth)
     ctx.close()
+
+
+def test_graph_replayed_after_larger_calls():
+    """A graph holds the addresses of the context's buffers: calls of larger sizes, which outgrow them, leave what
+    a replay writes and reads in place, so that it neither gives wrong words nor touches others' memory."""
+    from test_gpu_attention import attend
+
+    G.lib()
+    hip = ctypes.CDLL("libamdhip64.so.7")
+    vp, size = ctypes.c_void_p, ctypes.c_size_t
+    copy, stream, graph, run = hip.hipMemcpyAsync, vp(), vp(), vp()
+    copy.argtypes = [vp, vp, size, ctypes.c_int, vp]
+    hip.hipStreamBeginCapture.argtypes, hip.hipStreamEndCapture.argtypes = [vp, ctypes.c_int], [vp, ctypes.POINTER(vp)]
+    hip.hipGraphInstantiate.argtypes = [ctypes.POINTER(vp), vp, vp, vp, size]
+    hip.hipGraphLaunch.argtypes, hip.hipGraphExecDestroy.argtypes, hip.hipGraphDestroy.argtypes = [vp, vp], [vp], [vp]
+    assert hip.hipStreamCreate(ctypes.byref(stream)) == 0
+    ctx = G.Context(0, stream=stream.value)
+    rng = np.random.default_rng(21)
+    m, k, n, kv_len = 200, 5001, 300, 2000  # packed, with K splits that are joined
+    W = words(rng, (k, n), 1)
+    w, x, out = ctx.upload(W), ctx.zeros(m, k), ctx.zeros(m, n)
+    keys, values = words(rng, (kv_len, 64), 0), words(rng, (kv_len, 64), 0)
+    cache = ctx.kv_cache(1, 64, n_pages=200, max_seqs=3, max_tokens=9000)
+    seq, long = cache.new_sequence(), cache.new_sequence()
+    cache.append([seq], [kv_len], ctx.upload(keys), ctx.upload(values))
+    q, att = ctx.zeros(1, 128), ctx.zeros(1, 128)
+
+    def calls():
+        ctx.matmul_forward_fused(x, w, out)
+        ctx.attention_forward(cache, q, [seq], 2, att, score_offset=1 << 19)
+
+    calls()
+    ctx.synchronize()
+    thread_local = 1
+    assert hip.hipStreamBeginCapture(stream, thread_local) == 0
+    calls()
+    assert hip.hipStreamEndCapture(stream, ctypes.byref(graph)) == 0
+    assert hip.hipGraphInstantiate(ctypes.byref(run), graph, None, None, 0) == 0
+    others = []
+    for turn in range(4):
+        if turn:  # larger rows, K and splits than any before, and more of the heads' parts
+            M, K = 200 + 300 * turn, 5001 + 4000 * turn
+            A, B = words(rng, (M, K), 1), words(rng, (K, n), 1)
+            big = ctx.zeros(M, n)
+            ctx.matmul_forward_fused(ctx.upload(A), ctx.upload(B), big)
+            assert np.array_equal(big.download(), product(A, B))
+            more = words(rng, (2900, 64), 0)
+            cache.append([long], [2900], ctx.upload(more), ctx.upload(more))
+            wide = ctx.zeros(40 * turn, 128)
+            ctx.attention_forward(cache, ctx.zeros(40 * turn, 128), [long] * (40 * turn), 2, wide)
+            others += [ctx.zeros(1, e) for e in (1 << 16, 1 << 20, 1 << 22, 1 << 24)]  # where freed memory was
+        X, Q = words(rng, (m, k), turn % 2), words(rng, (1, 128), 0)
+        for dev, h in ((x, X), (q, Q)):
+            assert copy(dev.device_ptr, h.ctypes.data, h.nbytes, 1, stream) == 0
+        for _ in range(2):
+            assert hip.hipGraphLaunch(run, stream) == 0
+            assert np.array_equal(out.download(), product(X, W))
+            assert np.array_equal(att.download()[0], attend(Q[0], keys, values, 2, 1, 1 << 19, 20)[0])
+        assert not any(o.download().any() for o in others)
+    assert hip.hipGraphExecDestroy(run) == 0 and hip.hipGraphDestroy(graph) == 0
+    cache.free()
+    ctx.close()
+    assert hip.hipStreamDestroy(stream) == 0
