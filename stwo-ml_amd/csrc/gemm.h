@@ -408,6 +408,16 @@ static __global__ void __launch_bounds__(256) k_gemm_m31(const int8_t* __restric
     gemm_tile<1, 4, 1, 4>(Ap, a_plane_bytes, Bp, b_plane_bytes, m, n, nsteps, rt, ct, ctiles, s0, s1, out);
 }
 
+// 16 bytes a thread: `have` pieces of src, then zeros to `count` (a clear where
+// have is 0).  Kernels in place of copies and fills of the runtime's, whose
+// nodes in a captured graph are not to be relied on when it is replayed.
+static __global__ void __launch_bounds__(256) k_extend(const uint4* __restrict__ src, uint64_t have,
+                                                       uint4* __restrict__ dst, uint64_t count) {
+  for (uint64_t i = (uint64_t)blockIdx.x * 256 + threadIdx.x; i < count; i += (uint64_t)gridDim.x * 256)
+    dst[i] = i < have ? src[i] : make_uint4(0, 0, 0, 0);
+}
+inline dim3 extend_grid(uint64_t count) { return dim3((uint32_t)((count + 255) / 256 < 4096 ? (count + 255) / 256 : 4096)); }
+
 // C = sum over splits of the partials, mod P.
 static __global__ void k_gemm_reduce(const uint32_t* __restrict__ part, uint64_t count, int splits, uint32_t* __restrict__ C) {
   const uint64_t i = (uint64_t)blockIdx.x * blockDim.x + threadIdx.x;

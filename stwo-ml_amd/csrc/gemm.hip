@@ -76,12 +76,10 @@ int matmul_forward(gkr_ctx* c, const gkr_matrix* a, gkr_matrix* b, uint32_t* C) 
   if (!c->gemm_mask) {
     drain(c);
     uint32_t* w = nullptr;
-    HIP_TRY(hipMalloc(&w, 2 * sizeof(uint32_t)));
-    if (hipMemsetAsync(w, 0, 2 * sizeof(uint32_t), c->stream) != hipSuccess) {
-      (void)hipFree(w);
-      return fail(GKR_ERR_DEVICE, "clear of the digit masks failed");
-    }
+    HIP_TRY(hipMalloc(&w, 16));
     c->gemm_mask = w;
+    GKR_LAUNCH(c, k_extend, dim3(1), dim3(256), 0, nullptr, 0, (uint4*)w, 1);  // not run, all planes are taken to be there
+    HIP_TRY(hipGetLastError());
   }
   uint32_t* amask = c->gemm_mask + (c->gemm_turn & 1);
   uint32_t* next_mask = c->gemm_mask + (~c->gemm_turn & 1);
@@ -91,8 +89,10 @@ int matmul_forward(gkr_ctx* c, const gkr_matrix* a, gkr_matrix* b, uint32_t* C) 
   if (PB > b->bnplanes) {  // a 2- or 3-plane weight: extend with zero planes in scratch
     int8_t* ext;
     TRY(ensureT(c, S_GEMMB, (size_t)4 * b_plane, &ext));
-    HIP_TRY(hipMemcpyAsync(ext, b->bplanes, (size_t)b->bnplanes * b_plane, hipMemcpyDeviceToDevice, c->stream));
-    HIP_TRY(hipMemsetAsync(ext + (size_t)b->bnplanes * b_plane, 0, (size_t)(4 - b->bnplanes) * b_plane, c->stream));
+    const uint64_t count = 4 * b_plane / 16;
+    GKR_LAUNCH(c, k_extend, extend_grid(count), dim3(256), 0, (const uint4*)b->bplanes, b->bnplanes * b_plane / 16,
+               (uint4*)ext, count);
+    HIP_TRY(hipGetLastError());
     bp = ext;
   }
   const uint64_t waves = rtiles * ctiles, blocks_x = (waves + 3) / 4;

@@ -92,11 +92,10 @@ static int wit_masks(gkr_ctx* c, uint32_t** mask, uint32_t** next_mask) {
     drain(c);
     uint32_t* w = nullptr;
     HIP_TRY(hipMalloc(&w, 2 * words * sizeof(uint32_t)));
-    if (hipMemsetAsync(w, 0, 2 * words * sizeof(uint32_t), c->stream) != hipSuccess) {
-      (void)hipFree(w);
-      return fail(GKR_ERR_DEVICE, "clear of the digit masks failed");
-    }
     c->wit_mask = w;
+    const uint64_t count = 2 * words * sizeof(uint32_t) / 16;
+    GKR_LAUNCH(c, k_extend, extend_grid(count), dim3(256), 0, nullptr, 0, (uint4*)w, count);
+    TRY(check_launch(c));
   }
   *mask = c->wit_mask + (c->wit_turn & 1) * words;
   *next_mask = c->wit_mask + (~c->wit_turn & 1) * words;

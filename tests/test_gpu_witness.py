@@ -518,3 +518,64 @@ def test_graph_replayed_after_larger_calls():
     cache.free()
     ctx.close()
     assert hip.hipStreamDestroy(stream) == 0
+
+
+def test_captured_products_of_two_and_three_planes():
+    """The forward product by weights of two and three digit planes, which it extends to four in scratch, and a
+    fused product beyond the longest inner size, which takes the same path, captured and replayed with other
+    products in between that leave other planes there."""
+    G.lib()
+    hip = ctypes.CDLL("libamdhip64.so.7")
+    vp, size = ctypes.c_void_p, ctypes.c_size_t
+    copy, stream, graph, run = hip.hipMemcpyAsync, vp(), vp(), vp()
+    copy.argtypes = [vp, vp, size, ctypes.c_int, vp]
+    hip.hipStreamBeginCapture.argtypes, hip.hipStreamEndCapture.argtypes = [vp, ctypes.c_int], [vp, ctypes.POINTER(vp)]
+    hip.hipGraphInstantiate.argtypes = [ctypes.POINTER(vp), vp, vp, vp, size]
+    hip.hipGraphLaunch.argtypes, hip.hipGraphExecDestroy.argtypes, hip.hipGraphDestroy.argtypes = [vp, vp], [vp], [vp]
+    assert hip.hipStreamCreate(ctypes.byref(stream)) == 0
+    ctx = G.Context(0, stream=stream.value)
+    rng = np.random.default_rng(31)
+    shapes = ((33, 700, 90, 12), (5, 900, 200, 20), (3, 131073, 6, 12))
+    weights = [rng.integers(0, 1 << bits, size=(k, n), dtype=np.uint32) for _, k, n, bits in shapes]
+    ws = [ctx.upload(w) for w in weights]
+    xs, outs = [ctx.zeros(m, k) for m, k, _, _ in shapes], [ctx.zeros(m, n) for m, _, n, _ in shapes]
+    X = words(rng, (20, 700), 0)
+    full = words(rng, (700, 2500), 0)
+    full[:, ::2] = rng.integers(0, 1 << 20, size=(700, 1250))
+    other = rng.integers(0, 1 << 22, size=(131073, 40), dtype=np.uint32)
+    xo, wo, fo, oo = ctx.upload(words(rng, (3, 131073), 0)), ctx.upload(other), ctx.upload(full), ctx.zeros(3, 40)
+
+    def calls():
+        for i, (m, k, n, _) in enumerate(shapes):
+            if k > 131071:
+                ctx.matmul_forward_fused(xs[i], ws[i], outs[i], activation=RELU)
+            else:
+                ctx.matmul_forward_into(xs[i], ws[i], outs[i])
+
+    def between():
+        ctx.matmul_forward_into(xo, wo, oo)
+        out = ctx.zeros(20, 2500)
+        ctx.matmul_forward_into(ctx.upload(X), fo, out)
+        return out
+
+    between()
+    calls()
+    ctx.synchronize()
+    thread_local = 1
+    assert hip.hipStreamBeginCapture(stream, thread_local) == 0
+    calls()
+    assert hip.hipStreamEndCapture(stream, ctypes.byref(graph)) == 0
+    assert hip.hipGraphInstantiate(ctypes.byref(run), graph, None, None, 0) == 0
+    for turn in range(5):
+        host = [words(rng, (m, k), turn % 2) for m, k, _, _ in shapes]
+        for x, h in zip(xs, host):
+            assert copy(x.device_ptr, h.ctypes.data, h.nbytes, 1, stream) == 0
+        assert hip.hipGraphLaunch(run, stream) == 0
+        for i, (_, k, _, _) in enumerate(shapes):
+            z = product(host[i], weights[i])
+            assert np.array_equal(outs[i].download(), activate(z, RELU, 0) if k > 131071 else z), (turn, i)
+        if turn != 3:
+            assert np.array_equal(between().download(), product(X, full))
+    assert hip.hipGraphExecDestroy(run) == 0 and hip.hipGraphDestroy(graph) == 0
+    ctx.close()
+    assert hip.hipStreamDestroy(stream) == 0
