@@ -329,3 +329,34 @@ def test_every_refused_launch_is_told(int8, callers_stream):
             assert np.array_equal(out.download()[0], want), launch
     cache.free()
     ctx.close()
+
+
+@pytest.mark.parametrize("int8,kv", [(True, 4), (False, 1)])
+@pytest.mark.parametrize("short", [0, 1, 256])
+def test_longest_shares(gpu_ctx, int8, kv, short):
+    """128 rows of 131072 tokens, about the steps at which a workgroup's share is longest (255 of 256 tokens) and
+    then more workgroups than fit; weights and values whose lowest digits are -128, so that a share's digit sums
+    are at their largest, beside random ones."""
+    d, n, rows = 16, 131072, 128
+    rng = np.random.default_rng(short)
+    cache = gpu_ctx.kv_cache(kv, d, n_pages=n // 1024, page_tokens=1024, max_seqs=1, max_tokens=n, int8=int8)
+    k, v = words(rng, (n, kv * d), int8), words(rng, (n, kv * d), int8)
+    v[:, ::2] = P - (128 if int8 else 128 * 65793)
+    seq = cache.new_sequence()
+    cache.append([seq], [n], gpu_ctx.upload(k), gpu_ctx.upload(v))
+    lens = [n] * rows
+    lens[77] = 256 * (512 - short) - (short != 0)
+    q = np.zeros((rows, kv * d), np.uint32)  # scores are the offset: weights of 128
+    q[5], q[77] = words(rng, (kv * d,), int8), words(rng, (kv * d,), int8)
+    out, weighted, sums = (gpu_ctx.synthetic(rows, c, 0, 1) for c in (kv * d, kv * d, kv))
+    gpu_ctx.attention_forward(cache, gpu_ctx.upload(q), [seq] * rows, kv, out, lens=lens, score_offset=7 << 16,
+                              weighted=weighted, sums=sums)
+    got = out.download(), weighted.download(), sums.download()
+    for i in (0, 5, 77):
+        want = attend(q[i], k[:lens[i]], v[:lens[i]], kv, kv, 7 << 16, 20)
+        for j in (range(rows) if i == 0 else (i,)):
+            if i == 0 and j in (5, 77):
+                continue
+            for g, w in zip(got, want):
+                assert np.array_equal(g[j], w), j
+    cache.free()

@@ -579,3 +579,23 @@ def test_captured_products_of_two_and_three_planes():
     assert hip.hipGraphExecDestroy(run) == 0 and hip.hipGraphDestroy(graph) == 0
     ctx.close()
     assert hip.hipStreamDestroy(stream) == 0
+
+
+@pytest.mark.parametrize("m,k,n", [(1, 576, 192), (9, 300, 70), (40, 900, 333), (200, 2605, 5101), (300, 500, 4099),
+                                   (3, 131073, 5)])
+@pytest.mark.parametrize("wk", [1, 0])
+def test_every_call_writes_every_output(gpu_ctx, m, k, n, wk):
+    """Calls over outputs that hold other words each time, by weights whose planes are built and whose masks the
+    calls before have left set or clear."""
+    rng = np.random.default_rng(m)
+    B, C2 = words(rng, (k, n), wk), words(rng, (k, n), wk)
+    b, c2 = gpu_ctx.upload(B), gpu_ctx.upload(C2)
+    for turn, xk in enumerate((1, 0, 0, 1, 1)):
+        A = words(rng, (m, k), xk)
+        a, outs = gpu_ctx.upload(A), [gpu_ctx.synthetic(m, n, 0, 10 * turn + i) for i in range(6)]
+        gpu_ctx.matmul_forward_fused(a, b, outs[0], activation=GELU, pre=outs[1])
+        gpu_ctx.gated_forward(a, b, c2, outs[2], gate=outs[3], act=outs[4], up=outs[5])
+        z, u = product(A, B), product(A, C2)
+        act = activate(z, SILU, 0)
+        for i, (got, want) in enumerate(zip(outs, (activate(z, GELU, 0), z, act * u % P, z, act, u))):
+            assert np.array_equal(got.download(), want), (turn, i)
