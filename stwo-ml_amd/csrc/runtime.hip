@@ -453,7 +453,7 @@ static int create_context(int device, bool own_stream, hipStream_t stream, gkr_c
 }
 extern "C" int gkr_ctx_create(int device, gkr_ctx** out) { return create_context(device, true, nullptr, out); }
 extern "C" int gkr_ctx_create_on_stream(int device, void* stream, gkr_ctx** out) {
-  return create_context(device, false, (hipStream_t)stream, out);
+  return guarded([&] { return create_context(device, false, (hipStream_t)stream, out); });
 }
 extern "C" void gkr_ctx_destroy(gkr_ctx* c) {
   if (!c) return;
@@ -621,8 +621,12 @@ extern "C" int gkr_matrix_zeros(gkr_ctx* c, uint64_t rows, uint64_t cols, gkr_ma
     (void)hipFree(d);
     return fail(GKR_ERR_DEVICE, "matrix of zeros: %s", hipGetErrorString(e));
   }
-  *out = new_matrix(c, d, rows, cols, true);
-  return GKR_OK;
+  const int rc = guarded([&]() -> int {
+    *out = new_matrix(c, d, rows, cols, true);
+    return GKR_OK;
+  });
+  if (rc != GKR_OK) (void)hipFree(d);
+  return rc;
 }
 extern "C" int gkr_matrix_download(gkr_ctx* c, const gkr_matrix* m, uint32_t* host) {
   if (!c || !m || !host) return fail(GKR_ERR_INVALID, "null argument");
@@ -665,9 +669,9 @@ extern "C" int gkr_matrix_invalidate(gkr_ctx* c, gkr_matrix* m) {
   return drop_derived(c, m);
 }
 gkr_matrix* new_matrix(gkr_ctx* c, uint32_t* dev, uint64_t rows, uint64_t cols, bool owned) {
-  gkr_matrix* m = new gkr_matrix{c, dev, rows, cols, owned};
-  c->matrices.insert(m);
-  return m;
+  std::unique_ptr<gkr_matrix> m(new gkr_matrix{c, dev, rows, cols, owned});
+  c->matrices.insert(m.get());
+  return m.release();
 }
 extern "C" uint32_t gkr_synthetic_value(int kind, uint64_t seed, uint64_t i) { return synth_value(kind, seed, i); }
 
