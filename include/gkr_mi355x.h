@@ -413,7 +413,8 @@ int gkr_gated_forward(gkr_ctx* ctx, const gkr_matrix* a, const gkr_matrix* wg, c
  * by up to max_seqs sequences of up to max_tokens tokens (at most 2^21).  The
  * pages hold digit planes in the matrix cores' operand order: four bytes a
  * value, or one in an int8 cache (int8 != 0), whose values are -128 .. 127 as
- * words.  The cache belongs to its context; sequences are small numbers.     */
+ * words.  The cache belongs to its context; sequences are small numbers.  Pools
+ * of more than 2^48 bytes are GKR_ERR_INVALID, more than there is GKR_ERR_NOMEM. */
 typedef struct gkr_kv_cache gkr_kv_cache;
 int gkr_kv_cache_new(gkr_ctx* ctx, uint32_t n_kv_heads, uint32_t head_dim, uint32_t n_pages, uint32_t page_tokens,
                      uint32_t max_seqs, uint32_t max_tokens, int int8, gkr_kv_cache** out);
