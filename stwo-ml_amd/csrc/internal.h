@@ -54,11 +54,16 @@ int fail(int code, const char* fmt, ...);
 // context `c` in scope (launcher.h), so it never overtakes a launch queued
 // before it on that context.  HIP_CHECK is for calls that touch no stream
 // or device memory (device queries), made where no context exists yet.
+// The runtime keeps a failed call's error for hipGetLastError, where the next
+// call's check_launch would take it for its own launch's: it is taken here.
 #define HIP_CHECK(expr)                                                                     \
   do {                                                                                      \
     hipError_t e_ = (expr);                                                                 \
-    if (e_ != hipSuccess) return fail(GKR_ERR_DEVICE, "%s: %s (%s:%d)", #expr,              \
-                                      hipGetErrorString(e_), __FILE__, __LINE__);           \
+    if (e_ != hipSuccess) {                                                                 \
+      (void)hipGetLastError();                                                              \
+      return fail(GKR_ERR_DEVICE, "%s: %s (%s:%d)", #expr,                                  \
+                  hipGetErrorString(e_), __FILE__, __LINE__);                               \
+    }                                                                                       \
   } while (0)
 #define HIP_TRY(expr) \
   do {                \

@@ -599,3 +599,28 @@ def test_every_call_writes_every_output(gpu_ctx, m, k, n, wk):
         act = activate(z, SILU, 0)
         for i, (got, want) in enumerate(zip(outs, (activate(z, GELU, 0), z, act * u % P, z, act, u))):
             assert np.array_equal(got.download(), want), (turn, i)
+
+
+@pytest.mark.parametrize("callers_stream", [False, True])
+def test_an_allocation_that_fails_is_told_once(callers_stream):
+    """More memory than there is fails its own call; the calls behind it are not taken to have failed."""
+    ctx = G.Context(0, stream=0) if callers_stream else G.Context(0)
+    rng = np.random.default_rng(2)
+    A, B = words(rng, (3, 64), 1), words(rng, (64, 50), 1)
+    a, b = ctx.upload(A), ctx.upload(B)
+    cache = ctx.kv_cache(1, 16, n_pages=2, max_seqs=1, max_tokens=128)
+    seq, kv = cache.new_sequence(), ctx.upload(words(rng, (1, 16), 0))
+    for call in (lambda: ctx.zeros(1 << 19, 1 << 20), lambda: ctx.synthetic(1 << 19, 1 << 20, 1, 1),
+                 lambda: ctx.kv_cache(8, 128, n_pages=1 << 24, max_seqs=1, max_tokens=64)):
+        for behind in ("product", "append"):
+            with pytest.raises(G.GkrError):
+                call()
+            if behind == "append":
+                cache.append([seq], [1], kv, kv)
+            out = ctx.synthetic(3, 50, 0, 1)
+            ctx.matmul_forward_fused(a, b, out)
+            ctx.synchronize()
+            assert np.array_equal(out.download(), product(A, B))
+    assert cache.length(seq) == 3
+    cache.free()
+    ctx.close()
