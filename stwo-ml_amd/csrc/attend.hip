@@ -43,7 +43,6 @@ extern "C" int gkr_kv_cache_new(gkr_ctx* c, uint32_t kv_heads, uint32_t dim, uin
   gkr_kv_cache* k = nullptr;
   const int rc = guarded([&]() -> int {
     k = new gkr_kv_cache{c};
-    k->book.reset(new KvBook(n_pages, page_tokens, max_seqs, max_tokens));
     k->pool.width = width;
     k->pool.page_blocks = page_tokens / kAttBlock;
     k->pool.kv_heads = kv_heads;
@@ -64,6 +63,15 @@ extern "C" int gkr_kv_cache_new(gkr_ctx* c, uint32_t kv_heads, uint32_t dim, uin
     (void)hipGetLastError();
     gkr_kv_cache_free(k);
     return fail(GKR_ERR_NOMEM, "key-value cache: two pools of %llu bytes", (unsigned long long)bytes);
+  }
+  // after the pools: four bytes a page on the host, 16 GB for the most that can be asked for
+  const int booked = guarded([&]() -> int {
+    k->book.reset(new KvBook(n_pages, page_tokens, max_seqs, max_tokens));
+    return GKR_OK;
+  });
+  if (booked != GKR_OK) {
+    gkr_kv_cache_free(k);
+    return booked;
   }
   k->pool.pages = k->table;
   *k->bad = 0;

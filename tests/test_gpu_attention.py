@@ -1,6 +1,8 @@
 """Attention over the paged key-value cache (gkr_kv_cache_*, gkr_attention_forward) against whole-number
 arithmetic: head layouts, lengths from none to many pages, appends token by token and in runs, sequences that
 share rows, full-range and int8 caches, every output, and what is refused."""
+import resource
+
 import numpy as np
 import pytest
 
@@ -360,3 +362,12 @@ def test_longest_shares(gpu_ctx, int8, kv, short):
             for g, w in zip(got, want):
                 assert np.array_equal(g[j], w), j
     cache.free()
+
+
+def test_pools_that_do_not_fit_take_no_host_memory(gpu_ctx):
+    """The most pages that can be asked for, 4 TB of pools: refused before the host's book of them is made."""
+    before = resource.getrusage(resource.RUSAGE_SELF).ru_maxrss
+    with pytest.raises(G.GkrError) as e:
+        gpu_ctx.kv_cache(1, 1, n_pages=(1 << 32) - 1, max_seqs=1, max_tokens=64, int8=True)
+    assert e.value.code == 4
+    assert resource.getrusage(resource.RUSAGE_SELF).ru_maxrss - before < 1 << 20  # KiB
