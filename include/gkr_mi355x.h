@@ -408,6 +408,66 @@ int gkr_gated_forward(gkr_ctx* ctx, const gkr_matrix* a, const gkr_matrix* wg, c
                       uint32_t activation_type, uint32_t table_log_size, gkr_matrix* gate, gkr_matrix* act,
                       gkr_matrix* up, gkr_matrix* out);
 
+/* Products whose results are brought back to few bits, by whole scales r of the
+ * rows and s of the columns (any canonical words, as numbers 0 .. P - 1; NULL: 1):
+ *   Z = A B (mod P),  t = round(c(Z_ij) r_i s_j / 2^shift) + c(bias_j),
+ *   Y = t cut off at +-limit, + residual (mod P)
+ * with centered values c and halves rounded away from zero, exact for any words
+ * (shift 0 .. 63; limit 1 .. 2^30 - 1, 0 = 2^30 - 1).  With a limit of 127 or less
+ * Y are words that an int8 cache takes.  A is m x k, B k x n, row_scales m x 1,
+ * col_scales and bias 1 x n, residual, pre (Z) and out (Y) m x n; the residual may
+ * be the output itself.
+ *
+ * gkr_matmul_forward_quantized brings each row of A to 8 bits first: with a_i the
+ * largest |c(x)| of row i, q = round(c(x) levels / a_i) (0 where a_i = 0; levels
+ * 1 .. 127), Z = Q B and r_i = a_i.  x is about q a_i / levels, so 1 / levels belongs
+ * into the columns' scales.  Q into quantized (m x k) and a into row_scales (m x 1),
+ * where given: a walk's MatMul layer over Q and B proves Z.                     */
+int gkr_matmul_forward_scaled(gkr_ctx* ctx, const gkr_matrix* a, const gkr_matrix* b, const gkr_matrix* row_scales,
+                              const gkr_matrix* col_scales, uint32_t shift, uint32_t limit, const gkr_matrix* bias,
+                              const gkr_matrix* residual, gkr_matrix* pre, gkr_matrix* out);
+int gkr_matmul_forward_quantized(gkr_ctx* ctx, const gkr_matrix* a, const gkr_matrix* b, uint32_t levels,
+                                 const gkr_matrix* col_scales, uint32_t shift, uint32_t limit, const gkr_matrix* bias,
+                                 const gkr_matrix* residual, gkr_matrix* quantized, gkr_matrix* row_scales,
+                                 gkr_matrix* pre, gkr_matrix* out);
+
+/* Rotary positions.  A pair (x0, x1) of a head's values at a token of position p is
+ * turned by p f_i, f_i a whole number of 2^-64 turns a position (whole turns drop
+ * out, so the angles of far positions are exact):
+ *   y0 = round((c(x0) C - c(x1) S) / 2^shift), y1 = round((c(x1) C + c(x0) S) / 2^shift),
+ *   C = round(amplitude cos 2 pi p f_i), S = round(amplitude sin 2 pi p f_i)
+ * with halves rounded away from zero; amplitude 1 .. 2^30 (2^shift keeps lengths; a
+ * context's attention factor goes into it), shift 0 .. 30.
+ *
+ * gkr_rotary_frequencies (host): f_i = base^(-2 i / turned) / 2 pi turns, i < turned / 2,
+ *   PLAIN; LINEAR: divided by the factor; BASE: with the base times factor^(turned /
+ *   (turned - 2)); WAVES: with w = positions f_i waves in the context that was trained
+ *   on, divided by the factor where w <= low, kept where w >= high, and in between
+ *   f_i (g + (1 - g) / factor) with g = (w - low) / (high - low).  NULL: PLAIN.
+ * gkr_rotary_new: the table of C and S, eight bytes a pair and position (0 .. positions
+ *   - 1), on the context's device; the call returns when it is there.
+ * gkr_rotary_forward: counts[i] rows of sequence i at positions starts[i], starts[i] + 1
+ *   .. (NULL: 0 ..), the rows of q and, where given, of k in that order; their number
+ *   is the sum of the counts.  A row is whole heads of head_dim words, the first
+ *   `turned` of which are turned: dims i and turned / 2 + i a pair, or 2 i and 2 i + 1
+ *   (interleaved != 0); the others are copied.  limit 1 .. 2^30 - 1 cuts the turned
+ *   values off at +-limit (127 for an int8 cache), 0 takes them mod P.  An output may
+ *   be its own input.                                                          */
+enum { GKR_ROTARY_PLAIN = 0, GKR_ROTARY_LINEAR = 1, GKR_ROTARY_BASE = 2, GKR_ROTARY_WAVES = 3 };
+typedef struct {
+  uint32_t kind;
+  double factor;               /* > 0; all but PLAIN */
+  double positions, low, high; /* WAVES: 0 <= low < high */
+} gkr_rotary_scaling;
+int gkr_rotary_frequencies(uint32_t turned, double base, const gkr_rotary_scaling* scaling, uint64_t* freqs);
+typedef struct gkr_rotary gkr_rotary;
+int gkr_rotary_new(gkr_ctx* ctx, const uint64_t* freqs, uint32_t turned, uint32_t amplitude, uint32_t shift,
+                   uint32_t positions, gkr_rotary** out);
+void gkr_rotary_free(gkr_rotary* rotary);
+int gkr_rotary_forward(gkr_ctx* ctx, const gkr_rotary* rotary, uint32_t head_dim, int interleaved,
+                       const uint32_t* starts, const uint32_t* counts, size_t n, uint32_t limit, const gkr_matrix* q,
+                       gkr_matrix* q_out, const gkr_matrix* k, gkr_matrix* k_out);
+
 /* A paged cache of keys and values: n_pages pages of page_tokens tokens (a
  * multiple of 64) for n_kv_heads heads of head_dim values (1 .. 256), shared
  * by up to max_seqs sequences of up to max_tokens tokens (at most 2^21).  The
@@ -451,6 +511,19 @@ int gkr_attention_forward(gkr_ctx* ctx, const gkr_kv_cache* cache, const gkr_mat
                           const uint32_t* lens, size_t n_rows, uint32_t n_heads, uint32_t score_offset,
                           uint32_t table_log_size, gkr_matrix* weighted, gkr_matrix* sums, gkr_matrix* scores,
                           gkr_matrix* out);
+
+/* Causal attention of whole prompts: counts[i] tokens of sequence i (0 .. 131071), the
+ * rows of q (n_heads * head_dim words, head_dim at most 256), k and v (n_kv_heads *
+ * head_dim) in that order; their number is the sum of the counts.  A token sees
+ * itself and those before it in its sequence; weights, means and the other outputs
+ * as gkr_attention_forward has them for a cache with those keys and values (any
+ * canonical words; int8-range ones take an eighth of the products).  A prompt that
+ * goes on in a cache is also appended to it; tokens behind cached ones are
+ * gkr_attention_forward's.                                                    */
+int gkr_attention_prompt(gkr_ctx* ctx, const gkr_matrix* q, const gkr_matrix* k, const gkr_matrix* v,
+                         const uint32_t* counts, size_t n_seqs, uint32_t n_heads, uint32_t n_kv_heads,
+                         uint32_t score_offset, uint32_t table_log_size, gkr_matrix* weighted, gkr_matrix* sums,
+                         gkr_matrix* scores, gkr_matrix* out);
 
 /* MLE commitments: Poseidon Merkle roots (engine/src/crypto/poseidon_merkle.rs:255-280,
  * root_only_parallel) over securefield_to_felt leaves (poseidon_channel.rs:59-69),

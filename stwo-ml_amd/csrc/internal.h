@@ -112,7 +112,7 @@ enum Slot {
   S_MULT, S_MIN, S_MOUT, S_D0, S_D1, S_W0, S_W1, S_E0, S_M0, S_M1, S_COLPART,
   S_MK0, S_MK1, S_MKSTEP, S_MKROOT, S_OPL, S_OPI, S_GEMMA, S_GEMMB, S_GEMMP, S_FA2, S_FB2, S_EQPARTS, S_TRIPCNT, S_TRIPMB, S_LKINV, S_LKHIST, S_LDIG, S_R8FLAG, S_PTWAIT, S_EXTA, S_EXTB, S_GRAM, S_NORMSUM, S_NORMROW,
   S_LKARENA, S_LKFOLD, S_LKDESC, S_LKPART, S_LKRES, S_LKTAB,
-  S_BIND, S_BINDEQ, S_BINDDESC, S_BINDPART, S_BINDRES, S_BINDVIRT, S_WITG, S_WITU, S_ATTP, S_NSLOTS
+  S_BIND, S_BINDEQ, S_BINDDESC, S_BINDPART, S_BINDRES, S_BINDVIRT, S_WITG, S_WITU, S_ATTP, S_QUANT, S_QSCALE, S_PROMPTK, S_PROMPTV, S_NSLOTS
 };
 // Timer ids: device kernels (HIP events) and host-side phases (Fiat-Shamir
 // hashing inside the reducers, waiting for trip results, waiting for the
@@ -211,6 +211,8 @@ int check_operands(gkr_ctx* c, const char* what, std::initializer_list<const gkr
 int check_shape(const char* what, const char* name, const gkr_matrix* m, uint64_t rows, uint64_t cols);
 // attend.hip: frees a cache's device memory (its handle stays).
 void release_cache(gkr_kv_cache* cache);
+// rotary.hip: the same of a table of turns.
+void release_rotary(gkr_rotary* rotary);
 
 struct gkr_qvec {
   gkr_ctx* ctx;
@@ -280,6 +282,7 @@ struct gkr_ctx {
   std::set<gkr_matrix*> matrices;  // live matrices; detached when the context is destroyed
   std::set<gkr_qvec*> qvecs;       // live QM31 vectors; detached likewise
   std::set<gkr_kv_cache*> caches;  // live key-value caches; detached likewise
+  std::set<gkr_rotary*> rotaries;  // live tables of turns; detached likewise
   uint64_t mult_zero_entries = 0;  // leading entries of S_MULT known to be zero once the queued work is done
   std::map<uint64_t, uint32_t*> dev_tables;  // (tag << 32 | log) -> resident device copy of the table outputs
   std::map<uint64_t, felt> table_commitments;  // (tag << 32 | log) -> poseidon_hash_many([tag, log])

@@ -1,0 +1,136 @@
+// Causal attention of whole prompts (kernels in prompt.h).
+#include "activations.h"
+#include "prompt.h"
+#include "witness_launch.h"
+
+static int attention_prompt(gkr_ctx* c, const gkr_matrix* q, const gkr_matrix* k, const gkr_matrix* v,
+                            const uint32_t* counts, size_t n_seqs, uint32_t heads, uint32_t kv_heads, uint32_t offset,
+                            uint32_t table_log, gkr_matrix* weighted, gkr_matrix* sums, gkr_matrix* scores,
+                            gkr_matrix* out) {
+  static const char what[] = "prompt attention";
+  if (!c || !q || !k || !v || !out || (n_seqs && !counts)) return fail(GKR_ERR_INVALID, "null argument");
+  TRY(check_operands(c, what, {q, k, v}, {weighted, sums, scores, out}));
+  if (kv_heads == 0 || kv_heads > 4096 || heads == 0 || heads % kv_heads || heads > 65535)
+    return fail(GKR_ERR_INVALID, "%s: %u query heads on %u kv heads (at most 65535 on 4096)", what, heads, kv_heads);
+  if (q->cols % heads || q->cols / heads > 256)
+    return fail(GKR_ERR_INVALID, "%s: q has %llu columns, not %u heads of at most 256", what,
+                (unsigned long long)q->cols, heads);
+  if (offset >= P) return fail(GKR_ERR_INVALID, "%s: the offset %u is not a canonical M31", what, offset);
+  if (table_log > 24) return fail(GKR_ERR_INVALID, "%s: a table of 2^%u entries (at most 2^24)", what, table_log);
+  if (table_log == 0) table_log = act_default_log_size(ACT_SOFTMAX);
+  const uint32_t dim = (uint32_t)(q->cols / heads), chunks = (dim + 15) / 16, group = heads / kv_heads;
+  uint64_t rows = 0, blocks = 0, longest = 0;
+  for (size_t i = 0; i < n_seqs; i++) {
+    if (counts[i] > kMaxPrompt || (uint64_t)counts[i] * group > 0x7fffffffull)
+      return fail(GKR_ERR_INVALID, "%s: a sequence of %u tokens of %u heads each (at most %u, and 2^31 rows)", what, counts[i],
+                  group, kMaxPrompt);
+    rows += counts[i];
+    blocks += (counts[i] + kAttBlock - 1) / kAttBlock;
+    longest = std::max<uint64_t>(longest, counts[i]);
+  }
+  TRY(check_shape(what, "q", q, rows, (uint64_t)heads * dim));
+  TRY(check_shape(what, "k", k, rows, (uint64_t)kv_heads * dim));
+  TRY(check_shape(what, "v", v, rows, (uint64_t)kv_heads * dim));
+  TRY(check_shape(what, "the output", out, rows, (uint64_t)heads * dim));
+  TRY(check_shape(what, "weighted", weighted, rows, (uint64_t)heads * dim));
+  TRY(check_shape(what, "sums", sums, rows, heads));
+  if (scores) {
+    TRY(check_shape(what, "scores", scores, rows * heads, scores->cols));
+    if (scores->cols < longest || scores->cols > kMaxTokens)
+      return fail(GKR_ERR_INVALID, "%s: scores of %llu columns for sequences of up to %llu tokens (at most 2^21)", what,
+                  (unsigned long long)scores->cols, (unsigned long long)longest);
+  }
+  if (blocks > 0xffffffffull) return fail(GKR_ERR_INVALID, "%s: too many tokens", what);
+  HIP_TRY(hipSetDevice(c->device));
+  for (gkr_matrix* m : {weighted, sums, scores, out})
+    if (m) TRY(drop_derived(c, m));
+  const uint64_t head_bytes = blocks * (4 * 1024 * chunks);
+  int8_t *kd, *vd;
+  TRY(ensureT(c, S_PROMPTK, head_bytes * kv_heads, &kd));
+  TRY(ensureT(c, S_PROMPTV, head_bytes * kv_heads, &vd));
+  uint32_t *mask, *next_mask;
+  TRY(wit_masks(c, &mask, &next_mask));
+
+  PromptPack pack{};
+  pack.kv_heads = kv_heads;
+  pack.dim = dim;
+  pack.chunks = chunks;
+  pack.head_bytes = head_bytes;
+  uint32_t in_launch = 0;
+  uint64_t row = 0, at = 0;
+  auto launch_pack = [&]() -> int {
+    if (in_launch == 0) return GKR_OK;
+    GKR_LAUNCH(c, k_prompt_pack, dim3(in_launch, kv_heads), dim3(256), 0, pack, k->dev, v->dev, kd, vd, mask, next_mask);
+    pack.n = in_launch = 0;
+    return check_launch(c);
+  };
+  for (size_t i = 0; i < n_seqs; i++) {
+    if (counts[i] == 0) continue;
+    const uint32_t some = (counts[i] + kAttBlock - 1) / kAttBlock;
+    auto& e = pack.e[pack.n++];
+    e.block0 = in_launch;
+    e.len = counts[i];
+    e.at = (uint32_t)at;
+    e.row = row;
+    in_launch += some;
+    at += some;
+    row += counts[i];
+    if (pack.n == kPromptSeqs || in_launch > 1u << 22) TRY(launch_pack());
+  }
+  TRY(launch_pack());
+
+  PromptArgs a{};
+  a.k = kd;
+  a.v = vd;
+  a.q = q->dev;
+  a.mask = mask;
+  a.o = AttOut{out->dev, weighted ? weighted->dev : nullptr, sums ? sums->dev : nullptr, scores ? scores->dev : nullptr,
+               scores ? scores->cols : 0};
+  a.head_bytes = head_bytes;
+  a.kv_heads = kv_heads;
+  a.group = group;
+  a.dim = dim;
+  a.chunks = chunks;
+  a.offset = offset;
+  a.table_mask = (1u << table_log) - 1;
+  uint32_t items = 0;
+  auto launch = [&]() -> int {
+    if (items == 0) return GKR_OK;
+    auto one = [&](auto kernel) { GKR_LAUNCH(c, kernel, dim3(items), dim3(256), 0, a); };
+    if (dim <= 64) {
+      one(k_prompt<1, 1, 1>);
+      one(k_prompt<4, 1, 1>);
+    } else if (dim <= 128) {
+      one(k_prompt<1, 2, 1>);
+      one(k_prompt<4, 2, 1>);
+    } else {
+      one(k_prompt<1, 4, 1>);
+      one(k_prompt<4, 4, 1>);
+    }
+    a.n = items = 0;
+    return check_launch(c);
+  };
+  row = at = 0;
+  for (size_t i = 0; i < n_seqs; i++) {
+    if (counts[i] == 0) continue;
+    auto& e = a.e[a.n++];
+    e.item0 = items;
+    e.tiles = (counts[i] * group + 63) / 64;
+    e.len = counts[i];
+    e.at = (uint32_t)at;
+    e.row = row;
+    items += e.tiles * kv_heads;
+    at += (counts[i] + kAttBlock - 1) / kAttBlock;
+    row += counts[i];
+    if (a.n == kPromptSeqs || items > 1u << 22) TRY(launch());
+  }
+  return launch();
+}
+extern "C" int gkr_attention_prompt(gkr_ctx* c, const gkr_matrix* q, const gkr_matrix* k, const gkr_matrix* v,
+                                    const uint32_t* counts, size_t n_seqs, uint32_t heads, uint32_t kv_heads,
+                                    uint32_t offset, uint32_t table_log, gkr_matrix* weighted, gkr_matrix* sums,
+                                    gkr_matrix* scores, gkr_matrix* out) {
+  return guarded([&] {
+    return attention_prompt(c, q, k, v, counts, n_seqs, heads, kv_heads, offset, table_log, weighted, sums, scores, out);
+  });
+}

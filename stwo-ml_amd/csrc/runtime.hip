@@ -483,6 +483,7 @@ extern "C" void gkr_ctx_destroy(gkr_ctx* c) {
     v->ctx = nullptr;
   }
   for (gkr_kv_cache* k : c->caches) release_cache(k);
+  for (gkr_rotary* r : c->rotaries) release_rotary(r);
   for (int s = 0; s < S_NSLOTS; s++)
     if (c->buf[s]) (void)hipFree(c->buf[s]);
   for (void* b : c->outgrown) (void)hipFree(b);

@@ -45,11 +45,12 @@ __device__ __forceinline__ void wit_write(WitBuffer b, uint32_t at, uint32_t x) 
   __builtin_amdgcn_raw_buffer_store_b32((int)x, b, (int)at, 0, 0);
 }
 
-// What happens to a sum of the product (fused) or a pair of sums (gated), for E
-// elements (byte offsets `at` into the Tile) of a thread.  fetch() sends out the
+// What happens to a sum of the product (fused, scaled) or a pair of sums (gated),
+// for E elements (byte offsets `at` into the Tile, matrix rows `row`: those of a
+// tile's elements past m may be more) of a thread.  fetch() sends out the
 // loads that need no sums, begin() takes the sums and sends out those that do,
 // finish() stores, so that the next elements' loads can go out before these
-// ones' stores.  `bias`: the column's.
+// ones' stores.  `c`: what is the columns'.
 struct FusedEnd {
   ActArg act;
   const uint32_t* bias;      // n
@@ -59,6 +60,9 @@ struct FusedEnd {
   struct Tile {
     WitBuffer residual, pre, out;
   };
+  struct Column {
+    uint32_t bias;
+  };
   template <int E>
   struct Slot {
     uint32_t z[E], y[E], residual[E];
@@ -66,18 +70,18 @@ struct FusedEnd {
   __device__ __forceinline__ Tile tile(uint64_t first, uint64_t count) const {
     return Tile{wit_buffer(residual, first, count), wit_buffer(pre, first, count), wit_buffer(out, first, count)};
   }
-  __device__ __forceinline__ uint32_t column(uint64_t col, bool ok) const { return bias && ok ? bias[col] : 0u; }
+  __device__ __forceinline__ Column column(uint64_t col, bool ok) const { return Column{bias && ok ? bias[col] : 0u}; }
   template <int E>
-  __device__ __forceinline__ void fetch(Slot<E>& s, const Tile& t, const uint32_t (&at)[E]) const {
+  __device__ __forceinline__ void fetch(Slot<E>& s, const Tile& t, const uint32_t (&at)[E], const uint32_t (&)[E]) const {
     if (residual) {
 #pragma unroll
       for (int e = 0; e < E; e++) s.residual[e] = wit_read(t.residual, at[e]);
     }
   }
   template <int E>
-  __device__ __forceinline__ void begin(Slot<E>& s, uint32_t b, const uint32_t (&z)[1][E]) const {
+  __device__ __forceinline__ void begin(Slot<E>& s, const Column (&c)[E], const uint32_t (&z)[1][E]) const {
 #pragma unroll
-    for (int e = 0; e < E; e++) s.y[e] = s.z[e] = m31_add(z[0][e], b);
+    for (int e = 0; e < E; e++) s.y[e] = s.z[e] = m31_add(z[0][e], c[e].bias);
     activate(act, s.y);
   }
   template <int E>
@@ -100,6 +104,7 @@ struct GatedEnd {
   struct Tile {
     WitBuffer gate, act, up, out;
   };
+  struct Column {};
   template <int E>
   struct Slot {
     uint32_t z[E], y[E], u[E];
@@ -108,11 +113,11 @@ struct GatedEnd {
     return Tile{wit_buffer(gate, first, count), wit_buffer(act_out, first, count), wit_buffer(up, first, count),
                 wit_buffer(out, first, count)};
   }
-  __device__ __forceinline__ uint32_t column(uint64_t, bool) const { return 0; }
+  __device__ __forceinline__ Column column(uint64_t, bool) const { return {}; }
   template <int E>
-  __device__ __forceinline__ void fetch(Slot<E>&, const Tile&, const uint32_t (&)[E]) const {}
+  __device__ __forceinline__ void fetch(Slot<E>&, const Tile&, const uint32_t (&)[E], const uint32_t (&)[E]) const {}
   template <int E>
-  __device__ __forceinline__ void begin(Slot<E>& s, uint32_t, const uint32_t (&z)[2][E]) const {
+  __device__ __forceinline__ void begin(Slot<E>& s, const Column (&)[E], const uint32_t (&z)[2][E]) const {
 #pragma unroll
     for (int e = 0; e < E; e++) {
       s.y[e] = s.z[e] = z[0][e];
@@ -138,6 +143,86 @@ struct GatedEnd {
     for (int e = 0; e < E; e++) wit_write(t.out, at[e], m31_mul(s.y[e], s.u[e]));
   }
 };
+// Rescaled sums: t = round(c(z) r s / 2^shift) + c(bias), halves away from zero,
+// cut off at +-limit, with the row's and the column's scale as whole numbers.
+// |c(z)| r is below 2^61 and its product with s below 2^92, held in three words;
+// what is left of it after the shift is needed to 32 bits only, as limit and
+// bias are below 2^30.
+struct ScaledEnd {
+  const uint32_t* row_scales;  // m, or none (1)
+  const uint32_t* col_scales;  // n, or none
+  const uint32_t* bias;        // n
+  const uint32_t* residual;    // m x n; may be out
+  uint32_t *pre, *out;
+  uint32_t shift, last_row;  // at most 63; m - 1
+  int32_t limit;
+  struct Tile {
+    WitBuffer residual, pre, out;
+  };
+  struct Column {
+    uint32_t scale, bias;
+  };
+  template <int E>
+  struct Slot {
+    uint32_t z[E], y[E], residual[E], row[E];
+  };
+  __device__ __forceinline__ Tile tile(uint64_t first, uint64_t count) const {
+    return Tile{wit_buffer(residual, first, count), wit_buffer(pre, first, count), wit_buffer(out, first, count)};
+  }
+  __device__ __forceinline__ Column column(uint64_t col, bool ok) const {
+    return Column{col_scales && ok ? col_scales[col] : 1u, bias && ok ? bias[col] : 0u};
+  }
+  template <int E>
+  __device__ __forceinline__ void fetch(Slot<E>& s, const Tile& t, const uint32_t (&at)[E], const uint32_t (&row)[E]) const {
+#pragma unroll
+    for (int e = 0; e < E; e++) s.row[e] = row_scales ? row_scales[umin32(row[e], last_row)] : 1u;
+    if (residual) {
+#pragma unroll
+      for (int e = 0; e < E; e++) s.residual[e] = wit_read(t.residual, at[e]);
+    }
+  }
+  __device__ __forceinline__ uint32_t scale(uint32_t z, uint32_t r, const Column& c) const {
+    const int32_t v = center_m31(z), sign = v >> 31;
+    const uint64_t a = (uint64_t)(uint32_t)((v ^ sign) - sign) * r, half = shift ? 1ull << (shift - 1) : 0;
+    const uint64_t low = (uint64_t)(uint32_t)a * c.scale, mid = (a >> 32) * c.scale + (low >> 32);  // < 2^61
+    // mid 2^32 + (low mod 2^32), rounded: the half's upper word is below 2^31
+    const uint64_t bottom = (low & 0xffffffffu) + (half & 0xffffffffu), top = mid + (half >> 32) + (bottom >> 32);
+    const uint64_t t = shift >= 32 ? top >> (shift - 32)
+                       : top >> shift ? ~0ull >> 1  // more than 32 bits are left
+                                      : (top << (32 - shift)) | ((uint32_t)bottom >> shift);
+    const int64_t y0 = (int64_t)(t < 0xffffffffull ? t : 0xffffffffull);
+    int64_t y = ((y0 ^ sign) - sign) + center_m31(c.bias);
+    y = y < -(int64_t)limit ? -(int64_t)limit : y > limit ? limit : y;
+    return (uint32_t)y + ((uint32_t)((int32_t)y >> 31) & P);
+  }
+  template <int E>
+  __device__ __forceinline__ void begin(Slot<E>& s, const Column (&c)[E], const uint32_t (&z)[1][E]) const {
+#pragma unroll
+    for (int e = 0; e < E; e++) {
+      s.z[e] = z[0][e];
+      s.y[e] = scale(z[0][e], s.row[e], c[e]);
+    }
+  }
+  template <int E>
+  __device__ __forceinline__ void finish(Slot<E>& s, const Tile& t, const uint32_t (&at)[E]) const {
+    if (pre) {
+#pragma unroll
+      for (int e = 0; e < E; e++) wit_write(t.pre, at[e], s.z[e]);
+    }
+    if (residual) {
+#pragma unroll
+      for (int e = 0; e < E; e++) s.y[e] = m31_add(s.y[e], s.residual[e]);
+    }
+#pragma unroll
+    for (int e = 0; e < E; e++) wit_write(t.out, at[e], s.y[e]);
+  }
+};
+// Columns of elements that share one.
+template <int E, class Column>
+__device__ __forceinline__ void same_column(Column (&c)[E], const Column& of) {
+#pragma unroll
+  for (int e = 0; e < E; e++) c[e] = of;
+}
 // A split's sums, into its part of each matrix.
 template <int NW, int E>
 __device__ __forceinline__ void wit_parts(uint32_t* part, uint32_t split, uint64_t first, uint64_t count,
@@ -320,10 +405,11 @@ static __global__ void __launch_bounds__(64 * W, PB == 1 || !GATED ? 4 : 2)
   const uint32_t r = threadIdx.x / 32, c = threadIdx.x % 32, column = ct * kGemmTile + c;
   const bool ok = r < m && column < n;
   const uint32_t at[1] = {4 * (r * n + column)};  // inside the buffer: few_rows_fit
-  const uint32_t bias = end.column(column, ok);
+  const uint32_t row[1] = {r};
+  const typename End::Column of_column[1] = {end.column(column, ok)};
   typename End::template Slot<1> slot;
   const typename End::Tile tile = end.tile(0, (uint64_t)m * n);
-  if (ok) end.fetch(slot, tile, at);
+  if (ok) end.fetch(slot, tile, at, row);
   __syncthreads();
   if (!ok) return;
   uint32_t z[NW][1];
@@ -337,7 +423,7 @@ static __global__ void __launch_bounds__(64 * W, PB == 1 || !GATED ? 4 : 2)
     }
     z[i][0] = m31_reduce64(t);
   }
-  end.begin(slot, bias, z);
+  end.begin(slot, of_column, z);
   end.finish(slot, tile, at);
 }
 
@@ -507,16 +593,18 @@ __device__ __forceinline__ void wit_tiles(const WitProduct& g, int32_t* sums, ui
   static_assert(E * 64 * W == ALL || E == 1, "whole elements");
   const uint32_t c = threadIdx.x % 32;
   const uint64_t col = (uint64_t)cg * 32 + c, first = (uint64_t)rg * (TILES * ROWS) * g.n + (uint64_t)cg * 32;
-  uint32_t at[E], rows[E];
+  uint32_t at[E], rows[E], row[E];
 #pragma unroll
   for (int e = 0; e < E; e++) {
     rows[e] = threadIdx.x / 32 + e * 2 * W;
+    row[e] = rg * (TILES * ROWS) + rows[e];
     at[e] = rows[e] < TILES * ROWS && col < g.n ? 4 * (rows[e] * (uint32_t)g.n + c) : kOutside;
   }
-  const uint32_t bias = end.column(col, col < g.n);
+  typename End::Column of_column[E];
+  same_column(of_column, end.column(col, col < g.n));
   typename End::template Slot<E> slot;
   const typename End::Tile tile = end.tile(first, plan.splits == 1 ? g.m * g.n : 0);
-  end.fetch(slot, tile, at);
+  end.fetch(slot, tile, at, row);
   __syncthreads();
 #pragma unroll
   for (int i = 0; i < RT; i++)
@@ -553,7 +641,7 @@ __device__ __forceinline__ void wit_tiles(const WitProduct& g, int32_t* sums, ui
     }
   }
   if (plan.splits == 1) {
-    end.begin(slot, bias, z);
+    end.begin(slot, of_column, z);
     end.finish(slot, tile, at);
   } else {
     wit_parts(g.part, split, first, g.m * g.n, at, z);
@@ -695,7 +783,8 @@ __device__ __forceinline__ void wit_block(const WitProduct& g, v4i* lds, uint32_
     const uint32_t c = lane & 31, hi = lane >> 5, odd = wc & 1;
     const int32_t* const low = (const int32_t*)lds + (wave & ~2u) * 4096;
     const uint64_t col0 = ((uint64_t)cg * CT + wc / 2) * 32;
-    const uint32_t bias = end.column(col0 + c, col0 + c < g.n);
+    typename End::Column of_column[E];
+    same_column(of_column, end.column(col0 + c, col0 + c < g.n));
 #pragma unroll
     for (uint32_t part = 0; part < 2; part++) {
       if (part) __syncthreads();
@@ -705,14 +794,16 @@ __device__ __forceinline__ void wit_block(const WitProduct& g, v4i* lds, uint32_
         for (int v = 0; v < 16; v++)
           mine[t * 1024 + (8 * (v / 4) + 4 * hi + v % 4) * 32 + c] = acc[part * 2 + t / 2][t % 2][v];
       __syncthreads();
-      const uint64_t first = (uint64_t)(rg * 8 + wr * 4 + part * 2 + odd) * ROWS * g.n + col0;
+      const uint32_t row0 = (rg * 8 + wr * 4 + part * 2 + odd) * ROWS;
+      const uint64_t first = (uint64_t)row0 * g.n + col0;
       const typename End::Tile tile = end.tile(plan.splits == 1 ? first : 0, plan.splits == 1 ? g.m * g.n : 0);
 #pragma unroll 1
       for (uint32_t r0 = 0; r0 < ROWS; r0 += 2 * E) {
-        uint32_t at[E], z[1][E];
+        uint32_t at[E], row[E], z[1][E];
 #pragma unroll
         for (int e = 0; e < E; e++) {
           const uint32_t r = r0 + 2 * e + hi;
+          row[e] = row0 + r;
           at[e] = col0 + c < g.n ? 4 * (r * (uint32_t)g.n + c) : kOutside;
           uint64_t sum = 0;
 #pragma unroll
@@ -731,8 +822,8 @@ __device__ __forceinline__ void wit_block(const WitProduct& g, v4i* lds, uint32_
         }
         if (plan.splits == 1) {
           typename End::template Slot<E> slot;
-          end.fetch(slot, tile, at);
-          end.begin(slot, bias, z);
+          end.fetch(slot, tile, at, row);
+          end.begin(slot, of_column, z);
           end.finish(slot, tile, at);
         } else {
           wit_parts(g.part, split, first, g.m * g.n, at, z);
@@ -755,7 +846,9 @@ __device__ __forceinline__ void wit_block(const WitProduct& g, v4i* lds, uint32_
     const uint32_t tile0 = rg * 8 + wr * 4 + (GATED ? part * TI : 0), c = lane & 31, hi = lane >> 5;
     const uint64_t col0 = ((uint64_t)cg * CT + (GATED ? wc : wc * 2 + part)) * 32;
     const uint64_t first = (uint64_t)tile0 * ROWS * g.n + col0;
-    const uint32_t bias = end.column(col0 + c, col0 + c < g.n), pitch = 8 * (uint32_t)g.n;  // bytes of two rows
+    typename End::Column of_column[E];
+    same_column(of_column, end.column(col0 + c, col0 + c < g.n));
+    const uint32_t pitch = 8 * (uint32_t)g.n;  // bytes of two rows
     const uint32_t at0 = col0 + c < g.n ? 4 * (hi * (uint32_t)g.n + c) : kOutside;
     const int32_t* const from = mine + hi * (FOUR ? 128 : 32) + c;
     // rows r0 + 2 e + hi, r0 a multiple of 16
@@ -782,11 +875,13 @@ __device__ __forceinline__ void wit_block(const WitProduct& g, v4i* lds, uint32_
       const typename End::Tile tile = end.tile(first, g.m * g.n);
       typename End::template Slot<E> slot[2];
       auto begin = [&](int i, uint32_t r0) {
-        uint32_t at[E], z[NW][E];
+        uint32_t at[E], row[E], z[NW][E];
         places(r0, at);
-        end.fetch(slot[i], tile, at);
+#pragma unroll
+        for (int e = 0; e < E; e++) row[e] = tile0 * ROWS + r0 + 2 * e + hi;
+        end.fetch(slot[i], tile, at, row);
         values(r0, z);
-        end.begin(slot[i], bias, z);
+        end.begin(slot[i], of_column, z);
       };
       auto finish = [&](int i, uint32_t r0) {
         uint32_t at[E];
@@ -864,14 +959,20 @@ static __global__ void __launch_bounds__(256) k_wit_join(WitProduct g, End end) 
   const uint64_t count = g.m * g.n;
   constexpr int E = 4;
   for (uint64_t first = (uint64_t)blockIdx.x * (256 * E); first < count; first += (uint64_t)gridDim.x * (256 * E)) {
-    const uint32_t column = (uint32_t)(first % g.n);
+    const uint32_t row0 = (uint32_t)(first / g.n), column0 = (uint32_t)(first - (uint64_t)row0 * g.n);
     uint64_t t[NW][E] = {};
-    uint32_t at[E], z[NW][E];
+    uint32_t at[E], row[E], z[NW][E];
+    typename End::Column of_column[E];
 #pragma unroll
-    for (int e = 0; e < E; e++) at[e] = 4 * (threadIdx.x + 256 * e);
+    for (int e = 0; e < E; e++) {
+      const uint32_t in = column0 + threadIdx.x + 256 * e;
+      row[e] = row0 + in / (uint32_t)g.n;
+      of_column[e] = end.column(in % (uint32_t)g.n, true);
+      at[e] = 4 * (threadIdx.x + 256 * e);
+    }
     typename End::template Slot<E> slot;
     const typename End::Tile tile = end.tile(first, count);
-    end.fetch(slot, tile, at);
+    end.fetch(slot, tile, at, row);
     for (uint32_t s0 = 0; s0 < splits; s0 += kJoinParts) {  // those past the last have no bytes and read zero
       uint32_t part[kJoinParts][NW][E];
 #pragma unroll
@@ -893,11 +994,8 @@ static __global__ void __launch_bounds__(256) k_wit_join(WitProduct g, End end) 
 #pragma unroll
     for (int x = 0; x < NW; x++)
 #pragma unroll
-      for (int e = 0; e < E; e++) {
-        z[x][e] = m31_reduce64(t[x][e]);
-        if (x == 0) z[0][e] = m31_add(z[0][e], end.column((column + threadIdx.x + 256 * e) % (uint32_t)g.n, true));
-      }
-    end.begin(slot, 0, z);
+      for (int e = 0; e < E; e++) z[x][e] = m31_reduce64(t[x][e]);
+    end.begin(slot, of_column, z);
     end.finish(slot, tile, at);
   }
 }
@@ -908,14 +1006,16 @@ static __global__ void __launch_bounds__(256) k_wit_end(const uint32_t* __restri
                                                         uint64_t count, uint64_t n, End end) {
   for (uint64_t first = (uint64_t)blockIdx.x * 256; first < count; first += (uint64_t)gridDim.x * 256) {
     const uint64_t i = first + threadIdx.x < count ? first + threadIdx.x : count - 1;
-    const uint32_t at[1] = {4 * threadIdx.x}, bias = end.column(i % n, true);
+    const uint64_t r = i / n;
+    const uint32_t at[1] = {4 * threadIdx.x}, row[1] = {(uint32_t)r};
+    const typename End::Column of_column[1] = {end.column(i - r * n, true)};
     uint32_t z[GATED ? 2 : 1][1];
     z[0][0] = z0[i];
     if constexpr (GATED) z[1][0] = z1[i];
     typename End::template Slot<1> slot;
     const typename End::Tile tile = end.tile(first, count);
-    end.fetch(slot, tile, at);
-    end.begin(slot, bias, z);
+    end.fetch(slot, tile, at, row);
+    end.begin(slot, of_column, z);
     end.finish(slot, tile, at);
   }
 }

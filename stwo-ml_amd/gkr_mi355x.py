@@ -43,6 +43,11 @@ class GkrPolicy(C.Structure):
     _fields_ = [(f, C.c_uint8) for f in POLICY_FIELDS]
 
 
+class GkrRotaryScaling(C.Structure):
+    _fields_ = [("kind", C.c_uint32), ("factor", C.c_double), ("positions", C.c_double), ("low", C.c_double),
+                ("high", C.c_double)]
+
+
 class GkrMulOut(C.Structure):
     _fields_ = [("eq_round_polys", C.POINTER(GkrQM31)), ("lhs_eval", GkrQM31), ("rhs_eval", GkrQM31),
                 ("alpha", GkrQM31), ("next_value", GkrQM31), ("n_vars", C.c_uint32)]
@@ -86,6 +91,7 @@ class GkrNormOut(C.Structure):
                 ("gamma_commitment", GkrFelt), ("gamma_eval", GkrQM31)]
 
 
+ROTARY_PLAIN, ROTARY_LINEAR, ROTARY_BASE, ROTARY_WAVES = 0, 1, 2, 3
 STEP_MATMUL, STEP_MUL, STEP_ACTIVATION, STEP_LAYERNORM, STEP_RMSNORM = 0, 2, 3, 4, 8
 NORM_TABLE_LOG = 16
 # norm proof dict keys holding one QM31 (the oracle's norm proof dicts use the same names)
@@ -229,6 +235,15 @@ SIGNATURES = [
     ("gkr_matmul_forward_into", C.c_int, [_P, _P, _P, _P]),
     ("gkr_matmul_forward_fused", C.c_int, [_P, _P, _P, _P, C.c_uint32, C.c_uint32, _P, _P, _P]),
     ("gkr_gated_forward", C.c_int, [_P, _P, _P, _P, C.c_uint32, C.c_uint32, _P, _P, _P, _P]),
+    ("gkr_matmul_forward_scaled", C.c_int, [_P, _P, _P, _P, _P, C.c_uint32, C.c_uint32, _P, _P, _P, _P]),
+    ("gkr_matmul_forward_quantized", C.c_int, [_P, _P, _P, C.c_uint32, _P, C.c_uint32, C.c_uint32, _P, _P, _P, _P, _P, _P]),
+    ("gkr_rotary_frequencies", C.c_int, [C.c_uint32, C.c_double, C.POINTER(GkrRotaryScaling), C.POINTER(C.c_uint64)]),
+    ("gkr_rotary_new", C.c_int, [_P, C.POINTER(C.c_uint64), C.c_uint32, C.c_uint32, C.c_uint32, C.c_uint32,
+                                 C.POINTER(_P)]),
+    ("gkr_rotary_free", None, [_P]),
+    ("gkr_rotary_forward", C.c_int, [_P, _P, C.c_uint32, C.c_int, _U32P, _U32P, C.c_size_t, C.c_uint32, _P, _P, _P, _P]),
+    ("gkr_attention_prompt", C.c_int, [_P, _P, _P, _P, _U32P, C.c_size_t, C.c_uint32, C.c_uint32, C.c_uint32, C.c_uint32,
+                                       _P, _P, _P, _P]),
     ("gkr_kv_cache_new", C.c_int, [_P, C.c_uint32, C.c_uint32, C.c_uint32, C.c_uint32, C.c_uint32, C.c_uint32, C.c_int,
                                    C.POINTER(_P)]),
     ("gkr_kv_cache_free", None, [_P]),
@@ -336,6 +351,14 @@ def policy_commitment(policy: dict) -> int:
     out = GkrFelt()
     _check(lib().gkr_policy_commitment(C.byref(p), C.byref(out)))
     return felt_from_c(out)
+
+
+def rotary_frequencies(turned: int, base: float = 10000.0, kind: int = ROTARY_PLAIN, factor: float = 1.0,
+                       positions: float = 0.0, low: float = 0.0, high: float = 0.0) -> np.ndarray:
+    """gkr_rotary_frequencies: turned / 2 frequencies in 2^-64 turns a position."""
+    out = (C.c_uint64 * max(1, turned // 2))()
+    _check(lib().gkr_rotary_frequencies(turned, base, C.byref(GkrRotaryScaling(kind, factor, positions, low, high)), out))
+    return np.array(out, dtype=np.uint64)
 
 
 class PoseidonChannel:
@@ -655,6 +678,46 @@ class Context:
         _check(lib().gkr_gated_forward(self._h, a.handle, wg.handle, wu.handle, activation, table_log_size,
                                        _handle(gate), _handle(act), _handle(up), out.handle))
 
+    def matmul_forward_scaled(self, a: "Matrix", b: "Matrix", out: "Matrix", row_scales: Optional["Matrix"] = None,
+                              col_scales: Optional["Matrix"] = None, shift: int = 0, limit: int = 0,
+                              bias: Optional["Matrix"] = None, residual: Optional["Matrix"] = None,
+                              pre: Optional["Matrix"] = None) -> None:
+        """gkr_matmul_forward_scaled: out = round(c(A B) r s / 2^shift) + bias, cut off at +-limit, + residual mod P."""
+        _check(lib().gkr_matmul_forward_scaled(self._h, a.handle, b.handle, _handle(row_scales), _handle(col_scales),
+                                               shift, limit, _handle(bias), _handle(residual), _handle(pre),
+                                               out.handle))
+
+    def matmul_forward_quantized(self, a: "Matrix", b: "Matrix", out: "Matrix", levels: int = 127,
+                                 col_scales: Optional["Matrix"] = None, shift: int = 0, limit: int = 0,
+                                 bias: Optional["Matrix"] = None, residual: Optional["Matrix"] = None,
+                                 quantized: Optional["Matrix"] = None, row_scales: Optional["Matrix"] = None,
+                                 pre: Optional["Matrix"] = None) -> None:
+        """gkr_matmul_forward_quantized: the same of A's rows brought to +-levels, each by its largest magnitude."""
+        _check(lib().gkr_matmul_forward_quantized(self._h, a.handle, b.handle, levels, _handle(col_scales), shift,
+                                                  limit, _handle(bias), _handle(residual), _handle(quantized),
+                                                  _handle(row_scales), _handle(pre), out.handle))
+
+    def rotary(self, frequencies: Sequence[int], max_positions: int, amplitude: int = 1 << 15,
+               shift: int = 15) -> "Rotary":
+        """gkr_rotary_new: the turns of every position, for rotary_forward."""
+        f = [int(x) for x in frequencies]
+        h = C.c_void_p()
+        _check(lib().gkr_rotary_new(self._h, (C.c_uint64 * max(1, len(f)))(*f), 2 * len(f), amplitude, shift,
+                                    max_positions, C.byref(h)))
+        return Rotary(self, h.value)
+
+    def rotary_forward(self, rotary: "Rotary", q: "Matrix", q_out: "Matrix", counts: Sequence[int], head_dim: int,
+                       starts: Optional[Sequence[int]] = None, k: Optional["Matrix"] = None,
+                       k_out: Optional["Matrix"] = None, interleaved: bool = False, limit: int = 0) -> None:
+        """gkr_rotary_forward: the heads of counts[i] tokens of each sequence i, at positions starts[i] (0) onward."""
+        n = len(counts)
+        if starts is not None and len(starts) != n:
+            raise ValueError(f"{n} counts and {len(starts)} starts")
+        c_starts = None if starts is None else (C.c_uint32 * max(1, n))(*starts)
+        _check(lib().gkr_rotary_forward(self._h, rotary.handle, head_dim, int(interleaved), c_starts,
+                                        (C.c_uint32 * max(1, n))(*counts), n, limit, q.handle, q_out.handle, _handle(k),
+                                        _handle(k_out)))
+
     def kv_cache(self, n_kv_heads: int, head_dim: int, n_pages: int, page_tokens: int = 64, max_seqs: int = 64,
                  max_tokens: int = 65536, int8: bool = False) -> "KvCache":
         """gkr_kv_cache_new: a paged key-value cache on this context."""
@@ -675,6 +738,16 @@ class Context:
         _check(lib().gkr_attention_forward(self._h, cache.handle, q.handle, (C.c_uint32 * max(1, n))(*seqs), c_lens, n,
                                            n_heads, score_offset, table_log_size, _handle(weighted), _handle(sums),
                                            _handle(scores), out.handle))
+
+    def attention_prompt(self, q: "Matrix", k: "Matrix", v: "Matrix", counts: Sequence[int], n_heads: int,
+                         n_kv_heads: int, out: "Matrix", score_offset: int = 0, table_log_size: int = 0,
+                         weighted: Optional["Matrix"] = None, sums: Optional["Matrix"] = None,
+                         scores: Optional["Matrix"] = None) -> None:
+        """gkr_attention_prompt: causal attention of packed sequences of counts[i] tokens."""
+        n = len(counts)
+        _check(lib().gkr_attention_prompt(self._h, q.handle, k.handle, v.handle, (C.c_uint32 * max(1, n))(*counts), n,
+                                          n_heads, n_kv_heads, score_offset, table_log_size, _handle(weighted),
+                                          _handle(sums), _handle(scores), out.handle))
 
     def weight_commitment(self, b: "Matrix") -> int:
         """gkr_weight_commitment: commit_mle_root_only(matrix_to_mle_col_major_padded(B))."""
@@ -1031,6 +1104,26 @@ class Matrix:
 
 def _handle(m: Optional["Matrix"]) -> Optional[int]:
     return None if m is None else m.handle
+
+
+class Rotary:
+    """A table of turns (gkr_rotary); made by Context.rotary."""
+
+    def __init__(self, ctx: "Context", handle: int):
+        self.ctx, self._h = ctx, handle
+
+    @property
+    def handle(self) -> int:
+        return self._h
+
+    def free(self) -> None:
+        if self._h:
+            lib().gkr_rotary_free(self._h)
+            self._h = None
+
+    def __del__(self):
+        if _lib is not None and getattr(self, "_h", None):
+            self.free()
 
 
 class KvCache:
