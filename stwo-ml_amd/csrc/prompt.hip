@@ -93,38 +93,49 @@ static int attention_prompt(gkr_ctx* c, const gkr_matrix* q, const gkr_matrix* k
   a.chunks = chunks;
   a.offset = offset;
   a.table_mask = (1u << table_log) - 1;
-  uint32_t items = 0;
-  auto launch = [&]() -> int {
-    if (items == 0) return GKR_OK;
-    auto one = [&](auto kernel) { GKR_LAUNCH(c, kernel, dim3(items), dim3(256), 0, a); };
-    if (dim <= 64) {
-      one(k_prompt<1, 1, 1>);
-      one(k_prompt<4, 1, 1>);
-    } else if (dim <= 128) {
-      one(k_prompt<1, 2, 1>);
-      one(k_prompt<4, 2, 1>);
-    } else {
-      one(k_prompt<1, 4, 1>);
-      one(k_prompt<4, 4, 1>);
+  // the sequences' items, in workgroups of `tile` rows
+  auto launch_all = [&](uint32_t tile, auto kernel) -> int {
+    a.n = 0;
+    uint32_t items = 0;
+    uint64_t row = 0, at = 0;
+    auto launch = [&]() -> int {
+      if (items == 0) return GKR_OK;
+      TRY(kernel(items));
+      a.n = items = 0;
+      return check_launch(c);
+    };
+    for (size_t i = 0; i < n_seqs; i++) {
+      if (counts[i] == 0) continue;
+      auto& e = a.e[a.n++];
+      e.item0 = items;
+      e.tiles = (counts[i] * group + tile - 1) / tile;
+      e.len = counts[i];
+      e.at = (uint32_t)at;
+      e.row = row;
+      items += e.tiles * kv_heads;
+      at += (counts[i] + kAttBlock - 1) / kAttBlock;
+      row += counts[i];
+      if (a.n == kPromptSeqs || items > 1u << 22) TRY(launch());
     }
-    a.n = items = 0;
-    return check_launch(c);
+    return launch();
   };
-  row = at = 0;
-  for (size_t i = 0; i < n_seqs; i++) {
-    if (counts[i] == 0) continue;
-    auto& e = a.e[a.n++];
-    e.item0 = items;
-    e.tiles = (counts[i] * group + 63) / 64;
-    e.len = counts[i];
-    e.at = (uint32_t)at;
-    e.row = row;
-    items += e.tiles * kv_heads;
-    at += (counts[i] + kAttBlock - 1) / kAttBlock;
-    row += counts[i];
-    if (a.n == kPromptSeqs || items > 1u << 22) TRY(launch());
+#define GKR_PROMPT(NP, DT, R, W)                                                              \
+  launch_all(16 * R * W, [&](uint32_t items) -> int {                                         \
+    if (scores) GKR_LAUNCH(c, (k_prompt<NP, DT, R, W, true>), dim3(items), dim3(64 * W), 0, a); \
+    else GKR_LAUNCH(c, (k_prompt<NP, DT, R, W, false>), dim3(items), dim3(64 * W), 0, a);     \
+    return GKR_OK;                                                                            \
+  })
+  if (dim <= 64) {
+    TRY(GKR_PROMPT(1, 1, 2, 4));
+    return GKR_PROMPT(4, 1, 1, 4);
   }
-  return launch();
+  if (dim <= 128) {
+    TRY(GKR_PROMPT(1, 2, 2, 4));
+    return GKR_PROMPT(4, 2, 1, 8);
+  }
+  TRY(GKR_PROMPT(1, 4, 1, 4));
+  return GKR_PROMPT(4, 4, 1, 4);
+#undef GKR_PROMPT
 }
 extern "C" int gkr_attention_prompt(gkr_ctx* c, const gkr_matrix* q, const gkr_matrix* k, const gkr_matrix* v,
                                     const uint32_t* counts, size_t n_seqs, uint32_t heads, uint32_t kv_heads,
