@@ -22,6 +22,12 @@ namespace gkr {
 
 constexpr uint32_t kPromptSeqs = 128;      // sequences per launch
 constexpr uint32_t kMaxPrompt = 131071;    // tokens of one: digit sums stay below 2^31
+// Words of the mask (witness.h) that the packing sets: every wave of the products
+// reads them all, a line each.
+constexpr uint32_t kPromptWords = 16;
+__device__ __forceinline__ uint32_t prompt_mask(const uint32_t* mask) {  // this lane's
+  return mask[kMaskStride * (threadIdx.x & (kPromptWords - 1))];
+}
 
 struct PromptPack {
   uint32_t n, kv_heads, dim, chunks;
@@ -99,7 +105,7 @@ static __global__ void __launch_bounds__(256) k_prompt_pack(PromptPack a, const 
     }
   }
   if (__any(high != 0) && lane == 0) {
-    volatile uint32_t* const word = mask + kMaskStride * ((blockIdx.x * 4 + (threadIdx.x >> 6)) % kMaskWords);
+    volatile uint32_t* const word = mask + kMaskStride * ((blockIdx.x * 4 + (threadIdx.x >> 6)) % kPromptWords);
     if (!*word) *word = 1;
   }
 }
@@ -132,6 +138,7 @@ struct PromptArgs {
   uint64_t head_bytes;
   uint32_t n, kv_heads, group, dim, chunks;
   uint32_t offset, table_mask;
+  uint32_t* todo;  // a word an item: whether the int8 kernel left it
   struct {
     uint32_t item0, tiles;  // its first item of this launch, its tiles of rows
     uint32_t len, at;       // tokens; its first block
@@ -163,6 +170,10 @@ __device__ __forceinline__ uint32_t prompt_low(uint32_t g, uint32_t upper) {
 __device__ __forceinline__ uint32_t prompt_high(uint32_t g, uint32_t upper) {
   return __builtin_amdgcn_perm(0xfcfcfcfcu, 0xfcfcfeffu, g ^ 0x08080808u) & upper;
 }
+// Bits 16 .. 23 of four words, a byte each.
+__device__ __forceinline__ uint32_t prompt_places(const uint32_t (&x)[4]) {
+  return __builtin_amdgcn_perm(x[1], x[0], 0x0c0c0602u) | __builtin_amdgcn_perm(x[3], x[2], 0x06020c0cu);
+}
 // Tables of more than 2^20 entries have places past 15: 15 for them.
 __device__ __forceinline__ uint32_t prompt_cap(uint32_t g) {
   uint32_t high = g & 0xf0f0f0f0u;
@@ -183,16 +194,98 @@ __device__ __forceinline__ uint32_t prompt_mean(int64_t total, uint32_t z, doubl
   return total < 0 ? m31_neg(r) : r;
 }
 
+// The same of int8-range values, from the negated total and -1 / z, to a word: the
+// quotient is at most 128, |total| / z + 1/2 a multiple of 1 / 2 z, 2^-28 and more,
+// and its error in 53 bits below 2^-43, so 2^-30 more decides it; the conversion
+// cuts towards zero.
+__device__ __forceinline__ uint32_t prompt_mean(double negated, double inv) {
+  const int32_t r = (int32_t)__builtin_fma(negated, inv, __builtin_copysign(0.5 + 0x1p-30, -negated));
+  return umin32((uint32_t)r, (uint32_t)r + P);
+}
+
+// Four scores of a row, its tokens first .. first + 3: kept as words, 0 where they
+// are not seen.
+__device__ __forceinline__ void prompt_keep(const AttOut& o, uint64_t at, uint32_t first, uint32_t seen, const v4i& y,
+                                            int32_t add) {
+  if (seen == 0) return;  // no such row
+  v4i_word x;
+#pragma unroll
+  for (int v = 0; v < 4; v++) x[v] = first + v < seen ? (int)signed32_mod_p(y[v] + add) : 0;
+  if (first + 4 <= o.score_cols) {
+    *(v4i_word*)(o.scores + at + first) = x;
+  } else {
+#pragma unroll
+    for (int v = 0; v < 4; v++)
+      if (first + v < o.score_cols) o.scores[at + first + v] = (uint32_t)x[v];
+  }
+}
+// Scores behind a wave's last block (`mine` of them) are cleared.
+template <int R>
+__device__ __forceinline__ void prompt_clear(const PromptArgs& a, uint32_t i, uint32_t kvh, uint32_t row0, uint32_t mine) {
+  const uint32_t rows = a.e[i].len * a.group, end = row0 + 16 * R < rows ? row0 + 16 * R : rows;
+  for (uint32_t row = row0; row < end; row++) {
+    const uint32_t token = row / a.group;
+    const uint64_t at = ((a.e[i].row + token) * a.kv_heads + kvh) * a.group + (row - token * a.group);
+    for (uint64_t t = (uint64_t)mine * kAttBlock + (threadIdx.x & 63); t < a.o.score_cols; t += 64) a.o.scores[at * a.o.score_cols + t] = 0;
+  }
+}
+// The end of a wave's rows: acc and z as the tiles leave them.
+template <int NP, int DT, int R, bool TRACE>
+__device__ __forceinline__ void prompt_end(const PromptArgs& a, uint32_t i, uint32_t kvh, uint32_t row0, uint32_t mine,
+                                           const v4i (&acc)[R][4 * DT][NP + 1], const int32_t (&z)[R][2]) {
+  constexpr int CH = 4 * DT, NV = NP + 1;
+  const uint32_t lane = threadIdx.x & 63, col = lane & 15, quarter = lane >> 4;
+  const uint32_t rows = a.e[i].len * a.group, wave_end = row0 + 16 * R < rows ? row0 + 16 * R : rows;
+  auto whole_total = [&](int r, int d, int v) {
+    if constexpr (NP == 1) return -((int64_t)acc[r][d][0][v] + ((int64_t)acc[r][d][1][v] << 3));
+    int64_t total = 0;
+#pragma unroll
+    for (int g = 0; g < NV; g++) total -= (int64_t)acc[r][d][g][v] << (8 * g);
+    return total;
+  };
+#pragma unroll
+  for (int r = 0; r < R; r++) {
+    uint32_t zc = (uint32_t)-(NP == 1 ? z[r][0] + 8 * z[r][1] : z[r][0] + 256 * z[r][1]);
+    zc += __shfl_xor(zc, 16);
+    zc += __shfl_xor(zc, 32);
+#pragma unroll
+    for (int v = 0; v < 4; v++) {
+      const uint32_t row = row0 + 16 * r + 4 * quarter + v, zr = __shfl(zc, 4 * quarter + v);
+      if (row >= rows) continue;
+      const uint32_t token = row / a.group;
+      const uint64_t at = ((a.e[i].row + token) * a.kv_heads + kvh) * a.group + (row - token * a.group);
+      if (a.o.sums && col == 0) a.o.sums[at] = shift16(m31_from_u32(zr));
+      const double inv = (NP == 1 ? -1.0 : 0.5) / zr;
+#pragma unroll
+      for (int d = 0; d < (int)CH; d++) {
+        const bool there = 16 * d + col < a.dim;
+        if constexpr (NP == 1) {
+          const double total = __builtin_fma(8.0, (double)acc[r][d][1][v], (double)acc[r][d][0][v]);  // negated
+          const uint32_t mean = prompt_mean(total, inv);
+          if (there) a.o.out[at * a.dim + 16 * d + col] = mean;
+        } else {
+          const uint32_t mean = prompt_mean(whole_total(r, d, v), zr, inv);
+          if (there) a.o.out[at * a.dim + 16 * d + col] = mean;
+        }
+      }
+      if (TRACE && a.o.weighted) {
+#pragma unroll
+        for (int d = 0; d < (int)CH; d++)
+          if (16 * d + col < a.dim) a.o.weighted[at * a.dim + 16 * d + col] = shift16(signed_mod_p(whole_total(r, d, v)));
+      }
+    }
+  }
+  if (TRACE && a.o.scores && row0 < rows) prompt_clear<R>(a, i, kvh, row0, mine);
+}
 // A workgroup's W waves have R tiles of 16 rows each and take the blocks in step:
 // keys and values of a block go through LDS, each on its way from memory while
 // the other is used.
 template <int NP, int NQ, int DT, int R, int W, bool TRACE>
-__device__ __forceinline__ void prompt_tile(const PromptArgs& a, v4i* lds, uint32_t i, uint32_t kvh, uint32_t tile0,
-                                            uint32_t row0, const v4i (&qd)[R][DT][NQ]) {
+__device__ __forceinline__ void prompt_tile(const PromptArgs& a, v4i* __restrict__ lk, v4i* __restrict__ lv, uint32_t i,
+                                            uint32_t kvh, uint32_t tile0, uint32_t row0, const v4i (&qd)[R][DT][NQ]) {
   constexpr int NG = NP + NQ - 1, NV = NP + 1;  // NP = 1: sums of the small and of the wide weights
   constexpr uint32_t CH = 4 * DT;               // chunks of 16 dims in LDS
-  constexpr int ND = (int)(CH * NP / W);        // 1 KB pieces of keys, and of values, a wave copies
-  v4i *const lk = lds, *const lv = lds + NP * CH * 64;
+  constexpr int ND = (int)((CH * NP + W - 1) / W);  // 1 KB pieces of keys, and of values, a wave copies
   const uint32_t lane = threadIdx.x & 63, col = lane & 15, quarter = lane >> 4;
   const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const uint32_t len = a.e[i].len, rows = len * a.group, plane = 1024 * a.chunks;
@@ -209,18 +302,21 @@ __device__ __forceinline__ void prompt_tile(const PromptArgs& a, v4i* lds, uint3
     seen[r] = row < rows ? row / a.group + 1 : 0;
   }
   const uint64_t base = kvh * a.head_bytes + (uint64_t)a.e[i].at * (4 * plane) + 16 * lane;
-  v4i in[ND];
-  auto load = [&](const int8_t* from, uint32_t b) {
+  uint32_t from[ND];  // of this wave's pieces; chunks past the last are the last one again (the query is zero there)
 #pragma unroll
-    for (int j = 0; j < ND; j++) {
-      const uint32_t piece = wave * ND + j, p = piece / CH, chunk = piece % CH;
-      if (CH == 4 && a.chunks < CH && chunk >= a.chunks) continue;
-      in[j] = *(const v4i*)(from + base + (uint64_t)b * (4 * plane) + p * plane + 1024 * (chunk < a.chunks ? chunk : a.chunks - 1));
-    }
+  for (int j = 0; j < ND; j++) {
+    const uint32_t piece = wave * ND + j, chunk = piece % CH < a.chunks ? piece % CH : a.chunks - 1;
+    from[j] = piece < CH * NP ? piece / CH * plane + 1024 * chunk : 0;
+  }
+  auto load = [&](v4i (&in)[ND], const int8_t* m, uint32_t b) {  // past the last block: again, unused
+    const int8_t* const block = m + base + (uint64_t)(b < blocks ? b : blocks - 1) * (4 * plane);
+#pragma unroll
+    for (int j = 0; j < ND; j++) in[j] = *(const v4i*)(block + from[j]);
   };
-  auto put = [&](v4i* to) {
+  auto put = [&](const v4i (&in)[ND], v4i* to) {
 #pragma unroll
-    for (int j = 0; j < ND; j++) to[(wave * ND + j) * 64 + lane] = in[j];
+    for (int j = 0; j < ND; j++)
+      if (ND * W == CH * NP || wave * ND + j < CH * NP) to[(wave * ND + j) * 64 + lane] = in[j];
   };
   v4i acc[R][CH][NV];
 #pragma unroll
@@ -233,12 +329,13 @@ __device__ __forceinline__ void prompt_tile(const PromptArgs& a, v4i* lds, uint3
   const int32_t off = a.offset > P / 2 ? (int32_t)(a.offset - P) : (int32_t)a.offset;
   const uint32_t place_mask = (a.table_mask >> 16) * 0x01010101u;
   const bool many = a.table_mask >> 20 != 0;
-  load(a.k, 0);
-  put(lk);
+  v4i in[ND];
+  load(in, a.k, 0);
+  put(in, lk);
 #pragma unroll 1
   for (uint32_t b = 0; b < blocks; b++) {
     __syncthreads();  // the keys are there, the values' place is free
-    load(a.v, b);
+    load(in, a.v, b);
     uint32_t w0[R][4], w1[R][4];  // NP = 1: small and wide weights; else the digits base 256
     bool some_small = false;
     const bool busy = b < mine;
@@ -269,9 +366,7 @@ __device__ __forceinline__ void prompt_tile(const PromptArgs& a, v4i* lds, uint3
           uint32_t x[4];
 #pragma unroll
           for (int v = 0; v < 4; v++) {
-            if constexpr (NG == 1) {
-              x[v] = signed32_mod_p(sc[r][0][v]);
-            } else if constexpr (NG == 4) {
+            if constexpr (NG == 4) {
               // |sc[g]| <= 2^22 and the offset: pairs in 32 bits, the upper one turned by 16 of 31 bits
               const uint32_t low = signed32_mod_p(sc[r][0][v]), mid = signed32_mod_p(sc[r][1][v] << 8);
               const uint32_t high = signed32_mod_p(sc[r][2][v] + (sc[r][3][v] << 8));
@@ -280,64 +375,59 @@ __device__ __forceinline__ void prompt_tile(const PromptArgs& a, v4i* lds, uint3
               x[v] = prompt_score<(DT <= 2)>(sc[r], v, off);
             }
           }
-          if (TRACE) {
-            const uint32_t first = b * kAttBlock + 16 * t + 4 * quarter;
+          if (TRACE && a.o.scores) {
             const uint32_t row = row0 + 16 * r + col, token = row / a.group;
-            const uint64_t at = (((a.e[i].row + token) * a.kv_heads + kvh) * a.group + (row - token * a.group)) * a.o.score_cols + first;
-            if (seen[r]) {
-              if (first + 4 <= a.o.score_cols) {
-                v4i_word kept;
-#pragma unroll
-                for (int v = 0; v < 4; v++) kept[v] = first + v < seen[r] ? (int)x[v] : 0;
-                *(v4i_word*)(a.o.scores + at) = kept;
-              } else {
-#pragma unroll
-                for (int v = 0; v < 4; v++)
-                  if (first + v < a.o.score_cols) a.o.scores[at + v] = first + v < seen[r] ? x[v] : 0u;
-              }
-            }
+            const uint64_t at = (((a.e[i].row + token) * a.kv_heads + kvh) * a.group + (row - token * a.group)) * a.o.score_cols;
+            prompt_keep(a.o, at, b * kAttBlock + 16 * t + 4 * quarter, seen[r], v4i{(int)x[0], (int)x[1], (int)x[2], (int)x[3]}, 0);
           }
-          w0[r][t] = pick_bytes<2>(x) & place_mask;
+          w0[r][t] = prompt_places(x) & place_mask;
         }
       }
-      if (many) {  // uniform
+      {
+        if (many) {  // uniform
 #pragma unroll
-        for (int r = 0; r < R; r++)
+          for (int r = 0; r < R; r++)
 #pragma unroll
-          for (int t = 0; t < 4; t++) w0[r][t] = prompt_cap(w0[r][t]);
-      }
-#pragma unroll
-      for (int r = 0; r < R; r++)
-#pragma unroll
-        for (int t = 0; t < 4; t++) {
-          const uint32_t g = w0[r][t], upper = prompt_upper(g);
-          w0[r][t] = NP == 1 ? prompt_small(g, upper) : prompt_low(g, upper);
-          w1[r][t] = NP == 1 ? prompt_wide(g, upper) : prompt_high(g, upper);
+            for (int t = 0; t < 4; t++) w0[r][t] = prompt_cap(w0[r][t]);
         }
-      if (b >= whole) {  // uniform: tokens that a row does not see have no weight
 #pragma unroll
         for (int r = 0; r < R; r++)
 #pragma unroll
           for (int t = 0; t < 4; t++) {
-            const uint32_t in_sight = prompt_seen((int)(seen[r] - (b * kAttBlock + 16 * t + 4 * quarter)));
-            w0[r][t] &= in_sight;
-            w1[r][t] &= in_sight;
+            const uint32_t g = w0[r][t], upper = prompt_upper(g);
+            w0[r][t] = NP == 1 ? prompt_small(g, upper) : prompt_low(g, upper);
+            w1[r][t] = NP == 1 ? prompt_wide(g, upper) : prompt_high(g, upper);
           }
+        if (b >= whole) {  // uniform: tokens that a row does not see have no weight
+#pragma unroll
+          for (int r = 0; r < R; r++)
+#pragma unroll
+            for (int t = 0; t < 4; t++) w0[r][t] &= prompt_seen((int)(seen[r] - (b * kAttBlock + 16 * t + 4 * quarter)));
+        }
+        uint32_t any_small = 0;
+#pragma unroll
+        for (int r = 0; r < R; r++)
+#pragma unroll
+          for (int t = 0; t < 4; t++) {
+            any_small |= w0[r][t];
+            z[r][0] = __builtin_amdgcn_sdot4((int)w0[r][t], 0x01010101, z[r][0], false);
+          }
+        some_small = __any(any_small != 0);
       }
-      uint32_t any_small = 0;
+      if (b >= whole) {
+#pragma unroll
+        for (int r = 0; r < R; r++)
+#pragma unroll
+          for (int t = 0; t < 4; t++) w1[r][t] &= prompt_seen((int)(seen[r] - (b * kAttBlock + 16 * t + 4 * quarter)));
+      }
 #pragma unroll
       for (int r = 0; r < R; r++)
 #pragma unroll
-        for (int t = 0; t < 4; t++) {
-          any_small |= w0[r][t];
-          z[r][0] = __builtin_amdgcn_sdot4((int)w0[r][t], 0x01010101, z[r][0], false);
-          z[r][1] = __builtin_amdgcn_sdot4((int)w1[r][t], 0x01010101, z[r][1], false);
-        }
-      some_small = __any(any_small != 0);
+        for (int t = 0; t < 4; t++) z[r][1] = __builtin_amdgcn_sdot4((int)w1[r][t], 0x01010101, z[r][1], false);
     }
-    put(lv);
+    put(in, lv);
     __syncthreads();  // the values are there, the keys' place is free
-    if (b + 1 < blocks) load(a.k, b + 1);
+    load(in, a.k, b + 1);
     if (busy) {
       auto product = [&](int r, int d, int g, const uint32_t (&w)[4], const v4i& vd) {
         const v4i wd = {(int)w[0], (int)w[1], (int)w[2], (int)w[3]};
@@ -372,51 +462,242 @@ __device__ __forceinline__ void prompt_tile(const PromptArgs& a, v4i* lds, uint3
           }
       }
     }
-    if (b + 1 < blocks) put(lk);
+    put(in, lk);
   }
+  prompt_end<NP, DT, R, TRACE>(a, i, kvh, row0, mine, acc, z);
+}
+// The four digit planes of a wave's R tiles of queries.
+template <int DT, int R>
+__device__ __forceinline__ void prompt_query(const PromptArgs& a, uint32_t i, uint32_t kvh, uint32_t row0, v4i (&qd)[R][DT][4]) {
+  const uint32_t lane = threadIdx.x & 63, col = lane & 15, quarter = lane >> 4, rows = a.e[i].len * a.group;
 #pragma unroll
   for (int r = 0; r < R; r++) {
-    uint32_t zc = (uint32_t)-(NP == 1 ? z[r][0] + 8 * z[r][1] : z[r][0] + 256 * z[r][1]);
-    zc += __shfl_xor(zc, 16);
-    zc += __shfl_xor(zc, 32);
+    const uint32_t here = row0 + 16 * r + col, row = here < rows ? here : rows - 1, token = row / a.group;
+    const uint32_t* const from =
+        a.q + (((a.e[i].row + token) * a.kv_heads + kvh) * a.group + (row - token * a.group)) * a.dim;
+    v4i w[DT][4];
+    if (a.dim % 4 == 0) {  // uniform
 #pragma unroll
-    for (int v = 0; v < 4; v++) {
-      const uint32_t row = row0 + 16 * r + 4 * quarter + v, zr = __shfl(zc, 4 * quarter + v);
-      if (row >= rows) continue;
-      const uint32_t token = row / a.group;
-      const uint64_t at = ((a.e[i].row + token) * a.kv_heads + kvh) * a.group + (row - token * a.group);
-      if (a.o.sums && col == 0) a.o.sums[at] = shift16(m31_from_u32(zr));
-      const double inv = 0.5 / zr;
+      for (int s = 0; s < DT; s++)
 #pragma unroll
-      for (int d = 0; d < (int)CH; d++) {
-        int64_t total = 0;
-        if constexpr (NP == 1) {
-          total = -((int64_t)acc[r][d][0][v] + ((int64_t)acc[r][d][1][v] << 3));
-        } else {
-#pragma unroll
-          for (int g = 0; g < NV; g++) total -= (int64_t)acc[r][d][g][v] << (8 * g);
+        for (uint32_t j = 0; j < 4; j++) {
+          const uint32_t d = 64 * s + 16 * quarter + 4 * j;
+          w[s][j] = *(const v4i_word*)(from + (d < a.dim ? d : 0));
         }
-        if (16 * d + col < a.dim) {
-          a.o.out[at * a.dim + 16 * d + col] = prompt_mean(total, zr, inv);
-          if (a.o.weighted) a.o.weighted[at * a.dim + 16 * d + col] = shift16(signed_mod_p(total));
+    } else {
+#pragma unroll
+      for (int s = 0; s < DT; s++)
+#pragma unroll
+        for (uint32_t j = 0; j < 4; j++)
+#pragma unroll
+          for (uint32_t t = 0; t < 4; t++) {
+            const uint32_t d = 64 * s + 16 * quarter + 4 * j + t;
+            w[s][j][t] = (int)from[d < a.dim ? d : 0];
+          }
+    }
+#pragma unroll
+    for (int s = 0; s < DT; s++)
+#pragma unroll
+      for (uint32_t j = 0; j < 4; j++) {
+        uint32_t x[4], out[4];
+#pragma unroll
+        for (uint32_t t = 0; t < 4; t++) x[t] = 64 * s + 16 * quarter + 4 * j + t < a.dim ? digit_bytes((uint32_t)w[s][j][t]) : 0u;
+        transpose_bytes(x, out);
+#pragma unroll
+        for (int p = 0; p < 4; p++) qd[r][s][p][j] = (int)out[p];
+      }
+  }
+}
+// Rows of a wave: token and head of row x counted from the first (x below 2^17), by
+// a product with 1 / group: x / group is 0.5 / group away from the next whole
+// number, more than the product's error.
+struct PromptRows {
+  uint32_t token0, head0, group;  // of the first row
+  float inv;
+  __device__ __forceinline__ PromptRows(uint32_t row0, uint32_t group_) : group(group_), inv(1.0f / (float)group_) {
+    token0 = row0 / group_;
+    head0 = row0 - token0 * group_;
+  }
+  __device__ __forceinline__ void at(uint32_t x, uint32_t& token, uint32_t& head) const {  // token from token0 on
+    x += head0;
+    token = (uint32_t)(((float)x + 0.5f) * inv);
+    head = x - token * group;
+  }
+};
+
+// One pass over the blocks of a wave's R tiles of 16 rows, int8-range words on all
+// sides: sums of the values by the wide weights (SMALL: by the small ones).  A
+// block's keys and values come straight into LDS while the block before it is
+// used, a wave's share of them a piece of 1 KB at a time: two halves of LDS, which
+// are arrays of their own, so that a read of one does not wait for the other; one
+// barrier a block.  The blocks where a small weight was met are marked in `marks`, a
+// bit each, and the small weights' pass visits those only.
+template <int DT, int R, int W, bool SMALL, bool TRACE>
+struct PromptPass {
+  static constexpr uint32_t CH = 4 * DT;
+  const PromptArgs& a;
+  const int8_t *k, *v;  // block 0's piece of this wave
+  uint32_t i, kvh, row0, wave, lane, blocks, mine, whole;
+  const uint32_t (&seen)[R];  // tokens that row 16 r + lane % 16 of the wave sees
+  const v4i (&qd)[R][DT];
+  v4i (&acc)[R][CH];
+  int32_t (&z)[R];
+  uint32_t* marks;
+
+  __device__ __forceinline__ void load(uint32_t b, v4i* keys, v4i* values) const {
+    const uint64_t at = (uint64_t)b * (4 * 1024 * a.chunks);
+#pragma unroll
+    for (uint32_t j = 0; j < CH / W; j++) {
+      const uint32_t piece = wave * (CH / W) + j;
+      if (piece >= a.chunks) continue;  // uniform; not multiplied by anything, or not stored
+      __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(k + at + 1024 * j),
+                                       (__attribute__((address_space(3))) void*)(keys + piece * 64), 16, 0, 0);
+      __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(v + at + 1024 * j),
+                                       (__attribute__((address_space(3))) void*)(values + piece * 64), 16, 0, 0);
+    }
+  }
+  // The loads into LDS have arrived (they are not among what a barrier waits for)
+  // and all waves are here.
+  __device__ __forceinline__ void arrive() const {
+    __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0)
+    __syncthreads();
+  }
+  __device__ __forceinline__ uint32_t sight(uint32_t b, int r, int t) const {
+    return prompt_seen((int)(seen[r] - (b * kAttBlock + 16 * t + 4 * (lane >> 4))));
+  }
+  // the first marked block from b on, or `blocks`
+  __device__ __forceinline__ uint32_t marked(uint32_t b) const {
+    while (b < blocks) {
+      const uint32_t word = (uint32_t)__builtin_amdgcn_readfirstlane((int)marks[b / 32]) >> (b % 32);
+      if (word) return min(b + (uint32_t)__builtin_ctz(word), blocks);
+      b = (b / 32 + 1) * 32;
+    }
+    return blocks;
+  }
+  __device__ __forceinline__ void block(uint32_t b, uint32_t next, const v4i* __restrict__ keys, const v4i* __restrict__ values,
+                                        v4i* __restrict__ next_keys, v4i* __restrict__ next_values) {
+    arrive();
+    if (next < blocks) load(next, next_keys, next_values);
+    if (b >= mine) return;  // uniform in the wave
+    const uint32_t col = lane & 15, quarter = lane >> 4;
+    // scores less `low` 2^16, not reduced: below 0 where the place is below `low` or the score negative
+    const uint32_t places = a.table_mask >> 16, low = places < 8 ? 0 : 3;
+    const int32_t start = (a.offset > P / 2 ? (int32_t)(a.offset - P) : (int32_t)a.offset) - (int32_t)(low << 16);
+    v4i y[R][4];
+#pragma unroll
+    for (int t = 0; t < 4; t++) {
+#pragma unroll
+      for (int r = 0; r < R; r++) y[r][t] = v4i{start, start, start, start};
+#pragma unroll
+      for (int s = 0; s < DT; s++) {
+        const v4i kd = keys[(4 * s + quarter) * 64 + 16 * t + col];
+#pragma unroll
+        for (int r = 0; r < R; r++) y[r][t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(kd, qd[r][s], y[r][t], 0, 0, 0);
+      }
+    }
+    if (TRACE && !SMALL && a.o.scores) {
+      const uint32_t rows = a.e[i].len * a.group;
+#pragma unroll
+      for (int r = 0; r < R; r++) {
+        const uint32_t row = row0 + 16 * r + col < rows ? row0 + 16 * r + col : rows - 1, token = row / a.group;
+        const uint64_t at = (((a.e[i].row + token) * a.kv_heads + kvh) * a.group + (row - token * a.group)) * a.o.score_cols;
+#pragma unroll
+        for (int t = 0; t < 4; t++) prompt_keep(a.o, at, b * kAttBlock + 16 * t + 4 * quarter, seen[r], y[r][t], low << 16);
+      }
+    }
+    uint32_t w[R][4], most[R] = {}, left = 0;
+    if (!SMALL) {
+#pragma unroll
+      for (int r = 0; r < R; r++)
+#pragma unroll
+        for (int t = 0; t < 4; t++) most[r] = max(max(most[r], max((uint32_t)y[r][t][0], (uint32_t)y[r][t][1])), max((uint32_t)y[r][t][2], (uint32_t)y[r][t][3]));
+#pragma unroll
+      for (int r = 1; r < R; r++) most[0] = max(most[0], most[r]);
+    }
+    if (!SMALL && !__any(most[0] > a.table_mask - (low << 16))) {  // all places at `low` and above: cut off at 10
+      const uint32_t top = low ? 0x7ffffu : 0xffffffu;
+#pragma unroll
+      for (int r = 0; r < R; r++)
+#pragma unroll
+        for (int t = 0; t < 4; t++) {
+          uint32_t x[4];
+#pragma unroll
+          for (int j = 0; j < 4; j++) x[j] = min((uint32_t)y[r][t][j], top);
+          w[r][t] = __builtin_amdgcn_perm(0x80c0e0f0u, 0xf8fcfeffu, prompt_places(x));
         }
+    } else {
+      const uint32_t place_mask = places * 0x01010101u;
+#pragma unroll
+      for (int r = 0; r < R; r++)
+#pragma unroll
+        for (int t = 0; t < 4; t++) {
+          uint32_t x[4];
+#pragma unroll
+          for (int j = 0; j < 4; j++) x[j] = signed32_mod_p(y[r][t][j] + (int32_t)(low << 16));
+          uint32_t g = prompt_places(x) & place_mask;
+          if (places > 15) g = prompt_cap(g);  // uniform
+          const uint32_t upper = prompt_upper(g);
+          if (low == 0) {  // uniform: places 0 .. 7, no other weights
+            w[r][t] = prompt_low(g, upper);
+          } else if (SMALL) {
+            w[r][t] = prompt_small(g, upper);
+          } else {
+            w[r][t] = prompt_wide(g, upper);
+            left |= prompt_small(g, upper) & sight(b, r, t);
+          }
+        }
+    }
+    if (!SMALL && __any(left != 0) && lane == 0) atomicOr(&marks[b / 32], 1u << (b % 32));
+    if (b >= whole) {  // uniform: tokens that a row does not see have no weight
+#pragma unroll
+      for (int r = 0; r < R; r++)
+#pragma unroll
+        for (int t = 0; t < 4; t++) w[r][t] &= sight(b, r, t);
+    }
+#pragma unroll
+    for (int r = 0; r < R; r++)
+#pragma unroll
+      for (int t = 0; t < 4; t++) z[r] = __builtin_amdgcn_sdot4((int)w[r][t], 0x01010101, z[r], false);
+#pragma unroll
+    for (int d = 0; d < (int)CH; d++) {
+      const v4i vd = values[d * 64 + lane];
+#pragma unroll
+      for (int r = 0; r < R; r++) {
+        const v4i wd = {(int)w[r][0], (int)w[r][1], (int)w[r][2], (int)w[r][3]};
+        acc[r][d] = __builtin_amdgcn_mfma_i32_16x16x64_i8(wd, vd, acc[r][d], 0, 0, 0);
       }
     }
   }
-  if (TRACE && row0 < rows)  // behind the last block they are cleared
-    for (uint32_t row = row0; row < wave_end; row++) {
-      const uint32_t token = row / a.group;
-      const uint64_t at = ((a.e[i].row + token) * a.kv_heads + kvh) * a.group + (row - token * a.group);
-      for (uint64_t t = (uint64_t)mine * kAttBlock + lane; t < a.o.score_cols; t += 64) a.o.scores[at * a.o.score_cols + t] = 0;
+  // k0 and v0 hold the first block (on its way)
+  __device__ __forceinline__ void run(v4i* k0, v4i* v0, v4i* k1, v4i* v1) {
+#pragma unroll
+    for (int r = 0; r < R; r++) {
+#pragma unroll
+      for (int d = 0; d < (int)CH; d++) acc[r][d] = v4i{0, 0, 0, 0};
+      z[r] = 0;
     }
-}
-// NP planes of the keys and values; NP = 1 takes four of the queries where a row
-// of its workgroup has them, a tile at a time.
-template <int NP, int DT, int R, int W, bool TRACE>
-__global__ void __launch_bounds__(64 * W, DT == 4 ? 1 : 2) k_prompt(PromptArgs a) {
-  __shared__ v4i lds[2 * NP * 4 * DT * 64];
-  __shared__ uint32_t general;
-  if (wit_four(a.mask) != (NP > 1)) return;  // uniform
+    uint32_t b = SMALL ? marked(0) : 0;
+#pragma unroll 1
+    while (b < blocks) {
+      const uint32_t second = SMALL ? marked(b + 1) : b + 1;
+      block(b, second, k0, v0, k1, v1);
+      if (second >= blocks) break;
+      b = SMALL ? marked(second + 1) : second + 1;
+      block(second, b, k1, v1, k0, v0);
+    }
+  }
+};
+
+// The int8 kernel.  A workgroup's W waves have R tiles of 16 rows each.
+template <int DT, int R, int W, int OCC, bool TRACE>
+static __global__ void __launch_bounds__(64 * W, OCC) k_prompt_int8(PromptArgs a) {
+  constexpr uint32_t CH = 4 * DT, KB = CH * 64;
+  __shared__ v4i k0[KB], v0[KB], k1[KB], v1[KB];
+  __shared__ uint32_t general[W], marks[(kMaxPrompt + kAttBlock) / kAttBlock / 32 + 1];
+  const uint32_t flagged = prompt_mask(a.mask);
+  const uint32_t lane = threadIdx.x & 63, col = lane & 15, quarter = lane >> 4;
+  const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  for (uint32_t w = threadIdx.x; w < sizeof(marks) / 4; w += 64 * W) marks[w] = 0;
   const uint32_t item = blockIdx.x;
   uint32_t i = 0;
   for (uint32_t up = a.n; up - i > 1;) {  // the last sequence that begins at or before this item
@@ -424,62 +705,198 @@ __global__ void __launch_bounds__(64 * W, DT == 4 ? 1 : 2) k_prompt(PromptArgs a
     if (a.e[mid].item0 <= item) i = mid;
     else up = mid;
   }
-  const uint32_t in = item - a.e[i].item0, tile = a.e[i].tiles - 1 - in / a.kv_heads, kvh = in % a.kv_heads;
-  const uint32_t lane = threadIdx.x & 63, col = lane & 15, quarter = lane >> 4;
-  const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const uint32_t in = item - a.e[i].item0, turn = in / a.kv_heads, tile = a.e[i].tiles - 1 - turn, kvh = in - turn * a.kv_heads;
   const uint32_t tile0 = tile * (16 * R * W), row0 = tile0 + wave * (16 * R), rows = a.e[i].len * a.group;
+  const uint32_t first = row0 < rows ? row0 : rows - 1;  // a wave without rows has the last one again, unused
+  const PromptRows place(first, a.group);
+  // word offsets of rows from `origin`: 2^32 bytes are enough for a tile's (4096 kv heads of 256, 256 rows)
+  const uint64_t origin = ((a.e[i].row + place.token0) * a.kv_heads + kvh) * (uint64_t)a.group * a.dim;
+  const uint32_t token_words = a.kv_heads * a.group * a.dim;
+
+  // the queries' words, whole rows at a time, to bytes in the operand order through
+  // LDS (the second half of the blocks' place), a wave 16 R rows in its share of it.
+  // c(x) mod 2^31 is x, or x + 1 for a negative number: its low byte, where the rest
+  // is the byte's sign
+  static_assert(2 * KB * 16 >= W * R * CH * 256, "the queries' place");
+  int8_t* const mine_q = (int8_t*)(wave < W / 2 ? k1 : v1) + (wave % (W / 2)) * (R * CH * 256);
   uint32_t high = 0;
-  auto query = [&](uint32_t at, auto& qd, auto planes) {  // of 16 rows
-    const uint32_t row = at + col < rows ? at + col : rows - 1, token = row / a.group;
-    const uint32_t* const from =
-        a.q + (((a.e[i].row + token) * a.kv_heads + kvh) * a.group + (row - token * a.group)) * a.dim;
 #pragma unroll
-    for (int s = 0; s < DT; s++)
+  for (int r = 0; r < R; r++) {
+    constexpr uint32_t VR = 16 * DT, N = 16 * VR / 64;  // vectors of four words of a row; a lane's of 16 rows
+    v4i w[N];
+    const uint32_t d = lane % VR * 4;
 #pragma unroll
-      for (uint32_t j = 0; j < 4; j++) {
-        const uint32_t d = 64 * s + 16 * quarter + 4 * j;
-        uint32_t x[4], out[4];
-        if (d + 4 <= a.dim) {
-          const v4i_word w = *(const v4i_word*)(from + d);
+    for (uint32_t j = 0; j < N; j++) {
+      const uint32_t x = 16 * r + j * (64 / VR) + lane / VR;
+      uint32_t token, head;
+      place.at(first + x < rows ? x : rows - 1 - first, token, head);
+      const uint32_t* const from = a.q + origin + (uint64_t)token * token_words + head * a.dim;
+      if (a.dim % 4 == 0) {  // uniform
+        w[j] = *(const v4i_word*)(from + (d < a.dim ? d : 0));
+      } else {
 #pragma unroll
-          for (int t = 0; t < 4; t++) x[t] = digit_bytes((uint32_t)w[t]);
-        } else {
-#pragma unroll
-          for (uint32_t t = 0; t < 4; t++) x[t] = d + t < a.dim ? digit_bytes(from[d + t]) : 0u;
-        }
-        transpose_bytes(x, out);
-        high |= out[1] | out[2] | out[3];
-#pragma unroll
-        for (int p = 0; p < decltype(planes)::value; p++) qd[s][p][j] = (int)out[p];
+        for (uint32_t t = 0; t < 4; t++) w[j][t] = (int)from[d + t < a.dim ? d + t : 0];
       }
-  };
-  if constexpr (NP == 1) {
-    v4i qd[R][DT][1];
-    if (threadIdx.x == 0) general = 0;
-    __syncthreads();
-#pragma unroll
-    for (int r = 0; r < R; r++) query(row0 + 16 * r, qd[r], std::integral_constant<int, 1>{});
-    if (__any(high != 0) && lane == 0) general = 1;
-    __syncthreads();
-    if (!general) {  // uniform
-      prompt_tile<1, 1, DT, R, W, TRACE>(a, lds, i, kvh, tile0, row0, qd);
-      return;
     }
-#pragma unroll 1
-    for (int r = 0; r < R; r++) {
-      const uint32_t start = tile0 + r * (16 * W);
-      if (start >= rows) return;  // uniform
-      v4i qg[1][DT][4];
-      query(start + 16 * wave, qg[0], std::integral_constant<int, 4>{});
-      prompt_tile<1, 4, DT, 1, W, TRACE>(a, lds, i, kvh, start, start + 16 * wave, qg);
-      __syncthreads();  // LDS is written again
-    }
-  } else {
-    v4i qd[R][DT][4];
 #pragma unroll
-    for (int r = 0; r < R; r++) query(row0 + 16 * r, qd[r], std::integral_constant<int, 4>{});
-    prompt_tile<NP, 4, DT, R, W, TRACE>(a, lds, i, kvh, tile0, row0, qd);
+    for (uint32_t j = 0; j < N; j++) {
+      const uint32_t x = j * (64 / VR) + lane / VR;
+      uint32_t b[4];
+#pragma unroll
+      for (uint32_t t = 0; t < 4; t++) {
+        b[t] = (uint32_t)w[j][t];
+        b[t] += b[t] >> 30;
+        if (d + t >= a.dim) b[t] = 0;
+        high |= b[t] + 128;
+      }
+      // chunk by chunk 16 rows of 16 bytes, in another order in each chunk: neither side meets its own banks
+      *(uint32_t*)(mine_q + ((r * CH + d / 16) * 16 + (x ^ (d / 16 & 15))) * 16 + d % 16) = pick_bytes<0>(b);
+    }
   }
+  high &= 0x7fffff00u;
+  if (__any(flagged != 0)) return;  // uniform: the general kernel's
+  const uint64_t block0 = kvh * a.head_bytes + (uint64_t)a.e[i].at * (4 * 1024 * a.chunks) + 1024 * wave * (CH / W) + 16 * lane;
+  const uint32_t tile_end = tile0 + 16 * R * W < rows ? tile0 + 16 * R * W : rows;
+  const uint32_t blocks = ((tile_end - 1) / a.group + kAttBlock) / kAttBlock;
+  uint32_t seen[R], last_seen;
+  {
+    uint32_t token, head;
+#pragma unroll
+    for (int r = 0; r < R; r++) {
+      place.at(16 * r + col, token, head);
+      seen[r] = row0 + 16 * r + col < rows ? place.token0 + token + 1 : 0;
+    }
+    place.at(first + 16 * R < rows ? 16 * R - 1 : rows - 1 - first, token, head);
+    last_seen = place.token0 + token + 1;
+  }
+  // blocks up to this wave's last row's end, and whole ones up to its first row's
+  const uint32_t my_blocks = (uint32_t)__builtin_amdgcn_readfirstlane((int)((last_seen + kAttBlock - 1) / kAttBlock));
+  const uint32_t whole = (uint32_t)__builtin_amdgcn_readfirstlane((int)((place.token0 + 1) / kAttBlock));
+  v4i qd[R][DT], acc[R][CH];
+  int32_t z[R];
+  auto pass = [&](auto small) {
+    constexpr bool SMALL = decltype(small)::value;
+    return PromptPass<DT, R, W, SMALL, TRACE>{a, a.k + block0, a.v + block0, i, kvh, row0, wave, lane, blocks,
+                                              row0 < rows ? my_blocks : 0u, whole, seen, qd, acc, z, marks};
+  };
+  auto wide = pass(std::false_type{});
+  wide.load(0, k0, v0);
+  {
+    const bool any_high = __any(high != 0);
+    if (lane == 0) general[wave] = any_high;
+  }
+  wave_exchange();
+#pragma unroll
+  for (int r = 0; r < R; r++)
+#pragma unroll
+    for (int s = 0; s < DT; s++) {
+      const uint32_t chunk = 4 * s + quarter;
+      qd[r][s] = *(const v4i*)(mine_q + ((r * CH + chunk) * 16 + (col ^ (chunk & 15))) * 16);
+    }
+  wide.arrive();
+  uint32_t some = 0;
+#pragma unroll
+  for (int w = 0; w < W; w++) some |= general[w];
+  if (threadIdx.x == 0) a.todo[item] = some;
+  if (some) return;  // uniform: queries of four planes are the other kernel's
+  wide.run(k0, v0, k1, v1);
+  __syncthreads();
+  const uint32_t first_marked = wide.marked(0);
+  const bool again = first_marked < blocks;
+
+  // the ends: a lane has rows 16 r + 4 quarter + v, dims 16 d + col
+  const WitBuffer out = wit_buffer(a.o.out, origin, ~0ull);
+  uint32_t at[R][4];  // byte offsets from origin; none for rows that are not there
+#pragma unroll
+  for (int r = 0; r < R; r++)
+#pragma unroll
+    for (int v = 0; v < 4; v++) {
+      const uint32_t x = 16 * r + 4 * quarter + v;
+      uint32_t token, head;
+      place.at(x, token, head);
+      at[r][v] = row0 + x < rows ? 4 * (token * token_words + head * a.dim + col) : kOutside;
+    }
+  uint32_t zs[R];
+  auto negate = [&](uint32_t by) {
+#pragma unroll
+    for (int r = 0; r < R; r++) {
+      uint32_t s = (uint32_t)-z[r] * by;
+      s += __shfl_xor(s, 16);
+      s += __shfl_xor(s, 32);
+      zs[r] = by == 1 && again ? zs[r] + s : s;
+    }
+  };
+  const uint32_t unit = a.table_mask >> 19 ? 8 : 1;  // of the wide weights
+  negate(unit);
+  if (again) {  // small weights too: the wide ones' sums wait in the output
+#pragma unroll
+    for (int d = 0; d < (int)CH; d++)
+#pragma unroll
+      for (int r = 0; r < R; r++)
+#pragma unroll
+        for (int v = 0; v < 4; v++)
+          if (16 * d + col < a.dim) wit_write(out, at[r][v] == kOutside ? kOutside : at[r][v] + 64 * d, (uint32_t)acc[r][d][v]);
+    auto rest = pass(std::true_type{});
+    rest.load(first_marked, k0, v0);  // all waves are past the loop
+    rest.run(k0, v0, k1, v1);
+    negate(1);
+  }
+  uint32_t zv[R][4];
+  double inv[R][4];
+#pragma unroll
+  for (int r = 0; r < R; r++)
+#pragma unroll
+    for (int v = 0; v < 4; v++) {
+      zv[r][v] = __shfl(zs[r], 4 * quarter + v);
+      // 1 / z to 2^-45 by a step of Newton's from the reciprocal's 2^-23 or better
+      const double zd = zv[r][v], guess = __builtin_amdgcn_rcp(zd);
+      inv[r][v] = -__builtin_fma(guess, __builtin_fma(-zd, guess, 1.0), guess);
+      if (a.o.sums && col == 0 && at[r][v] != kOutside) {
+        uint32_t token, head;
+        place.at(16 * r + 4 * quarter + v, token, head);
+        a.o.sums[((a.e[i].row + place.token0 + token) * a.kv_heads + kvh) * a.group + head] = shift16(m31_from_u32(zv[r][v]));
+      }
+    }
+#pragma unroll
+  for (int d = 0; d < (int)CH; d++) {
+    const bool there = 16 * d + col < a.dim;
+#pragma unroll
+    for (int r = 0; r < R; r++)
+#pragma unroll
+      for (int v = 0; v < 4; v++) {
+        const uint32_t to = there && at[r][v] != kOutside ? at[r][v] + 64 * d : kOutside;
+        double total;
+        if (again) total = __builtin_fma((double)unit, (double)(int32_t)wit_read(out, to), (double)acc[r][d][v]);
+        else total = (double)unit * (double)acc[r][d][v];
+        if (TRACE && a.o.weighted && to != kOutside)
+          a.o.weighted[origin + to / 4] = shift16(signed_mod_p(-(int64_t)total));
+        wit_write(out, to, prompt_mean(total, inv[r][v]));
+      }
+  }
+  if (TRACE && a.o.scores && row0 < rows)  // behind the last block they are cleared
+    prompt_clear<R>(a, i, kvh, row0, wide.mine);
+}
+// Words that are not int8-range: keys or values (by the packing's mask), or the
+// queries of an item (a.todo, by the int8 kernel, whose items are the same).
+template <int DT, int R, int W, int OCC, bool TRACE>
+static __global__ void __launch_bounds__(64 * W, OCC) k_prompt(PromptArgs a) {
+  __shared__ v4i lk[4 * 4 * DT * 64], lv[4 * 4 * DT * 64];
+  const bool flagged = __any(prompt_mask(a.mask) != 0);
+  const uint32_t item = blockIdx.x;
+  if (!flagged && !a.todo[item]) return;  // uniform
+  uint32_t i = 0;
+  for (uint32_t up = a.n; up - i > 1;) {  // the last sequence that begins at or before this item
+    const uint32_t mid = (i + up) / 2;
+    if (a.e[mid].item0 <= item) i = mid;
+    else up = mid;
+  }
+  const uint32_t in = item - a.e[i].item0, tile = a.e[i].tiles - 1 - in / a.kv_heads, kvh = in % a.kv_heads;
+  const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const uint32_t tile0 = tile * (16 * R * W), row0 = tile0 + wave * (16 * R);
+  v4i qd[R][DT][4];
+  prompt_query<DT, R>(a, i, kvh, row0, qd);
+  if (flagged) prompt_tile<4, 4, DT, R, W, TRACE>(a, lk, lv, i, kvh, tile0, row0, qd);
+  else prompt_tile<1, 4, DT, R, W, TRACE>(a, lk, lv, i, kvh, tile0, row0, qd);
 }
 
 }  // namespace gkr

@@ -93,16 +93,18 @@ static int attention_prompt(gkr_ctx* c, const gkr_matrix* q, const gkr_matrix* k
   a.chunks = chunks;
   a.offset = offset;
   a.table_mask = (1u << table_log) - 1;
-  // the sequences' items, in workgroups of `tile` rows
-  auto launch_all = [&](uint32_t tile, auto kernel) -> int {
-    a.n = 0;
+  // The sequences' items, in workgroups of `tile` rows: the int8 kernel's launch,
+  // then the other's, one of which finds nothing to do.
+  auto launch_all = [&](uint32_t tile, auto kernels) -> int {
+    uint64_t row = 0, at = 0, most = 0;
+    for (size_t i = 0; i < n_seqs; i++) most += (counts[i] * group + tile - 1) / tile;
+    TRY(ensureT(c, S_PROMPTQ, std::min<uint64_t>(most * kv_heads, (1ull << 22) + (0x7fffffffull / tile + 1) * kv_heads), &a.todo));
     uint32_t items = 0;
-    uint64_t row = 0, at = 0;
     auto launch = [&]() -> int {
       if (items == 0) return GKR_OK;
-      TRY(kernel(items));
+      TRY(kernels(items));
       a.n = items = 0;
-      return check_launch(c);
+      return GKR_OK;
     };
     for (size_t i = 0; i < n_seqs; i++) {
       if (counts[i] == 0) continue;
@@ -119,23 +121,30 @@ static int attention_prompt(gkr_ctx* c, const gkr_matrix* q, const gkr_matrix* k
     }
     return launch();
   };
-#define GKR_PROMPT(NP, DT, R, W)                                                              \
-  launch_all(16 * R * W, [&](uint32_t items) -> int {                                         \
-    if (scores) GKR_LAUNCH(c, (k_prompt<NP, DT, R, W, true>), dim3(items), dim3(64 * W), 0, a); \
-    else GKR_LAUNCH(c, (k_prompt<NP, DT, R, W, false>), dim3(items), dim3(64 * W), 0, a);     \
-    return GKR_OK;                                                                            \
+  // R1 and W1 of the int8 kernel, R4 and W4 of the other: tiles of 16 rows a wave, waves
+#define GKR_PROMPT_(DT, R1, W1, OCC1, R4, W4, OCC4)                                                                  \
+  static_assert(R1 * W1 == R4 * W4, "the same items");                                                               \
+  return launch_all(16 * R1 * W1, [&](uint32_t items) -> int {                                                       \
+    if (scores || weighted) GKR_LAUNCH(c, (k_prompt_int8<DT, R1, W1, OCC1, true>), dim3(items), dim3(64 * W1), 0, a); \
+    else GKR_LAUNCH(c, (k_prompt_int8<DT, R1, W1, OCC1, false>), dim3(items), dim3(64 * W1), 0, a);                  \
+    TRY(check_launch(c));                                                                                            \
+    if (scores || weighted) GKR_LAUNCH(c, (k_prompt<DT, R4, W4, OCC4, true>), dim3(items), dim3(64 * W4), 0, a);     \
+    else GKR_LAUNCH(c, (k_prompt<DT, R4, W4, OCC4, false>), dim3(items), dim3(64 * W4), 0, a);                       \
+    return check_launch(c);                                                                                          \
   })
+#define GKR_PROMPT(...) GKR_PROMPT_(__VA_ARGS__)
+#ifndef PV
+#define PV 2, 2, 4, 3, 1, 8, 2
+#endif
   if (dim <= 64) {
-    TRY(GKR_PROMPT(1, 1, 2, 4));
-    return GKR_PROMPT(4, 1, 1, 4);
+    GKR_PROMPT(1, 2, 4, 3, 1, 8, 2);
   }
   if (dim <= 128) {
-    TRY(GKR_PROMPT(1, 2, 2, 4));
-    return GKR_PROMPT(4, 2, 1, 8);
+    GKR_PROMPT(PV);
   }
-  TRY(GKR_PROMPT(1, 4, 1, 4));
-  return GKR_PROMPT(4, 4, 1, 4);
+  GKR_PROMPT(4, 1, 4, 2, 1, 4, 1);
 #undef GKR_PROMPT
+#undef GKR_PROMPT_
 }
 extern "C" int gkr_attention_prompt(gkr_ctx* c, const gkr_matrix* q, const gkr_matrix* k, const gkr_matrix* v,
                                     const uint32_t* counts, size_t n_seqs, uint32_t heads, uint32_t kv_heads,
