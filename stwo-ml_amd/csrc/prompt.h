@@ -31,11 +31,11 @@ __device__ __forceinline__ uint32_t prompt_mask(const uint32_t* mask) {  // this
 
 struct PromptPack {
   uint32_t n, kv_heads, dim, chunks;
-  uint64_t head_bytes;  // of a kv head's blocks, all sequences'
+  uint32_t n_blocks, blocks, counters;  // blocks of this launch; blocks of a kv head, all sequences'; launches of the products to come
+  uint32_t* counter;
   struct {
     uint32_t block0, len, at;  // its first block in this launch; tokens; its first block of all
-    uint32_t pad;
-    uint64_t row;              // its first row of k and v
+    uint32_t row;              // its first row of k and v
   } e[kPromptSeqs];
 };
 // Bytes of plane p of a block begin at p * chunks * 1024.
@@ -43,70 +43,112 @@ __device__ __forceinline__ uint32_t prompt_key(uint32_t token, uint32_t chunk) {
 __device__ __forceinline__ uint32_t prompt_value(uint32_t quarter, uint32_t dim) {
   return dim / 16 * 1024 + 256 * quarter + 16 * (dim % 16);
 }
-// A workgroup packs a block of 64 tokens of one kv head, a wave 16 dims at a time.
-// Words of the mask are set where a digit above plane 0 is not zero, and `clear`,
-// the mask of the next operator on the stream, is zeroed, as in k_wit_pack.
+// A workgroup packs a block of 64 tokens of one kv head, a wave 16 dims of its keys
+// or of its values at a time (so that all words are asked for at once).
+// A digit above plane 0 is rare: the three upper planes are stored only where the
+// block's keys, or values, have such a digit, which its word of `upper` tells the
+// products (bit 0 keys, bit 1 values); then a word of the mask is set too, as in
+// k_wit_pack, and `clear`, the mask of the next operator on the stream, is zeroed.
 // Places behind a sequence's last token get its words again: they have no weight.
-static __global__ void __launch_bounds__(256) k_prompt_pack(PromptPack a, const uint32_t* __restrict__ k,
-                                                            const uint32_t* __restrict__ v, int8_t* __restrict__ ko,
-                                                            int8_t* __restrict__ vo, uint32_t* __restrict__ mask,
-                                                            uint32_t* __restrict__ clear) {
-  if (blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x < kMaskWords) clear[kMaskStride * threadIdx.x] = 0;
+// The workgroups of an XCD (blockIdx 8 apart) take the heads of a block one after
+// another, so that it reads whole rows: all heads' first, then the next block's. With
+// one head after the other all that run at a time read the same few channels of the
+// caches (62 us, and 13 so).
+constexpr uint32_t kPackHeads = 64;  // along one grid dimension
+constexpr uint32_t kPackWaves = 16;
+template <uint32_t PIECES>  // a wave's: of 32 there are at most
+static __global__ void __launch_bounds__(64 * kPackWaves) k_prompt_pack(PromptPack a, const uint32_t* __restrict__ k,
+                                                             const uint32_t* __restrict__ v, int8_t* __restrict__ ko,
+                                                             int8_t* __restrict__ vo, uint32_t* __restrict__ upper,
+                                                             uint32_t* __restrict__ mask, uint32_t* __restrict__ clear) {
+  __shared__ uint32_t highs[kPackWaves];  // of the waves: bit 0 keys, bit 1 values
+  const uint32_t waves = blockDim.x / 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  if (blockIdx.x == 0 && blockIdx.y == 0) {
+    if (threadIdx.x < kMaskWords) clear[kMaskStride * threadIdx.x] = 0;
+    for (uint32_t c = threadIdx.x; c < a.counters; c += blockDim.x) a.counter[c] = 0;
+  }
+  const uint32_t wide = a.kv_heads < kPackHeads ? a.kv_heads : kPackHeads;
+  const uint32_t head = blockIdx.x / 8 % wide + blockIdx.y * kPackHeads, at = blockIdx.x / 8 / wide * 8 + blockIdx.x % 8;
+  if (at >= a.n_blocks || head >= a.kv_heads) return;  // uniform
   uint32_t i = 0;
   for (uint32_t up = a.n; up - i > 1;) {  // the last sequence that begins at or before this block
     const uint32_t mid = (i + up) / 2;
-    if (a.e[mid].block0 <= blockIdx.x) i = mid;
+    if (a.e[mid].block0 <= at) i = mid;
     else up = mid;
   }
-  const uint32_t in = blockIdx.x - a.e[i].block0, first = in * kAttBlock, last = a.e[i].len - 1, head = blockIdx.y;
-  const uint64_t width = (uint64_t)a.kv_heads * a.dim;
-  const uint64_t to = head * a.head_bytes + (uint64_t)(a.e[i].at + in) * (4 * 1024 * a.chunks);
+  const uint32_t in = at - a.e[i].block0, first = in * kAttBlock, last = a.e[i].len - 1;
+  const uint64_t width = (uint64_t)a.kv_heads * a.dim, block = (uint64_t)head * a.blocks + a.e[i].at + in;
   const uint32_t lane = threadIdx.x & 63, q = lane & 3, plane = 1024 * a.chunks;
-  uint32_t high = 0;
-  auto words = [&](const uint32_t* m, uint32_t token, uint32_t d, uint32_t (&x)[4]) {
-    const uint32_t t = first + token < last ? first + token : last;
-    const uint32_t* const from = m + (a.e[i].row + t) * width + (uint64_t)head * a.dim + d;
-    if (d + 4 <= a.dim) {
-      const v4i_word w = *(const v4i_word*)from;
+  const uint64_t to = block * (4 * plane);
+  uint32_t d[PIECES][4][4];  // digits: keys [16 tokens][plane], values [dim][plane]: a word each
 #pragma unroll
-      for (int j = 0; j < 4; j++) x[j] = digit_bytes((uint32_t)w[j]);
+  for (uint32_t j = 0; j < PIECES; j++) {
+    // keys: lane 4 t + q has dims 4 q .. + 3 of tokens t, 16 + t ..;
+    // values: lane 16 c + 4 g + t has tokens 16 t + 4 c .. + 3 of dims 4 g .. + 3
+    const uint32_t piece = wave + j * waves, chunk = piece / 2, values = piece & 1;
+    if (piece >= 2 * a.chunks) break;  // uniform
+    const uint32_t dim0 = 16 * chunk + 4 * (values ? lane / 4 % 4 : q);
+    uint32_t x[4][4];
+    const uint32_t* from[4];
+#pragma unroll
+    for (uint32_t t = 0; t < 4; t++) {
+      const uint32_t token = first + (values ? 16 * q + 4 * (lane / 16) + t : 16 * t + lane / 4);
+      from[t] = (values ? v : k) + ((uint64_t)a.e[i].row + (token < last ? token : last)) * width + (uint64_t)head * a.dim;
+    }
+    if (a.dim % 4 == 0) {  // uniform
+      const uint32_t at0 = dim0 < a.dim ? dim0 : 0;
+      v4i_word w[4];
+#pragma unroll
+      for (uint32_t t = 0; t < 4; t++) w[t] = *(const v4i_word*)(from[t] + at0);
+#pragma unroll
+      for (uint32_t t = 0; t < 4; t++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) x[t][e] = (uint32_t)w[t][e];
     } else {
 #pragma unroll
-      for (uint32_t j = 0; j < 4; j++) x[j] = d + j < a.dim ? digit_bytes(from[j]) : 0u;
-    }
-  };
-  for (uint32_t chunk = threadIdx.x >> 6; chunk < a.chunks; chunk += 4) {
-    // keys: lane 4 t + q has token t's dims 4 q .. + 3, and stores plane q of its 16
+      for (uint32_t t = 0; t < 4; t++)
 #pragma unroll
-    for (uint32_t t0 = 0; t0 < 64; t0 += 16) {
-      uint32_t x[4], out[4];
-      words(k, t0 + lane / 4, 16 * chunk + 4 * q, x);
-      transpose_bytes(x, out);
-      high |= out[1] | out[2] | out[3];
-      quad_transpose(out);
-      *(uint4*)(ko + to + q * plane + prompt_key(t0 + lane / 4, chunk)) = make_uint4(out[0], out[1], out[2], out[3]);
+        for (uint32_t e = 0; e < 4; e++) x[t][e] = from[t][dim0 + e < a.dim ? dim0 + e : 0];
     }
-    // values: lane 16 c + 4 g + t has tokens 16 t + 4 c .. + 3 of dims 4 g .. + 3
-    const uint32_t c = lane / 16, g = lane / 4 % 4;
-    uint32_t x[4][4], y[4][4];  // [token][dim], [dim][plane]
 #pragma unroll
-    for (uint32_t j = 0; j < 4; j++) words(v, 16 * q + 4 * c + j, 16 * chunk + 4 * g, x[j]);
+    for (uint32_t t = 0; t < 4; t++)
 #pragma unroll
-    for (uint32_t d = 0; d < 4; d++) {
-      const uint32_t of[4] = {x[0][d], x[1][d], x[2][d], x[3][d]};
-      transpose_bytes(of, y[d]);
-      high |= y[d][1] | y[d][2] | y[d][3];
+      for (uint32_t e = 0; e < 4; e++) x[t][e] = dim0 + e < a.dim ? digit_bytes(x[t][e]) : 0u;
+    uint32_t high = 0;
+#pragma unroll
+    for (uint32_t t = 0; t < 4; t++) {
+      const uint32_t of[4] = {values ? x[0][t] : x[t][0], values ? x[1][t] : x[t][1], values ? x[2][t] : x[t][2],
+                              values ? x[3][t] : x[t][3]};
+      transpose_bytes(of, d[j][t]);
+      high |= d[j][t][1] | d[j][t][2] | d[j][t][3];
     }
+    const uint32_t any = (uint32_t)__any(high != 0) << values;
+    if (lane == 0) highs[wave] = j ? highs[wave] | any : any;
+  }
+  __syncthreads();
+  uint32_t all = 0;
+  if (lane < waves) all = highs[lane];  // every wave has a piece
+  all = (uint32_t)__any(all & 1) | (uint32_t)__any(all >> 1) << 1;
+#pragma unroll
+  for (uint32_t j = 0; j < PIECES; j++) {
+    const uint32_t piece = wave + j * waves, chunk = piece / 2, values = piece & 1;
+    if (piece >= 2 * a.chunks) break;  // uniform
+    const uint32_t planes = all >> values & 1 ? 4 : 1;
+    // of a quad lane q takes the 16 bytes of token 16 q + lane / 4, or of dim 4 g + q
+    int8_t* const out = (values ? vo + prompt_value(lane / 16, 16 * chunk + 4 * (lane / 4 % 4) + q)
+                                : ko + prompt_key(16 * q + lane / 4, chunk)) + to;
 #pragma unroll
     for (uint32_t p = 0; p < 4; p++) {
-      uint32_t w[4] = {y[0][p], y[1][p], y[2][p], y[3][p]};
-      quad_transpose(w);  // lane q of a quad: dim 4 g + q, all of t
-      *(uint4*)(vo + to + p * plane + prompt_value(c, 16 * chunk + 4 * g + q)) = make_uint4(w[0], w[1], w[2], w[3]);
+      if (p >= planes) break;
+      uint32_t w[4] = {d[j][0][p], d[j][1][p], d[j][2][p], d[j][3][p]};
+      quad_transpose(w);
+      *(uint4*)(out + p * plane) = make_uint4(w[0], w[1], w[2], w[3]);
     }
   }
-  if (__any(high != 0) && lane == 0) {
-    volatile uint32_t* const word = mask + kMaskStride * ((blockIdx.x * 4 + (threadIdx.x >> 6)) % kPromptWords);
-    if (!*word) *word = 1;
+  if (threadIdx.x == 0) {
+    upper[block] = all;
+    volatile uint32_t* const word = mask + kMaskStride * (blockIdx.x % kPromptWords);
+    if (all && !*word) *word = 1;
   }
 }
 
@@ -131,18 +173,22 @@ __device__ __forceinline__ uint32_t prompt_score(const S& s, int v, int32_t offs
   }
 }
 
+constexpr uint32_t kPromptCounters = 9;  // a launch's words of PromptArgs::counter
 struct PromptArgs {
   const int8_t *k, *v;
   const uint32_t *q, *mask;
   AttOut o;
-  uint64_t head_bytes;
+  uint32_t blocks;  // of a kv head, all sequences'
   uint32_t n, kv_heads, group, dim, chunks;
   uint32_t offset, table_mask;
-  uint32_t* todo;  // a word an item: whether the int8 kernel left it
+  const uint32_t* upper;  // the packing's, a word a block
+  // todo: a word an item, whether the int8 kernel left it; counter: how many items of
+  // each eighth the other has taken, and whether any word of todo is set
+  uint32_t items, general_items, *todo, *counter;
   struct {
-    uint32_t item0, tiles;  // its first item of this launch, its tiles of rows
-    uint32_t len, at;       // tokens; its first block
-    uint64_t row;           // its first row of q
+    uint32_t item0, tiles;  // its first item of this launch, its tiles of rows (int8 kernel)
+    uint32_t general0;      // its first item of the other kernel, whose tiles are `per` of these
+    uint32_t len, at, row;  // tokens; its first block; its first row of q
   } e[kPromptSeqs];
 };
 
@@ -225,7 +271,7 @@ __device__ __forceinline__ void prompt_clear(const PromptArgs& a, uint32_t i, ui
   const uint32_t rows = a.e[i].len * a.group, end = row0 + 16 * R < rows ? row0 + 16 * R : rows;
   for (uint32_t row = row0; row < end; row++) {
     const uint32_t token = row / a.group;
-    const uint64_t at = ((a.e[i].row + token) * a.kv_heads + kvh) * a.group + (row - token * a.group);
+    const uint64_t at = (((uint64_t)a.e[i].row + token) * a.kv_heads + kvh) * a.group + (row - token * a.group);
     for (uint64_t t = (uint64_t)mine * kAttBlock + (threadIdx.x & 63); t < a.o.score_cols; t += 64) a.o.scores[at * a.o.score_cols + t] = 0;
   }
 }
@@ -253,7 +299,7 @@ __device__ __forceinline__ void prompt_end(const PromptArgs& a, uint32_t i, uint
       const uint32_t row = row0 + 16 * r + 4 * quarter + v, zr = __shfl(zc, 4 * quarter + v);
       if (row >= rows) continue;
       const uint32_t token = row / a.group;
-      const uint64_t at = ((a.e[i].row + token) * a.kv_heads + kvh) * a.group + (row - token * a.group);
+      const uint64_t at = (((uint64_t)a.e[i].row + token) * a.kv_heads + kvh) * a.group + (row - token * a.group);
       if (a.o.sums && col == 0) a.o.sums[at] = shift16(m31_from_u32(zr));
       const double inv = (NP == 1 ? -1.0 : 0.5) / zr;
 #pragma unroll
@@ -301,17 +347,24 @@ __device__ __forceinline__ void prompt_tile(const PromptArgs& a, v4i* __restrict
     const uint32_t row = row0 + 16 * r + col;
     seen[r] = row < rows ? row / a.group + 1 : 0;
   }
-  const uint64_t base = kvh * a.head_bytes + (uint64_t)a.e[i].at * (4 * plane) + 16 * lane;
+  const uint64_t block0 = (uint64_t)kvh * a.blocks + a.e[i].at, base = block0 * (4 * plane) + 16 * lane;
   uint32_t from[ND];  // of this wave's pieces; chunks past the last are the last one again (the query is zero there)
 #pragma unroll
   for (int j = 0; j < ND; j++) {
     const uint32_t piece = wave * ND + j, chunk = piece % CH < a.chunks ? piece % CH : a.chunks - 1;
     from[j] = piece < CH * NP ? piece / CH * plane + 1024 * chunk : 0;
   }
-  auto load = [&](v4i (&in)[ND], const int8_t* m, uint32_t b) {  // past the last block: again, unused
+  // the upper planes of keys or values that have none are zero and not in memory; the
+  // word that tells goes a block ahead
+  uint32_t upper = NP > 1 ? a.upper[block0] : 0;
+  auto load = [&](v4i (&in)[ND], const int8_t* m, uint32_t b, uint32_t bit) {  // past the last block: again, unused
     const int8_t* const block = m + base + (uint64_t)(b < blocks ? b : blocks - 1) * (4 * plane);
+    const bool have = __builtin_amdgcn_readfirstlane((int)upper) >> bit & 1;
 #pragma unroll
-    for (int j = 0; j < ND; j++) in[j] = *(const v4i*)(block + from[j]);
+    for (int j = 0; j < ND; j++) {
+      if (NP == 1 || wave * ND + j < CH || have) in[j] = *(const v4i*)(block + from[j]);  // uniform
+      else in[j] = v4i{0, 0, 0, 0};
+    }
   };
   auto put = [&](const v4i (&in)[ND], v4i* to) {
 #pragma unroll
@@ -330,12 +383,13 @@ __device__ __forceinline__ void prompt_tile(const PromptArgs& a, v4i* __restrict
   const uint32_t place_mask = (a.table_mask >> 16) * 0x01010101u;
   const bool many = a.table_mask >> 20 != 0;
   v4i in[ND];
-  load(in, a.k, 0);
+  load(in, a.k, 0, 0);
   put(in, lk);
 #pragma unroll 1
   for (uint32_t b = 0; b < blocks; b++) {
     __syncthreads();  // the keys are there, the values' place is free
-    load(in, a.v, b);
+    load(in, a.v, b, 1);
+    if (NP > 1) upper = a.upper[block0 + (b + 1 < blocks ? b + 1 : b)];
     uint32_t w0[R][4], w1[R][4];  // NP = 1: small and wide weights; else the digits base 256
     bool some_small = false;
     const bool busy = b < mine;
@@ -377,7 +431,7 @@ __device__ __forceinline__ void prompt_tile(const PromptArgs& a, v4i* __restrict
           }
           if (TRACE && a.o.scores) {
             const uint32_t row = row0 + 16 * r + col, token = row / a.group;
-            const uint64_t at = (((a.e[i].row + token) * a.kv_heads + kvh) * a.group + (row - token * a.group)) * a.o.score_cols;
+            const uint64_t at = ((((uint64_t)a.e[i].row + token) * a.kv_heads + kvh) * a.group + (row - token * a.group)) * a.o.score_cols;
             prompt_keep(a.o, at, b * kAttBlock + 16 * t + 4 * quarter, seen[r], v4i{(int)x[0], (int)x[1], (int)x[2], (int)x[3]}, 0);
           }
           w0[r][t] = prompt_places(x) & place_mask;
@@ -427,7 +481,7 @@ __device__ __forceinline__ void prompt_tile(const PromptArgs& a, v4i* __restrict
     }
     put(in, lv);
     __syncthreads();  // the values are there, the keys' place is free
-    load(in, a.k, b + 1);
+    load(in, a.k, b + 1, 0);
     if (busy) {
       auto product = [&](int r, int d, int g, const uint32_t (&w)[4], const v4i& vd) {
         const v4i wd = {(int)w[0], (int)w[1], (int)w[2], (int)w[3]};
@@ -474,7 +528,7 @@ __device__ __forceinline__ void prompt_query(const PromptArgs& a, uint32_t i, ui
   for (int r = 0; r < R; r++) {
     const uint32_t here = row0 + 16 * r + col, row = here < rows ? here : rows - 1, token = row / a.group;
     const uint32_t* const from =
-        a.q + (((a.e[i].row + token) * a.kv_heads + kvh) * a.group + (row - token * a.group)) * a.dim;
+        a.q + ((((uint64_t)a.e[i].row + token) * a.kv_heads + kvh) * a.group + (row - token * a.group)) * a.dim;
     v4i w[DT][4];
     if (a.dim % 4 == 0) {  // uniform
 #pragma unroll
@@ -600,7 +654,7 @@ struct PromptPass {
 #pragma unroll
       for (int r = 0; r < R; r++) {
         const uint32_t row = row0 + 16 * r + col < rows ? row0 + 16 * r + col : rows - 1, token = row / a.group;
-        const uint64_t at = (((a.e[i].row + token) * a.kv_heads + kvh) * a.group + (row - token * a.group)) * a.o.score_cols;
+        const uint64_t at = ((((uint64_t)a.e[i].row + token) * a.kv_heads + kvh) * a.group + (row - token * a.group)) * a.o.score_cols;
 #pragma unroll
         for (int t = 0; t < 4; t++) prompt_keep(a.o, at, b * kAttBlock + 16 * t + 4 * quarter, seen[r], y[r][t], low << 16);
       }
@@ -710,7 +764,7 @@ static __global__ void __launch_bounds__(64 * W, OCC) k_prompt_int8(PromptArgs a
   const uint32_t first = row0 < rows ? row0 : rows - 1;  // a wave without rows has the last one again, unused
   const PromptRows place(first, a.group);
   // word offsets of rows from `origin`: 2^32 bytes are enough for a tile's (4096 kv heads of 256, 256 rows)
-  const uint64_t origin = ((a.e[i].row + place.token0) * a.kv_heads + kvh) * (uint64_t)a.group * a.dim;
+  const uint64_t origin = (((uint64_t)a.e[i].row + place.token0) * a.kv_heads + kvh) * (uint64_t)a.group * a.dim;
   const uint32_t token_words = a.kv_heads * a.group * a.dim;
 
   // the queries' words, whole rows at a time, to bytes in the operand order through
@@ -720,11 +774,11 @@ static __global__ void __launch_bounds__(64 * W, OCC) k_prompt_int8(PromptArgs a
   static_assert(2 * KB * 16 >= W * R * CH * 256, "the queries' place");
   int8_t* const mine_q = (int8_t*)(wave < W / 2 ? k1 : v1) + (wave % (W / 2)) * (R * CH * 256);
   uint32_t high = 0;
+  constexpr uint32_t VR = 16 * DT, N = 16 * VR / 64;  // vectors of four words of a row; a lane's of 16 rows
+  const uint32_t d = lane % VR * 4;
+  v4i w[R][N];
 #pragma unroll
-  for (int r = 0; r < R; r++) {
-    constexpr uint32_t VR = 16 * DT, N = 16 * VR / 64;  // vectors of four words of a row; a lane's of 16 rows
-    v4i w[N];
-    const uint32_t d = lane % VR * 4;
+  for (int r = 0; r < R; r++)
 #pragma unroll
     for (uint32_t j = 0; j < N; j++) {
       const uint32_t x = 16 * r + j * (64 / VR) + lane / VR;
@@ -732,19 +786,22 @@ static __global__ void __launch_bounds__(64 * W, OCC) k_prompt_int8(PromptArgs a
       place.at(first + x < rows ? x : rows - 1 - first, token, head);
       const uint32_t* const from = a.q + origin + (uint64_t)token * token_words + head * a.dim;
       if (a.dim % 4 == 0) {  // uniform
-        w[j] = *(const v4i_word*)(from + (d < a.dim ? d : 0));
+        w[r][j] = *(const v4i_word*)(from + (d < a.dim ? d : 0));
       } else {
 #pragma unroll
-        for (uint32_t t = 0; t < 4; t++) w[j][t] = (int)from[d + t < a.dim ? d + t : 0];
+        for (uint32_t t = 0; t < 4; t++) w[r][j][t] = (int)from[d + t < a.dim ? d + t : 0];
       }
     }
+  if (__any(flagged != 0)) return;  // uniform: the other kernel's
+#pragma unroll
+  for (int r = 0; r < R; r++)
 #pragma unroll
     for (uint32_t j = 0; j < N; j++) {
       const uint32_t x = j * (64 / VR) + lane / VR;
       uint32_t b[4];
 #pragma unroll
       for (uint32_t t = 0; t < 4; t++) {
-        b[t] = (uint32_t)w[j][t];
+        b[t] = (uint32_t)w[r][j][t];
         b[t] += b[t] >> 30;
         if (d + t >= a.dim) b[t] = 0;
         high |= b[t] + 128;
@@ -752,10 +809,8 @@ static __global__ void __launch_bounds__(64 * W, OCC) k_prompt_int8(PromptArgs a
       // chunk by chunk 16 rows of 16 bytes, in another order in each chunk: neither side meets its own banks
       *(uint32_t*)(mine_q + ((r * CH + d / 16) * 16 + (x ^ (d / 16 & 15))) * 16 + d % 16) = pick_bytes<0>(b);
     }
-  }
   high &= 0x7fffff00u;
-  if (__any(flagged != 0)) return;  // uniform: the general kernel's
-  const uint64_t block0 = kvh * a.head_bytes + (uint64_t)a.e[i].at * (4 * 1024 * a.chunks) + 1024 * wave * (CH / W) + 16 * lane;
+  const uint64_t block0 = ((uint64_t)kvh * a.blocks + a.e[i].at) * (4 * 1024 * a.chunks) + 1024 * wave * (CH / W) + 16 * lane;
   const uint32_t tile_end = tile0 + 16 * R * W < rows ? tile0 + 16 * R * W : rows;
   const uint32_t blocks = ((tile_end - 1) / a.group + kAttBlock) / kAttBlock;
   uint32_t seen[R], last_seen;
@@ -797,7 +852,10 @@ static __global__ void __launch_bounds__(64 * W, OCC) k_prompt_int8(PromptArgs a
   uint32_t some = 0;
 #pragma unroll
   for (int w = 0; w < W; w++) some |= general[w];
-  if (threadIdx.x == 0) a.todo[item] = some;
+  if (threadIdx.x == 0) {
+    a.todo[item] = some;
+    if (some) a.counter[8] = 1;
+  }
   if (some) return;  // uniform: queries of four planes are the other kernel's
   wide.run(k0, v0, k1, v1);
   __syncthreads();
@@ -854,7 +912,7 @@ static __global__ void __launch_bounds__(64 * W, OCC) k_prompt_int8(PromptArgs a
       if (a.o.sums && col == 0 && at[r][v] != kOutside) {
         uint32_t token, head;
         place.at(16 * r + 4 * quarter + v, token, head);
-        a.o.sums[((a.e[i].row + place.token0 + token) * a.kv_heads + kvh) * a.group + head] = shift16(m31_from_u32(zv[r][v]));
+        a.o.sums[(((uint64_t)a.e[i].row + place.token0 + token) * a.kv_heads + kvh) * a.group + head] = shift16(m31_from_u32(zv[r][v]));
       }
     }
 #pragma unroll
@@ -877,26 +935,49 @@ static __global__ void __launch_bounds__(64 * W, OCC) k_prompt_int8(PromptArgs a
     prompt_clear<R>(a, i, kvh, row0, wide.mine);
 }
 // Words that are not int8-range: keys or values (by the packing's mask), or the
-// queries of an item (a.todo, by the int8 kernel, whose items are the same).
-template <int DT, int R, int W, int OCC, bool TRACE>
+// queries of an item (a.todo, by the int8 kernel; PER of its items are one here).  No more
+// workgroups than fit at once: the items are taken in turn, the longest first, and
+// with nothing to do the launch is short (3 us; 7 with a workgroup for each of 2432
+// items).  The workgroups of an XCD (blockIdx 8 apart) take every eighth item, which
+// with eight kv heads are one head's (1501 general tokens: 174 us; any item 202).
+template <int DT, int R, int W, int OCC, uint32_t PER, bool TRACE>
 static __global__ void __launch_bounds__(64 * W, OCC) k_prompt(PromptArgs a) {
   __shared__ v4i lk[4 * 4 * DT * 64], lv[4 * 4 * DT * 64];
+  __shared__ uint32_t taken;
+  const uint32_t left = a.counter[8];
   const bool flagged = __any(prompt_mask(a.mask) != 0);
-  const uint32_t item = blockIdx.x;
-  if (!flagged && !a.todo[item]) return;  // uniform
-  uint32_t i = 0;
-  for (uint32_t up = a.n; up - i > 1;) {  // the last sequence that begins at or before this item
-    const uint32_t mid = (i + up) / 2;
-    if (a.e[mid].item0 <= item) i = mid;
-    else up = mid;
-  }
-  const uint32_t in = item - a.e[i].item0, tile = a.e[i].tiles - 1 - in / a.kv_heads, kvh = in % a.kv_heads;
+  if (!flagged && !left) return;  // uniform
   const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const uint32_t tile0 = tile * (16 * R * W), row0 = tile0 + wave * (16 * R);
-  v4i qd[R][DT][4];
-  prompt_query<DT, R>(a, i, kvh, row0, qd);
-  if (flagged) prompt_tile<4, 4, DT, R, W, TRACE>(a, lk, lv, i, kvh, tile0, row0, qd);
-  else prompt_tile<1, 4, DT, R, W, TRACE>(a, lk, lv, i, kvh, tile0, row0, qd);
+  uint32_t item = blockIdx.x;
+#pragma unroll 1
+  for (;; item += gridDim.x) {
+    if (flagged) {
+      const uint32_t eighths = gridDim.x < 8 ? 1 : 8, mine = blockIdx.x % eighths;
+      if (threadIdx.x == 0) taken = atomicAdd(a.counter + mine, 1u) * eighths + mine;
+      __syncthreads();
+      item = taken;
+    }
+    if (item >= a.general_items) return;  // uniform
+    uint32_t i = 0;
+    for (uint32_t up = a.n; up - i > 1;) {  // the last sequence that begins at or before this item
+      const uint32_t mid = (i + up) / 2;
+      if (a.e[mid].general0 <= item) i = mid;
+      else up = mid;
+    }
+    const uint32_t in = item - a.e[i].general0, tiles = a.e[i].tiles, tile = (tiles + PER - 1) / PER - 1 - in / a.kv_heads;
+    const uint32_t kvh = in % a.kv_heads, tile0 = tile * (16 * R * W), row0 = tile0 + wave * (16 * R);
+    if (!flagged) {
+      uint32_t some = 0;
+      for (uint32_t t = PER * tile; t < PER * tile + PER && t < tiles; t++)
+        some |= a.todo[a.e[i].item0 + (tiles - 1 - t) * a.kv_heads + kvh];
+      if (!some) continue;  // uniform
+    }
+    v4i qd[R][DT][4];
+    prompt_query<DT, R>(a, i, kvh, row0, qd);
+    if (flagged) prompt_tile<4, 4, DT, R, W, TRACE>(a, lk, lv, i, kvh, tile0, row0, qd);
+    else prompt_tile<1, 4, DT, R, W, TRACE>(a, lk, lv, i, kvh, tile0, row0, qd);
+    __syncthreads();  // LDS is written again
+  }
 }
 
 }  // namespace gkr

@@ -40,44 +40,56 @@ static int attention_prompt(gkr_ctx* c, const gkr_matrix* q, const gkr_matrix* k
       return fail(GKR_ERR_INVALID, "%s: scores of %llu columns for sequences of up to %llu tokens (at most 2^21)", what,
                   (unsigned long long)scores->cols, (unsigned long long)longest);
   }
-  if (blocks > 0xffffffffull) return fail(GKR_ERR_INVALID, "%s: too many tokens", what);
+  if (rows > 0xffffffffull || blocks > 0xffffffffull) return fail(GKR_ERR_INVALID, "%s: too many tokens", what);
   HIP_TRY(hipSetDevice(c->device));
   for (gkr_matrix* m : {weighted, sums, scores, out})
     if (m) TRY(drop_derived(c, m));
-  const uint64_t head_bytes = blocks * (4 * 1024 * chunks);
+  const uint64_t pool = blocks * (4 * 1024 * chunks) * kv_heads;
   int8_t *kd, *vd;
-  TRY(ensureT(c, S_PROMPTK, head_bytes * kv_heads, &kd));
-  TRY(ensureT(c, S_PROMPTV, head_bytes * kv_heads, &vd));
+  uint32_t* upper;
+  TRY(ensureT(c, S_PROMPTK, pool, &kd));
+  TRY(ensureT(c, S_PROMPTV, pool, &vd));
+  TRY(ensureT(c, S_PROMPTU, blocks * kv_heads, &upper));
   uint32_t *mask, *next_mask;
   TRY(wit_masks(c, &mask, &next_mask));
 
-  PromptPack pack{};
-  pack.kv_heads = kv_heads;
-  pack.dim = dim;
-  pack.chunks = chunks;
-  pack.head_bytes = head_bytes;
-  uint32_t in_launch = 0;
-  uint64_t row = 0, at = 0;
-  auto launch_pack = [&]() -> int {
-    if (in_launch == 0) return GKR_OK;
-    GKR_LAUNCH(c, k_prompt_pack, dim3(in_launch, kv_heads), dim3(256), 0, pack, k->dev, v->dev, kd, vd, mask, next_mask);
-    pack.n = in_launch = 0;
-    return check_launch(c);
+  auto pack_all = [&](uint32_t* counter, uint32_t counters) -> int {
+    PromptPack pack{};
+    pack.kv_heads = kv_heads;
+    pack.dim = dim;
+    pack.chunks = chunks;
+    pack.blocks = (uint32_t)blocks;
+    pack.counter = counter;
+    pack.counters = counters;
+    uint32_t in_launch = 0;
+    uint64_t row = 0, at = 0;
+    auto launch = [&]() -> int {
+      if (in_launch == 0) return GKR_OK;
+      pack.n_blocks = in_launch;
+      const dim3 grid((in_launch + 7) / 8 * 8 * std::min(kv_heads, kPackHeads), (kv_heads + kPackHeads - 1) / kPackHeads);
+      auto one = [&](auto kernel) {
+        GKR_LAUNCH(c, kernel, grid, dim3(64 * std::min(kPackWaves, 2 * chunks)), 0, pack, k->dev, v->dev, kd, vd, upper, mask, next_mask);
+      };
+      if (2 * chunks <= kPackWaves) one(k_prompt_pack<1>);
+      else one(k_prompt_pack<2>);
+      pack.n = in_launch = pack.counters = 0;  // cleared by the first
+      return check_launch(c);
+    };
+    for (size_t i = 0; i < n_seqs; i++) {
+      if (counts[i] == 0) continue;
+      const uint32_t some = (counts[i] + kAttBlock - 1) / kAttBlock;
+      auto& e = pack.e[pack.n++];
+      e.block0 = in_launch;
+      e.len = counts[i];
+      e.at = (uint32_t)at;
+      e.row = (uint32_t)row;
+      in_launch += some;
+      at += some;
+      row += counts[i];
+      if (pack.n == kPromptSeqs || in_launch > 1u << 14) TRY(launch());
+    }
+    return launch();
   };
-  for (size_t i = 0; i < n_seqs; i++) {
-    if (counts[i] == 0) continue;
-    const uint32_t some = (counts[i] + kAttBlock - 1) / kAttBlock;
-    auto& e = pack.e[pack.n++];
-    e.block0 = in_launch;
-    e.len = counts[i];
-    e.at = (uint32_t)at;
-    e.row = row;
-    in_launch += some;
-    at += some;
-    row += counts[i];
-    if (pack.n == kPromptSeqs || in_launch > 1u << 22) TRY(launch_pack());
-  }
-  TRY(launch_pack());
 
   PromptArgs a{};
   a.k = kd;
@@ -86,65 +98,71 @@ static int attention_prompt(gkr_ctx* c, const gkr_matrix* q, const gkr_matrix* k
   a.mask = mask;
   a.o = AttOut{out->dev, weighted ? weighted->dev : nullptr, sums ? sums->dev : nullptr, scores ? scores->dev : nullptr,
                scores ? scores->cols : 0};
-  a.head_bytes = head_bytes;
+  a.blocks = (uint32_t)blocks;
+  a.upper = upper;
   a.kv_heads = kv_heads;
   a.group = group;
   a.dim = dim;
   a.chunks = chunks;
   a.offset = offset;
   a.table_mask = (1u << table_log) - 1;
-  // The sequences' items, in workgroups of `tile` rows: the int8 kernel's launch,
-  // then the other's, one of which finds nothing to do.
-  auto launch_all = [&](uint32_t tile, auto kernels) -> int {
-    uint64_t row = 0, at = 0, most = 0;
-    for (size_t i = 0; i < n_seqs; i++) most += (counts[i] * group + tile - 1) / tile;
-    TRY(ensureT(c, S_PROMPTQ, std::min<uint64_t>(most * kv_heads, (1ull << 22) + (0x7fffffffull / tile + 1) * kv_heads), &a.todo));
-    uint32_t items = 0;
+  // The sequences' items, in workgroups of `tile` rows: the packing, then for up to
+  // kPromptSeqs sequences and 2^22 items (and one sequence's more, at most 2^23, so
+  // that a grid has fewer than 2^32 threads) the int8 kernel's launch and the
+  // other's, one of which finds nothing to do.
+  auto launch_all = [&](uint32_t tile, uint32_t per, auto kernels) -> int {
+    uint64_t all = 0;
+    for (size_t i = 0; i < n_seqs; i++) {
+      const uint64_t items = ((uint64_t)counts[i] * group + tile - 1) / tile * kv_heads;
+      if (items > 1u << 23) return fail(GKR_ERR_INVALID, "%s: too many tokens and heads for one launch", what);
+      all += items;
+    }
+    const uint64_t launches = n_seqs / kPromptSeqs + (all >> 22) + 2, room = std::min<uint64_t>(all, (1u << 22) + (1u << 23));
+    TRY(ensureT(c, S_PROMPTQ, room + kPromptCounters * launches, &a.todo));
+    a.counter = a.todo + room;
+    TRY(pack_all(a.counter, (uint32_t)(kPromptCounters * launches)));
+    uint64_t row = 0, at = 0;
     auto launch = [&]() -> int {
-      if (items == 0) return GKR_OK;
-      TRY(kernels(items));
-      a.n = items = 0;
+      if (a.items == 0) return GKR_OK;
+      TRY(kernels());
+      a.n = a.items = a.general_items = 0;
+      a.counter += kPromptCounters;
       return GKR_OK;
     };
     for (size_t i = 0; i < n_seqs; i++) {
       if (counts[i] == 0) continue;
       auto& e = a.e[a.n++];
-      e.item0 = items;
+      e.item0 = a.items;
+      e.general0 = a.general_items;
       e.tiles = (counts[i] * group + tile - 1) / tile;
       e.len = counts[i];
       e.at = (uint32_t)at;
-      e.row = row;
-      items += e.tiles * kv_heads;
+      e.row = (uint32_t)row;
+      a.items += e.tiles * kv_heads;
+      a.general_items += (e.tiles + per - 1) / per * kv_heads;
       at += (counts[i] + kAttBlock - 1) / kAttBlock;
       row += counts[i];
-      if (a.n == kPromptSeqs || items > 1u << 22) TRY(launch());
+      if (a.n == kPromptSeqs || a.items > 1u << 22) TRY(launch());
     }
     return launch();
   };
   // R1 and W1 of the int8 kernel, R4 and W4 of the other: tiles of 16 rows a wave, waves
-#define GKR_PROMPT_(DT, R1, W1, OCC1, R4, W4, OCC4)                                                                  \
-  static_assert(R1 * W1 == R4 * W4, "the same items");                                                               \
-  return launch_all(16 * R1 * W1, [&](uint32_t items) -> int {                                                       \
-    if (scores || weighted) GKR_LAUNCH(c, (k_prompt_int8<DT, R1, W1, OCC1, true>), dim3(items), dim3(64 * W1), 0, a); \
-    else GKR_LAUNCH(c, (k_prompt_int8<DT, R1, W1, OCC1, false>), dim3(items), dim3(64 * W1), 0, a);                  \
-    TRY(check_launch(c));                                                                                            \
-    if (scores || weighted) GKR_LAUNCH(c, (k_prompt<DT, R4, W4, OCC4, true>), dim3(items), dim3(64 * W4), 0, a);     \
-    else GKR_LAUNCH(c, (k_prompt<DT, R4, W4, OCC4, false>), dim3(items), dim3(64 * W4), 0, a);                       \
-    return check_launch(c);                                                                                          \
+#define GKR_PROMPT(DT, R1, W1, OCC1, R4, W4, OCC4)                                                                    \
+  return launch_all(16 * R1 * W1, R4 * W4 / (R1 * W1), [&]() -> int {                                                  \
+    constexpr uint32_t PER = R4 * W4 / (R1 * W1);                                                                      \
+    static_assert(PER * R1 * W1 == R4 * W4, "whole items");                                                            \
+    if (scores || weighted) GKR_LAUNCH(c, (k_prompt_int8<DT, R1, W1, OCC1, true>), dim3(a.items), dim3(64 * W1), 0, a); \
+    else GKR_LAUNCH(c, (k_prompt_int8<DT, R1, W1, OCC1, false>), dim3(a.items), dim3(64 * W1), 0, a);                  \
+    TRY(check_launch(c));                                                                                              \
+    const dim3 grid(std::min(a.general_items, 256u * (OCC4 * 4 / W4)));                                                \
+    if (scores || weighted) GKR_LAUNCH(c, (k_prompt<DT, R4, W4, OCC4, PER, true>), grid, dim3(64 * W4), 0, a);         \
+    else GKR_LAUNCH(c, (k_prompt<DT, R4, W4, OCC4, PER, false>), grid, dim3(64 * W4), 0, a);                           \
+    return check_launch(c);                                                                                            \
   })
-#define GKR_PROMPT(...) GKR_PROMPT_(__VA_ARGS__)
-#ifndef PV
-#define PV 2, 2, 4, 3, 1, 8, 2
-#endif
-  if (dim <= 64) {
-    GKR_PROMPT(1, 2, 4, 3, 1, 8, 2);
-  }
-  if (dim <= 128) {
-    GKR_PROMPT(PV);
-  }
+  if (dim <= 64) GKR_PROMPT(1, 1, 4, 4, 1, 8, 2);
+  if (dim <= 128) GKR_PROMPT(2, 1, 4, 4, 1, 8, 2);
   GKR_PROMPT(4, 1, 4, 2, 1, 4, 1);
 #undef GKR_PROMPT
-#undef GKR_PROMPT_
 }
 extern "C" int gkr_attention_prompt(gkr_ctx* c, const gkr_matrix* q, const gkr_matrix* k, const gkr_matrix* v,
                                     const uint32_t* counts, size_t n_seqs, uint32_t heads, uint32_t kv_heads,

@@ -165,7 +165,7 @@ def test_refusals(gpu_ctx):
 def test_weights_of_every_place(gpu_ctx, spread, table):
     """Scores all in a few places or over all of the table and past it, small weights in no block, few or all."""
     rng = np.random.default_rng(spread + table)
-    counts, heads, kv, d = [700, 130], 6, 2, 64
+    counts, heads, kv, d = [310, 70], 4, 2, 64
     rows = sum(counts)
     for lonely in (False, True):
         t = []
@@ -173,8 +173,8 @@ def test_weights_of_every_place(gpu_ctx, spread, table):
             v = rng.integers(-spread, spread + 1, size=(rows, h * d))
             t.append(v)
         if lonely:  # one key far below the others, and one far above
-            t[1][5], t[1][333] = -127, 127
-            t[0][600, :d] = 127
+            t[1][5], t[1][133] = -127, 127
+            t[0][300, :d] = 127
         t = [np.where(v < 0, v + P, v).astype(np.uint32) for v in t]
         for offset in (1 << 19, 5 << 16, 0):
             check(gpu_ctx, counts, heads, kv, d, qkv=t, offset=offset, log=table)
