@@ -281,7 +281,7 @@ __device__ __forceinline__ void prompt_end(const PromptArgs& a, uint32_t i, uint
                                            const v4i (&acc)[R][4 * DT][NP + 1], const int32_t (&z)[R][2]) {
   constexpr int CH = 4 * DT, NV = NP + 1;
   const uint32_t lane = threadIdx.x & 63, col = lane & 15, quarter = lane >> 4;
-  const uint32_t rows = a.e[i].len * a.group, wave_end = row0 + 16 * R < rows ? row0 + 16 * R : rows;
+  const uint32_t rows = a.e[i].len * a.group;
   auto whole_total = [&](int r, int d, int v) {
     if constexpr (NP == 1) return -((int64_t)acc[r][d][0][v] + ((int64_t)acc[r][d][1][v] << 3));
     int64_t total = 0;

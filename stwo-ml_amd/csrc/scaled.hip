@@ -89,19 +89,23 @@ static int quantized_forward(gkr_ctx* c, const gkr_matrix* a, const gkr_matrix* 
   for (gkr_matrix* w : {quantized, row_scales, pre, out})
     if (w) TRY(drop_derived(c, w));
   TRY(weight_planes(c, const_cast<gkr_matrix*>(b)));
-  gkr_matrix q{c, nullptr, m, k, false};
   uint32_t* scales;
-  if (quantized) q.dev = quantized->dev;
-  else TRY(ensureT(c, S_QUANT, m * k, &q.dev));
   if (row_scales) scales = row_scales->dev;
   else TRY(ensureT(c, S_QSCALE, m, &scales));
-  for (uint64_t row = 0; row < m; row += 1u << 23) {  // as many workgroups as one grid dimension holds
-    const uint64_t some = std::min<uint64_t>(m - row, 1u << 23);
-    GKR_LAUNCH(c, k_quantize_rows, dim3((uint32_t)some), dim3(256), 0, a->dev + row * k, k, levels, q.dev + row * k,
+  const WitRows rows = wit_rows(a);
+  const WitQuant quant{levels, quantized ? quantized->dev : nullptr, scales};
+  if (quantized_rows_fit(rows, b)) return rows_product<false, true>(c, rows, b, b, e, quant);
+  e.row_scales = scales;
+  if (!few_rows(rows, b, b) && packable(m, k, b->cols)) return packed_product<false>(c, rows, b, b, e, &quant);
+  gkr_matrix q{c, nullptr, m, k, false};
+  if (quantized) q.dev = quantized->dev;
+  else TRY(ensureT(c, S_QUANT, m * k, &q.dev));
+  for (uint64_t row = 0; row < m; row += 1u << 21) {  // as many workgroups as one grid dimension holds
+    const uint64_t some = std::min<uint64_t>(m - row, 1u << 21);
+    GKR_LAUNCH(c, k_quantize_rows, dim3((uint32_t)some), dim3(1024), 0, a->dev + row * k, k, levels, q.dev + row * k,
                scales + row);
     TRY(check_launch(c));
   }
-  e.row_scales = scales;
   return scaled_product(c, &q, b, e);
 }
 

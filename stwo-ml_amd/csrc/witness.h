@@ -247,6 +247,35 @@ __device__ __forceinline__ uint32_t digit_sum_mod_p(const int32_t (&s)[4]) {
   return m31_reduce64((uint64_t)(t + ((int64_t)P << 26)));
 }
 
+// round(c(x) levels / a), halves away from zero, for |c(x)| <= a < 2^30 and levels <
+// 128.  The product with a rounded ratio is off by less than 127 2^-21, its nearest
+// whole number q by one at most; the rest |c| levels - q a, below 1.5 a and so whole
+// in 32 bits, says which way.
+struct Quantizer {
+  float ratio;
+  uint32_t a, levels;
+  __device__ __forceinline__ Quantizer(uint32_t most, uint32_t to)
+      : ratio(most ? (float)to / (float)most : 0.0f), a(most), levels(to) {}
+  __device__ __forceinline__ int32_t operator()(uint32_t x) const {
+    const int32_t v = center_m31(x), sign = v >> 31;
+    const uint32_t c = (uint32_t)((v ^ sign) - sign), q = (uint32_t)__builtin_fmaf((float)c, ratio, 0.5f);
+    const int32_t rest = (int32_t)(c * levels - q * a), half = (int32_t)(a >> 1);
+    const int32_t r = (int32_t)q + (rest < -half ? -1 : rest > (int32_t)(a - 1) - half && a ? 1 : 0);
+    return (r ^ sign) - sign;
+  }
+};
+__device__ __forceinline__ uint32_t word_of(int32_t v) { return (uint32_t)v + ((uint32_t)(v >> 31) & P); }
+__device__ __forceinline__ uint32_t size_of_word(uint32_t x) {  // |c(x)|
+  const int32_t v = center_m31(x);
+  return (uint32_t)(v < 0 ? -v : v);
+}
+// Rows that are brought to 8 bits before they are multiplied: levels, and where
+// their words (m x k) and scales (m) go, if anywhere.
+struct WitQuant {
+  uint32_t levels;
+  uint32_t *words, *scales;
+};
+
 // Few rows.  The rows' digit planes are rows of one product: row' 4 i + p is
 // plane p of row i, 16 of them to a v_mfma_i32_16x16x64_i8, so general words cost
 // no more than int8-range ones, and lane 16 j + c of the accumulator of tile t
@@ -265,14 +294,21 @@ __device__ __forceinline__ uint32_t digit_sum_mod_p(const int32_t (&s)[4]) {
 // us, also with sixteen waves for the gated pair's 432 column tiles).
 // W waves: sixteen, or eight, of which two workgroups fit a CU, where there are
 // more column tiles than CUs.
-template <int MR, int PB, bool GATED, int W, class End>
+// QUANT: every workgroup brings the rows, up to kQuantFew words that its threads
+// hold, to 8 bits itself, from their largest magnitudes (1 x 13824 x 5120 33.2 us
+// with a launch of a workgroup a row that does it, 16.5 so); the words that are asked
+// for are stored by all of them, each a part.
+constexpr uint32_t kQuantFew = 16384;
+template <int MR, int PB, bool GATED, int W, bool QUANT, class End>
 static __global__ void __launch_bounds__(64 * W, PB == 1 || !GATED ? 4 : 2)
-    k_rows(const uint32_t* __restrict__ X, WitWeight w0, WitWeight w1, uint32_t m, uint32_t k, uint32_t n, End end) {
+    k_rows(const uint32_t* __restrict__ X, WitWeight w0, WitWeight w1, uint32_t m, uint32_t k, uint32_t n, End end,
+           WitQuant quant) {
   constexpr int NW = GATED ? 2 : 1, RT = MR <= 4 ? 1 : MR / 4, U = PB > 1 ? 1 : MR > 4 ? 2 : 4;
   constexpr uint32_t kChunk = kRowLds / (4 * MR);  // K per LDS fill
   static_assert(MR > 4 || kChunk / 64 % (W * U) == 0, "a fill ends where the loads in flight start over");
   extern __shared__ __align__(16) int8_t digits[];  // [K / 16][4 MR][16]
   __shared__ int32_t sums[NW][PB][MR][4][32];
+  __shared__ uint32_t most[MR];  // QUANT: largest magnitudes
   const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6, ct = blockIdx.x;
   const uint32_t nsteps = (k + kGemmK - 1) / kGemmK, npairs = (nsteps + 1) / 2;
   const uint64_t plane = (uint64_t)((n + kGemmTile - 1) / kGemmTile) * nsteps * kGemmBlockBytes;
@@ -318,7 +354,7 @@ static __global__ void __launch_bounds__(64 * W, PB == 1 || !GATED ? 4 : 2)
   };
   // the first rows' words go out before the weights' loads, which are then in
   // flight while the words are laid out
-  constexpr int XQ = 4;
+  constexpr int XQ = QUANT ? (int)(kQuantFew / (256 * W)) : 4;
   uint32_t x[XQ][4];
   {
     const uint32_t left = k < kChunk ? k : kChunk, quads = (left + 63) / 64 * 16;
@@ -329,6 +365,54 @@ static __global__ void __launch_bounds__(64 * W, PB == 1 || !GATED ? 4 : 2)
 #pragma unroll
   for (int u = 0; u < U; u++) load(u, wave + u * W);
   for (uint32_t i = threadIdx.x; i < NW * PB * MR * 128; i += blockDim.x) (&sums[0][0][0][0][0])[i] = 0;
+  if constexpr (QUANT) {
+    if (threadIdx.x < MR) most[threadIdx.x] = 0;
+    __syncthreads();
+    // The words wait where their digits go to; a loop takes them from there, since a
+    // short launch takes as long as its instructions' way from memory (with them in
+    // registers and the loop unrolled 20.9 us).
+    const uint32_t quads = (k + 63) / 64 * 16;
+    auto place = [&](uint32_t t) {
+      const uint32_t i = t / quads, kk = t % quads * 4;
+      return (uint32_t*)(digits + (kk / 16 * (4 * MR) + 4 * i) * 16 + kk % 16);
+    };
+#pragma unroll
+    for (int q = 0; q < XQ; q++) {
+      const uint32_t t = threadIdx.x + q * 64 * W;
+      if (t >= MR * quads) break;  // sixteen lanes together, which have the same row
+      uint32_t* const to = place(t);
+      uint32_t a = 0;
+#pragma unroll
+      for (int j = 0; j < 4; j++) {
+        a = max(a, size_of_word(x[q][j]));
+        to[4 * j] = x[q][j];
+      }
+      a = max(a, (uint32_t)__builtin_amdgcn_mov_dpp((int)a, 0xb1, 0xf, 0xf, true));   // lane ^ 1
+      a = max(a, (uint32_t)__builtin_amdgcn_mov_dpp((int)a, 0x4e, 0xf, 0xf, true));   // lane ^ 2
+      a = max(a, (uint32_t)__builtin_amdgcn_mov_dpp((int)a, 0x141, 0xf, 0xf, true));  // lane ^ 7
+      a = max(a, (uint32_t)__builtin_amdgcn_mov_dpp((int)a, 0x140, 0xf, 0xf, true));  // lane ^ 15
+      if ((threadIdx.x & 15) == 0) atomicMax(&most[t / quads], a);
+    }
+    __syncthreads();
+#pragma unroll 1
+    for (uint32_t t = threadIdx.x; t < MR * quads; t += 64 * W) {
+      const uint32_t i = t / quads, kk = t % quads * 4;
+      const Quantizer quantizer(most[i], quant.levels);
+      uint32_t* const to = place(t);
+      uint32_t b[4];
+#pragma unroll
+      for (int j = 0; j < 4; j++) b[j] = (uint32_t)quantizer(to[4 * j]);
+      to[0] = __builtin_amdgcn_perm(b[1], b[0], 0x0c0c0400u) | __builtin_amdgcn_perm(b[3], b[2], 0x04000c0cu);
+#pragma unroll
+      for (int p = 1; p < 4; p++) to[4 * p] = 0;
+      if (quant.words && i < m && t / 64 % gridDim.x == ct) {
+#pragma unroll
+        for (int j = 0; j < 4; j++)
+          if (kk + j < k) quant.words[i * k + kk + j] = word_of((int32_t)b[j]);
+      }
+    }
+    if (quant.scales && ct == 0 && threadIdx.x < m) quant.scales[threadIdx.x] = most[threadIdx.x];
+  }
   v4i acc[NW][PB][2][RT];
 #pragma unroll
   for (int i = 0; i < NW; i++)
@@ -343,12 +427,12 @@ static __global__ void __launch_bounds__(64 * W, PB == 1 || !GATED ? 4 : 2)
     const uint32_t left = k - k0 < kChunk ? k - k0 : kChunk, fill = (left + 63) / 64 * 64;
     if (k0) __syncthreads();
     uint32_t t = threadIdx.x;
-    if (k0 == 0) {
+    if (!QUANT && k0 == 0) {
 #pragma unroll
       for (int q = 0; q < XQ; q++, t += 64 * W)
         if (t < MR * (fill / 4)) lay_out(t, fill / 4, x[q]);
     }
-    for (; t < MR * (fill / 4); t += 64 * W) {
+    for (; !QUANT && t < MR * (fill / 4); t += 64 * W) {
       uint32_t later[4];
       words(t, k0, left, fill / 4, later);
       lay_out(t, fill / 4, later);
@@ -410,6 +494,7 @@ static __global__ void __launch_bounds__(64 * W, PB == 1 || !GATED ? 4 : 2)
   typename End::template Slot<1> slot;
   const typename End::Tile tile = end.tile(0, (uint64_t)m * n);
   if (ok) end.fetch(slot, tile, at, row);
+  if constexpr (QUANT) slot.row[0] = most[r < MR ? r : 0];
   __syncthreads();
   if (!ok) return;
   uint32_t z[NW][1];
@@ -489,6 +574,97 @@ static __global__ void __launch_bounds__(256) k_wit_pack(const uint32_t* __restr
     // on lines of their own, and only while a word is not set
     volatile uint32_t* const word = mask + kMaskStride * (blockIdx.x % kMaskWords);
     if (!*word) *word = 1;
+  }
+}
+
+// The packing of rows that are brought to 8 bits: a workgroup has two rows, 256
+// threads each, and goes over their words twice, the second time back from the end:
+// the last of them are in registers and the others in this XCD's cache, where 32
+// workgroups of 110 KB fit (four rows a workgroup, the words of 16 turns in registers
+// and both loops unrolled: 512 x 13824 24.5 us, 37 x 1537 8.1, most of it the
+// instructions' way from memory; so 19.0 and 6.2).  Plane 0 alone is stored, 16 bytes a lane:
+// a quad's lanes exchange the words of four turns.
+constexpr uint32_t kQuantRows = 2;
+static __global__ void __launch_bounds__(256 * kQuantRows) k_wit_quantize(const uint32_t* __restrict__ X, uint64_t m, uint64_t k,
+                                                                          uint32_t nsteps, int8_t* __restrict__ one,
+                                                                          WitQuant quant) {
+  __shared__ uint32_t most[kQuantRows][4];
+  const uint32_t r = threadIdx.x / 256, t = threadIdx.x % 256, q = threadIdx.x & 3;
+  const uint64_t row = (uint64_t)blockIdx.x * kQuantRows + r;
+  const uint32_t groups = (nsteps * (kGemmK / 4) + 1023) / 1024;  // of four turns
+  const uint32_t* const from = X + (row < m ? row : m - 1) * k;
+  const bool whole = k % 4 == 0;  // uniform
+  uint32_t x[4][4];
+  auto words = [&](uint32_t group) {
+    uint32_t at[4];  // k is below 2^31
+#pragma unroll
+    for (int i = 0; i < 4; i++) at[i] = 4 * ((4 * group + i) * 256 + t);
+    if (whole) {
+      v4i_word w[4];
+#pragma unroll
+      for (int i = 0; i < 4; i++) w[i] = *(const v4i_word*)(from + (at[i] < k ? at[i] : 0));
+#pragma unroll
+      for (int i = 0; i < 4; i++)
+#pragma unroll
+        for (int j = 0; j < 4; j++) x[i][j] = at[i] < k ? (uint32_t)w[i][j] : 0u;
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; i++)
+#pragma unroll
+        for (int j = 0; j < 4; j++) x[i][j] = from[at[i] + j < k ? at[i] + j : 0];
+#pragma unroll
+      for (int i = 0; i < 4; i++)
+#pragma unroll
+        for (int j = 0; j < 4; j++) x[i][j] = at[i] + j < k ? x[i][j] : 0u;
+    }
+  };
+  uint32_t a = 0;
+#pragma unroll 1
+  for (uint32_t g = 0; g < groups; g++) {
+    words(g);
+#pragma unroll
+    for (int i = 0; i < 4; i++)
+#pragma unroll
+      for (int j = 0; j < 4; j++) a = max(a, size_of_word(x[i][j]));
+  }
+#pragma unroll
+  for (int off = 32; off > 0; off >>= 1) a = max(a, (uint32_t)__shfl_xor(a, off));
+  if ((threadIdx.x & 63) == 0) most[r][t / 64] = a;
+  __syncthreads();
+  a = max(max(most[r][0], most[r][1]), max(most[r][2], most[r][3]));
+  const Quantizer quantizer(a, quant.levels);
+  if (row >= m) return;
+  if (t == 0) quant.scales[row] = a;
+#pragma unroll 1
+  for (uint32_t g = groups; g-- > 0;) {
+    if (g + 1 < groups) words(g);
+    uint32_t bytes[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      uint32_t b[4];
+#pragma unroll
+      for (int j = 0; j < 4; j++) b[j] = (uint32_t)quantizer(x[i][j]);
+      bytes[i] = __builtin_amdgcn_perm(b[1], b[0], 0x0c0c0400u) | __builtin_amdgcn_perm(b[3], b[2], 0x04000c0cu);
+    }
+    if (quant.words) {
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        const uint32_t at = 4 * ((4 * g + i) * 256 + t);
+        uint32_t w[4];
+#pragma unroll
+        for (int j = 0; j < 4; j++) w[j] = word_of((int8_t)(bytes[i] >> (8 * j)));
+        uint32_t* const to = quant.words + row * k + at;
+        if (whole && at < k) *(v4i_word*)to = v4i_word{(int)w[0], (int)w[1], (int)w[2], (int)w[3]};
+#pragma unroll
+        for (int j = 0; j < 4; j++)
+          if (!whole && at + j < k) to[j] = w[j];
+      }
+    }
+    quad_transpose(bytes);  // lane q of a quad: 16 bytes of turn q
+    const uint32_t k16 = ((4 * g + q) * 256 + t) / 4;  // from 16 K on
+    if (k16 < 2 * nsteps)
+      *(uint4*)(one + ((row >> 5) * nsteps + k16 / 2) * kGemmBlockBytes + 512 * (k16 & 1) + 16 * (row & 31)) =
+          make_uint4(bytes[0], bytes[1], bytes[2], bytes[3]);
   }
 }
 

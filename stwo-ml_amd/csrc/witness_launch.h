@@ -18,31 +18,35 @@ inline bool overlap(const gkr_matrix* x, const gkr_matrix* y) {
 static WitWeight wit_weight(const gkr_matrix* w) { return WitWeight{w->bplanes, (uint32_t)w->bnplanes}; }
 
 static dim3 end_grid(uint64_t count) { return dim3((uint32_t)std::min<uint64_t>((count + 255) / 256, 1u << 20)); }
-// Few rows (k_rows).
-template <bool GATED, class End>
-static int rows_product(gkr_ctx* c, const WitRows& a, const gkr_matrix* w0, const gkr_matrix* w1, const End& end) {
+// Few rows (k_rows); with QUANT they are quantized_rows_fit.
+template <bool GATED, bool QUANT = false, class End>
+static int rows_product(gkr_ctx* c, const WitRows& a, const gkr_matrix* w0, const gkr_matrix* w1, const End& end,
+                        const WitQuant& quant = {}) {
   const uint32_t m = (uint32_t)a.m, k = (uint32_t)a.k;
   const uint64_t n = w0->cols, ctiles = (n + kGemmTile - 1) / kGemmTile;
   const bool one = w0->bnplanes == 1 && w1->bnplanes == 1;
   auto launch = [&](auto kernel, uint32_t mr, uint32_t waves) {
     const uint32_t lds = std::min<uint32_t>(kRowLds, 4 * mr * ((k + 63) / 64 * 64));
     GKR_LAUNCH(c, kernel, dim3((uint32_t)ctiles), dim3(64 * waves), lds, a.x, wit_weight(w0), wit_weight(w1), m, k,
-               (uint32_t)n, end);
+               (uint32_t)n, end, quant);
   };
   const bool many = ctiles > 256;
   // two matrices of general weights: eight waves of twice the registers
-#define GKR_ROWS(MR)                                                                \
-  do {                                                                              \
-    if (!one && (many || GATED)) launch(k_rows<MR, 4, GATED, 8, End>, MR, 8);       \
-    else if (!one) launch(k_rows<MR, 4, GATED, GATED ? 8 : 16, End>, MR, 16);       \
-    else if (many) launch(k_rows<MR, 1, GATED, 8, End>, MR, 8);                     \
-    else launch(k_rows<MR, 1, GATED, 16, End>, MR, 16);                             \
+#define GKR_ROWS_ONE(MR) \
+  (many ? launch(k_rows<MR, 1, GATED, 8, QUANT, End>, MR, 8) : launch(k_rows<MR, 1, GATED, 16, QUANT, End>, MR, 16))
+#define GKR_ROWS(MR)                                                                                     \
+  do {                                                                                                   \
+    if constexpr (QUANT) GKR_ROWS_ONE(MR);                                                               \
+    else if (one) GKR_ROWS_ONE(MR);                                                                      \
+    else if (many || GATED) launch(k_rows<MR, 4, GATED, 8, QUANT, End>, MR, 8);                          \
+    else launch(k_rows<MR, 4, GATED, GATED ? 8 : 16, QUANT, End>, MR, 16);                               \
   } while (0)
   if (m == 1) GKR_ROWS(1);
   else if (m == 2) GKR_ROWS(2);
   else if (m <= 4) GKR_ROWS(4);
-  else if (m <= 8) many ? launch(k_rows<8, 1, GATED, 8, End>, 8, 8) : launch(k_rows<8, 1, GATED, 16, End>, 8, 16);
-  else many ? launch(k_rows<16, 1, GATED, 8, End>, 16, 8) : launch(k_rows<16, 1, GATED, 16, End>, 16, 16);
+  else if (m <= 8) GKR_ROWS_ONE(8);
+  else GKR_ROWS_ONE(16);
+#undef GKR_ROWS_ONE
 #undef GKR_ROWS
   return check_launch(c);
 }
@@ -50,22 +54,31 @@ static bool few_rows(const WitRows& a, const gkr_matrix* w0, const gkr_matrix* w
   return few_rows_fit(a.m, a.k, w0->cols, w0->bnplanes == 1 && w1->bnplanes == 1);
 }
 
+static bool quantized_rows_fit(const WitRows& a, const gkr_matrix* w) {
+  const uint64_t mr = a.m == 1 ? 1 : a.m == 2 ? 2 : a.m <= 4 ? 4 : a.m <= 8 ? 8 : 16;
+  static_assert(4 * kQuantFew <= kRowLds, "one fill");
+  return w->bnplanes == 1 && few_rows(a, w, w) && mr * ((a.k + 63) / 64 * 64) <= kQuantFew;
+}
+
 // Two masks of the packing, used in turn: the packing of one product clears the
 // other's.  A mask that is set says that rows may have four planes, which is right
-// for all rows: a captured product may find its own from the last replay.
+// for all rows: a captured product may find its own from the last replay.  A third
+// is never set, for rows that have one plane.
+constexpr uint32_t kMaskAll = kMaskWords * kMaskStride;
+static int wit_mask_words(gkr_ctx* c) {
+  if (c->wit_mask) return GKR_OK;
+  drain(c);
+  uint32_t* w = nullptr;
+  HIP_TRY(hipMalloc(&w, 3 * kMaskAll * sizeof(uint32_t)));
+  c->wit_mask = w;
+  const uint64_t count = 3 * kMaskAll * sizeof(uint32_t) / 16;
+  GKR_LAUNCH(c, k_extend, extend_grid(count), dim3(256), 0, nullptr, 0, (uint4*)w, count);
+  return check_launch(c);
+}
 static int wit_masks(gkr_ctx* c, uint32_t** mask, uint32_t** next_mask) {
-  constexpr uint32_t words = kMaskWords * kMaskStride;
-  if (!c->wit_mask) {
-    drain(c);
-    uint32_t* w = nullptr;
-    HIP_TRY(hipMalloc(&w, 2 * words * sizeof(uint32_t)));
-    c->wit_mask = w;
-    const uint64_t count = 2 * words * sizeof(uint32_t) / 16;
-    GKR_LAUNCH(c, k_extend, extend_grid(count), dim3(256), 0, nullptr, 0, (uint4*)w, count);
-    TRY(check_launch(c));
-  }
-  *mask = c->wit_mask + (c->wit_turn & 1) * words;
-  *next_mask = c->wit_mask + (~c->wit_turn & 1) * words;
+  TRY(wit_mask_words(c));
+  *mask = c->wit_mask + (c->wit_turn & 1) * kMaskAll;
+  *next_mask = c->wit_mask + (~c->wit_turn & 1) * kMaskAll;
   c->wit_turn++;
   return GKR_OK;
 }
@@ -97,9 +110,11 @@ static double blocks_us(uint64_t groups, uint32_t nsteps, uint64_t elements, uin
   return best;
 }
 
-// More rows: packed, multiplied (k_wit_tiles) and, where K is split, joined.
+// More rows: packed, multiplied (k_wit_tiles) and, where K is split, joined.  With
+// `quant` they are brought to 8 bits as they are packed, and have one plane.
 template <bool GATED, class End>
-static int packed_product(gkr_ctx* c, const WitRows& a, const gkr_matrix* w0, const gkr_matrix* w1, const End& end) {
+static int packed_product(gkr_ctx* c, const WitRows& a, const gkr_matrix* w0, const gkr_matrix* w1, const End& end,
+                          const WitQuant* quant = nullptr) {
   const uint64_t m = a.m, k = a.k, n = w0->cols;
   WitProduct g{};
   g.m = m;
@@ -111,21 +126,29 @@ static int packed_product(gkr_ctx* c, const WitRows& a, const gkr_matrix* w0, co
   g.w[1] = wit_weight(w1);
   const uint64_t one_tiles = (m + 31) / 32, four_tiles = (m + 7) / 8;
   int8_t* packed;
-  TRY(ensureT(c, S_GEMMA, (one_tiles + four_tiles) * g.nsteps * kGemmBlockBytes, &packed));
+  TRY(ensureT(c, S_GEMMA, (one_tiles + (quant ? 0 : four_tiles)) * g.nsteps * kGemmBlockBytes, &packed));
   g.one = packed;
   g.four = packed + one_tiles * g.nsteps * kGemmBlockBytes;
-  uint32_t *mask, *next_mask;
-  TRY(wit_masks(c, &mask, &next_mask));
-  g.mask = mask;
   static_assert(kProductStep == kGemmK, "packable");
-  const dim3 pack_grid((uint32_t)pack_groups(m, k));
-  GKR_LAUNCH(c, k_wit_pack, pack_grid, dim3(kPackThreads), 0, a.x, m, k, g.nsteps, packed,
-             const_cast<int8_t*>(g.four), mask, next_mask);
+  if (quant) {
+    TRY(wit_mask_words(c));
+    g.mask = c->wit_mask + 2 * kMaskAll;
+    GKR_LAUNCH(c, k_wit_quantize, dim3((uint32_t)((m + kQuantRows - 1) / kQuantRows)), dim3(256 * kQuantRows), 0, a.x, m, k,
+               g.nsteps, packed, *quant);
+  } else {
+    uint32_t *mask, *next_mask;
+    TRY(wit_masks(c, &mask, &next_mask));
+    g.mask = mask;
+    const dim3 pack_grid((uint32_t)pack_groups(m, k));
+    GKR_LAUNCH(c, k_wit_pack, pack_grid, dim3(kPackThreads), 0, a.x, m, k, g.nsteps, packed,
+               const_cast<int8_t*>(g.four), mask, next_mask);
+  }
   TRY(check_launch(c));
 
   uint32_t max_splits = 1, max_rgroups = 1;
   // group: row tiles of a workgroup, for rows of one plane and of four
   auto plan = [&](int four, uint32_t group, uint32_t splits) -> int {
+    if (four && quant) return GKR_OK;
     const uint64_t tiles = four ? four_tiles : one_tiles;
     WitPlan& p = g.plan[four];
     p.rtiles = (uint32_t)tiles;
@@ -153,7 +176,7 @@ static int packed_product(gkr_ctx* c, const WitRows& a, const gkr_matrix* w0, co
   const uint64_t bgroups = (ctiles * NW * (general ? 4 : 1) + 7) / 8, elements = m * n * NW;
   uint32_t splits[2] = {1, 1};
   const double blocks[2] = {blocks_us((one_tiles + 7) / 8 * bgroups, g.nsteps, elements, &splits[0]),
-                            blocks_us((four_tiles + 7) / 8 * bgroups, g.nsteps, elements, &splits[1])};
+                            quant ? 0 : blocks_us((four_tiles + 7) / 8 * bgroups, g.nsteps, elements, &splits[1])};
   // rows1: row tiles a workgroup has of rows of one plane that it streams the weights for; 0: blocks as for four
   auto launch_blocks = [&](auto kernel, uint32_t rows1) -> int {
     g.cgroups = (uint32_t)bgroups;
@@ -173,7 +196,7 @@ static int packed_product(gkr_ctx* c, const WitRows& a, const gkr_matrix* w0, co
   constexpr int W = GATED ? 8 : 16;
   if (general) {
     const double tiles = tiles_us(one_tiles * ctiles, 256, g.nsteps, 1 + 4 * NW) +
-                         tiles_us((four_tiles + 1) / 2 * ctiles, 256, g.nsteps, 2 * (1 + 4 * NW));
+                         (quant ? 0 : tiles_us((four_tiles + 1) / 2 * ctiles, 256, g.nsteps, 2 * (1 + 4 * NW)));
     if (GATED || tiles <= blocks[0] + blocks[1]) {
       TRY(GKR_WIT_TILES(1, 4, W, 1, 2));
     } else if constexpr (!GATED) {
@@ -185,7 +208,8 @@ static int packed_product(gkr_ctx* c, const WitRows& a, const gkr_matrix* w0, co
   else if (m <= 64) TRY(GKR_WIT_TILES(2, 1, W, 1, 4));
   else {
     const uint64_t rows64 = (m + 63) / 64;
-    const double tiles = tiles_us(rows64 * ctiles, 512, g.nsteps, 2 + NW) + tiles_us(rows64 * ctiles, 512, g.nsteps, 4 * (2 + NW));
+    const double tiles = tiles_us(rows64 * ctiles, 512, g.nsteps, 2 + NW) +
+                         (quant ? 0 : tiles_us(rows64 * ctiles, 512, g.nsteps, 4 * (2 + NW)));
     constexpr uint32_t RT = GATED ? 2 : 4, WR = GATED ? 2 : 1;
     const uint32_t down = m <= 128 ? WR : 2 * WR;  // waves down the rows of k_wit_mixed
     const double mixed = m <= 256 ? tiles_us(ctiles, 256, g.nsteps, down * (RT + NW)) + blocks[1] : 1e30;
