@@ -525,7 +525,7 @@ static __global__ void __launch_bounds__(64 * W, PB == 1 || !GATED ? 4 : 2)
 // Rows past m are left as they are (their sums are not stored).
 constexpr uint32_t kMaskWords = 64, kMaskStride = 32;
 __device__ __forceinline__ bool wit_four(const uint32_t* mask) {  // the same in every wave
-  return __any(mask[kMaskStride * (threadIdx.x & 63)] != 0);
+  return mask && __any(mask[kMaskStride * (threadIdx.x & 63)] != 0);
 }
 // Word p of a quad's lane q and word q of its lane p change places.
 __device__ __forceinline__ void quad_transpose(uint32_t (&x)[4]) {
@@ -675,7 +675,7 @@ struct WitPlan {
 };
 struct WitProduct {
   const int8_t *one, *four;  // the packed rows
-  const uint32_t* mask;
+  const uint32_t* mask;  // none: rows of one plane
   WitWeight w[2];
   uint64_t m, n;
   uint32_t nsteps, ctiles, cgroups;

@@ -62,23 +62,20 @@ static bool quantized_rows_fit(const WitRows& a, const gkr_matrix* w) {
 
 // Two masks of the packing, used in turn: the packing of one product clears the
 // other's.  A mask that is set says that rows may have four planes, which is right
-// for all rows: a captured product may find its own from the last replay.  A third
-// is never set, for rows that have one plane.
-constexpr uint32_t kMaskAll = kMaskWords * kMaskStride;
-static int wit_mask_words(gkr_ctx* c) {
-  if (c->wit_mask) return GKR_OK;
-  drain(c);
-  uint32_t* w = nullptr;
-  HIP_TRY(hipMalloc(&w, 3 * kMaskAll * sizeof(uint32_t)));
-  c->wit_mask = w;
-  const uint64_t count = 3 * kMaskAll * sizeof(uint32_t) / 16;
-  GKR_LAUNCH(c, k_extend, extend_grid(count), dim3(256), 0, nullptr, 0, (uint4*)w, count);
-  return check_launch(c);
-}
+// for all rows: a captured product may find its own from the last replay.
 static int wit_masks(gkr_ctx* c, uint32_t** mask, uint32_t** next_mask) {
-  TRY(wit_mask_words(c));
-  *mask = c->wit_mask + (c->wit_turn & 1) * kMaskAll;
-  *next_mask = c->wit_mask + (~c->wit_turn & 1) * kMaskAll;
+  constexpr uint32_t words = kMaskWords * kMaskStride;
+  if (!c->wit_mask) {
+    drain(c);
+    uint32_t* w = nullptr;
+    HIP_TRY(hipMalloc(&w, 2 * words * sizeof(uint32_t)));
+    c->wit_mask = w;
+    const uint64_t count = 2 * words * sizeof(uint32_t) / 16;
+    GKR_LAUNCH(c, k_extend, extend_grid(count), dim3(256), 0, nullptr, 0, (uint4*)w, count);
+    TRY(check_launch(c));
+  }
+  *mask = c->wit_mask + (c->wit_turn & 1) * words;
+  *next_mask = c->wit_mask + (~c->wit_turn & 1) * words;
   c->wit_turn++;
   return GKR_OK;
 }
@@ -131,8 +128,6 @@ static int packed_product(gkr_ctx* c, const WitRows& a, const gkr_matrix* w0, co
   g.four = packed + one_tiles * g.nsteps * kGemmBlockBytes;
   static_assert(kProductStep == kGemmK, "packable");
   if (quant) {
-    TRY(wit_mask_words(c));
-    g.mask = c->wit_mask + 2 * kMaskAll;
     GKR_LAUNCH(c, k_wit_quantize, dim3((uint32_t)((m + kQuantRows - 1) / kQuantRows)), dim3(256 * kQuantRows), 0, a.x, m, k,
                g.nsteps, packed, *quant);
   } else {

@@ -1,0 +1,229 @@
+"""Products with scales, rotary positions and attention over prompts as callers use them: on a stream of the
+caller's, captured into a graph that is replayed between other calls, over outputs that hold other words, from
+several contexts and threads, and with launches that are refused."""
+import ctypes
+import threading
+
+import numpy as np
+import pytest
+
+import gkr_mi355x as G
+from test_gpu_prompt import attend
+from test_gpu_rotary import table, turn
+from test_gpu_scaled import check, quantize, rescale
+from test_gpu_witness import product, words
+
+pytestmark = pytest.mark.gpu
+P = G.P
+HEADS, KV, DIM, OFFSET = 4, 2, 32, 1 << 19
+
+
+class Calls:
+    """One of each operator over inputs of `kind` (int8-range or any words), with what it has to give."""
+
+    def __init__(self, ctx, m, counts, seed, n=90, k=500):
+        self.ctx, self.m, self.counts, self.n, self.k = ctx, m, counts, n, k
+        rng = self.rng = np.random.default_rng(seed)
+        self.W, self.S = words(rng, (k, n), 1), rng.integers(1 << 14, 1 << 15, size=n)
+        self.w, self.s = ctx.upload(self.W), ctx.upload(self.S.reshape(1, n).astype(np.uint32))
+        tokens = sum(counts)
+        self.freqs = G.rotary_frequencies(DIM)
+        self.rotary = ctx.rotary(self.freqs, 1000)
+        self.inputs = {"a": ctx.zeros(m, k), "q": ctx.zeros(tokens, HEADS * DIM), "k": ctx.zeros(tokens, KV * DIM),
+                       "v": ctx.zeros(tokens, KV * DIM)}
+        shapes = {"scaled": (m, n), "quantized": (m, n), "rows": (m, k), "scales": (m, 1), "pre": (m, n),
+                  "q_turned": (tokens, HEADS * DIM), "k_turned": (tokens, KV * DIM), "attended": (tokens, HEADS * DIM)}
+        self.outputs = {name: ctx.synthetic(*shape, 0, 40 + i) for i, (name, shape) in enumerate(shapes.items())}
+
+    def __call__(self):
+        i, o, ctx = self.inputs, self.outputs, self.ctx
+        ctx.matmul_forward_scaled(i["a"], self.w, o["scaled"], col_scales=self.s, shift=20)
+        ctx.matmul_forward_quantized(i["a"], self.w, o["quantized"], col_scales=self.s, shift=40, limit=1 << 20,
+                                     quantized=o["rows"], row_scales=o["scales"], pre=o["pre"])
+        ctx.rotary_forward(self.rotary, i["q"], o["q_turned"], self.counts, DIM, starts=[7] * len(self.counts), k=i["k"],
+                           k_out=o["k_turned"], limit=127)
+        ctx.attention_prompt(o["q_turned"], o["k_turned"], i["v"], self.counts, HEADS, KV, o["attended"],
+                             score_offset=OFFSET)
+
+    def fresh(self, kind):
+        """New words for the inputs: name -> array."""
+        return {name: words(self.rng, (t.rows, t.cols), kind) for name, t in self.inputs.items()}
+
+    def matches(self, x):
+        want = {"scaled": rescale(product(x["a"], self.W), np.ones(self.m, np.int64), self.S, 20, 0)}
+        rows, scales = quantize(x["a"], 127)
+        want["rows"], want["scales"] = rows, scales[:, None]
+        want["pre"] = product(rows.astype(np.uint32), self.W)
+        want["quantized"] = rescale(want["pre"], scales, self.S, 40, 1 << 20)
+        at = np.concatenate([7 + np.arange(n) for n in self.counts])
+        c, s = table(self.freqs, at, 1 << 15)
+        want["q_turned"], want["k_turned"] = (turn(x[t], c, s, DIM, 15, False, 127) for t in "qk")
+        out, row = [], 0
+        for n in filter(None, self.counts):
+            part = [t[row : row + n] for t in (want["q_turned"], want["k_turned"], x["v"])]
+            out.append(attend(*part, HEADS, KV, OFFSET, 20, n)[0])
+            row += n
+        want["attended"] = np.concatenate(out)
+        for name, t in want.items():
+            assert np.array_equal(self.outputs[name].download(), t), name
+
+
+def upload(ctx, calls, x, copy, stream):
+    for name, host in x.items():
+        assert copy(calls.inputs[name].device_ptr, host.ctypes.data, host.nbytes, 1, stream) == 0
+
+
+def runtime():
+    G.lib()
+    hip = ctypes.CDLL("libamdhip64.so.7")  # the runtime the library has loaded
+    vp, size = ctypes.c_void_p, ctypes.c_size_t
+    hip.hipMemcpyAsync.argtypes = [vp, vp, size, ctypes.c_int, vp]
+    hip.hipStreamBeginCapture.argtypes, hip.hipStreamEndCapture.argtypes = [vp, ctypes.c_int], [vp, ctypes.POINTER(vp)]
+    hip.hipGraphInstantiate.argtypes = [ctypes.POINTER(vp), vp, vp, vp, size]
+    hip.hipGraphLaunch.argtypes, hip.hipGraphExecDestroy.argtypes, hip.hipGraphDestroy.argtypes = [vp, vp], [vp], [vp]
+    return hip
+
+
+def test_on_the_callers_stream():
+    hip, stream = runtime(), ctypes.c_void_p()
+    assert hip.hipStreamCreate(ctypes.byref(stream)) == 0
+    for s in (stream, ctypes.c_void_p()):
+        ctx = G.Context(0, stream=s.value or 0)
+        for m, counts in ((1, [1]), (40, [33, 0, 5])):
+            calls = Calls(ctx, m, counts, m)
+            for turn_ in range(4):
+                x = calls.fresh(turn_ % 2)
+                upload(ctx, calls, x, hip.hipMemcpyAsync, s)
+                calls()
+                calls.matches(x)
+        ctx.close()
+    assert hip.hipStreamDestroy(stream) == 0
+
+
+@pytest.mark.parametrize("m,counts", [(1, [1]), (9, [9]), (200, [150, 1, 0, 70])])
+def test_captured_into_a_graph(m, counts):
+    """Captured once and replayed over changed inputs, int8-range and general in turn, with calls of the context's
+    own between, of the same sizes and of larger ones, whose buffers outgrow the graph's."""
+    hip, stream = runtime(), ctypes.c_void_p()
+    graph, run = ctypes.c_void_p(), ctypes.c_void_p()
+    assert hip.hipStreamCreate(ctypes.byref(stream)) == 0
+    ctx = G.Context(0, stream=stream.value)
+    calls, same = Calls(ctx, m, counts, 5), Calls(ctx, m, counts, 6)
+    upload(ctx, calls, calls.fresh(0), hip.hipMemcpyAsync, stream)
+    calls()  # planes, tables and buffers are there from here on
+    ctx.synchronize()
+    thread_local = 1
+    assert hip.hipStreamBeginCapture(stream, thread_local) == 0
+    calls()
+    assert hip.hipStreamEndCapture(stream, ctypes.byref(graph)) == 0
+    assert hip.hipGraphInstantiate(ctypes.byref(run), graph, None, None, 0) == 0
+    others = []
+    for turn_ in range(5):
+        x = calls.fresh(turn_ % 2)
+        upload(ctx, calls, x, hip.hipMemcpyAsync, stream)
+        for _ in range(2):
+            assert hip.hipGraphLaunch(run, stream) == 0
+            calls.matches(x)
+        between = same if turn_ < 2 else Calls(ctx, m + 150 * turn_, [200 * turn_, 40], turn_, k=500 + 900 * turn_)
+        y = between.fresh(1 - turn_ % 2)
+        upload(ctx, between, y, hip.hipMemcpyAsync, stream)
+        between()
+        between.matches(y)
+        others += [ctx.zeros(1, e) for e in (1 << 16, 1 << 20, 1 << 22)]  # where freed memory was
+        assert not any(o.download().any() for o in others)
+    assert hip.hipGraphExecDestroy(run) == 0 and hip.hipGraphDestroy(graph) == 0
+    ctx.close()
+    assert hip.hipStreamDestroy(stream) == 0
+
+
+def test_two_contexts_from_two_threads():
+    failed = []
+
+    def work(seed):
+        try:
+            ctx = G.Context(0)
+            calls = [Calls(ctx, m, counts, seed + m) for m, counts in ((1, [1]), (70, [64, 6]), (300, [257]))]
+            for turn_ in range(4):
+                for c in calls:
+                    x = c.fresh((turn_ + seed) % 2)
+                    for name, host in x.items():
+                        c.inputs[name] = ctx.upload(host)
+                    c()
+                    c.matches(x)
+            ctx.close()
+        except BaseException as e:  # told by the test
+            failed.append(e)
+
+    threads = [threading.Thread(target=work, args=(s,)) for s in (1, 2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not failed, failed
+
+
+@pytest.mark.parametrize("callers_stream", [False, True])
+@pytest.mark.parametrize("m,counts,k", [(1, [1], 64), (4, [3], 5000), (40, [70], 64), (300, [40, 33], 13825)])
+def test_every_refused_launch_is_told(m, counts, k, callers_stream):
+    """Whichever launch of the four operators is refused, a call or the wait behind them says so, and the next
+    calls write every output again."""
+    ctx = G.Context(0, stream=0) if callers_stream else G.Context(0)
+    calls = Calls(ctx, m, counts, m, n=1030, k=k)
+    x = calls.fresh(0)
+    for name, host in x.items():
+        calls.inputs[name] = ctx.upload(host)
+    calls()
+    ctx.synchronize()  # planes and buffers are there
+
+    refused = 0
+    for nth in range(1, 40):
+        for name, t in calls.outputs.items():
+            calls.outputs[name] = ctx.synthetic(t.rows, t.cols, 0, nth)
+        ctx.synchronize()
+        ctx.debug(G.DEBUG_REFUSE_LAUNCH, nth)
+        try:
+            calls()
+            ctx.synchronize()
+        except G.GkrError as e:
+            assert e.code == 2
+            refused += 1
+        else:
+            ctx.debug(G.DEBUG_REFUSE_LAUNCH, 0)
+            break
+        ctx.debug(G.DEBUG_REFUSE_LAUNCH, 0)
+        ctx.synchronize()  # told once
+        calls()
+        calls.matches(x)
+    assert 5 <= refused < 39  # a launch of each, the prompt's two
+    calls.matches(x)
+    ctx.close()
+
+
+# the longest rows that a few rows' product quantizes by itself, and one more
+@pytest.mark.parametrize("m,k", [(1, 16384), (1, 16385), (2, 8192), (2, 8193), (4, 4096), (3, 4097), (8, 2048), (16, 1024),
+                                 (7, 1985), (1, 65), (1, 70001), (17, 16385), (40, 20000)])
+@pytest.mark.parametrize("n", [70, 8300])
+def test_longest_rows_quantized_by_the_product(gpu_ctx, m, k, n):
+    if n * k > 1 << 28:
+        n = 333
+    check(gpu_ctx, m, k, n, 0, 1, 50, 127, levels=127)
+    check(gpu_ctx, m, k, n, 1, 1, 40, 0, levels=3, residual=False, bias=False)
+
+
+@pytest.mark.parametrize("levels", [1, 2, 127])
+@pytest.mark.parametrize("m", [1, 40])
+def test_quantized_halves(gpu_ctx, m, levels):
+    """Every magnitude about the halves between two levels, for largest magnitudes of every size."""
+    rng = np.random.default_rng(m)
+    for a in (0, 1, 2, 3, 126, 127, 128, 255, 65537, (1 << 24) - 1, 1 << 29, (1 << 30) - 1):
+        half = [(2 * i + 1) * a // (2 * levels) + d for i in range(levels) for d in (-1, 0, 1)]
+        c = np.array([a] + [min(a, max(0, h)) for h in half] + [0], dtype=np.int64)
+        c = c * rng.choice([-1, 1], size=(m, len(c)))
+        x = (c % P).astype(np.uint32)
+        k, out = x.shape[1], gpu_ctx.zeros(m, 2)
+        q, s = gpu_ctx.synthetic(m, k, 0, 1), gpu_ctx.synthetic(m, 1, 0, 2)
+        gpu_ctx.matmul_forward_quantized(gpu_ctx.upload(x), gpu_ctx.upload(words(rng, (k, 2), 1)), out, levels=levels,
+                                         quantized=q, row_scales=s)
+        want, scale = quantize(x, levels)
+        assert np.array_equal(q.download(), want), a
+        assert np.array_equal(s.download()[:, 0], scale), a
