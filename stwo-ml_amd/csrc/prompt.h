@@ -51,9 +51,10 @@ __device__ __forceinline__ uint32_t prompt_value(uint32_t quarter, uint32_t dim)
 // k_wit_pack, and `clear`, the mask of the next operator on the stream, is zeroed.
 // Places behind a sequence's last token get its words again: they have no weight.
 // The workgroups of an XCD (blockIdx 8 apart) take the heads of a block one after
-// another, so that it reads whole rows: all heads' first, then the next block's. With
-// one head after the other all that run at a time read the same few channels of the
-// caches (62 us, and 13 so).
+// another, so that it reads whole rows.  All of a wave's loads go out before a branch on
+// a dim's place in its head (heads of a multiple of four dims: whole 16 bytes, and one
+// branch for all; 8125 tokens of 8 x 128 62 -> 36 us), and a lane stores the 16 bytes
+// that it holds of a plane (36 -> 23 us, 4096 tokens 9.3).
 constexpr uint32_t kPackHeads = 64;  // along one grid dimension
 constexpr uint32_t kPackWaves = 16;
 template <uint32_t PIECES>  // a wave's: of 32 there are at most
@@ -173,7 +174,7 @@ __device__ __forceinline__ uint32_t prompt_score(const S& s, int v, int32_t offs
   }
 }
 
-constexpr uint32_t kPromptCounters = 9;  // a launch's words of PromptArgs::counter
+constexpr uint32_t kPromptCounters = 2;  // a launch's words of PromptArgs::counter
 struct PromptArgs {
   const int8_t *k, *v;
   const uint32_t *q, *mask;
@@ -182,8 +183,8 @@ struct PromptArgs {
   uint32_t n, kv_heads, group, dim, chunks;
   uint32_t offset, table_mask;
   const uint32_t* upper;  // the packing's, a word a block
-  // todo: a word an item, whether the int8 kernel left it; counter: how many items of
-  // each eighth the other has taken, and whether any word of todo is set
+  // todo: a word an item, whether the int8 kernel left it; counter: how many items the
+  // other has taken, and whether any word of todo is set
   uint32_t items, general_items, *todo, *counter;
   struct {
     uint32_t item0, tiles;  // its first item of this launch, its tiles of rows (int8 kernel)
@@ -854,7 +855,7 @@ static __global__ void __launch_bounds__(64 * W, OCC) k_prompt_int8(PromptArgs a
   for (int w = 0; w < W; w++) some |= general[w];
   if (threadIdx.x == 0) {
     a.todo[item] = some;
-    if (some) a.counter[8] = 1;
+    if (some) a.counter[1] = 1;
   }
   if (some) return;  // uniform: queries of four planes are the other kernel's
   wide.run(k0, v0, k1, v1);
@@ -937,14 +938,14 @@ static __global__ void __launch_bounds__(64 * W, OCC) k_prompt_int8(PromptArgs a
 // Words that are not int8-range: keys or values (by the packing's mask), or the
 // queries of an item (a.todo, by the int8 kernel; PER of its items are one here).  No more
 // workgroups than fit at once: the items are taken in turn, the longest first, and
-// with nothing to do the launch is short (3 us; 7 with a workgroup for each of 2432
-// items).  The workgroups of an XCD (blockIdx 8 apart) take every eighth item, which
-// with eight kv heads are one head's (1501 general tokens: 174 us; any item 202).
+// with nothing to do the launch is short (4.7 us; 7.5 with a workgroup for each of 2432
+// items).  Items of one kv head for the workgroups of an XCD gain nothing (1501 general
+// tokens, 40 heads on 8 x 128: 205 us either way).
 template <int DT, int R, int W, int OCC, uint32_t PER, bool TRACE>
 static __global__ void __launch_bounds__(64 * W, OCC) k_prompt(PromptArgs a) {
   __shared__ v4i lk[4 * 4 * DT * 64], lv[4 * 4 * DT * 64];
   __shared__ uint32_t taken;
-  const uint32_t left = a.counter[8];
+  const uint32_t left = a.counter[1];
   const bool flagged = __any(prompt_mask(a.mask) != 0);
   if (!flagged && !left) return;  // uniform
   const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -952,8 +953,7 @@ static __global__ void __launch_bounds__(64 * W, OCC) k_prompt(PromptArgs a) {
 #pragma unroll 1
   for (;; item += gridDim.x) {
     if (flagged) {
-      const uint32_t eighths = gridDim.x < 8 ? 1 : 8, mine = blockIdx.x % eighths;
-      if (threadIdx.x == 0) taken = atomicAdd(a.counter + mine, 1u) * eighths + mine;
+      if (threadIdx.x == 0) taken = atomicAdd(a.counter, 1u);
       __syncthreads();
       item = taken;
     }

@@ -12,6 +12,7 @@ from __future__ import annotations
 
 import ctypes as C
 import os
+from array import array
 from typing import List, Optional, Sequence, Tuple
 
 import numpy as np
@@ -713,10 +714,9 @@ class Context:
         n = len(counts)
         if starts is not None and len(starts) != n:
             raise ValueError(f"{n} counts and {len(starts)} starts")
-        c_starts = None if starts is None else (C.c_uint32 * max(1, n))(*starts)
-        _check(lib().gkr_rotary_forward(self._h, rotary.handle, head_dim, int(interleaved), c_starts,
-                                        (C.c_uint32 * max(1, n))(*counts), n, limit, q.handle, q_out.handle, _handle(k),
-                                        _handle(k_out)))
+        c_starts = None if starts is None else _words(starts)
+        _check(lib().gkr_rotary_forward(self._h, rotary.handle, head_dim, int(interleaved), c_starts, _words(counts), n,
+                                        limit, q.handle, q_out.handle, _handle(k), _handle(k_out)))
 
     def kv_cache(self, n_kv_heads: int, head_dim: int, n_pages: int, page_tokens: int = 64, max_seqs: int = 64,
                  max_tokens: int = 65536, int8: bool = False) -> "KvCache":
@@ -745,9 +745,9 @@ class Context:
                          scores: Optional["Matrix"] = None) -> None:
         """gkr_attention_prompt: causal attention of packed sequences of counts[i] tokens."""
         n = len(counts)
-        _check(lib().gkr_attention_prompt(self._h, q.handle, k.handle, v.handle, (C.c_uint32 * max(1, n))(*counts), n,
-                                          n_heads, n_kv_heads, score_offset, table_log_size, _handle(weighted),
-                                          _handle(sums), _handle(scores), out.handle))
+        _check(lib().gkr_attention_prompt(self._h, q.handle, k.handle, v.handle, _words(counts), n, n_heads, n_kv_heads,
+                                          score_offset, table_log_size, _handle(weighted), _handle(sums),
+                                          _handle(scores), out.handle))
 
     def weight_commitment(self, b: "Matrix") -> int:
         """gkr_weight_commitment: commit_mle_root_only(matrix_to_mle_col_major_padded(B))."""
@@ -1104,6 +1104,12 @@ class Matrix:
 
 def _handle(m: Optional["Matrix"]) -> Optional[int]:
     return None if m is None else m.handle
+
+
+def _words(values: Sequence[int]) -> C.Array:
+    """A list of u32 for a call; one by one into a ctypes array, 64 of them take 8 us and so 2."""
+    a = array("I", values)
+    return (C.c_uint32 * len(a)).from_buffer(a)
 
 
 class Rotary:
