@@ -836,6 +836,98 @@ static __global__ void __launch_bounds__(64 * W) k_wit_tiles(WitProduct g, uint3
     wit_tiles<RT, PB, GATED, W, WR1, false>(g, sums, rg, cg, blockIdx.y, end);
 }
 
+// Some hundred rows of one plane by weights of one plane: a workgroup has RT row tiles
+// by CT column tiles and all of K, and its eight waves take the K steps in turn, each
+// all of the tiles, straight from memory into registers.  No operand is read twice by
+// a workgroup, nothing waits for another wave until the waves' sums meet in LDS, and
+// no parts go through memory: where k_wit_blocks' 256 x 256 leave most CUs without a
+// workgroup or split K (scales, no residual: 512 x 5120 x 5120 38 us with the join, 25
+// so; 512 x 13824 x 5120 58 and 47; 700 x 576 x 1536 27 and 8).  Bound by a CU's way to
+// its second-level cache, 7 KB a K step at 78 GB/s (two, three or four steps in flight,
+// 2 x 4 and 2 x 5 tiles: the same).
+template <int RT, int CT, class End>
+__device__ __forceinline__ void wit_wide(const WitProduct& g, int32_t* sums, uint32_t rg, uint32_t cg, const End& end) {
+  constexpr int W = 8, U = 2;
+  const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int8_t *ab[RT], *bb[CT];  // tiles past an edge are the last one again, and not stored
+#pragma unroll
+  for (int i = 0; i < RT; i++)
+    ab[i] = g.one + (uint64_t)umin32(rg * RT + i, g.plan[0].rtiles - 1) * g.nsteps * kGemmBlockBytes;
+#pragma unroll
+  for (int j = 0; j < CT; j++)
+    bb[j] = g.w[0].planes + (uint64_t)umin32(cg * CT + j, g.ctiles - 1) * g.nsteps * kGemmBlockBytes;
+  v4i a[U][RT], b[U][CT];
+  auto load = [&](int u, uint32_t s) {
+    const uint32_t at = umin32(s, g.nsteps - 1) * kGemmBlockBytes + 16 * lane;  // past the end: again, unused
+#pragma unroll
+    for (int j = 0; j < CT; j++) b[u][j] = *(const v4i*)(bb[j] + at);
+#pragma unroll
+    for (int i = 0; i < RT; i++) a[u][i] = *(const v4i*)(ab[i] + at);
+  };
+#pragma unroll
+  for (int u = 0; u < U; u++) load(u, wave + u * W);
+#pragma unroll 1
+  for (uint32_t i = threadIdx.x; i < RT * CT * 256; i += 64 * W) ((v4i*)sums)[i] = v4i{0, 0, 0, 0};
+  v16i acc[RT][CT];
+#pragma unroll
+  for (int i = 0; i < RT; i++)
+#pragma unroll
+    for (int j = 0; j < CT; j++)
+#pragma unroll
+      for (int v = 0; v < 16; v++) acc[i][j][v] = 0;
+  auto multiply = [&](int u) {
+#pragma unroll
+    for (int j = 0; j < CT; j++)
+#pragma unroll
+      for (int i = 0; i < RT; i++) acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(a[u][i], b[u][j], acc[i][j], 0, 0, 0);
+  };
+  uint32_t s = wave;
+  // U steps at a time without a branch between: with one, a wait for any load would be for all
+#pragma unroll 1
+  for (; s + (U - 1) * W < g.nsteps; s += U * W) {
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+      multiply(u);
+      load(u, s + (u + U) * W);
+    }
+  }
+#pragma unroll
+  for (int u = 0; u < U - 1; u++)
+    if (s + u * W < g.nsteps) multiply(u);
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < RT; i++)
+#pragma unroll
+    for (int j = 0; j < CT; j++)
+#pragma unroll
+      for (int v = 0; v < 16; v++)
+        atomicAdd(&sums[((j * RT + i) * 32 + 8 * (v / 4) + 4 * (lane >> 5) + v % 4) * 32 + (lane & 31)], acc[i][j][v]);
+  __syncthreads();
+  // the end, a column tile at a time
+  constexpr int E = RT * 1024 / (64 * W);
+  const uint32_t c = threadIdx.x % 32, r0 = threadIdx.x / 32;
+#pragma unroll 1
+  for (int j = 0; j < CT; j++) {
+    const uint64_t col0 = ((uint64_t)cg * CT + j) * 32, col = col0 + c;
+    if (col0 >= g.n) return;  // uniform
+    const typename End::Tile tile = end.tile((uint64_t)rg * (RT * 32) * g.n + col0, g.m * g.n);
+    uint32_t at[E], row[E], z[1][E];
+#pragma unroll
+    for (int e = 0; e < E; e++) {
+      const uint32_t r = r0 + e * 2 * W;
+      row[e] = rg * (RT * 32) + r;
+      at[e] = col < g.n ? 4 * (r * (uint32_t)g.n + c) : kOutside;
+      z[0][e] = gemm_mod_p(sums[(j * RT * 32 + r) * 32 + c]);
+    }
+    typename End::Column of_column[E];
+    same_column(of_column, end.column(col, col < g.n));
+    typename End::template Slot<E> slot;
+    end.fetch(slot, tile, at, row);
+    end.begin(slot, of_column, z);
+    end.finish(slot, tile, at);
+  }
+}
+
 // Between a wave's stores to LDS and its lanes' reads of each other's words, and
 // between those reads and the next stores: the wave's LDS instructions run in
 // order, but the compiler sees one lane's addresses, which it may prove apart
@@ -1106,6 +1198,18 @@ static __global__ void __launch_bounds__(512) k_wit_blocks(WitProduct g, End end
     wit_block<PB, GATED, true>(g, lds, rg, cg, split, end);
   else
     wit_block<PB, GATED, false>(g, lds, rg, cg, split, end);
+}
+template <int RT, int CT, class End>
+static __global__ void __launch_bounds__(512) k_wit_wide(WitProduct g, End end) {
+  __shared__ v4i lds[2 * 16 * kBlockStage * 64];
+  static_assert(RT * CT * 4096 <= sizeof(lds), "the waves' sums");
+  const bool four = wit_four(g.mask);
+  uint32_t rg, cg, split;
+  if (!wit_group(g.plan[four ? 1 : 0], four ? g.cgroups : (g.ctiles + CT - 1) / CT, rg, cg, split)) return;  // uniform
+  if (four)
+    wit_block<1, false, true>(g, lds, rg, cg, split, end);
+  else
+    wit_wide<RT, CT>(g, (int32_t*)lds, rg, cg, end);
 }
 // 65 to 256 rows: rows of one plane are still a stream of the weights
 // (wit_tiles, all of the rows in a workgroup), rows of four are blocks.

@@ -107,6 +107,15 @@ static double blocks_us(uint64_t groups, uint32_t nsteps, uint64_t elements, uin
   return best;
 }
 
+// k_wit_wide, 128 x 96 a workgroup: fitted to 24 products of 300 to 2048 rows, k 576 to
+// 13824, n 1024 to 8000, 8 to 228 us without the packing, within a seventh; a quarter
+// more, as the others' times are only that well known.  Beyond two rounds the rows and
+// weights no longer lie in the second-level caches (5000 x 13824 x 5120 in nine rounds
+// 640 us, k_wit_blocks 440).
+static double wide_us(uint64_t groups, uint32_t nsteps) {
+  return groups > 512 ? 1e30 : 1.25 * (2.0 + (double)((groups + 255) / 256) * (9.0 + 0.09 * nsteps));
+}
+
 // More rows: packed, multiplied (k_wit_tiles) and, where K is split, joined.  With
 // `quant` they are brought to 8 bits as they are packed, and have one plane.
 template <bool GATED, class End>
@@ -185,6 +194,15 @@ static int packed_product(gkr_ctx* c, const WitRows& a, const gkr_matrix* w0, co
     GKR_LAUNCH(c, kernel, dim3((uint32_t)grid), dim3(512), 0, g, end);
     return check_launch(c);
   };
+  auto launch_wide = [&](auto kernel, uint32_t rt, uint32_t ct) -> int {
+    g.cgroups = (uint32_t)bgroups;
+    TRY(plan(0, rt, 1));
+    TRY(plan(1, 8, splits[1]));
+    const uint64_t wide = (uint64_t)g.plan[0].rgroups * ((g.ctiles + ct - 1) / ct);
+    const uint64_t other = ((uint64_t)g.plan[1].rgroups * g.cgroups + 7) / 8 * 8 * g.plan[1].splits;
+    GKR_LAUNCH(c, kernel, dim3((uint32_t)std::max((wide + 7) / 8 * 8, other)), dim3(512), 0, g, end);
+    return check_launch(c);
+  };
 #define GKR_WIT_TILES(RT, PB, W, WR1, WR4) launch_tiles(k_wit_tiles<RT, PB, GATED, W, WR1, WR4, End>, RT, W, WR1, WR4)
   // sixteen waves a workgroup for one matrix, eight for two: the registers of
   // sixteen hold no more accumulators
@@ -208,8 +226,12 @@ static int packed_product(gkr_ctx* c, const WitRows& a, const gkr_matrix* w0, co
     constexpr uint32_t RT = GATED ? 2 : 4, WR = GATED ? 2 : 1;
     const uint32_t down = m <= 128 ? WR : 2 * WR;  // waves down the rows of k_wit_mixed
     const double mixed = m <= 256 ? tiles_us(ctiles, 256, g.nsteps, down * (RT + NW)) + blocks[1] : 1e30;
-    if (tiles <= std::min(mixed, blocks[0] + blocks[1])) TRY(GKR_WIT_TILES(2, 1, W, 1, 4));
-    else if (mixed > blocks[0] + blocks[1]) TRY(launch_blocks(k_wit_blocks<1, GATED, End>, 0));
+    const double wide = GATED ? 1e30 : wide_us((m + 127) / 128 * ((ctiles + 2) / 3), g.nsteps);
+    const double most = std::min(wide, blocks[0]) + blocks[1];
+    if (tiles <= std::min(mixed, most)) TRY(GKR_WIT_TILES(2, 1, W, 1, 4));
+    else if (mixed > most && wide < blocks[0]) {
+      if constexpr (!GATED) TRY(launch_wide(k_wit_wide<4, 3, End>, 4, 3));
+    } else if (mixed > most) TRY(launch_blocks(k_wit_blocks<1, GATED, End>, 0));
     else if (m <= 128) TRY(launch_blocks(k_wit_mixed<RT, WR, GATED, End>, RT * WR));
     else TRY(launch_blocks(k_wit_mixed<RT, 2 * WR, GATED, End>, 2 * RT * WR));
   }

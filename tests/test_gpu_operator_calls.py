@@ -11,7 +11,7 @@ import gkr_mi355x as G
 from test_gpu_prompt import attend
 from test_gpu_rotary import table, turn
 from test_gpu_scaled import check, quantize, rescale
-from test_gpu_witness import product, words
+from test_gpu_witness import GELU, check_fused, product, words
 
 pytestmark = pytest.mark.gpu
 P = G.P
@@ -227,3 +227,16 @@ def test_quantized_halves(gpu_ctx, m, levels):
         want, scale = quantize(x, levels)
         assert np.array_equal(q.download(), want), a
         assert np.array_equal(s.download()[:, 0], scale), a
+
+
+# rows between the sizes of the streamed kernels and those that fill the chip with blocks; ragged in both
+@pytest.mark.parametrize("m,k,n", [(300, 700, 5001), (257, 1001, 8111), (700, 65, 4100), (1000, 333, 1551), (385, 2100, 5000)])
+def test_some_hundred_rows(gpu_ctx, m, k, n):
+    check(gpu_ctx, m, k, n, 1, 1, 40, 127)
+    check(gpu_ctx, m, k, n, 0, 1, 50, 0, residual=False, pre=False)
+    check(gpu_ctx, m, k, n, 0, 1, 50, 1 << 20, levels=127)
+    x = np.zeros((m, k), np.uint32)
+    x[m // 2, k - 1] = 12345  # one word above a byte
+    check(gpu_ctx, m, k, n, 1, 1, 0, 0, x=x)
+    check_fused(gpu_ctx, m, k, n, 1, 1, act=GELU, log=0)
+    check_fused(gpu_ctx, m, k, n, 0, 1)
