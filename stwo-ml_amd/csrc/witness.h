@@ -143,6 +143,7 @@ struct GatedEnd {
     for (int e = 0; e < E; e++) wit_write(t.out, at[e], m31_mul(s.y[e], s.u[e]));
   }
 };
+__device__ __forceinline__ uint32_t word_of(int32_t v) { return (uint32_t)v + ((uint32_t)(v >> 31) & P); }
 // Rescaled sums: t = round(c(z) r s / 2^shift) + c(bias), halves away from zero,
 // cut off at +-limit, with the row's and the column's scale as whole numbers.
 // |c(z)| r is below 2^61 and its product with s below 2^92, held in three words;
@@ -181,19 +182,21 @@ struct ScaledEnd {
       for (int e = 0; e < E; e++) s.residual[e] = wit_read(t.residual, at[e]);
     }
   }
+  // In three words: |c(z)| r s + half below 2^93, its bits from `shift` on in a word, or
+  // all ones where there are more.  The bias moves the bounds: what is cut off at them
+  // plus the bias is what the sum would be cut off to.
   __device__ __forceinline__ uint32_t scale(uint32_t z, uint32_t r, const Column& c) const {
-    const int32_t v = center_m31(z), sign = v >> 31;
+    const int32_t v = center_m31(z), sign = v >> 31, bias_of = center_m31(c.bias);
     const uint64_t a = (uint64_t)(uint32_t)((v ^ sign) - sign) * r, half = shift ? 1ull << (shift - 1) : 0;
-    const uint64_t low = (uint64_t)(uint32_t)a * c.scale, mid = (a >> 32) * c.scale + (low >> 32);  // < 2^61
-    // mid 2^32 + (low mod 2^32), rounded: the half's upper word is below 2^31
-    const uint64_t bottom = (low & 0xffffffffu) + (half & 0xffffffffu), top = mid + (half >> 32) + (bottom >> 32);
-    const uint64_t t = shift >= 32 ? top >> (shift - 32)
-                       : top >> shift ? ~0ull >> 1  // more than 32 bits are left
-                                      : (top << (32 - shift)) | ((uint32_t)bottom >> shift);
-    const int64_t y0 = (int64_t)(t < 0xffffffffull ? t : 0xffffffffull);
-    int64_t y = ((y0 ^ sign) - sign) + center_m31(c.bias);
-    y = y < -(int64_t)limit ? -(int64_t)limit : y > limit ? limit : y;
-    return (uint32_t)y + ((uint32_t)((int32_t)y >> 31) & P);
+    const uint64_t low = (uint64_t)(uint32_t)a * c.scale + (uint32_t)half;
+    const uint64_t top = (a >> 32) * c.scale + ((low >> 32) + (half >> 32));  // < 2^61
+    const bool far = shift >= 32;  // uniform
+    const uint32_t w0 = far ? (uint32_t)top : (uint32_t)low, w1 = far ? (uint32_t)(top >> 32) : (uint32_t)top;
+    const uint32_t over = ((far ? 0u : (uint32_t)(top >> 32)) | w1 >> (shift & 31));
+    const uint32_t t = over ? ~0u : __builtin_amdgcn_alignbit(w1, w0, shift & 31);
+    const int32_t y = (int32_t)umin32(t, 0x7fffffffu);
+    const int32_t cut = max(min((y ^ sign) - sign, limit - bias_of), -limit - bias_of) + bias_of;
+    return word_of(cut);
   }
   template <int E>
   __device__ __forceinline__ void begin(Slot<E>& s, const Column (&c)[E], const uint32_t (&z)[1][E]) const {
@@ -264,7 +267,6 @@ struct Quantizer {
     return (r ^ sign) - sign;
   }
 };
-__device__ __forceinline__ uint32_t word_of(int32_t v) { return (uint32_t)v + ((uint32_t)(v >> 31) & P); }
 __device__ __forceinline__ uint32_t size_of_word(uint32_t x) {  // |c(x)|
   const int32_t v = center_m31(x);
   return (uint32_t)(v < 0 ? -v : v);
