@@ -527,7 +527,7 @@ static __global__ void __launch_bounds__(64 * W, PB == 1 || !GATED ? 4 : 2)
 // Rows past m are left as they are (their sums are not stored).
 constexpr uint32_t kMaskWords = 64, kMaskStride = 32;
 __device__ __forceinline__ bool wit_four(const uint32_t* mask) {  // the same in every wave
-  return mask && __any(mask[kMaskStride * (threadIdx.x & 63)] != 0);
+  return __any(mask[kMaskStride * (threadIdx.x & 63)] != 0);
 }
 // Word p of a quad's lane q and word q of its lane p change places.
 __device__ __forceinline__ void quad_transpose(uint32_t (&x)[4]) {
@@ -585,12 +585,15 @@ static __global__ void __launch_bounds__(256) k_wit_pack(const uint32_t* __restr
 // workgroups of 110 KB fit (four rows a workgroup, the words of 16 turns in registers
 // and both loops unrolled: 512 x 13824 24.5 us, 37 x 1537 8.1, most of it the
 // instructions' way from memory; so 19.0 and 6.2).  Plane 0 alone is stored, 16 bytes a lane:
-// a quad's lanes exchange the words of four turns.
+// a quad's lanes exchange the words of four turns.  Both masks are zeroed, the product's own
+// too: there are no rows of four planes.
 constexpr uint32_t kQuantRows = 2;
 static __global__ void __launch_bounds__(256 * kQuantRows) k_wit_quantize(const uint32_t* __restrict__ X, uint64_t m, uint64_t k,
                                                                           uint32_t nsteps, int8_t* __restrict__ one,
-                                                                          WitQuant quant) {
+                                                                          WitQuant quant, uint32_t* __restrict__ mask,
+                                                                          uint32_t* __restrict__ clear) {
   __shared__ uint32_t most[kQuantRows][4];
+  if (blockIdx.x == 0 && threadIdx.x < kMaskWords) mask[kMaskStride * threadIdx.x] = clear[kMaskStride * threadIdx.x] = 0;
   const uint32_t r = threadIdx.x / 256, t = threadIdx.x % 256, q = threadIdx.x & 3;
   const uint64_t row = (uint64_t)blockIdx.x * kQuantRows + r;
   const uint32_t groups = (nsteps * (kGemmK / 4) + 1023) / 1024;  // of four turns
@@ -677,7 +680,7 @@ struct WitPlan {
 };
 struct WitProduct {
   const int8_t *one, *four;  // the packed rows
-  const uint32_t* mask;  // none: rows of one plane
+  const uint32_t* mask;
   WitWeight w[2];
   uint64_t m, n;
   uint32_t nsteps, ctiles, cgroups;

@@ -135,14 +135,14 @@ static int packed_product(gkr_ctx* c, const WitRows& a, const gkr_matrix* w0, co
   TRY(ensureT(c, S_GEMMA, (one_tiles + (quant ? 0 : four_tiles)) * g.nsteps * kGemmBlockBytes, &packed));
   g.one = packed;
   g.four = packed + one_tiles * g.nsteps * kGemmBlockBytes;
+  uint32_t *mask, *next_mask;
+  TRY(wit_masks(c, &mask, &next_mask));
+  g.mask = mask;
   static_assert(kProductStep == kGemmK, "packable");
   if (quant) {
     GKR_LAUNCH(c, k_wit_quantize, dim3((uint32_t)((m + kQuantRows - 1) / kQuantRows)), dim3(256 * kQuantRows), 0, a.x, m, k,
-               g.nsteps, packed, *quant);
+               g.nsteps, packed, *quant, mask, next_mask);
   } else {
-    uint32_t *mask, *next_mask;
-    TRY(wit_masks(c, &mask, &next_mask));
-    g.mask = mask;
     const dim3 pack_grid((uint32_t)pack_groups(m, k));
     GKR_LAUNCH(c, k_wit_pack, pack_grid, dim3(kPackThreads), 0, a.x, m, k, g.nsteps, packed,
                const_cast<int8_t*>(g.four), mask, next_mask);
@@ -152,9 +152,12 @@ static int packed_product(gkr_ctx* c, const WitRows& a, const gkr_matrix* w0, co
   uint32_t max_splits = 1, max_rgroups = 1;
   // group: row tiles of a workgroup, for rows of one plane and of four
   auto plan = [&](int four, uint32_t group, uint32_t splits) -> int {
-    if (four && quant) return GKR_OK;
-    const uint64_t tiles = four ? four_tiles : one_tiles;
     WitPlan& p = g.plan[four];
+    if (four && quant) {  // there are none; a mask that is set all the same (a refused packing) finds nothing to do
+      p = WitPlan{1, 1, 0, 0};
+      return GKR_OK;
+    }
+    const uint64_t tiles = four ? four_tiles : one_tiles;
     p.rtiles = (uint32_t)tiles;
     p.rgroups = (uint32_t)((tiles + group - 1) / group);
     p.splits = splits;
