@@ -10,7 +10,7 @@ import pytest
 import gkr_mi355x as G
 from test_gpu_prompt import attend
 from test_gpu_rotary import table, turn
-from test_gpu_scaled import check, quantize, rescale
+from test_gpu_scaled import centered, check, quantize, rescale
 from test_gpu_witness import GELU, check_fused, product, words
 
 pytestmark = pytest.mark.gpu
@@ -240,3 +240,82 @@ def test_some_hundred_rows(gpu_ctx, m, k, n):
     check(gpu_ctx, m, k, n, 1, 1, 0, 0, x=x)
     check_fused(gpu_ctx, m, k, n, 1, 1, act=GELU, log=0)
     check_fused(gpu_ctx, m, k, n, 0, 1)
+
+
+def tail(ctx, m, rows):
+    """The last rows of a matrix, as a matrix over the same memory."""
+    return ctx.wrap_device(m.device_ptr + 4 * (m.rows - rows) * m.cols, rows, m.cols)
+
+
+@pytest.mark.parametrize("kind", [1, 0])
+def test_prompts_and_turns_past_4_gib(gpu_ctx, kind):
+    """Packed sequences whose queries and outputs pass 2^32 bytes: the last ones equal a call with them alone."""
+    each, n, heads, kv, d = 1000, 215, 40, 8, 128
+    q, k, v = (gpu_ctx.synthetic(each * n, h * d, kind, 3 + i) for i, h in enumerate((heads, kv, kv)))
+    out, sums = gpu_ctx.synthetic(each * n, heads * d, 0, 1), gpu_ctx.synthetic(each * n, heads, 0, 2)
+    counts = [each] * (n - 3) + [each + 7, each - 7, each]
+    gpu_ctx.attention_prompt(q, k, v, counts, heads, kv, out, score_offset=OFFSET, sums=sums)
+    rows = counts[-1] + counts[-2]
+    alone, alone_sums = gpu_ctx.zeros(rows, heads * d), gpu_ctx.zeros(rows, heads)
+    gpu_ctx.attention_prompt(tail(gpu_ctx, q, rows), tail(gpu_ctx, k, rows), tail(gpu_ctx, v, rows), counts[-2:], heads, kv,
+                             alone, score_offset=OFFSET, sums=alone_sums)
+    assert np.array_equal(tail(gpu_ctx, out, rows).download(), alone.download())
+    assert np.array_equal(tail(gpu_ctx, sums, rows).download(), alone_sums.download())
+    rotary = gpu_ctx.rotary(G.rotary_frequencies(d), 2 * each)
+    starts = [i % 900 for i in range(n)]
+    gpu_ctx.rotary_forward(rotary, q, out, counts, d, starts=starts, k=k, k_out=k, limit=127)
+    gpu_ctx.rotary_forward(rotary, tail(gpu_ctx, q, rows), alone, counts[-2:], d, starts=starts[-2:], limit=127)
+    assert np.array_equal(tail(gpu_ctx, out, rows).download(), alone.download())
+    rotary.free()
+
+
+def test_scores_past_4_gib(gpu_ctx):
+    heads, n, d = 64, 4200, 16
+    rng = np.random.default_rng(5)
+    Q, K = words(rng, (n, heads * d), 1), words(rng, (n, d), 1)
+    q, k = gpu_ctx.upload(Q), gpu_ctx.upload(K)
+    out, scores = gpu_ctx.zeros(n, heads * d), gpu_ctx.zeros(n * heads, n + 1)
+    gpu_ctx.attention_prompt(q, k, k, [n], heads, 1, out, score_offset=OFFSET, scores=scores)
+    want = (OFFSET + centered(Q[-1]).reshape(heads, d) @ centered(K).T) % P
+    got = tail(gpu_ctx, scores, 65).download()  # the last token's, and one of the token before
+    assert np.array_equal(got[1:, :n], want) and not got[:, n].any() and got[0, n - 1] == 0 and got[0, n - 2] != 0
+
+
+def test_scaled_results_past_4_gib(gpu_ctx):
+    m, k, n = 70001, 64, 16400
+    rows = 300
+    a, b, s = gpu_ctx.synthetic(m, k, 1, 1), gpu_ctx.synthetic(k, n, 1, 2), gpu_ctx.synthetic(1, n, 0, 3)
+    out, alone = gpu_ctx.synthetic(m, n, 0, 4), gpu_ctx.zeros(rows, n)
+    gpu_ctx.matmul_forward_scaled(a, b, out, col_scales=s, shift=38, limit=127)
+    gpu_ctx.matmul_forward_scaled(tail(gpu_ctx, a, rows), b, alone, col_scales=s, shift=38, limit=127)
+    assert np.array_equal(tail(gpu_ctx, out, rows).download(), alone.download())
+    gpu_ctx.matmul_forward_quantized(a, b, out, col_scales=s, shift=45, limit=127)
+    gpu_ctx.matmul_forward_quantized(tail(gpu_ctx, a, rows), b, alone, col_scales=s, shift=45, limit=127)
+    assert np.array_equal(tail(gpu_ctx, out, rows).download(), alone.download())
+
+
+@pytest.mark.parametrize("general", [False, True])
+def test_longest_prompt(gpu_ctx, general):
+    """The most tokens of one sequence, with weights and values that fill the sums: rows of it against whole
+    numbers."""
+    n, d = 131071, 16
+    rng = np.random.default_rng(9)
+    place = 7 if general else 10  # the largest weights of a plane
+    Q, K = np.zeros((n, d), np.uint32), words(rng, (n, d), 0 if general else 1)
+    V = np.full((n, d), (P - (128 + (128 << 8) + (128 << 16) + (62 << 24))) if general else P - 128, np.uint32)
+    Q[n // 2 :] = words(rng, (n - n // 2, d), 0 if general else 1)  # the earlier rows have one weight
+    Q[-1] = 0
+    V[::7] = words(rng, V[::7].shape, 0 if general else 1)
+    V[1::7] = V[2]
+    out, weighted, sums = gpu_ctx.zeros(n, d), gpu_ctx.zeros(n, d), gpu_ctx.zeros(n, 1)
+    gpu_ctx.attention_prompt(gpu_ctx.upload(Q), gpu_ctx.upload(K), gpu_ctx.upload(V), [n], 1, 1, out,
+                             score_offset=place << 16, weighted=weighted, sums=sums)
+    out, weighted, sums = out.download(), weighted.download(), sums.download()
+    ck, cv = centered(K), centered(V)
+    for t in (0, 1, 63, 64, 4097, n // 2 - 1, n // 2, n - 65, n - 2, n - 1):
+        x = ((place << 16) + (ck[: t + 1] * centered(Q[t]) % P).sum(axis=1)) % P
+        w = np.int64(1) << np.minimum((x % (1 << 20)) >> 16, 10)
+        z, total = int(w.sum()), [int(c) for c in w @ cv[: t + 1]]
+        assert sums[t, 0] == (z << 16) % P, t
+        assert [int(c) for c in weighted[t]] == [(c << 16) % P for c in total], t
+        assert [int(c) for c in out[t]] == [(1 if c > 0 else -1) * ((2 * abs(c) + z) // (2 * z)) % P for c in total], t
