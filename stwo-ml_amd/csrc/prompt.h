@@ -53,7 +53,7 @@ __device__ __forceinline__ uint32_t prompt_value(uint32_t quarter, uint32_t dim)
 // The workgroups of an XCD (blockIdx 8 apart) take the heads of a block one after
 // another, so that it reads whole rows.  All of a wave's loads go out before a branch on
 // a dim's place in its head (heads of a multiple of four dims: whole 16 bytes, and one
-// branch for all; 8125 tokens of 8 x 128 62 -> 36 us), and a lane stores the 16 bytes
+// branch for all; 7599 tokens of 8 x 128 62 -> 36 us), and a lane stores the 16 bytes
 // that it holds of a plane (36 -> 23 us, 4096 tokens 9.3).
 constexpr uint32_t kPackHeads = 64;  // along one grid dimension
 constexpr uint32_t kPackWaves = 16;
