@@ -396,8 +396,9 @@ int gkr_matmul_forward_into(gkr_ctx* ctx, const gkr_matrix* a, const gkr_matrix*
 
 /* Z = A B + bias, Y = act(Z) + residual (mod P): Y into out, Z into pre.
  * A is m x k, B k x n; bias 1 x n, residual, pre and out m x n.  The residual
- * may be the output itself (added in place).  Replaces the reference's GEMM,
- * add, ReLU and table kernels of the forward pass (engine/src/gpu_sumcheck.rs:418-512). */
+ * may be the output itself (added in place), also by another handle of the same
+ * memory.  Replaces the reference's GEMM, add, ReLU and table kernels of the
+ * forward pass (engine/src/gpu_sumcheck.rs:418-512).                          */
 int gkr_matmul_forward_fused(gkr_ctx* ctx, const gkr_matrix* a, const gkr_matrix* b, const gkr_matrix* bias,
                              uint32_t activation_type, uint32_t table_log_size, const gkr_matrix* residual,
                              gkr_matrix* pre, gkr_matrix* out);
@@ -416,7 +417,7 @@ int gkr_gated_forward(gkr_ctx* ctx, const gkr_matrix* a, const gkr_matrix* wg, c
  * (shift 0 .. 63; limit 1 .. 2^30 - 1, 0 = 2^30 - 1).  With a limit of 127 or less
  * Y are words that an int8 cache takes.  A is m x k, B k x n, row_scales m x 1,
  * col_scales and bias 1 x n, residual, pre (Z) and out (Y) m x n; the residual may
- * be the output itself.
+ * be the output itself, also by another handle of the same memory.
  *
  * gkr_matmul_forward_quantized brings each row of A to 8 bits first: with a_i the
  * largest |c(x)| of row i, q = round(c(x) levels / a_i) (0 where a_i = 0; levels

@@ -63,8 +63,8 @@ static int scaled_forward(gkr_ctx* c, const gkr_matrix* a, const gkr_matrix* b, 
   TRY(check_shape(what, "the rows' scales", row_scales, a->rows, 1));
   e.row_scales = row_scales ? row_scales->dev : nullptr;
   HIP_TRY(hipSetDevice(c->device));
-  for (gkr_matrix* w : {pre, out})
-    if (w) TRY(drop_derived(c, w));
+  if (pre) TRY(drop_derived(c, pre));
+  TRY(drop_output(c, out, residual));
   TRY(weight_planes(c, const_cast<gkr_matrix*>(b)));
   return scaled_product(c, a, b, e);
 }
@@ -86,8 +86,9 @@ static int quantized_forward(gkr_ctx* c, const gkr_matrix* a, const gkr_matrix* 
     if (residual && w && overlap(residual, w))
       return fail(GKR_ERR_INVALID, "%s: the residual shares part of an output's memory", what);
   HIP_TRY(hipSetDevice(c->device));
-  for (gkr_matrix* w : {quantized, row_scales, pre, out})
+  for (gkr_matrix* w : {quantized, row_scales, pre})
     if (w) TRY(drop_derived(c, w));
+  TRY(drop_output(c, out, residual));
   TRY(weight_planes(c, const_cast<gkr_matrix*>(b)));
   uint32_t* scales;
   if (row_scales) scales = row_scales->dev;

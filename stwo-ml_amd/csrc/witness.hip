@@ -68,7 +68,7 @@ static int fused_forward(gkr_ctx* c, const gkr_matrix* a, const gkr_matrix* b, c
   e.residual = residual ? residual->dev : nullptr;
   e.pre = pre ? pre->dev : nullptr;
   e.out = out->dev;
-  TRY(drop_derived(c, out));
+  TRY(drop_output(c, out, residual));
   if (pre) TRY(drop_derived(c, pre));
   TRY(weight_planes(c, const_cast<gkr_matrix*>(b)));
   if (few_rows(wit_rows(a), b, b)) return rows_product<false>(c, wit_rows(a), b, b, e);

@@ -15,6 +15,12 @@ inline bool overlap(const gkr_matrix* x, const gkr_matrix* y) {
   const uint32_t *x1 = x->dev + x->rows * x->cols, *y1 = y->dev + y->rows * y->cols;
   return x->dev < y1 && y->dev < x1;
 }
+// The contents of an output change; a residual may be the same memory by another
+// handle, whose derived copies go too.
+inline int drop_output(gkr_ctx* c, gkr_matrix* out, const gkr_matrix* residual) {
+  if (residual && residual != out && residual->dev == out->dev) TRY(drop_derived(c, const_cast<gkr_matrix*>(residual)));
+  return drop_derived(c, out);
+}
 static WitWeight wit_weight(const gkr_matrix* w) { return WitWeight{w->bplanes, (uint32_t)w->bnplanes}; }
 
 static dim3 end_grid(uint64_t count) { return dim3((uint32_t)std::min<uint64_t>((count + 255) / 256, 1u << 20)); }
