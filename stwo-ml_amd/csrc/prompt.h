@@ -175,16 +175,18 @@ __device__ __forceinline__ uint32_t prompt_score(const S& s, int v, int32_t offs
 }
 
 constexpr uint32_t kPromptCounters = 2;  // a launch's words of PromptArgs::counter
+constexpr uint32_t kPromptSome = 1, kPromptAll = 2;
 struct PromptArgs {
   const int8_t *k, *v;
   const uint32_t *q, *mask;
+  uint32_t* clear;  // the mask once more, for the call's last launch, else none
   AttOut o;
   uint32_t blocks;  // of a kv head, all sequences'
   uint32_t n, kv_heads, group, dim, chunks;
   uint32_t offset, table_mask;
   const uint32_t* upper;  // the packing's, a word a block
   // todo: a word an item, whether the int8 kernel left it; counter: how many items the
-  // other has taken, and whether any word of todo is set
+  // other has taken, and whether it has some of them (kPromptSome, by todo) or all
   uint32_t items, general_items, *todo, *counter;
   struct {
     uint32_t item0, tiles;  // its first item of this launch, its tiles of rows (int8 kernel)
@@ -793,7 +795,10 @@ static __global__ void __launch_bounds__(64 * W, OCC) k_prompt_int8(PromptArgs a
         for (uint32_t t = 0; t < 4; t++) w[r][j][t] = (int)from[d + t < a.dim ? d + t : 0];
       }
     }
-  if (__any(flagged != 0)) return;  // uniform: the other kernel's
+  if (__any(flagged != 0)) {  // uniform: the other kernel's
+    if (item == 0 && threadIdx.x == 0) a.counter[1] = kPromptAll;
+    return;
+  }
 #pragma unroll
   for (int r = 0; r < R; r++)
 #pragma unroll
@@ -855,7 +860,7 @@ static __global__ void __launch_bounds__(64 * W, OCC) k_prompt_int8(PromptArgs a
   for (int w = 0; w < W; w++) some |= general[w];
   if (threadIdx.x == 0) {
     a.todo[item] = some;
-    if (some) a.counter[1] = 1;
+    if (some) a.counter[1] = kPromptSome;
   }
   if (some) return;  // uniform: queries of four planes are the other kernel's
   wide.run(k0, v0, k1, v1);
@@ -940,14 +945,18 @@ static __global__ void __launch_bounds__(64 * W, OCC) k_prompt_int8(PromptArgs a
 // workgroups than fit at once: the items are taken in turn, the longest first, and
 // with nothing to do the launch is short (4.7 us; 7.5 with a workgroup for each of 2432
 // items).  Items of one kv head for the workgroups of an XCD gain nothing (1501 general
-// tokens, 40 heads on 8 x 128: 205 us either way).
+// tokens, 40 heads on 8 x 128: 205 us either way).  The mask is the int8 kernel's to
+// read; the last launch of a call zeroes it, so that a graph of one prompt, whose
+// replays all have the same mask, does not find it set by general words of an earlier
+// one (1500 int8 tokens, 16 heads of 128: 46 us, and 176 for every replay behind such).
 template <int DT, int R, int W, int OCC, uint32_t PER, bool TRACE>
 static __global__ void __launch_bounds__(64 * W, OCC) k_prompt(PromptArgs a) {
   __shared__ v4i lk[4 * 4 * DT * 64], lv[4 * 4 * DT * 64];
   __shared__ uint32_t taken;
-  const uint32_t left = a.counter[1];
-  const bool flagged = __any(prompt_mask(a.mask) != 0);
-  if (!flagged && !left) return;  // uniform
+  const uint32_t left = (uint32_t)__builtin_amdgcn_readfirstlane((int)a.counter[1]);
+  if (!left) return;  // uniform
+  const bool flagged = left == kPromptAll;
+  if (flagged && a.clear && blockIdx.x == 0 && threadIdx.x < kPromptWords) a.clear[kMaskStride * threadIdx.x] = 0;
   const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   uint32_t item = blockIdx.x;
 #pragma unroll 1

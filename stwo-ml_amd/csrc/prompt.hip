@@ -136,7 +136,6 @@ static int attention_prompt(gkr_ctx* c, const gkr_matrix* q, const gkr_matrix* k
     a.counter = a.todo + room;
     TRY(pack_all(a.counter, (uint32_t)(kPromptCounters * launches)));
     auto launch = [&]() -> int {
-      if (a.items == 0) return GKR_OK;
       TRY(kernels());
       a.n = a.items = a.general_items = 0;
       a.counter += kPromptCounters;
@@ -152,9 +151,11 @@ static int attention_prompt(gkr_ctx* c, const gkr_matrix* q, const gkr_matrix* k
       e.row = first_row[i];
       a.items += e.tiles * kv_heads;
       a.general_items += (e.tiles + per - 1) / per * kv_heads;
-      if (a.n == kPromptSeqs || a.items > 1u << 22) TRY(launch());
+      const bool last = i == order.back();
+      if (last) a.clear = mask;
+      if (last || a.n == kPromptSeqs || a.items > 1u << 22) TRY(launch());
     }
-    return launch();
+    return GKR_OK;
   };
   // R1 and W1 of the int8 kernel, R4 and W4 of the other: tiles of 16 rows a wave, waves
 #define GKR_PROMPT(DT, R1, W1, OCC1, R4, W4, OCC4)                                                                    \

@@ -68,7 +68,8 @@ static bool quantized_rows_fit(const WitRows& a, const gkr_matrix* w) {
 
 // Two masks of the packing, used in turn: the packing of one product clears the
 // other's.  A mask that is set says that rows may have four planes, which is right
-// for all rows: a captured product may find its own from the last replay.
+// for all rows: a captured product may find its own from the last replay.  A prompt
+// zeroes its own too (k_prompt), as there the kernel of general words costs more.
 static int wit_masks(gkr_ctx* c, uint32_t** mask, uint32_t** next_mask) {
   constexpr uint32_t words = kMaskWords * kMaskStride;
   if (!c->wit_mask) {
