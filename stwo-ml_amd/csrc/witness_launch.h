@@ -4,6 +4,7 @@
 #include "gemm.h"
 #include "internal.h"
 #include "witness.h"
+#include "witness_cost.h"
 
 // The m x k words that the weights are multiplied by.
 struct WitRows {
@@ -87,42 +88,6 @@ static int wit_masks(gkr_ctx* c, uint32_t** mask, uint32_t** next_mask) {
   return GKR_OK;
 }
 
-// What the two kinds of kernel take, in us, to choose between them; fitted to 27
-// products of 40 to 512 rows, k 100 to 13824, n 900 to 13824, rows and weights
-// of one plane and of four, which each kind took 10 to 330 us for: within a
-// quarter, and the better one taken in all but two (by 1.1 and 1.2 times).
-// k_wit_tiles: 8 us for each round of the workgroups that fit at once (`slots`),
-// and the operands' way from the second-level cache, 17 GB/ms; kb is a
-// workgroup's K step.
-static double tiles_us(uint64_t groups, uint32_t slots, uint32_t nsteps, uint32_t kb) {
-  return 8.0 * (double)((groups + slots - 1) / slots) + (double)groups * nsteps * kb / 17000.0;
-}
-// k_wit_blocks: a workgroup fills a CU; a K step takes it 0.27 us where few run
-// and 0.5 on all 256 (the matrix cores slow down).  K splits fill the last
-// round, against the parts' way through memory and a launch to join them.
-static double blocks_us(uint64_t groups, uint32_t nsteps, uint64_t elements, uint32_t* splits) {
-  double best = 0;
-  for (uint32_t s = 1; s <= 16 && (s == 1 || nsteps / s >= 16); s++) {
-    const uint64_t rounds = (groups * s + 255) / 256, steps = (nsteps + s - 1) / s;
-    const double step = 0.27 + 0.23 * std::min(1.0, (double)(groups * s) / 256);
-    const double us = 12.0 + step * (double)(rounds * steps) + (s > 1 ? 5.0 + (double)s * (double)elements * 2e-6 : 0.0);
-    if (s == 1 || us < best) {
-      best = us;
-      *splits = s;
-    }
-  }
-  return best;
-}
-
-// k_wit_wide, 128 x 96 a workgroup: fitted to 24 products of 300 to 2048 rows, k 576 to
-// 13824, n 1024 to 8000, 8 to 228 us without the packing, within a seventh; a quarter
-// more, as the others' times are only that well known.  Beyond two rounds the rows and
-// weights no longer lie in the second-level caches (5000 x 13824 x 5120 in nine rounds
-// 640 us, k_wit_blocks 440).
-static double wide_us(uint64_t groups, uint32_t nsteps) {
-  return groups > 512 ? 1e30 : 1.25 * (2.0 + (double)((groups + 255) / 256) * (9.0 + 0.09 * nsteps));
-}
-
 // More rows: packed, multiplied (k_wit_tiles) and, where K is split, joined.  With
 // `quant` they are brought to 8 bits as they are packed, and have one plane.
 template <bool GATED, class End>
@@ -184,18 +149,16 @@ static int packed_product(gkr_ctx* c, const WitRows& a, const gkr_matrix* w0, co
     GKR_LAUNCH(c, kernel, grid, dim3(64 * waves), 0, g, rg, end);
     return check_launch(c);
   };
-  // the block kernels' column groups, and what they take (splits[]) for rows of one plane and of four
+  // the block kernels' column groups, and what they take for rows of one plane and of four
   constexpr uint32_t NW = GATED ? 2 : 1;
   const bool general = w0->bnplanes > 1 || w1->bnplanes > 1;
-  const uint64_t bgroups = (ctiles * NW * (general ? 4 : 1) + 7) / 8, elements = m * n * NW;
-  uint32_t splits[2] = {1, 1};
-  const double blocks[2] = {blocks_us((one_tiles + 7) / 8 * bgroups, g.nsteps, elements, &splits[0]),
-                            quant ? 0 : blocks_us((four_tiles + 7) / 8 * bgroups, g.nsteps, elements, &splits[1])};
+  const uint64_t bgroups = (ctiles * NW * (general ? 4 : 1) + 7) / 8;
+  const PackedCost cost(m, n, g.nsteps, GATED, general, quant != nullptr);
   // rows1: row tiles a workgroup has of rows of one plane that it streams the weights for; 0: blocks as for four
   auto launch_blocks = [&](auto kernel, uint32_t rows1) -> int {
     g.cgroups = (uint32_t)bgroups;
-    TRY(plan(0, rows1 ? rows1 : 8, rows1 ? 1 : splits[0]));
-    TRY(plan(1, 8, splits[1]));
+    TRY(plan(0, rows1 ? rows1 : 8, rows1 ? 1 : cost.splits[0]));
+    TRY(plan(1, 8, cost.splits[1]));
     uint64_t grid = 0;
     for (int i = 0; i < 2; i++) {
       const uint64_t groups = (uint64_t)g.plan[i].rgroups * (i == 0 && rows1 ? g.ctiles : g.cgroups);
@@ -207,7 +170,7 @@ static int packed_product(gkr_ctx* c, const WitRows& a, const gkr_matrix* w0, co
   auto launch_wide = [&](auto kernel, uint32_t rt, uint32_t ct) -> int {
     g.cgroups = (uint32_t)bgroups;
     TRY(plan(0, rt, 1));
-    TRY(plan(1, 8, splits[1]));
+    TRY(plan(1, 8, cost.splits[1]));
     const uint64_t wide = (uint64_t)g.plan[0].rgroups * ((g.ctiles + ct - 1) / ct);
     const uint64_t other = ((uint64_t)g.plan[1].rgroups * g.cgroups + 7) / 8 * 8 * g.plan[1].splits;
     GKR_LAUNCH(c, kernel, dim3((uint32_t)std::max((wide + 7) / 8 * 8, other)), dim3(512), 0, g, end);
@@ -220,7 +183,7 @@ static int packed_product(gkr_ctx* c, const WitRows& a, const gkr_matrix* w0, co
   if (general) {
     const double tiles = tiles_us(one_tiles * ctiles, 256, g.nsteps, 1 + 4 * NW) +
                          (quant ? 0 : tiles_us((four_tiles + 1) / 2 * ctiles, 256, g.nsteps, 2 * (1 + 4 * NW)));
-    if (GATED || tiles <= blocks[0] + blocks[1]) {
+    if (GATED || tiles <= cost.blocks[0] + cost.blocks[1]) {
       TRY(GKR_WIT_TILES(1, 4, W, 1, 2));
     } else if constexpr (!GATED) {
       TRY(launch_blocks(k_wit_blocks<4, false, End>, 0));
@@ -230,20 +193,17 @@ static int packed_product(gkr_ctx* c, const WitRows& a, const gkr_matrix* w0, co
   else if (m <= 32) TRY(GKR_WIT_TILES(1, 1, W, 1, 4));
   else if (m <= 64) TRY(GKR_WIT_TILES(2, 1, W, 1, 4));
   else {
-    const uint64_t rows64 = (m + 63) / 64;
-    const double tiles = tiles_us(rows64 * ctiles, 512, g.nsteps, 2 + NW) +
-                         (quant ? 0 : tiles_us(rows64 * ctiles, 512, g.nsteps, 4 * (2 + NW)));
-    constexpr uint32_t RT = GATED ? 2 : 4, WR = GATED ? 2 : 1;
-    const uint32_t down = m <= 128 ? WR : 2 * WR;  // waves down the rows of k_wit_mixed
-    const double mixed = m <= 256 ? tiles_us(ctiles, 256, g.nsteps, down * (RT + NW)) + blocks[1] : 1e30;
-    const double wide = GATED ? 1e30 : wide_us((m + 127) / 128 * ((ctiles + 2) / 3), g.nsteps);
-    const double most = std::min(wide, blocks[0]) + blocks[1];
-    if (tiles <= std::min(mixed, most)) TRY(GKR_WIT_TILES(2, 1, W, 1, 4));
-    else if (mixed > most && wide < blocks[0]) {
-      if constexpr (!GATED) TRY(launch_wide(k_wit_wide<4, 3, End>, 4, 3));
-    } else if (mixed > most) TRY(launch_blocks(k_wit_blocks<1, GATED, End>, 0));
-    else if (m <= 128) TRY(launch_blocks(k_wit_mixed<RT, WR, GATED, End>, RT * WR));
-    else TRY(launch_blocks(k_wit_mixed<RT, 2 * WR, GATED, End>, 2 * RT * WR));
+    constexpr uint32_t RT = GATED ? 2 : 4, WR = GATED ? 2 : 1;  // k_wit_mixed: row tiles of a wave, waves down the rows
+    switch (cost.kernel(m, n, g.nsteps, GATED, quant != nullptr)) {
+      case PackedKernel::kTiles: TRY(GKR_WIT_TILES(2, 1, W, 1, 4)); break;
+      case PackedKernel::kWide:
+        if constexpr (!GATED) TRY(launch_wide(k_wit_wide<4, 3, End>, 4, 3));
+        break;
+      case PackedKernel::kBlocks: TRY(launch_blocks(k_wit_blocks<1, GATED, End>, 0)); break;
+      case PackedKernel::kMixed:
+        if (m <= 128) TRY(launch_blocks(k_wit_mixed<RT, WR, GATED, End>, RT * WR));
+        else TRY(launch_blocks(k_wit_mixed<RT, 2 * WR, GATED, End>, 2 * RT * WR));
+    }
   }
 #undef GKR_WIT_TILES
   if (max_splits > 1) {
