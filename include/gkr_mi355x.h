@@ -445,6 +445,7 @@ int gkr_matmul_forward_quantized(gkr_ctx* ctx, const gkr_matrix* a, const gkr_ma
  *   (turned - 2)); WAVES: with w = positions f_i waves in the context that was trained
  *   on, divided by the factor where w <= low, kept where w >= high, and in between
  *   f_i (g + (1 - g) / factor) with g = (w - low) / (high - low).  NULL: PLAIN.
+ *   A frequency or a changed base that a float64 does not hold is refused.
  * gkr_rotary_new: the table of C and S, eight bytes a pair and position (0 .. positions
  *   - 1), on the context's device; the call returns when it is there.
  * gkr_rotary_forward: counts[i] rows of sequence i at positions starts[i], starts[i] + 1

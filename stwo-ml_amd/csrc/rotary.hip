@@ -29,6 +29,8 @@ extern "C" int gkr_rotary_frequencies(uint32_t turned, double base, const gkr_ro
                                      !(s.high > s.low) || !isfinite(s.high)))
     return fail(GKR_ERR_INVALID, "rotary frequencies: %g positions, waves between %g and %g", s.positions, s.low, s.high);
   if (s.kind == GKR_ROTARY_BASE && turned > 2) base *= pow(s.factor, turned / (turned - 2.0));
+  if (!(base > 0) || !isfinite(base))
+    return fail(GKR_ERR_INVALID, "rotary frequencies: a base changed by a factor of %g to %g", s.factor, base);
   for (uint32_t i = 0; i < turned / 2; i++) {
     double f = pow(base, -2.0 * i / turned) / 6.283185307179586476925;  // turns a position
     if (s.kind == GKR_ROTARY_LINEAR) f /= s.factor;
@@ -36,6 +38,7 @@ extern "C" int gkr_rotary_frequencies(uint32_t turned, double base, const gkr_ro
       const double keep = fmin(fmax((s.positions * f - s.low) / (s.high - s.low), 0.0), 1.0);
       f *= keep + (1 - keep) / s.factor;
     }
+    if (!isfinite(f)) return fail(GKR_ERR_INVALID, "rotary frequencies: a base of %g and a factor of %g", base, s.factor);
     f -= floor(f);  // whole turns are none
     out[i] = f < 1 ? (uint64_t)(f * 18446744073709551616.0) : 0;
   }

@@ -53,3 +53,13 @@ def test_refusals():
         assert e.value.code == 1, args
     assert G.lib().gkr_rotary_frequencies(4, 1e4, None, None) == 1
     assert len(np.unique(G.rotary_frequencies(128))) == 64
+
+
+def test_frequencies_past_float64_are_refused():
+    """Turns a position, or a changed base, that a float64 does not hold: not zeros for them."""
+    for args in ((128, 1e-320), (128, 1e4, G.ROTARY_LINEAR, 1e-320), (128, 1e308, G.ROTARY_BASE, 1e10),
+                 (128, 1e-308, G.ROTARY_BASE, 1e-30), (4, 1e4, G.ROTARY_BASE, 1e300)):
+        with pytest.raises(G.GkrError, match="base") as e:
+            G.rotary_frequencies(*args)
+        assert e.value.code == 1, args
+    assert close(turns(G.rotary_frequencies(2, 1e308)), [1 / (2 * math.pi)])
