@@ -415,7 +415,7 @@ int gkr_gated_forward(gkr_ctx* ctx, const gkr_matrix* a, const gkr_matrix* wg, c
  *   Y = t cut off at +-limit, + residual (mod P)
  * with centered values c and halves rounded away from zero, exact for any words
  * (shift 0 .. 63; limit 1 .. 2^30 - 1, 0 = 2^30 - 1).  With a limit of 127 or less
- * Y are words that an int8 cache takes.  A is m x k, B k x n, row_scales m x 1,
+ * and no residual Y are words that an int8 cache takes.  A is m x k, B k x n, row_scales m x 1,
  * col_scales and bias 1 x n, residual, pre (Z) and out (Y) m x n; the residual may
  * be the output itself, also by another handle of the same memory.
  *
@@ -515,11 +515,12 @@ int gkr_attention_forward(gkr_ctx* ctx, const gkr_kv_cache* cache, const gkr_mat
                           gkr_matrix* out);
 
 /* Causal attention of whole prompts: counts[i] tokens of sequence i (0 .. 131071), the
- * rows of q (n_heads * head_dim words, head_dim at most 256), k and v (n_kv_heads *
- * head_dim) in that order; their number is the sum of the counts.  A token sees
+ * rows of q (n_heads * head_dim words, head_dim at most 256, up to 65535 heads), k and v
+ * (n_kv_heads * head_dim, up to 4096 heads) in that order; their number is the sum of the
+ * counts.  A sequence of more than 2^29 tokens times query heads may be refused.  A token sees
  * itself and those before it in its sequence; weights, means and the other outputs
  * as gkr_attention_forward has them for a cache with those keys and values (any
- * canonical words; int8-range ones take an eighth of the products).  A prompt that
+ * canonical words; int8-range ones on all sides take a twelfth of the products).  A prompt that
  * goes on in a cache is also appended to it; tokens behind cached ones are
  * gkr_attention_forward's.                                                    */
 int gkr_attention_prompt(gkr_ctx* ctx, const gkr_matrix* q, const gkr_matrix* k, const gkr_matrix* v,

@@ -245,8 +245,9 @@ __device__ __forceinline__ uint32_t prompt_mean(int64_t total, uint32_t z, doubl
 
 // The same of int8-range values, from the negated total and -1 / z, to a word: the
 // quotient is at most 128, |total| / z + 1/2 a multiple of 1 / 2 z, 2^-28 and more,
-// and its error in 53 bits below 2^-43, so 2^-30 more decides it; the conversion
-// cuts towards zero.
+// and its error below 2^-37 (1 / z to 2^-45 by k_prompt_int8's step of Newton's, so
+// 2^-38 of the quotient; prompt_end divides, to 2^-53), so 2^-30 more decides it; the
+// conversion cuts towards zero.
 __device__ __forceinline__ uint32_t prompt_mean(double negated, double inv) {
   const int32_t r = (int32_t)__builtin_fma(negated, inv, __builtin_copysign(0.5 + 0x1p-30, -negated));
   return umin32((uint32_t)r, (uint32_t)r + P);
@@ -945,7 +946,12 @@ static __global__ void __launch_bounds__(64 * W, OCC) k_prompt_int8(PromptArgs a
 // workgroups than fit at once: the items are taken in turn, the longest first, and
 // with nothing to do the launch is short (4.7 us; 7.5 with a workgroup for each of 2432
 // items).  Items of one kv head for the workgroups of an XCD gain nothing (1501 general
-// tokens, 40 heads on 8 x 128: 205 us either way).  The mask is the int8 kernel's to
+// tokens, 40 heads on 8 x 128: the same either way).  Those tokens take 180 us here
+// where it runs again and again (203 in the first few dozen calls under a tracer, when
+// the clock is lower), 7.7 in the packing and 6 in the int8 kernel; the call 191 without
+// a tracer.  The matrix cores are busy a third of the cycles: a wave holds the five digit
+// sums of all dims, and registers spill (116 at up to 128 dims, 810 above; with traces 247
+// and 899).  The mask is the int8 kernel's to
 // read; the last launch of a call zeroes it, so that a graph of one prompt, whose
 // replays all have the same mask, does not find it set by general words of an earlier
 // one (1500 int8 tokens, 16 heads of 128: 46 us, and 176 for every replay behind such).

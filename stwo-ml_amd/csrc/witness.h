@@ -846,10 +846,13 @@ static __global__ void __launch_bounds__(64 * W) k_wit_tiles(WitProduct g, uint3
 // all of the tiles, straight from memory into registers.  No operand is read twice by
 // a workgroup, nothing waits for another wave until the waves' sums meet in LDS, and
 // no parts go through memory: where k_wit_blocks' 256 x 256 leave most CUs without a
-// workgroup or split K (scales, no residual: 512 x 5120 x 5120 38 us with the join, 25
-// so; 512 x 13824 x 5120 58 and 47; 700 x 576 x 1536 27 and 8).  Bound by a CU's way to
-// its second-level cache, 7 KB a K step at 78 GB/s (two, three or four steps in flight,
-// 2 x 4 and 2 x 5 tiles: the same).
+// workgroup or split K (scales, no residual, operands in the caches: 512 x 5120 x 5120
+// 38 us with the join, 25 so; 512 x 13824 x 5120 58 and 47; 700 x 576 x 1536 27 and 8; with
+// the packing and operands from memory 512 x 5120 x 5120 40 and 29, 512 x 13824 x 5120,
+// quantized, 82.6 and 78.8).  Between start and end bound by a CU's way to its
+// second-level cache, 7 KB a K step at 78 GB/s (two, three or four steps in flight, 2 x 4
+// and 2 x 5 tiles: the same); over the whole kernel the matrix cores are busy two fifths
+// of the cycles, as all the waves' sums meet at the end and nothing is there at the start.
 template <int RT, int CT, class End>
 __device__ __forceinline__ void wit_wide(const WitProduct& g, int32_t* sums, uint32_t rg, uint32_t cg, const End& end) {
   constexpr int W = 8, U = 2;
